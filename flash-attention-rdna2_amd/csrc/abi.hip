@@ -45,6 +45,9 @@ extern "C" size_t fable_attn_struct_size(int which) {
     case 5: return sizeof(FwdParams);
     case 6: return sizeof(BwdParams);
     case 7: return sizeof(DecParams);
+    case 8: return sizeof(FableCache8);
+    case 9: return sizeof(FableAppendParams);
+    case 10: return sizeof(FableGatherParams);
     default: return 0;
   }
 }

@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "attn_device.hpp"
+#include "dec_common.hpp"
 #include "fwd_common.hpp"
 #include "status.hpp"
 
@@ -37,147 +38,10 @@ static int dec_checked(FableDecParams p, int dtype, void* stream, const void* ne
 
 constexpr int kDecChunk = 32;  // keys per wave iteration of the fp32 kernel; splits are multiples
 constexpr int kDecKeys = 16;   // keys per wave iteration of the fp16/bf16 kernel
-constexpr int kDecWaves = 4;
 static_assert(kDecKeys <= 16, "a chunk spans at most two pages of >= 16 rows (SPT)");
 
-__device__ __forceinline__ float xor16_max(float x) {
-  return fmaxf(x, __shfl_xor(x, 16));
-}
-__device__ __forceinline__ float xor16_sum(float x) { return x + __shfl_xor(x, 16); }
-
-// Rows of a (sequence, K/V head): its nq new tokens x the gqa q heads of its group, token first;
-// workgroups take them in groups of 16. The keys of a sequence some row sees are [lo, hi); row
-// masks cut them down (a row of token tk sees [max(leftpad, pos - window + 1), ctx + (append ? tk +
-// 1 : 0))). With `append` the span reaches down to ctx, so that it holds every new key.
-struct DecSpan {
-  int ctx, lo, hi;
-};
-// The lengths and tables are read as constant memory, which no kernel here writes: uniform entries
-// then come by scalar loads (the kernels' own stores otherwise turn them into vector loads, whose
-// in-order counter they would share with the row loads: C4 311 -> 319 us).
-typedef const __attribute__((address_space(4))) int* cint_ptr;
-__device__ __forceinline__ cint_ptr cmem(const int* p) { return (cint_ptr)(uintptr_t)p; }
-__device__ __forceinline__ int dec_room(const FableDecParams& p) {
-  return (int)min((long long)p.max_blocks * p.page, 0x7FFFFFFFLL);
-}
-__device__ __forceinline__ int dec_lo(const FableDecParams& p, int b, int ctx, int tk) {
-  int lo = p.leftpad ? cmem(p.leftpad)[b] : 0;
-  if (p.window >= 0) lo = max(lo, ctx + tk - p.window + 1);
-  return max(lo, 0);
-}
-__device__ __forceinline__ int dec_hi(const FableDecParams& p, int ctx, int tk, int append) {
-  return min(ctx + (append ? tk + 1 : 0), dec_room(p));
-}
-__device__ __forceinline__ DecSpan dec_span(const FableDecParams& p, int b, int append) {
-  DecSpan r;
-  r.ctx = cmem(p.ctx_len)[b];
-  r.lo = dec_lo(p, b, r.ctx, 0);
-  if (append) r.lo = max(min(r.lo, r.ctx), 0);
-  r.hi = dec_hi(p, r.ctx, p.nq - 1, append);
-  return r;
-}
-
-// How a call's keys are shared out when the caller sets no split count (p.nsplit 0). The lengths
-// stay on the device, so every workgroup works out the shares by itself, from units of kUnit keys (a
-// sequence has one at least):
-//  * even: `parts` workgroups per (K/V head, row group); each sequence is cut into runs of `per`
-//    units, `per` the least for which the runs fit the parts, so every workgroup has one run at
-//    most. Taken where that is at most a quarter above an even share (few or alike sequences), or
-//    kSegUnits units: a stream's workgroup pays a second segment, which costs about as much.
-//  * stream: otherwise (many sequences of unequal lengths) the sequences' units follow one another
-//    and each workgroup (two per part when there are more sequences than parts) takes as many, whatever sequences they belong to.
-// A sequence that lies in one workgroup is finished there; of the others each writes a partial record
-// (a stream's workgroup one for a sequence it goes on with, slot 0, and one for a sequence that goes
-// on after it, slot 1). Two equal splits per sequence, the host's choice before, left 48 requests of 64
-// to 8192 keys (Hq 64 / Hk 8, D 128) waiting for the longest: 142 us, 125 as a stream.
+// keys of a unit of a share (DecShare)
 constexpr int kUnit = kDecKeys * kDecWaves;
-__device__ __forceinline__ int dec_units(const DecSpan& r) { return max((r.hi - r.lo + kUnit - 1) / kUnit, 1); }
-// inclusive prefix sum over the wave (row shifts within 16 lanes, then two broadcasts)
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
-__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-// Every wave for itself: lane l holds the span of sequence base + l, read from memory once for
-// batches of up to 64 sequences (a chain of dependent loads ahead of the first row load is what a
-// short segment takes longest for).
-struct DecShare {
-  DecSpan mine;
-  int units;        // of sequence base + lane; 0 past the batch
-  int base;
-  int total, per;   // units of the call, units per run (even) or workgroup (stream)
-  bool even;
-  __device__ __forceinline__ void load(const FableDecParams& p, int append, int b0, int lane) {
-    base = b0;
-    mine = DecSpan{0, 0, 0};
-    units = 0;
-    if (b0 + lane < p.batch) {
-      mine = dec_span(p, b0 + lane, append);
-      units = dec_units(mine);
-    }
-  }
-  // sum over the batch of f(units); sequence 0's lanes are loaded afterwards
-  template <typename F>
-  __device__ __forceinline__ int sum(const FableDecParams& p, int append, int lane, F&& f) {
-    int t = 0;
-#pragma nounroll
-    for (int b0 = (p.batch - 1) & ~63; b0 >= 0; b0 -= 64) {
-      if (b0 != base) load(p, append, b0, lane);
-      t += wave_sum(f(units));
-    }
-    return t;
-  }
-  __device__ __forceinline__ void init(const FableDecParams& p, int append, int parts, int lane) {
-    load(p, append, 0, lane);
-    total = sum(p, append, lane, [](int u) { return u; });
-    const int least = max((int)((unsigned)(total + parts - 1) / (unsigned)parts), 1);
-    even = false;
-    if (p.batch <= parts) {
-#pragma nounroll
-      for (per = least; 4 * per <= 5 * least || per <= least + kSegUnits; per += max(per >> 4, 1)) {
-        if (sum(p, append, lane, [=](int u) { return (int)((unsigned)(u + per - 1) / (unsigned)per); }) <= parts) {
-          even = true;
-          break;
-        }
-      }
-    }
-    if (!even) per = p.batch <= parts ? least : (least + 1) / 2;
-  }
-  // items: runs (even) or units (stream) of a sequence
-  __device__ __forceinline__ int items(int u) const { return even ? (int)((unsigned)(u + per - 1) / (unsigned)per) : u; }
-  __device__ __forceinline__ DecSpan span(int b) const {
-    const int l = b - base;
-    return DecSpan{__builtin_amdgcn_readlane(mine.ctx, l), __builtin_amdgcn_readlane(mine.lo, l), __builtin_amdgcn_readlane(mine.hi, l)};
-  }
-  // the sequence that holds item `at`, and its first item (p.batch: no such item); after init
-  __device__ __forceinline__ int seek(const FableDecParams& p, int append, int at, int lane, int& first) {
-    first = 0;
-#pragma nounroll
-    for (;;) {
-      const int inc = wave_scan(items(units)), sum = __builtin_amdgcn_readlane(inc, 63);
-      if (at >= first + sum) {
-        first += sum;
-        if (base + 64 >= p.batch) return p.batch;
-        load(p, append, base + 64, lane);
-        continue;
-      }
-      const int n = __popcll(__builtin_amdgcn_ballot_w64(first + inc <= at));   // sequences that end before `at`
-      if (n > 0) first += __builtin_amdgcn_readlane(inc, n - 1);
-      return base + n;
-    }
-  }
-  // (at least 4 units per run and streams from a quarter above the even share on: 24 sequences of 500 keys, Hq 32 /
-  // Hk 8, D 128, 21.3 us, 19.0 now; 3 of 500 13.7 and 11.6; 5 of 300 14.1 and 11.2)
-  static constexpr int kSegUnits = 6;
-};
-
-// floats ahead of the records: two ints per sequence, for the combine
-__host__ __device__ inline long long dec_meta_floats(const FableDecParams& p) { return (2ll * p.batch + 63) / 64 * 64; }
 
 // The partial kernel's argument. The phases that only some workgroups run (the shares, the append)
 // read it again from the kernel argument segment: the phases together use most of the 40 fields,
@@ -254,7 +118,7 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
     return p;
   };
   // segments: a stream part's (sequence, run of keys), or the one split of the grid
-  DecShare str;
+  DecShare<kUnit> str;
   int at = 0, at_end = 0, sq = 0, first = 0;  // (units; sq: the sequence that holds `at`, first: its first)
   if constexpr (SHARE) {
     const DecArgs p = dec_reload();
@@ -296,7 +160,7 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
     const DecArgs p = dec_reload();
     if (b >= str.base + 64) str.load(p, append, b, lane);
     sp = str.span(b);
-    const int units = dec_units(sp), stop = min(at_end, first + units);
+    const int units = dec_units<kUnit>(sp), stop = min(at_end, first + units);
     start = sp.lo + (at - first) * kUnit;
     end = min(sp.lo + (stop - first) * kUnit, sp.hi);
     const bool begins = at == first;
@@ -926,27 +790,6 @@ __global__ __launch_bounds__(256) void dec_append_kernel(FableDecParams p, const
   ((T*)p.Vc)[dst] = nv[src + d];
 }
 
-// row groups of 16 per (sequence, K/V head)
-static int dec_groups(const FableDecParams& p) { return (int)(((long long)p.nq * p.gqa + 15) / 16); }
-
-// Parts of a call (DecShare): one workgroup per CU (more in flight per CU read a batch of alike
-// sequences slower: C4 0.96x with two, 0.86x with three), or two where the (K/V head, row group) count
-// leaves more than an eighth of the CUs out of a round of one.
-static int dec_parts(const FableDecParams& p) {
-  const long long X = (long long)(p.NH / p.gqa) * dec_groups(p);
-  long long parts = 256 / X;
-  if (parts * X < 224) parts = (512 + X - 1) / X;
-  const long long units = (long long)p.batch * (((long long)p.max_blocks * p.page + kUnit - 1) / kUnit + 1);
-  parts = parts < units ? parts : units;
-  return parts > 1 ? (int)parts : 1;
-}
-// workgroups per (K/V head, row group) (DecShare::init)
-static int dec_share_wgs(const FableDecParams& p) { return p.batch <= dec_parts(p) ? dec_parts(p) : 2 * dec_parts(p); }
-// scratch: two records of 16 rows per workgroup
-static long long dec_share_bytes(const FableDecParams& p) {
-  return (dec_meta_floats(p) + (long long)dec_share_wgs(p) * 2 * (p.NH / p.gqa) * dec_groups(p) * 16 * (p.HD + 2)) * 4;
-}
-
 template <typename T, int HD>
 static int launch_dec_partial(const FableDecParams& p, dim3 grid, int page_shift, int flags, int parts, hipStream_t st, const void* nk,
                               const void* nv) {
@@ -991,6 +834,25 @@ static bool dec_fuses_append(const FableDecParams& p, const void* nv) {
   return !std::is_same<T, float>::value && p.nq == 1 && (!p.block_table || p.batch == 1) && ((uintptr_t)nv & 15) == 0;
 }
 
+// merge of the fixed grid's partials
+template <typename T, int HD>
+static int launch_dec_combine(const FableDecParams& p, hipStream_t st) {
+  const dim3 cg(p.batch * p.nq, p.NH);
+  if (p.nsplit <= 2)
+    hipLaunchKernelGGL((dec_combine_kernel<T, HD, 2>), cg, dim3(HD), 0, st, p, 0);
+  else if (p.nsplit <= 4)
+    hipLaunchKernelGGL((dec_combine_kernel<T, HD, 4>), cg, dim3(HD), 0, st, p, 0);
+  else
+    hipLaunchKernelGGL((dec_combine_kernel<T, HD, 8>), cg, dim3(HD), 0, st, p, 0);
+  return launch_status("fable_attn_dec (combine)");
+}
+// and of the shares'
+template <typename T, int HD>
+static int launch_dec_share_combine(const FableDecParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((dec_combine_kernel<T, HD, 8, true>), dim3(p.batch * p.nq, p.NH), dim3(HD), 0, st, p, dec_groups(p));
+  return launch_status("fable_attn_dec (combine)");
+}
+
 template <typename T, int HD>
 static int launch_dec(const FableDecParams& p, hipStream_t st, const void* nk, const void* nv) {
   const int page_shift = __builtin_ctz((unsigned)p.page);
@@ -1013,28 +875,36 @@ static int launch_dec(const FableDecParams& p, hipStream_t st, const void* nk, c
     if (p.nsplit == 1) return FA_OK;
   }
   if (int rc = launch_status("fable_attn_dec (partial)")) return rc;
-  const dim3 cg(p.batch * p.nq, p.NH);
-  if (p.nsplit <= 2)
-    hipLaunchKernelGGL((dec_combine_kernel<T, HD, 2>), cg, dim3(HD), 0, st, p, 0);
-  else if (p.nsplit <= 4)
-    hipLaunchKernelGGL((dec_combine_kernel<T, HD, 4>), cg, dim3(HD), 0, st, p, 0);
-  else
-    hipLaunchKernelGGL((dec_combine_kernel<T, HD, 8>), cg, dim3(HD), 0, st, p, 0);
-  return launch_status("fable_attn_dec (combine)");
+  return launch_dec_combine<T, HD>(p, st);
 }
 
 // the call with its shares worked out on the device (p.nsplit 0)
 template <typename T, int HD>
 static int launch_dec_share(const FableDecParams& p, hipStream_t st, const void* nk, const void* nv) {
-  const int ngrp = dec_groups(p), X = p.NH / p.gqa * ngrp, parts = dec_parts(p);
+  const int ngrp = dec_groups(p), X = p.NH / p.gqa * ngrp, parts = dec_parts(p, kUnit);
   const bool fuse = dec_fuses_append<T>(p, nv);
   if (nk && !fuse)
     if (int rc = launch_dec_append<T, HD>(p, st, nk, nv)) return rc;
-  if (int rc = launch_dec_partial<T, HD>(p, dim3((unsigned)X, (unsigned)dec_share_wgs(p)), __builtin_ctz((unsigned)p.page), nk ? kDecAppend : 0, parts,
+  if (int rc = launch_dec_partial<T, HD>(p, dim3((unsigned)X, (unsigned)dec_share_wgs(p, kUnit)), __builtin_ctz((unsigned)p.page), nk ? kDecAppend : 0, parts,
                                          st, fuse ? nk : nullptr, nv))
     return rc;
-  hipLaunchKernelGGL((dec_combine_kernel<T, HD, 8, true>), dim3(p.batch * p.nq, p.NH), dim3(HD), 0, st, p, ngrp);
-  return launch_status("fable_attn_dec (combine)");
+  return launch_dec_share_combine<T, HD>(p, st);
+}
+
+// the merge of an 8-bit cache's partials (dec_common.hpp), in the kernel of the next width
+template <typename T>
+static int dec_combine_dispatch(const FableDecParams& p, hipStream_t st, bool share) {
+  auto go = [&](auto w) {
+    constexpr int HD = decltype(w)::value;
+    return share ? launch_dec_share_combine<T, HD>(p, st) : launch_dec_combine<T, HD>(p, st);
+  };
+  if (p.HD <= 64) return go(std::integral_constant<int, 64>{});
+  if (p.HD <= 128) return go(std::integral_constant<int, 128>{});
+  if (p.HD <= 192) return go(std::integral_constant<int, 192>{});
+  return go(std::integral_constant<int, 256>{});
+}
+int dec_combine(const FableDecParams& p, int dtype, hipStream_t st, bool share) {
+  return dtype == FA_F16 ? dec_combine_dispatch<_Float16>(p, st, share) : dec_combine_dispatch<__bf16>(p, st, share);
 }
 
 // fp16/bf16: every head dim that is a multiple of 8 up to 256 runs in the kernel of the next
@@ -1382,7 +1252,7 @@ constexpr long long kShareBytes = 128LL << 20;
 static bool dec_shares(const FableDecParams& p, int dtype) {
   if (dtype == FA_F32 || p.nsplit > 0 || p.batch < 2 || p.gqa <= 0 || p.page < 16) return false;
   if ((long long)p.batch * p.max_blocks * p.page * (p.NH / p.gqa) * p.HD * 4 < kShareBytes) return false;
-  const int parts = fa::dec_parts(p);
+  const int parts = fa::dec_parts(p, fa::kUnit);
   return p.batch > parts || parts % p.batch != 0;
 }
 // splits per sequence otherwise: its rows are packed into dec_groups groups
@@ -1404,7 +1274,7 @@ extern "C" int64_t fable_attn_dec_ws_bytes(FableDecParams p, int dtype, int appe
     if (launch_fwd_paged(f, pg, dtype, p.rotary != 0, nullptr, fw) != FA_OK) return -1;
     return 2 * dec_q_bytes(p) + fw.need;
   }
-  if (dec_shares(p, dtype)) return dec_share_bytes(p);
+  if (dec_shares(p, dtype)) return dec_share_bytes(p, kUnit);
   p.nsplit = dec_fixed_splits(p, dtype);
   return dec_uses_scratch(p, dtype) ? (int64_t)p.batch * p.nq * p.NH * p.nsplit * (p.HD + 2) * 4 : 0;
 }
@@ -1425,7 +1295,7 @@ extern "C" int fable_attn_dec_ws(FableDecParams p, int dtype, void* ws, int64_t 
                            : launch_dec_tiles<__bf16>(p, dtype, hint, (char*)ws, ws_bytes, (hipStream_t)stream_, new_k, new_v);
   long long need;
   if (share) {
-    need = dec_share_bytes(p);
+    need = dec_share_bytes(p, kUnit);
   } else {
     p.nsplit = hint;
     p.nsplit = dec_fixed_splits(p, dtype);

@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "attn_device.hpp"
+#include "cache8.hpp"
 #include "fwd_common.hpp"
 #include "status.hpp"
 
@@ -227,4 +228,43 @@ extern "C" int64_t fable_attn_fwd_paged_ws_bytes(FableFwdParams p, FablePagedKV 
 extern "C" int fable_attn_fwd_paged(FableFwdParams p, FablePagedKV kv, int dtype, void* ws_ptr, int64_t ws_bytes, void* stream) {
   fa::FwdWs ws{ws_ptr, ws_bytes, false, 0};
   return fa::paged_run(p, kv, dtype, ws, (hipStream_t)stream);
+}
+
+// ------------------------------------------------------------------ packed prompts over an 8-bit cache
+namespace fa {
+
+static int paged8_run(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype, FwdWs& ws, hipStream_t st) {
+  const char* what = "fable_attn_fwd_paged8";
+  const long long room = (long long)kv.max_blocks * kv.page;
+  if (!p.cu_q || !p.cu_k) return fail(FA_ERR_ARG, "%s: cu_q and cu_k are needed", what);
+  if (!ws.query && (!kv.block_table || !c.k_scale || !c.v_scale)) return fail(FA_ERR_ARG, "%s: null block_table or scales", what);
+  if (kv.max_blocks < 1 || room > 0x7FFFFFFF || (long long)p.batch * kv.max_blocks > 0x7FFFFFFF)
+    return fail(FA_ERR_ARG, "%s: max_blocks=%d page=%d batch=%d", what, kv.max_blocks, kv.page, p.batch);
+  if (dtype != FA_F16 && dtype != FA_BF16) return fail(FA_ERR_DTYPE, "%s: dtype %d not implemented (fp16/bf16)", what, dtype);
+  if (p.dropout_p > 0.0f) return fail(FA_ERR_ARG, "%s: no dropout over a cache", what);
+  if (int rc = cache8_check(what, c, p.HD, kv.page)) return rc;
+  if (c.k.b > 0x7FFFFFFF || c.v.b > 0x7FFFFFFF) return fail(FA_ERR_ARG, "%s: pages of 2 GiB", what);
+  p.SK = (int)room;
+  p.sK = fa_strides{0, c.k.h, c.k.s};
+  p.sV = fa_strides{0, c.v.h, c.v.s};
+  int rc;
+  if (fwd_check(p, dtype, ws.query, rc)) return rc;
+  FwdPaged8 pg;
+  (FwdPaged&)pg = FwdPaged{kv.block_table, -1, kv.max_blocks, __builtin_ctz((unsigned)kv.page), c.k.b, c.v.b, nullptr, 0, nullptr, nullptr, 1};
+  fwd_paged8_scales(pg, c, kv.page);
+  return launch_fwd_paged8(p, pg, dtype, false, st, ws);
+}
+
+}  // namespace fa
+
+extern "C" int64_t fable_attn_fwd_paged8_ws_bytes(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype) {
+  fa::FwdWs ws{nullptr, 0, true, 0};
+  if (fa::paged8_run(p, kv, c, dtype, ws, nullptr) != FA_OK) return -1;
+  return ws.need;
+}
+
+extern "C" int fable_attn_fwd_paged8(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype, void* ws_ptr, int64_t ws_bytes,
+                                     void* stream) {
+  fa::FwdWs ws{ws_ptr, ws_bytes, false, 0};
+  return fa::paged8_run(p, kv, c, dtype, ws, (hipStream_t)stream);
 }

@@ -112,6 +112,18 @@ struct FwdPaged {
   long long lse_sq;      // LSE stride of a query (1: packed prompts)
 };
 struct NoPaged {};
+// the same over an 8-bit cache (cache8.hpp): p.K / p.V are its codes, strides in bytes
+struct FwdPaged8 : FwdPaged {
+  const uint8_t *ks, *vs;   // scales [num_blocks][heads][subs]
+  int gshift, subs, num_blocks;
+};
+inline void fwd_paged8_scales(FwdPaged8& pg, const FableCache8& c, int page) {
+  pg.ks = c.k_scale;
+  pg.vs = c.v_scale;
+  pg.gshift = __builtin_ctz((unsigned)c.group);
+  pg.subs = page / c.group;
+  pg.num_blocks = c.num_blocks;
+}
 
 // lengths, key position of query 0 and row-0 offsets of sequence z (as seq_view; delta need not
 // be SK - SQ here: new tokens that are not in the cache follow its last key)
@@ -174,6 +186,14 @@ int launch_fwd_paged_d256(const FableFwdParams& p, const FwdPaged& pg, int dtype
 inline int launch_fwd_paged(const FableFwdParams& p, const FwdPaged& pg, int dtype, bool rot, hipStream_t st, FwdWs& ws) {
   return p.HD <= 64 ? launch_fwd_paged_d64(p, pg, dtype, rot, st, ws)
                     : (p.HD <= 128 ? launch_fwd_paged_d128(p, pg, dtype, rot, st, ws) : launch_fwd_paged_d256(p, pg, dtype, rot, st, ws));
+}
+// the same over an 8-bit cache (fwd_paged8_d64/d128/d256.hip)
+int launch_fwd_paged8_d64(const FableFwdParams& p, const FwdPaged8& pg, int dtype, bool rot, hipStream_t st, FwdWs& ws);
+int launch_fwd_paged8_d128(const FableFwdParams& p, const FwdPaged8& pg, int dtype, bool rot, hipStream_t st, FwdWs& ws);
+int launch_fwd_paged8_d256(const FableFwdParams& p, const FwdPaged8& pg, int dtype, bool rot, hipStream_t st, FwdWs& ws);
+inline int launch_fwd_paged8(const FableFwdParams& p, const FwdPaged8& pg, int dtype, bool rot, hipStream_t st, FwdWs& ws) {
+  return p.HD <= 64 ? launch_fwd_paged8_d64(p, pg, dtype, rot, st, ws)
+                    : (p.HD <= 128 ? launch_fwd_paged8_d128(p, pg, dtype, rot, st, ws) : launch_fwd_paged8_d256(p, pg, dtype, rot, st, ws));
 }
 // merge of the key-split partials (fwd.hip)
 int launch_fwd_split_combine(const FableFwdParams& p, int dtype, const FwdSplit& sp, hipStream_t st);

@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "attn_device.hpp"
+#include "cache8.hpp"
 #include "fwd_common.hpp"
 #include "status.hpp"
 
@@ -79,7 +80,11 @@ template <typename T, class C, bool CAUSAL, bool FEAT, bool DROP = false, class 
 __global__ __attribute__((amdgpu_flat_work_group_size(C::NT, C::NT),
                           amdgpu_waves_per_eu(C::WPE, C::WPE))) void
 fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
-  constexpr bool PG = std::is_same<PGT, FwdPaged>::value;
+  constexpr bool PG = std::is_base_of<FwdPaged, PGT>::value;
+  // Q8: the pages hold codes with scales (cache8.hpp); a row's chunk becomes T on its way to LDS, its scale in
+  // the conversion, and everything behind LDS is as over 16-bit pages
+  constexpr bool Q8 = std::is_same<PGT, FwdPaged8>::value;
+  using KT = std::conditional_t<Q8, uint8_t, T>;
   static_assert(!PG || (!CAUSAL && !DROP), "paged instances");
   using V8 = typename Dt<T>::V8;
   using V4 = typename Dt<T>::V4;
@@ -130,8 +135,8 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
   if (qb >= SQ) return;
 
   const T* Qg = (const T*)p.Q + sv.q0 + (long long)h * p.sQ.h;
-  const T* Kg = (const T*)p.K + sv.k0 + (long long)kvh * p.sK.h;
-  const T* Vg = (const T*)p.V + sv.v0 + (long long)kvh * p.sV.h;
+  const KT* Kg = (const KT*)p.K + sv.k0 + (long long)kvh * p.sK.h;
+  const KT* Vg = (const KT*)p.V + sv.v0 + (long long)kvh * p.sV.h;
   T* Og = (T*)p.O + sv.o0 + (long long)h * p.sO.h;
 
   // ---- block and wave key ranges
@@ -298,12 +303,14 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
       lvo[j] = live ? r * C::VSTR + 8 * c : -1;
     }
   }
-  u32x4 ldk[C::KJ], ldv[C::KJ];
+  using LD = std::conditional_t<Q8, u32x2, u32x4>;
+  LD ldk[C::KJ], ldv[C::KJ];
+  unsigned lsk[Q8 ? C::KJ : 1], lsv[Q8 ? C::KJ : 1];   // the scales of their rows
   // K and V tiles are loaded in key order, kstart, kstart+BC, ... (each through its own
   // cursor): the descriptor advances by additions instead of 64-bit products of the tile's key
   const long long k_step = (long long)C::BC * p.sK.s, v_step = (long long)C::BC * p.sV.s;
-  const T* k_cur = Kg + (long long)kstart * p.sK.s;
-  const T* v_cur = Vg + (long long)kstart * p.sV.s;
+  const KT* k_cur = Kg + (long long)kstart * p.sK.s;
+  const KT* v_cur = Vg + (long long)kstart * p.sV.s;
   long long k_left = (long long)(kvalid - kstart) * p.sK.s * 2, v_left = (long long)(kvalid - kstart) * p.sV.s * 2;
   // PG: the rows of one wave's load (64 / DCH of them, at most 16) lie in one page. The page of
   // each load of the next K tile is fetched a tile ahead by a vector load (a scalar one would
@@ -335,16 +342,25 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
       for (int j = 0; j < NE; j++) ent[j] = __builtin_amdgcn_raw_buffer_load_b32(r, (pg_index(j) & pg.tmask) * 4, 0, 0);
     }
   };
-  auto pg_load = [&](bool first, u32x4 (&ld)[C::KJ], const T* base, int key0, const int (&page)[NE], unsigned spg,
-                     unsigned srow, const int (&off)[C::KJ]) {
+  auto pg_load = [&](bool first, LD (&ld)[C::KJ], const KT* base, int key0, const int (&page)[NE], unsigned spg,
+                     unsigned srow, const int (&off)[C::KJ], unsigned (&lsc)[Q8 ? C::KJ : 1], const uint8_t* scales) {
     if constexpr (PG) {
 #pragma unroll
       for (int j = 0; j < NE; j++) {
         const int key = __builtin_amdgcn_readfirstlane(key0 + wrow + j * RSTEP);
         const unsigned in = key & ((1 << pg.page_shift) - 1);
         const unsigned rows = __builtin_amdgcn_readfirstlane(min(max(kvalid - key, 0), RW));   // (a med3: vector only)
-        const auto r = buf_rsrc32(base + ((uint64_t)(unsigned)page[j] * spg + (uint64_t)in * srow), rows * srow * 2u);
-        ld[j] = buf_load16(r, FEAT && first && key + lane / C::DCH < bk0 ? kBufZero : off[j]);
+        const auto r = buf_rsrc32(base + ((uint64_t)(unsigned)page[j] * spg + (uint64_t)in * srow), rows * srow * (unsigned)sizeof(KT));
+        const int row = lane / C::DCH;
+        const bool hide = FEAT && first && key + row < bk0;
+        if constexpr (Q8) {
+          // (rows that are not there get scale 0: their codes are zeros, and no scale's byte may make NaN of them)
+          const auto rs = buf_rsrc32(scales + ((uint64_t)(unsigned)page[j] * nheads + kvh) * pg.subs, (unsigned)pg.subs);
+          lsc[j] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(rs, hide || row >= (int)rows ? kBufZero : (int)(in + row) >> pg.gshift, 0, 0);
+          ld[j] = __builtin_amdgcn_raw_buffer_load_b64(r, hide ? kBufZero : off[j], 0, 0);
+        } else {
+          ld[j] = buf_load16(r, hide ? kBufZero : off[j]);
+        }
       }
     }
   };
@@ -353,8 +369,9 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
 #pragma unroll
     for (int j = 0; j < C::KJ; j++) {
       const int r = lane / C::DCH, c = tid % C::DCH;
-      koff[j] = 8 * c < HDr ? r * (int)(p.sK.s * 2) + 16 * c : kBufZero;
-      voff[j] = 8 * c < HDr ? r * (int)(p.sV.s * 2) + 16 * c : kBufZero;
+      constexpr int EL = sizeof(KT);
+      koff[j] = 8 * c < HDr ? r * (int)(p.sK.s * EL) + 8 * EL * c : kBufZero;
+      voff[j] = 8 * c < HDr ? r * (int)(p.sV.s * EL) + 8 * EL * c : kBufZero;
     }
     if (ntiles > 0) pg_fetch();
   }
@@ -365,41 +382,53 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
         pg_prev[j] = pg_cur[j];
         pg_cur[j] = __builtin_amdgcn_readfirstlane(ent[j]);
         if (!pg.tmask) pg_cur[j] = __builtin_amdgcn_readfirstlane(z * pg.max_blocks + pg_index(j));
+        if constexpr (Q8) pg_cur[j] = (int)min((unsigned)pg_cur[j], (unsigned)pg.num_blocks - 1);
       }
-      pg_load(first, ldk, Kg, ekey, pg_cur, (unsigned)pg.kpg, (unsigned)p.sK.s, koff);
+      const uint8_t* ks = nullptr;
+      if constexpr (Q8) ks = pg.ks;
+      pg_load(first, ldk, Kg, ekey, pg_cur, (unsigned)pg.kpg, (unsigned)p.sK.s, koff, lsk, ks);
       ekey += C::BC;
       pg_fetch();
-      return;
-    }
-    const auto r = buf_rsrc(k_cur, k_left);
+    } else {
+      const auto r = buf_rsrc(k_cur, k_left);
 #pragma unroll
-    for (int j = 0; j < C::KJ; j++) ldk[j] = buf_load16(r, koff[j]);
-    k_cur += k_step;
-    k_left -= 2 * k_step;
+      for (int j = 0; j < C::KJ; j++) ldk[j] = buf_load16(r, koff[j]);
+      k_cur += k_step;
+      k_left -= 2 * k_step;
+    }
   };
   // (PG: `ahead` K tiles have been loaded past this V tile, 0 or 1)
   auto gload_v = [&](int ahead = 1, bool first = false) {
     if constexpr (PG) {
-      pg_load(first, ldv, Vg, ekey - (1 + ahead) * C::BC, ahead ? pg_prev : pg_cur, (unsigned)pg.vpg, (unsigned)p.sV.s, voff);
-      return;
-    }
-    const auto r = buf_rsrc(v_cur, v_left);
+      const uint8_t* vs = nullptr;
+      if constexpr (Q8) vs = pg.vs;
+      pg_load(first, ldv, Vg, ekey - (1 + ahead) * C::BC, ahead ? pg_prev : pg_cur, (unsigned)pg.vpg, (unsigned)p.sV.s, voff, lsv, vs);
+    } else {
+      const auto r = buf_rsrc(v_cur, v_left);
 #pragma unroll
-    for (int j = 0; j < C::KJ; j++) ldv[j] = buf_load16(r, voff[j]);
-    v_cur += v_step;
-    v_left -= 2 * v_step;
+      for (int j = 0; j < C::KJ; j++) ldv[j] = buf_load16(r, voff[j]);
+      v_cur += v_step;
+      v_left -= 2 * v_step;
+    }
+  };
+  // what a chunk's load holds, as T
+  auto chunk_of = [&](const LD& x, unsigned scale) -> u32x4 {
+    if constexpr (Q8)
+      return bitcast<u32x4>(codes_to<T>(x, e8_f32(scale)));
+    else
+      return x;
   };
   auto lstore_k = [&](int st) {
     T* b = kl + st * C::KTILE;
 #pragma unroll
     for (int j = 0; j < C::KJ; j++)
-      if (!C::KTAIL || j < C::KJ - 1 || lko[j] >= 0) *(u32x4*)(b + lko[j]) = ldk[j];
+      if (!C::KTAIL || j < C::KJ - 1 || lko[j] >= 0) *(u32x4*)(b + lko[j]) = chunk_of(ldk[j], lsk[Q8 ? j : 0]);
   };
   auto lstore_v = [&](int st) {
     T* b = vl + st * C::VTILE;
 #pragma unroll
     for (int j = 0; j < C::KJ; j++)
-      if (!C::KTAIL || j < C::KJ - 1 || lvo[j] >= 0) *(u32x4*)(b + lvo[j]) = ldv[j];
+      if (!C::KTAIL || j < C::KJ - 1 || lvo[j] >= 0) *(u32x4*)(b + lvo[j]) = chunk_of(ldv[j], lsv[Q8 ? j : 0]);
   };
 
   // S^T = K . Q^T for the K tile in stage st, every query block: lane reads key row
@@ -928,8 +957,8 @@ struct CfgTag {
 // to kPagedSplitMax shares of at least kPagedSplitTiles tiles of the longest cache the table holds); a
 // split count of the caller's is taken as it is, up to kPagedSplitMax.
 constexpr int kPagedSplitMax = 32, kPagedSplitTiles = 4;
-template <typename T, class C, class CF>
-static int launch_fwd_pg(const FableFwdParams& p, const FwdPaged& pg, bool rot, hipStream_t st, FwdWs& ws) {
+template <typename T, class C, class CF, class PGT>
+static int launch_fwd_pg(const FableFwdParams& p, const PGT& pg, bool rot, hipStream_t st, FwdWs& ws) {
   const bool feat = p.softcap > 0.0f || p.alibi_slopes != nullptr || p.attn_chunk > 0 || p.win_left >= 0 || pg.leftpad ||
                     (p.win_right >= 0 && !(p.win_right == 0 && p.causal));
   auto go = [&](auto cfg, auto ft, auto rt) -> int {
@@ -956,7 +985,7 @@ static int launch_fwd_pg(const FableFwdParams& p, const FwdPaged& pg, bool rot, 
     }
     if (ws.query) return FA_OK;
     if (nblk * sp.n > 0x7FFFFFFF) return fail(FA_ERR_ARG, "fable_attn_fwd: grid too large");
-    hipLaunchKernelGGL((fwd_kernel<T, K, false, decltype(ft)::value, false, FwdPaged, decltype(rt)::value>),
+    hipLaunchKernelGGL((fwd_kernel<T, K, false, decltype(ft)::value, false, PGT, decltype(rt)::value>),
                        dim3((unsigned)(nblk * sp.n)), dim3(K::NT), 0, st, p, nqt, sp, pg);
     const int rc = launch_status("fable_attn_fwd (paged)");
     if (rc != FA_OK || sp.n == 1) return rc;

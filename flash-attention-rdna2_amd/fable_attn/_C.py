@@ -20,6 +20,8 @@ bound at :239-268) with the same names, argument order and meaning:
         rotary_sin, rotary_interleaved, scale, window, num_splits, cache_leftpad=None,
         return_lse=False, softcap=0.0, alibi=None, rotary_dim=0, rotary_pos=None) -> (out, lse)
     combine(out_partial, lse_partial, out_dtype) -> out
+Without counterparts there: dec8 and fwd_paged8 (caches held in 8 bits), append (packed or padded new
+tokens into a cache) and gather (cached rows as a packed batch).
 Tensor checks raise RuntimeError as TORCH_CHECK does there. torch only allocates outputs and
 workspaces and supplies the current stream; all compute is in libfable_attn_hip.so. There is
 no fallback: if the library is missing, importing this module raises ImportError.
@@ -456,6 +458,251 @@ def dec(q, k_cache, v_cache, block_table, cache_seqlens, new_k, new_v, rotary_co
         _lib.check(_L.fable_attn_dec_ws(p, _dt(q), _ptr(ws), max(ws_bytes, 0), _stream(q), _ptr(new_k),
                                         _ptr(new_v)), "fable_attn_dec")
     return out, lse
+
+
+# ----------------------------------------------------------------------------- caches in 8 bits, append, gather
+FP8, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _cache_strides(name, t, dev):
+    """(page, head, row) strides of a cache [num_blocks, page, nheads_k, D] that the kernels can address."""
+    _req(t.is_cuda and t.device == dev, f"{name}: must be on {dev}, got {t.device}")
+    _req(_rows_aligned(t), f"{name}: head_dim must be contiguous with 16-byte aligned rows")
+    return Strides(t.stride(0), t.stride(2), t.stride(1))
+
+
+def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev):
+    """Shapes and types of a cache pair: of `dtype`, or e4m3 codes with e8m0 scales. Returns (k strides, v strides,
+    tokens per scale; 0 without scales)."""
+    _req(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
+         "k_cache/v_cache must both be [num_blocks, page, nheads_k, D]")
+    _req((k_scale is None) == (v_scale is None), "k_scale and v_scale go together")
+    want = FP8 if k_scale is not None else dtype
+    nb, page, Hk, D = k_cache.shape
+    for n, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _req(t.dtype == want, f"{n}: dtype {want} expected, got {t.dtype}"
+             + ("" if k_scale is not None else " (8-bit caches need k_scale and v_scale)"))
+    _req(nb > 0, "the cache has no pages")
+    _req(page > 0 and (page & (page - 1)) == 0, "page must be a power of two")
+    ks, vs = _cache_strides("k_cache", k_cache, dev), _cache_strides("v_cache", v_cache, dev)
+    if k_scale is None:
+        return ks, vs, 0
+    _req(D % 16 == 0 and D <= 256, f"8-bit caches need a head_dim that is a multiple of 16 up to 256, got {D}")
+    _req(page >= 16, f"8-bit caches need pages of at least 16 rows, got {page}")
+    for n, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        _req(torch.is_tensor(t) and t.dtype == E8M0, f"{n}: {E8M0} expected")
+        _req(t.device == dev and t.is_contiguous(), f"{n}: must be contiguous on {dev}")
+        subs = t.shape[2] if t.dim() == 3 else 0
+        _req(t.dim() == 3 and t.shape[0] == nb and t.shape[1] == Hk and subs > 0 and page % subs == 0
+             and (subs & (subs - 1)) == 0 and page // subs <= 256,
+             f"{n}: must be [num_blocks, nheads_k, page / G] = [{nb}, {Hk}, {page} / G] with G a power of two up to "
+             f"min(page, 256), got {tuple(t.shape)}")
+    _req(v_scale.shape == k_scale.shape, "v_scale: must have the shape of k_scale")
+    subs = k_scale.shape[2]
+    return ks, vs, page // subs
+
+
+def _cache8(k_cache, v_cache, k_scale, v_scale, dtype, dev, rotary_rows=0):
+    ks, vs, group = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev)
+    return _lib.FableCache8(k_scale.data_ptr(), v_scale.data_ptr(), ks, vs, group, k_cache.shape[0], rotary_rows)
+
+
+def _check_table(block_table, batch, dev):
+    _check_index("block_table", block_table, dev)
+    _req(block_table.dim() == 2 and block_table.shape[0] == batch and block_table.shape[1] > 0,
+         f"block_table must be [batch, max_blocks], got {tuple(block_table.shape)} for batch={batch}")
+
+
+def _check_rotary(cos, sin, rotary_dim, D, dev):
+    _req((cos is None) == (sin is None), "rotary_cos and rotary_sin go together")
+    if cos is None:
+        return
+    _check_f32("rotary_cos", cos, dev)
+    _check_f32("rotary_sin", sin, dev)
+    _req(cos.dim() == 2 and sin.shape == cos.shape and cos.shape[0] > 0,
+         "rotary_cos/rotary_sin must be [seqlen_ro, rotary_dim/2]")
+    _req(cos.shape[1] * 2 == rotary_dim and 0 < rotary_dim <= D,
+         f"rotary tables of width {cos.shape[1]} do not fit a head_dim of {D}")
+
+
+def dec8(q, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, new_k, new_v, cos, sin, interleaved, scale,
+         window, num_splits, leftpad, return_lse, softcap, alibi, rotary_pos):
+    """dec over a cache in 8 bits: codes [num_blocks, page, Hk, D] (strided pages, rows and heads), scales
+    [num_blocks, Hk, page / G]. block_table None: a dense cache, sequence b in page b."""
+    _req(q.is_cuda, "GPU tensors required")
+    _req(q.dim() == 4 and q.is_contiguous() and q.data_ptr() % 16 == 0, "decode expects contiguous q [B,nq,Hq,D], 16-byte aligned")
+    _req(q.dtype in (torch.float16, torch.bfloat16), f"8-bit caches take fp16 or bf16 queries, got {q.dtype}")
+    B, NQ, Hq, D = q.shape
+    dev = q.device
+    _req(k_cache.dim() == 4 and k_cache.shape[3] == D, "k_cache/v_cache must both be [num_blocks, page, nheads_k, D] with q's D")
+    nb, page, Hk = k_cache.shape[:3]
+    _req(Hk > 0 and Hq % Hk == 0, "Hq must be a multiple of nheads_k (GQA)")
+    c = _cache8(k_cache, v_cache, k_scale, v_scale, q.dtype, dev, cos.shape[0] if cos is not None else 0)
+    if block_table is not None:
+        _check_table(block_table, B, dev)
+    else:
+        _req(nb >= B, f"a dense cache of {nb} rows for a batch of {B}")
+    _check_index("cache_seqlens", cache_seqlens, dev, B)
+    for n, t in (("cache_leftpad", leftpad), ("rotary_seqlens", rotary_pos)):
+        if t is not None:
+            _check_index(n, t, dev, B)
+    if alibi is not None:
+        _check_f32("alibi_slopes", alibi, dev, Hq)
+    rd = int(cos.shape[-1] * 2) if cos is not None else 0
+    _check_rotary(cos, sin, rd, D, dev)
+    _req((new_k is None) == (new_v is None), "new_k and new_v go together")
+    if new_k is not None:
+        for n, t in (("k", new_k), ("v", new_v)):
+            _req(tuple(t.shape) == (B, NQ, Hk, D) and t.dtype == q.dtype and t.device == dev and
+                 t.is_contiguous() and t.data_ptr() % 16 == 0,
+                 f"{n}: contiguous, 16-byte aligned [B, seqlen_q, nheads_k, D] of q's dtype")
+    out = torch.empty((B, NQ, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, NQ, Hq) if return_lse else (0,), dtype=torch.float32, device=dev)
+    p = FableDecParams()
+    p.q, p.Kc, p.Vc, p.o = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    p.block_table = block_table.data_ptr() if block_table is not None else None
+    p.ctx_len = cache_seqlens.data_ptr()
+    p.cos = cos.data_ptr() if cos is not None else None
+    p.sin = sin.data_ptr() if sin is not None else None
+    p.batch, p.NH, p.gqa, p.HD, p.page = B, Hq, Hq // Hk, D, page
+    p.max_blocks, p.nsplit, p.window = block_table.shape[1] if block_table is not None else 1, int(num_splits or 0), int(window)
+    p.rotary, p.rotary_dim = ((2 if interleaved else 1) if cos is not None else 0), rd
+    p.scale, p.softcap, p.nq = float(scale), float(softcap), NQ
+    p.leftpad = leftpad.data_ptr() if leftpad is not None else None
+    p.lse_out = lse.data_ptr() if return_lse else None
+    p.alibi = alibi.data_ptr() if alibi is not None else None
+    p.rotary_pos = rotary_pos.data_ptr() if rotary_pos is not None else None
+    need = int(_L.fable_attn_dec8_ws_bytes(p, c, _dt(q), 1 if new_k is not None else 0))
+    if need < 0:
+        _lib.check(1, "fable_attn_dec8")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    with _on(dev):
+        _lib.check(_L.fable_attn_dec8(p, c, _dt(q), _ptr(ws), need, _stream(q), _ptr(new_k), _ptr(new_v)), "fable_attn_dec8")
+    return out, lse
+
+
+def fwd_paged8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, scale, causal, win_left, win_right,
+               softcap, alibi, attn_chunk=0, seqused_q=None, seqused_k=None):
+    """fwd_paged over a cache in 8 bits (as dec8's)."""
+    _req(q.is_cuda, "GPU tensors required")
+    _req(q.dtype in (torch.float16, torch.bfloat16), f"8-bit caches take fp16 or bf16 queries, got {q.dtype}")
+    _req(q.dim() == 3 and _rows_aligned(q), "q: [total, H, D] with a contiguous head_dim and 16-byte aligned rows expected")
+    _req(k_cache.dim() == 4 and k_cache.shape[3] == q.shape[2], "k/v must be paged [num_blocks, page, nheads_k, D] with q's D")
+    Hq, D, page, Hk = q.shape[1], q.shape[2], k_cache.shape[1], k_cache.shape[2]
+    _req(Hk > 0 and Hq % Hk == 0, "Hq must be a multiple of nheads_k (GQA)")
+    c = _cache8(k_cache, v_cache, k_scale, v_scale, q.dtype, q.device)
+    batch = _check_varlen_index(q, cu_q, cu_k, seqused_q, seqused_k)
+    _check_table(block_table, batch, q.device)
+    al = _alibi(alibi, Hq, q.device)
+    p = FableFwdParams()
+    p.Q, p.K, p.V = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    p.sQ, p.sO = Strides(0, q.stride(1), q.stride(0)), Strides(0, D, Hq * D)
+    p.SQ, p.HD, p.NH, p.gqa = int(max_sq), D, Hq, Hq // Hk
+    p.scale, p.softcap = float(scale), float(softcap)
+    p.win_left, p.win_right, p.causal = int(win_left), int(win_right), 1 if causal else 0
+    p.alibi_slopes = al.data_ptr() if al is not None else None
+    p.cu_q, p.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    p.batch, p.attn_chunk = batch, int(attn_chunk)
+    p.seqused_q = seqused_q.data_ptr() if seqused_q is not None else None
+    p.seqused_k = seqused_k.data_ptr() if seqused_k is not None else None
+    kv = _lib.FablePagedKV(block_table.data_ptr(), block_table.shape[1], page, 0, 0)
+    need = int(_L.fable_attn_fwd_paged8_ws_bytes(p, kv, c, _dt(q)))
+    if need < 0:
+        _lib.check(1, "fable_attn_fwd_paged8")
+    make = torch.zeros if seqused_q is not None else torch.empty   # (rows past seqused_q stay 0)
+    out = make(tuple(q.shape), dtype=q.dtype, device=q.device)
+    p.O = out.data_ptr()
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    with _on(q.device):
+        _lib.check(_L.fable_attn_fwd_paged8(p, kv, c, _dt(q), _ptr(ws), need, _stream(q)), "fable_attn_fwd_paged8")
+    return out
+
+
+def append(k, v, k_cache, v_cache, cache_seqlens, q=None, cu=None, max_seqlen=0, block_table=None, leftpad=None, cos=None,
+           sin=None, interleaved=False, rotary_pos=None, k_scale=None, v_scale=None):
+    """New tokens k, v (and q, which comes back rotated) [B,N,H,D], or [total,H,D] with cu int32 [batch+1], into the
+    caches at positions cache_seqlens[b] + t. block_table None: a dense cache, sequence b in page b."""
+    dev = k.device
+    packed = cu is not None
+    _req(k.is_cuda, "GPU tensors required")
+    _req(k.dim() == (3 if packed else 4) and v.shape == k.shape, "k/v: [B,N,nheads_k,D], or [total,nheads_k,D] with cu_seqlens")
+    D, Hk = k.shape[-1], k.shape[-2]
+    for n, t in (("k", k), ("v", v)) + ((("q", q),) if q is not None else ()):
+        _req(t.dtype == k.dtype and t.device == dev, f"{n}: dtype and device of k")
+        _req(_rows_aligned(t), f"{n}: head_dim must be contiguous with 16-byte aligned rows")
+    if q is not None:
+        _req(q.dim() == k.dim() and q.shape[:-2] == k.shape[:-2] and q.shape[-1] == D, "q: the tokens and head_dim of k")
+    dt = _dt(k)
+    _req(k_cache.dim() == 4 and tuple(k_cache.shape[2:]) == (Hk, D),
+         f"k_cache/v_cache must be [num_blocks, page, {Hk}, {D}], got {tuple(k_cache.shape)}")
+    kc, vc, group = _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, dev)
+    _req(group == 0 or k.dtype != torch.float32, "8-bit caches take fp16 or bf16 tokens")
+    _req(D % 8 == 0 and D <= 256, f"head_dim must be a multiple of 8 up to 256, got {D}")
+    batch = cu.numel() - 1 if packed else k.shape[0]
+    _req(batch >= 0, "cu_seqlens must have batch+1 entries")
+    if packed:
+        _check_index("cu_seqlens", cu, dev)
+    _check_index("cache_seqlens", cache_seqlens, dev, batch)
+    for n, t in (("cache_leftpad", leftpad), ("rotary_seqlens", rotary_pos)):
+        if t is not None:
+            _check_index(n, t, dev, batch)
+    if block_table is not None:
+        _check_table(block_table, batch, dev)
+    else:
+        _req(k_cache.shape[0] >= batch, f"a dense cache of {k_cache.shape[0]} rows for a batch of {batch}")
+    rd = int(cos.shape[-1] * 2) if cos is not None else 0
+    _check_rotary(cos, sin, rd, D, dev)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q is not None else None
+    st = lambda t: Strides(0 if packed else t.stride(0), t.stride(-2), t.stride(-3))
+    p = _lib.FableAppendParams()
+    p.k, p.v, p.Kc, p.Vc = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    p.sk, p.sv, p.kc, p.vc = st(k), st(v), kc, vc
+    if q is not None:
+        p.q, p.q_out, p.sq, p.NH = q.data_ptr(), q_out.data_ptr(), st(q), q.shape[-2]
+    if group:
+        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    p.block_table = block_table.data_ptr() if block_table is not None else None
+    p.ctx_len = cache_seqlens.data_ptr()
+    p.cu = cu.data_ptr() if packed else None
+    p.leftpad = leftpad.data_ptr() if leftpad is not None else None
+    p.rotary_pos = rotary_pos.data_ptr() if rotary_pos is not None else None
+    p.batch, p.n, p.NKV, p.HD = batch, int(max_seqlen) if packed else k.shape[1], Hk, D
+    p.page, p.num_blocks, p.group = k_cache.shape[1], k_cache.shape[0], group
+    p.max_blocks = block_table.shape[1] if block_table is not None else 1
+    if cos is not None:
+        p.cos, p.sin, p.rotary, p.rotary_dim, p.rotary_rows = cos.data_ptr(), sin.data_ptr(), 2 if interleaved else 1, rd, cos.shape[0]
+    if k.numel():
+        with _on(dev):
+            _lib.check(_L.fable_attn_append(p, dt, _stream(k)), "fable_attn_append")
+    return q_out
+
+
+def gather(k_cache, v_cache, cu, total, dtype, block_table=None, k_scale=None, v_scale=None):
+    """The first cu[b+1] - cu[b] cached rows of every sequence as packed k, v [total, Hk, D] in dtype."""
+    dev = k_cache.device
+    kc, vc, group = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev)
+    nb, page, Hk, D = k_cache.shape
+    _req(D % 8 == 0 and D <= 256, f"head_dim must be a multiple of 8 up to 256, got {D}")
+    _check_index("cu_seqlens_k", cu, dev)
+    batch = cu.numel() - 1
+    _req(batch >= 0, "cu_seqlens_k must have batch+1 entries")
+    if block_table is not None:
+        _check_table(block_table, batch, dev)
+    else:
+        _req(nb >= batch, f"a dense cache of {nb} rows for a batch of {batch}")
+    k, v = (torch.empty((int(total), Hk, D), dtype=dtype, device=dev) for _ in range(2))
+    p = _lib.FableGatherParams()
+    p.Kc, p.Vc, p.k_out, p.v_out, p.kc, p.vc = k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(), v.data_ptr(), kc, vc
+    if group:
+        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    p.block_table = block_table.data_ptr() if block_table is not None else None
+    p.cu, p.total, p.batch, p.NKV, p.HD, p.page = cu.data_ptr(), int(total), batch, Hk, D, page
+    p.max_blocks = block_table.shape[1] if block_table is not None else 1
+    p.num_blocks, p.group = nb, group
+    if k.numel():
+        with _on(dev):
+            _lib.check(_L.fable_attn_gather(p, _dt(k), _stream(k)), "fable_attn_gather")
+    return k, v
 
 
 def combine(out_partial, lse_partial, out_dtype):

@@ -10,8 +10,10 @@ host-side mirror of the reference's Python interface (package/fable_attn/__init_
 import sys
 
 from .flash_attn_interface import (
+    flash_attn_append_kvcache,
     flash_attn_combine,
     flash_attn_func,
+    flash_attn_gather_kvcache,
     flash_attn_kvpacked_func,
     flash_attn_qkvpacked_func,
     flash_attn_varlen_func,
@@ -29,6 +31,7 @@ __all__ = [
     "flash_attn_func", "flash_attn_qkvpacked_func", "flash_attn_kvpacked_func",
     "flash_attn_varlen_func", "flash_attn_varlen_qkvpacked_func",
     "flash_attn_varlen_kvpacked_func", "flash_attn_combine", "flash_attn_with_kvcache",
+    "flash_attn_append_kvcache", "flash_attn_gather_kvcache",
     "install_as_flash_attn",
 ]
 

@@ -76,6 +76,30 @@ class FablePagedKV(ctypes.Structure):
                 ("k_page_stride", c_i64), ("v_page_stride", c_i64)]
 
 
+class FableCache8(ctypes.Structure):
+    _fields_ = [("k_scale", c_ptr), ("v_scale", c_ptr), ("k", Strides), ("v", Strides),
+                ("group", c_i32), ("num_blocks", c_i32), ("rotary_rows", c_i32)]
+
+
+class FableAppendParams(ctypes.Structure):
+    _fields_ = [("k", c_ptr), ("v", c_ptr), ("q", c_ptr), ("q_out", c_ptr), ("q_lo", c_ptr),
+                ("Kc", c_ptr), ("Vc", c_ptr), ("k_scale", c_ptr), ("v_scale", c_ptr),
+                ("sk", Strides), ("sv", Strides), ("sq", Strides), ("kc", Strides), ("vc", Strides),
+                ("block_table", c_ptr), ("ctx_len", c_ptr), ("cu", c_ptr), ("leftpad", c_ptr),
+                ("rotary_pos", c_ptr), ("cos", c_ptr), ("sin", c_ptr),
+                ("batch", c_i32), ("n", c_i32), ("NH", c_i32), ("NKV", c_i32), ("HD", c_i32),
+                ("page", c_i32), ("max_blocks", c_i32), ("num_blocks", c_i32), ("group", c_i32),
+                ("rotary", c_i32), ("rotary_dim", c_i32), ("rotary_rows", c_i32)]
+
+
+class FableGatherParams(ctypes.Structure):
+    _fields_ = [("Kc", c_ptr), ("Vc", c_ptr), ("k_scale", c_ptr), ("v_scale", c_ptr),
+                ("k_out", c_ptr), ("v_out", c_ptr), ("kc", Strides), ("vc", Strides),
+                ("block_table", c_ptr), ("cu", c_ptr), ("total", c_i64),
+                ("batch", c_i32), ("NKV", c_i32), ("HD", c_i32), ("page", c_i32),
+                ("max_blocks", c_i32), ("num_blocks", c_i32), ("group", c_i32)]
+
+
 # The reference's layouts (package/csrc/fa_iface.h:9-63), taken by fa_forward_launch,
 # fable_attn_backward_launch and fa_decode_launch.
 class RefStrides(ctypes.Structure):
@@ -119,13 +143,16 @@ class RefDecParams(ctypes.Structure):
 
 
 STRUCTS = {0: FableFwdParams, 1: FableBwdParams, 2: FableDecParams, 3: CombineParams,
-           4: Strides, 5: RefFwdParams, 6: RefBwdParams, 7: RefDecParams}
+           4: Strides, 5: RefFwdParams, 6: RefBwdParams, 7: RefDecParams,
+           8: FableCache8, 9: FableAppendParams, 10: FableGatherParams}
 
 # exported symbols of libfable_attn_hip.so (the C-ABI surface)
 EXPORTS = ("fa_forward_launch", "fable_attn_backward_launch", "fa_decode_launch",
            "fable_attn_fwd", "fable_attn_fwd_ws", "fable_attn_fwd_ws_bytes", "fable_attn_bwd", "fable_attn_dec", "fable_attn_dec_noalloc",
            "fable_attn_dec_noalloc_max_floats", "fable_attn_dec_ws", "fable_attn_dec_ws_bytes",
            "fable_attn_fwd_paged", "fable_attn_fwd_paged_ws_bytes", "fable_attn_bwd_zero_gaps",
+           "fable_attn_dec8", "fable_attn_dec8_ws_bytes", "fable_attn_fwd_paged8",
+           "fable_attn_fwd_paged8_ws_bytes", "fable_attn_append", "fable_attn_gather",
            "fa_decode_num_splits", "fa_combine_launch", "fable_attn_bwd_ds_bytes",
            "fable_attn_abi_version", "fable_attn_struct_size", "fable_attn_last_error")
 
@@ -162,7 +189,15 @@ def load():
     lib.fable_attn_fwd_paged_ws_bytes.argtypes = [FableFwdParams, FablePagedKV, c_i32]
     lib.fable_attn_fwd_paged_ws_bytes.restype = c_i64
     lib.fable_attn_bwd_zero_gaps.argtypes = [FableBwdParams, c_i32, c_i64, c_i64, c_ptr]
-    for f in ("fable_attn_bwd_zero_gaps", "fable_attn_dec_ws", "fable_attn_fwd_paged", "fable_attn_fwd", "fable_attn_fwd_ws", "fable_attn_bwd", "fable_attn_dec", "fable_attn_dec_noalloc",
+    lib.fable_attn_dec8.argtypes = [FableDecParams, FableCache8, c_i32, c_ptr, c_i64, c_ptr, c_ptr, c_ptr]
+    lib.fable_attn_dec8_ws_bytes.argtypes = [FableDecParams, FableCache8, c_i32, c_i32]
+    lib.fable_attn_dec8_ws_bytes.restype = c_i64
+    lib.fable_attn_fwd_paged8.argtypes = [FableFwdParams, FablePagedKV, FableCache8, c_i32, c_ptr, c_i64, c_ptr]
+    lib.fable_attn_fwd_paged8_ws_bytes.argtypes = [FableFwdParams, FablePagedKV, FableCache8, c_i32]
+    lib.fable_attn_fwd_paged8_ws_bytes.restype = c_i64
+    lib.fable_attn_append.argtypes = [FableAppendParams, c_i32, c_ptr]
+    lib.fable_attn_gather.argtypes = [FableGatherParams, c_i32, c_ptr]
+    for f in ("fable_attn_dec8", "fable_attn_fwd_paged8", "fable_attn_append", "fable_attn_gather", "fable_attn_bwd_zero_gaps", "fable_attn_dec_ws", "fable_attn_fwd_paged", "fable_attn_fwd", "fable_attn_fwd_ws", "fable_attn_bwd", "fable_attn_dec", "fable_attn_dec_noalloc",
               "fa_forward_launch",
               "fable_attn_backward_launch", "fa_decode_launch",
               "fa_decode_num_splits", "fa_combine_launch", "fable_attn_abi_version"):

@@ -544,6 +544,33 @@ def _paged_prefill(q, k_cache, v_cache, block_table, cu_q, cu_k, max_sq, max_sk,
                         idx(seqused_q), idx(seqused_k))
 
 
+def _no_grad8(q):
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise NotImplementedError("fable_attn: attention over an 8-bit cache has no gradient; run it under torch.no_grad()")
+
+
+def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, seqused_q, seqused_k, *,
+                    descale, hints, **kw):
+    """Packed prompts over a paged cache held in 8 bits, read through the block table."""
+    _no_grad8(q)
+    _reject_fp8(*descale)
+    if q.is_cuda and q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"fable_attn: 8-bit caches take fp16 or bf16 queries, got {q.dtype}")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or q.shape[2] != k_cache.shape[3]:
+        raise ValueError("fable_attn: with block_table, k and v must be paged (num_blocks, page_block_size, nheads_k, "
+                         f"headdim) with q's headdim; got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if q.shape[2] % 16:
+        raise NotImplementedError(f"fable_attn: 8-bit caches need a head_dim that is a multiple of 16, got {q.shape[2]}")
+    spec = _normalize(q, k_cache[0], v_cache[0], head_axis=1, hints=hints, **kw) if k_cache.shape[0] else None
+    if spec is None:
+        raise ValueError("fable_attn: the cache has no pages")
+    dev = q.device
+    idx = lambda t: _as_index(t, dev) if t is not None else None
+    return _C.fwd_paged8(_aligned(q), k_cache, v_cache, k_scale, v_scale, idx(block_table), idx(cu_q), idx(cu_k), int(max_sq),
+                         spec.scale, bool(spec.causal), spec.wl, spec.wr, spec.softcap, spec.alibi, spec.chunk,
+                         idx(seqused_q), idx(seqused_k))
+
+
 def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                            dropout_p=0.0, softmax_scale=None, causal=False,
                            window_size=(-1, -1), softcap=0.0, alibi_slopes=None,
@@ -552,14 +579,25 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
                            qv=None, attention_chunk=0,
                            q_descale=None, k_descale=None, v_descale=None,
                            num_splits=1, pack_gqa=None, sm_margin=0,
-                           block_table=None):
+                           block_table=None, k_scale=None, v_scale=None):
     """Packed variable-length sequences: q (total_q, nheads, d), k/v (total_k, nheads_k, d),
     cu_seqlens_* int32 (batch+1). One forward launch over all sequences and, with grad, one
     launch of each backward kernel (the reference loops over the sequences in Python on the
-    grad path, :523-540). With return_attn_probs: (out, [lse per sequence], [P per sequence])."""
+    grad path, :523-540). With return_attn_probs: (out, [lse per sequence], [P per sequence]).
+    With block_table, k and v are paged caches; with k_scale and v_scale too, caches held in 8 bits (see
+    flash_attn_append_kvcache), for inference: no gradient, dropout, qv or probabilities."""
     del deterministic
     if q.dim() != 3:
         raise ValueError(f"fable_attn: varlen expects (total, nheads, headdim), got {tuple(q.shape)}")
+    if k_scale is not None or v_scale is not None:
+        if block_table is None:
+            raise ValueError("fable_attn: k_scale and v_scale belong to a paged cache; pass block_table")
+        if dropout_p or qv is not None or return_attn_probs:
+            raise NotImplementedError("fable_attn: dropout, qv and return_attn_probs are not supported over an 8-bit cache")
+        return _paged_prefill8(q, k, v, k_scale, v_scale, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, seqused_q,
+                               seqused_k, softmax_scale=softmax_scale, causal=causal, window_size=window_size,
+                               softcap=softcap, alibi_slopes=alibi_slopes, attention_chunk=attention_chunk,
+                               descale=(q_descale, k_descale, v_descale), hints=(num_splits, pack_gqa, sm_margin))
     if block_table is not None:
         if not dropout_p and qv is None and not return_attn_probs:
             out = _paged_prefill(q, k, v, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
@@ -734,13 +772,13 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
                             q_descale=None, k_descale=None, v_descale=None,
                             pack_gqa=None, sm_margin=0, scheduler_metadata=None,
                             cu_seqlens_q=None, cu_seqlens_k_new=None, max_seqlen_q=None,
-                            rotary_seqlens=None):
+                            rotary_seqlens=None, k_scale=None, v_scale=None):
     """Decode against a paged or dense KV cache (arguments and results: _with_kvcache). A step of a
     serving loop repeats one signature (shapes, dtypes, options) with new tensors: the first call
     of a signature goes through all checks, and the launch parameters it came to are kept per
     thread (without any pointer), so later calls only fill in addresses and launch."""
     key = None
-    if (qv is None and cache_batch_idx is None and not attention_chunk and not return_softmax_lse
+    if (qv is None and k_scale is None and v_scale is None and cache_batch_idx is None and not attention_chunk and not return_softmax_lse
             and q_descale is None and k_descale is None and v_descale is None and cu_seqlens_q is None
             and cu_seqlens_k_new is None and rotary_seqlens is None and (page_table is None or block_table is None)
             and (num_splits is None or type(num_splits) is int) and (pack_gqa is None or type(pack_gqa) is bool)
@@ -766,7 +804,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
                         k_descale=k_descale, v_descale=v_descale, pack_gqa=pack_gqa, sm_margin=sm_margin,
                         scheduler_metadata=scheduler_metadata, cu_seqlens_q=cu_seqlens_q,
                         cu_seqlens_k_new=cu_seqlens_k_new, max_seqlen_q=max_seqlen_q,
-                        rotary_seqlens=rotary_seqlens)
+                        rotary_seqlens=rotary_seqlens, k_scale=k_scale, v_scale=v_scale)
     if key is not None and key not in plans:
         if len(plans) >= _MAX_PLANS:
             plans.clear()
@@ -785,14 +823,16 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
                   q_descale=None, k_descale=None, v_descale=None,
                   pack_gqa=None, sm_margin=0, scheduler_metadata=None,
                   cu_seqlens_q=None, cu_seqlens_k_new=None, max_seqlen_q=None,
-                  rotary_seqlens=None):
+                  rotary_seqlens=None, k_scale=None, v_scale=None):
     """Decode against a paged (k_cache/v_cache (num_blocks, page, nheads_k, d) + block_table)
     or dense ((batch, seqlen, nheads_k, d)) KV cache; split-KV kernels with an LSE combine.
     q: (batch, seqlen_q, nheads, d), or packed (total_q, nheads, d) with cu_seqlens_q; new
     token t of sequence b sits at cache_seqlens[b] + t. Without k/v every new token sees the
     cached keys [0, cache_seqlens[b]); k/v (batch, seqlen_q, nheads_k, d) are written into
     the cache first, and then token t also sees the new keys up to its own. Returns out, or
-    (out, softmax_lse (batch, nheads, seqlen_q)). Reference :583-771."""
+    (out, softmax_lse (batch, nheads, seqlen_q)). Reference :583-771.
+    k_scale and v_scale: the caches are held in 8 bits (flash_attn_append_kvcache says how); q, k and v are fp16
+    or bf16, and new k/v are quantised as that function does."""
     _reject_fp8(q_descale, k_descale, v_descale)
     _accept_hints(num_splits, pack_gqa, sm_margin)
     del scheduler_metadata      # the launcher plans each call itself (fa_decode_num_splits)
@@ -800,6 +840,15 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
         raise NotImplementedError(
             "fable_attn: cu_seqlens_k_new (ragged append) is not supported; append the same "
             "number of tokens to every batch element")
+    q8 = k_scale is not None or v_scale is not None
+    if q8:
+        if k_scale is None or v_scale is None:
+            raise ValueError("fable_attn: k_scale and v_scale go together")
+        if qv is not None or v_cache.shape != k_cache.shape or q.shape[-1] != k_cache.shape[-1] or q.shape[-1] % 16:
+            raise NotImplementedError(
+                "fable_attn: over an 8-bit cache keys and values share one head_dim, a multiple of 16, and qv is not supported")
+        if q.is_cuda and q.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"fable_attn: 8-bit caches take fp16 or bf16 queries, got {q.dtype}")
     if page_table is not None:
         if block_table is not None:
             raise ValueError("fable_attn: block_table and page_table are the same argument; pass one")
@@ -815,7 +864,8 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
                                  causal=causal, window_size=window_size, softcap=softcap,
                                  rotary_interleaved=rotary_interleaved,
                                  alibi_slopes=alibi_slopes, num_splits=num_splits,
-                                 attention_chunk=attention_chunk, rotary_seqlens=rotary_seqlens)
+                                 attention_chunk=attention_chunk, rotary_seqlens=rotary_seqlens,
+                                 k_scale=k_scale, v_scale=v_scale)
     if q.dim() != 4:
         raise ValueError(f"fable_attn: decode expects q (batch, seqlen_q, nheads, headdim), "
                          f"got {tuple(q.shape)}")
@@ -826,7 +876,7 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     if softmax_scale is None:
         softmax_scale = (q.shape[-1] + (qv.shape[-1] if qv is not None else 0)) ** -0.5
     appending = k is not None
-    if appending and (qv is not None or not (k_cache.is_contiguous() and v_cache.is_contiguous())):
+    if appending and not q8 and (qv is not None or not (k_cache.is_contiguous() and v_cache.is_contiguous())):
         raise NotImplementedError(
             "fable_attn: appending k/v needs the kernel to write the caller's cache in place: "
             "not possible with qv (the cache is widened into a temporary) or with a "
@@ -864,6 +914,12 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     sin = rotary_sin.to(torch.float32).contiguous() if rotary_sin is not None else None
     alibi = alibi_slopes.to(torch.float32).contiguous() if alibi_slopes is not None else None
     rpos = _as_index(rotary_seqlens, dev) if rotary_seqlens is not None else None
+    if q8:
+        out, lse = _C.dec8(_aligned(q, dense=True), k_cache, v_cache, k_scale, v_scale, table, lens,
+                           _aligned(k, dense=True) if appending else None, _aligned(v, dense=True) if appending else None,
+                           cos, sin, bool(rotary_interleaved), float(softmax_scale), int(keys_back), int(num_splits or 0),
+                           leftpad, bool(return_softmax_lse), float(softcap or 0.0), alibi, rpos)
+        return (out, lse.transpose(1, 2).contiguous()) if return_softmax_lse else out
     out, lse = _C.dec(_aligned(q, dense=True), kc.contiguous(), vc.contiguous(), table, lens,
                       _aligned(k, dense=True) if appending else None,
                       _aligned(v, dense=True) if appending else None,
@@ -918,3 +974,82 @@ def _kvcache_packed_q(q, k_cache, v_cache, k, qv, cu_seqlens_q, max_seqlen_q, re
         return out
     lse = r[1].transpose(1, 2).reshape(nseq * width, -1)[slot]   # (total_q, nheads)
     return out, lse.transpose(0, 1).contiguous()
+
+
+# ----------------------------------------------------------------------------- append and gather
+def _rows_of_cache(k_cache, block_table, cache_batch_idx, dev):
+    """The block table of a paged cache, or of a dense one with chosen rows; None for a dense cache in order."""
+    if block_table is not None:
+        if cache_batch_idx is not None:
+            raise ValueError("fable_attn: cache_batch_idx applies to a dense cache only; with a "
+                             "paged cache the block_table selects the rows")
+        return _as_index(block_table, dev)
+    if k_cache.shape[1] & (k_cache.shape[1] - 1):
+        raise NotImplementedError(
+            f"fable_attn: dense cache length {k_cache.shape[1]} must be a power of two (or pass block_table)")
+    return _as_index(cache_batch_idx, dev).view(-1, 1) if cache_batch_idx is not None else None
+
+
+@torch.no_grad()
+def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, cu_seqlens=None, max_seqlen=None,
+                              block_table=None, cache_batch_idx=None, cache_leftpad=None, rotary_cos=None,
+                              rotary_sin=None, rotary_interleaved=True, rotary_seqlens=None, k_scale=None, v_scale=None):
+    """Write new keys and values into a cache, the keys (and, if given, the queries) rotated on the way.
+    k, v (batch, seqlen_new, nheads_k, d); or packed (total, nheads_k, d) with cu_seqlens int32 (batch+1) and
+    max_seqlen, at least the longest sequence's count (a smaller one leaves tokens out; default: total). Token t of
+    sequence b goes to position cache_seqlens[b] + t, which the caller then adds to its lengths, and is rotated by row
+    rotary_seqlens[b] + t (default: its position) of the tables. k_cache, v_cache: (num_blocks, page, nheads_k, d) with
+    block_table, or dense (batch, seqlen, nheads_k, d), rows chosen by cache_batch_idx; pages, rows and heads may
+    be strided. Positions past the table and table entries that name no page of the cache are dropped. Returns
+    q's tokens (batch, seqlen_new, nheads, d) or (total, nheads, d) rotated, in a new tensor; else None.
+
+    Caches of k's dtype are written as they are. Caches held in 8 bits are torch.float8_e4m3fn with k_scale, v_scale
+    torch.float8_e8m0fnu (num_blocks, nheads_k, page / G): G consecutive tokens of a head share a power of two (G a
+    power of two, 1 to 256), and a value is code * scale. A block of G tokens gets the least scale that its largest
+    new token fits; if the sequence holds tokens in it already (from cache_leftpad on), the larger of that and the one
+    it has, and a scale that grows takes the older codes with it. Values that are not finite become NaN. Two
+    sequences of one call must not write to one block of G tokens. Head dims are multiples of 16 up to 256, pages
+    have 16 rows at least, k is fp16 or bf16."""
+    if not k.is_cuda:
+        raise ValueError("fable_attn: tensors must be on the GPU (k.is_cuda == False)")
+    if k.dtype not in _DTYPES:
+        raise ValueError(f"fable_attn: dtype {k.dtype} is not supported; use fp16, bf16 or fp32")
+    if k.dim() != (4 if cu_seqlens is None else 3) or v.shape != k.shape:
+        raise ValueError(f"fable_attn: k and v must be (batch, seqlen_new, nheads_k, headdim), or (total, nheads_k, headdim) "
+                         f"with cu_seqlens; got {tuple(k.shape)} and {tuple(v.shape)}")
+    if q is not None and rotary_cos is None:
+        raise ValueError("fable_attn: q is given to be rotated; pass rotary_cos and rotary_sin")
+    if k_cache.dim() != 4:
+        raise ValueError(f"fable_attn: k_cache must be (num_blocks, page, nheads_k, headdim), got {tuple(k_cache.shape)}")
+    dev = k.device
+    batch = k.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
+    if isinstance(cache_seqlens, int):
+        cache_seqlens = torch.full((batch,), cache_seqlens, dtype=torch.int32, device=dev)
+    idx = lambda t: _as_index(t, dev) if t is not None else None
+    f32 = lambda t: t.to(torch.float32).contiguous() if t is not None else None
+    return _C.append(_aligned(k), _aligned(v), k_cache, v_cache, idx(cache_seqlens), _aligned(q) if q is not None else None,
+                     idx(cu_seqlens), k.shape[0] if max_seqlen is None else int(max_seqlen),
+                     _rows_of_cache(k_cache, block_table, cache_batch_idx, dev), idx(cache_leftpad), f32(rotary_cos),
+                     f32(rotary_sin), bool(rotary_interleaved), idx(rotary_seqlens), k_scale, v_scale)
+
+
+@torch.no_grad()
+def flash_attn_gather_kvcache(k_cache, v_cache, cu_seqlens_k, total_k, *, block_table=None, cache_batch_idx=None,
+                              k_scale=None, v_scale=None, dtype=None):
+    """The first cu_seqlens_k[b+1] - cu_seqlens_k[b] cached rows of every sequence as packed (k, v), (total_k, nheads_k,
+    d) each: a cache's rows for flash_attn_varlen_func, or to be kept elsewhere. Caches as in
+    flash_attn_append_kvcache; dtype: of the result for a cache held in 8 bits (fp16 or bf16, the default), else
+    the cache's own. Rows past cu_seqlens_k[-1], and of pages the table does not name, are zeros."""
+    if not k_cache.is_cuda:
+        raise ValueError("fable_attn: tensors must be on the GPU (k_cache.is_cuda == False)")
+    if k_cache.dim() != 4:
+        raise ValueError(f"fable_attn: k_cache must be (num_blocks, page, nheads_k, headdim), got {tuple(k_cache.shape)}")
+    if k_scale is None:
+        if k_cache.dtype not in _DTYPES or dtype not in (None, k_cache.dtype):
+            raise ValueError(f"fable_attn: a cache of {k_cache.dtype} without scales comes back as it is (fp16, bf16 or fp32)")
+        dtype = k_cache.dtype
+    elif dtype not in (None, torch.float16, torch.bfloat16):
+        raise ValueError(f"fable_attn: a cache in 8 bits comes back in fp16 or bf16, not {dtype}")
+    dev = k_cache.device
+    return _C.gather(k_cache, v_cache, _as_index(cu_seqlens_k, dev), int(total_k), dtype or torch.bfloat16,
+                     _rows_of_cache(k_cache, block_table, cache_batch_idx, dev), k_scale, v_scale)

@@ -361,6 +361,91 @@ int fable_attn_dec_noalloc(FableDecParams p, int dtype, void* stream, const void
                            const void* new_v);
 int64_t fable_attn_dec_noalloc_max_floats(void);
 
+/* ---- Caches held in 8 bits. A row of HD values is HD e4m3 codes (four exponent bits, three of mantissa, no
+ * infinities; one byte each), and every `group` consecutive rows of a page share one scale per head: a
+ * byte b that stands for 2^(b-127) (e8m0), value = code * 2^(b-127). Codes sit at page, head and row strides
+ * in bytes (fa_strides .b, .h, .s; multiples of 16, rows below 2^26, the head dim contiguous); scales are
+ * dense, [num_blocks][NH/gqa][page/group]. group is a power of two of at most 256 and at most the page,
+ * pages are powers of two of at least 16 rows, head dims multiples of 16 up to 256. Table entries outside
+ * [0, num_blocks) are never followed: attention reads the last page in their place, an append
+ * drops the row and a gather gives zeros. No reference counterpart (the reference refuses FP8 caches). */
+typedef struct FableCache8 {
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  fa_strides k, v;
+  int32_t group, num_blocks;
+  int32_t rotary_rows;   /* decode: rows of the rotary tables (positions past them use the last row) */
+} FableCache8;
+
+/* fable_attn_dec_ws over an 8-bit cache (p.Kc / p.Vc: the codes): q and o in fp16 or bf16, any number of new
+ * tokens, p.block_table NULL for a dense cache. new_k / new_v (of q's type) are quantised into the cache
+ * first, as fable_attn_append does. Same arguments, workspace contract and results as there, with the K and
+ * V that the codes stand for. */
+int64_t fable_attn_dec8_ws_bytes(FableDecParams p, FableCache8 c, int dtype, int append);
+int fable_attn_dec8(FableDecParams p, FableCache8 c, int dtype, void* ws, int64_t ws_bytes, void* stream, const void* new_k,
+                    const void* new_v);
+
+/* fable_attn_fwd_paged over an 8-bit cache: p.K / p.V are the codes, c.k / c.v their strides (p.sK, p.sV and
+ * the page strides of kv are ignored). Head dims up to 256 in kernels of width 64, 128 and 256. */
+int64_t fable_attn_fwd_paged8_ws_bytes(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype);
+int fable_attn_fwd_paged8(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype, void* ws, int64_t ws_bytes,
+                          void* stream);
+
+/* New tokens into a cache. Token t of sequence b goes to position ctx_len[b] + t of the sequence: row
+ * position % page of page block_table[b*max_blocks + position / page] (block_table NULL: page b*max_blocks +
+ * position / page). Padded batches have n tokens per sequence (row t of sequence b at b*.b + t*.s elements);
+ * with cu (int32, batch+1) sequence b has the rows cu[b]..cu[b+1] (at row*.s, .b ignored) and n is the most
+ * any sequence has. Keys are rotated first, in fp32, as FableDecParams says (positions past the rotary_rows rows
+ * of the tables use the last row). k_scale NULL: the caches are of `dtype` (fp16, bf16, fp32; head dims
+ * multiples of 8). Otherwise they are in 8 bits (dtype fp16 or bf16), and every block of `group` rows that gets
+ * new ones takes the least scale its new rows fit (|code| <= 448), or the one it has, if rows of the sequence
+ * are in it already (from leftpad[b] on, if given) and theirs is larger; older rows are brought to a scale
+ * that grew. Values that are not finite become NaN codes; larger ones than a code can stand for in
+ * dtype's range (61440 in fp16, 448 * 2^119 in bf16) become that. Two sequences of a call must not write rows of one block. q (optional,
+ * NH heads): its rotated rows go to q_out, rounded to dtype, and what the rounding left to q_lo, if given;
+ * both are dense [tokens][NH][HD]. Positions outside the sequence's table are dropped. */
+typedef struct FableAppendParams {
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  void* q_lo;
+  void* Kc;
+  void* Vc;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  fa_strides sk, sv, sq;   /* new tokens (elements) */
+  fa_strides kc, vc;       /* caches: page, head, row (elements) */
+  const int32_t* block_table;
+  const int32_t* ctx_len;
+  const int32_t* cu;
+  const int32_t* leftpad;
+  const int32_t* rotary_pos;
+  const float* cos;
+  const float* sin;
+  int32_t batch, n, NH, NKV, HD, page, max_blocks, num_blocks, group;
+  int32_t rotary, rotary_dim, rotary_rows;
+} FableAppendParams;
+int fable_attn_append(FableAppendParams p, int dtype, void* stream);
+
+/* The first cu[b+1] - cu[b] cached rows of every sequence, packed: rows cu[b].. of the dense k_out / v_out
+ * [total][NKV][HD] in dtype (fp16, bf16; fp32 for a cache of that type). k_scale NULL: the caches are of
+ * `dtype`. Rows of [0, total) that no sequence has, or whose page the table does not name, become zeros. */
+typedef struct FableGatherParams {
+  const void* Kc;
+  const void* Vc;
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  void* k_out;
+  void* v_out;
+  fa_strides kc, vc;
+  const int32_t* block_table;
+  const int32_t* cu;
+  int64_t total;
+  int32_t batch, NKV, HD, page, max_blocks, num_blocks, group;
+} FableGatherParams;
+int fable_attn_gather(FableGatherParams p, int dtype, void* stream);
+
 /* split count chosen for a decode call (reference heuristic: dispatch.cpp:182-200, retuned for
  * 256 CUs); num_splits_hint > 0 is honoured (clamped to [1, 512]). */
 int fa_decode_num_splits(int batch, int nq, int NH, int gqa, int64_t ctx_bound, int num_splits_hint);
@@ -371,7 +456,8 @@ int fa_combine_launch(CombineParams p, void* stream);
 /* introspection for bindings and tests */
 int fable_attn_abi_version(void);
 /* sizeof of a struct: 0 FableFwdParams, 1 FableBwdParams, 2 FableDecParams, 3 CombineParams,
- * 4 fa_strides, 5 FwdParams, 6 BwdParams, 7 DecParams (0 for any other value) */
+ * 4 fa_strides, 5 FwdParams, 6 BwdParams, 7 DecParams, 8 FableCache8, 9 FableAppendParams, 10 FableGatherParams
+ * (0 for any other value) */
 size_t fable_attn_struct_size(int which);
 const char* fable_attn_last_error(void);
 
