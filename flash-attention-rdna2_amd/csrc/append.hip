@@ -40,82 +40,100 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // Rotation (AppendArgs::rot): none; halves or pairs in whole chunks of eight (half a multiple of 8, or the
 // width for pairs, tables 16-byte aligned); halves or pairs element by element (any even width).
 enum { kRotNone = 0, kRotHalves = 1, kRotPairs = 2, kRotHalvesAny = 3, kRotPairsAny = 4 };
+constexpr int kHeadsPerWave = 4;   // heads of a unit whose rows need no scale
 
 struct AppendArgs : FableAppendParams {
-  int page_shift, gshift, tshift, rot, rdim, tiles, nunits, nkv;   // nkv: NKV, or 0 where only q is rotated
+  int page_shift, gshift, tshift, rot, rdim, tiles, wgs;   // tiles of a sequence, workgroups of a tile
+  int ukv, uq;   // units (waves) of a tile: of K, and as many of V, and of q
 };
 
 // A lane's two chunks of eight values of a row: with halves in whole chunks, one of the first half and its
-// partner, so a rotation needs no other lane; else two neighbours.
+// partner, so a rotation needs no other lane; else two neighbours. (Chunks past the head dim: chunk 0, not ok.)
 struct Chunks {
   int c[2];
-  bool ok[2];
+  bool ok[2], turn;   // turn: halves, and this lane's chunks are in the rotated columns
 };
 __device__ __forceinline__ Chunks chunks_of(const AppendArgs& p, int u, bool rotated) {
   Chunks k;
-  const int half = p.rdim / 2;
+  k.c[0] = 2 * u;
+  k.c[1] = 2 * u + 1;
+  k.turn = false;
   if (rotated && p.rot == kRotHalves) {
-    const int n = half / 8;
-    k.c[0] = u < n ? u : 2 * n + 2 * (u - n);
-    k.c[1] = u < n ? u + n : k.c[0] + 1;
-  } else {
-    k.c[0] = 2 * u;
-    k.c[1] = 2 * u + 1;
+    const int n = p.rdim / 16;
+    k.turn = u < n;
+    k.c[0] = u < n ? u : 2 * u;   // (past the rotated columns: 2n + 2(u - n))
+    k.c[1] = u < n ? u + n : 2 * u + 1;
   }
-  k.ok[0] = 8 * k.c[0] < p.HD;
-  k.ok[1] = 8 * k.c[1] < p.HD;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    k.ok[i] = 8 * k.c[i] < p.HD;
+    k.c[i] = k.ok[i] ? k.c[i] : 0;
+  }
   return k;
 }
 
-// the lane's values of one row, rotated at row rp of the tables if asked (row: in bounds, rp too)
-template <typename T>
-__device__ __forceinline__ void load_row(const AppendArgs& p, const T* row, const Chunks& k, bool rotated, int rp, float (&x)[2][8]) {
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    if (k.ok[i]) {
-      load8(row + 8 * k.c[i], x[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-    }
-  }
-  if (!rotated || p.rot == kRotNone) return;
+// cosines and sines for a lane's chunks at row rp of the tables (in bounds; only p.rot < kRotHalvesAny)
+struct Angles {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_angles(const AppendArgs& p, const Chunks& k, int rp, Angles& a) {
   const int half = p.rdim / 2;
   const float* cos = p.cos + (long long)rp * half;
   const float* sin = p.sin + (long long)rp * half;
   if (p.rot == kRotHalves) {
-    if (8 * k.c[0] < half) {
-      float c[8], s[8];
-      load8(cos + 8 * k.c[0], c);
-      load8(sin + 8 * k.c[0], s);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float a = x[0][e], b = x[1][e];
-        x[0][e] = a * c[e] - b * s[e];
-        x[1][e] = b * c[e] + a * s[e];
-      }
-    }
+    const int at = k.turn ? 8 * k.c[0] : 0;
+    load8(cos + at, a.c);
+    load8(sin + at, a.s);
   } else if (p.rot == kRotPairs) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      if (k.ok[i] && 8 * k.c[i] < p.rdim) {
-        const f32x4 c = *(const f32x4*)(cos + 4 * k.c[i]), s = *(const f32x4*)(sin + 4 * k.c[i]);
+      const int at = 8 * k.c[i] < p.rdim ? 4 * k.c[i] : 0;
+      const f32x4 c = *(const f32x4*)(cos + at), s = *(const f32x4*)(sin + at);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float a = x[i][2 * e], b = x[i][2 * e + 1];
-          x[i][2 * e] = a * c[e] - b * s[e];
-          x[i][2 * e + 1] = b * c[e] + a * s[e];
+      for (int e = 0; e < 4; e++) {
+        a.c[4 * i + e] = c[e];
+        a.s[4 * i + e] = s[e];
+      }
+    }
+  }
+}
+// (ANY: the element-by-element forms only, which read the partner from the row)
+template <bool ANY, typename T>
+__device__ __forceinline__ void turn(const AppendArgs& p, const Chunks& k, const Angles& an, const T* row, int rp, float (&x)[2][8]) {
+  if constexpr (!ANY) {
+    if (p.rot == kRotHalves) {
+      if (k.turn) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float a = x[0][e], b = x[1][e];
+          x[0][e] = a * an.c[e] - b * an.s[e];
+          x[1][e] = b * an.c[e] + a * an.s[e];
+        }
+      }
+    } else if (p.rot == kRotPairs) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        if (8 * k.c[i] < p.rdim) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float a = x[i][2 * e], b = x[i][2 * e + 1], c = an.c[4 * i + e], s = an.s[4 * i + e];
+            x[i][2 * e] = a * c - b * s;
+            x[i][2 * e + 1] = b * c + a * s;
+          }
         }
       }
     }
   } else {
+    const int half = p.rdim / 2;
+    const float* cos = p.cos + (long long)rp * half;
+    const float* sin = p.sin + (long long)rp * half;
     const bool halves = p.rot == kRotHalvesAny;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const int d = 8 * k.c[i] + e;
-        if (k.ok[i] && d < p.rdim) {
+        if (d < p.rdim) {
           const int j = halves ? (d < half ? d : d - half) : d / 2;
           const bool first = halves ? d < half : (d & 1) == 0;
           const int other = halves ? (first ? d + half : d - half) : d ^ 1;
@@ -126,178 +144,231 @@ __device__ __forceinline__ void load_row(const AppendArgs& p, const T* row, cons
   }
 }
 
-// A wave takes a tile of 2^tshift consecutive positions of one sequence, aligned to the tile, and one head of
-// the keys, values or queries; LPR lanes share a row (16 values each), so a pass covers 64 / LPR rows. In 8
-// bits a tile holds whole blocks of `group` rows, which no other wave touches: their largest value is a
-// reduction within the wave, and older rows of a block whose scale grew are rewritten by the same lanes.
-// NP: passes of a tile, whose rows stay in registers between the search for the largest value and the
-// rounding; 0: any number, read twice (the second time from L2).
-// What bounds it: a step of few tokens the launch and two dependent memory latencies (lengths, then rows);
-// prompts the bytes read and written.
-template <typename T, bool Q8, int NP, int LPR>
+// A unit takes a tile of 2^tshift consecutive positions of one sequence, aligned to the tile; LPR lanes share a
+// row (16 values each), so a pass of a wave covers 64 / LPR rows. In 8 bits a tile holds whole blocks of `group`
+// rows, which no other unit touches: their largest value is a reduction over the unit, and older rows of a block
+// whose scale grew are rewritten by the same lanes. A unit is WB waves of NP passes each, whose rows stay in
+// registers between the search for the largest value and the rounding (NP 0: any number of passes, read twice,
+// the second time from L2), and HB heads of the keys or values, which share their angles: a head of 128 has half as many
+// bytes as its angles, which came from L2 for every head before (8192 tokens of 8 heads, blocks of 16: 24.3 us,
+// 17.3 without a rotation). Rows that need no scale (queries, caches of 16 and 32 bits) go four heads to a unit of
+// one wave and one pass. The units of a tile follow one another in the grid, so that the heads of a token are
+// read together (rather than the tiles of a head one after another).
+// Loads carry no lane condition (a row that is not there reads the sequence's first or last token), so those of a
+// tile are in flight together. What bounds it: a step of few tokens the launch and two dependent
+// memory latencies (lengths, then rows); prompts the bytes read and written.
+template <typename T, bool Q8, int NP, int HB, int WB, int LPR, bool ANY>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
   constexpr int R = 64 / LPR, NH = NP > 0 ? NP : 1;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.x / p.tiles, tile = blockIdx.x - b * p.tiles;
-  const int unit = blockIdx.y * 4 + wave;
-  if (unit >= p.nunits) return;
-  // units: the key heads, the value heads, the query heads
-  const int kind = unit < p.nkv ? 0 : (unit < 2 * p.nkv ? 1 : 2), head = unit - kind * p.nkv;
+  const int bt = blockIdx.x / p.wgs, wg = blockIdx.x - bt * p.wgs;
+  const int b = bt / p.tiles, tile = bt - b * p.tiles;
+  // units of K and V, padded to whole workgroups where they are of several waves, then those of q
+  const int kvw = WB > 1 ? (2 * p.ukv * WB + 3) / 4 * 4 : 2 * p.ukv, at = wg * 4 + wave;
+  const int unit = at < kvw ? at / WB : 2 * p.ukv + at - kvw;
+  if (WB == 1 || at >= kvw) {
+    if (unit >= 2 * p.ukv + p.uq) return;
+  }
+  const int kind = at >= kvw ? 2 : (unit < p.ukv ? 0 : 1);   // q, K, V
   const int ctx = p.ctx_len[b], c0 = p.cu ? p.cu[b] : 0, n = p.cu ? p.cu[b + 1] - c0 : p.n;
   const long long base = (((long long)max(ctx, 0) >> p.tshift) + tile) << p.tshift, stop = (long long)ctx + n;
-  if (base >= stop) return;
+  if (n <= 0 || base >= stop) return;
   const int r = lane / LPR;
-  const bool rotated = kind != 1;
+  const bool rotated = kind != 1 && p.rot != kRotNone;
   const Chunks ch = chunks_of(p, lane % LPR, rotated);
   const fa_strides st = kind == 0 ? p.sk : (kind == 1 ? p.sv : p.sq);
-  const T* src = (const T*)(kind == 0 ? p.k : (kind == 1 ? p.v : p.q)) + (long long)head * st.h + (p.cu ? (long long)c0 * st.s : (long long)b * st.b);
-  const long long rp0 = (p.rotary_pos && p.rot ? p.rotary_pos[b] : ctx);
-  const int passes = NP > 0 ? NP : max((1 << p.tshift) / R, 1);
+  const T* src = (const T*)(kind == 0 ? p.k : (kind == 1 ? p.v : p.q)) + (p.cu ? (long long)c0 * st.s : (long long)b * st.b);
+  const long long rp0 = rotated && p.rotary_pos ? p.rotary_pos[b] : ctx;
+  const int passes = NP > 0 ? NP : max((1 << p.tshift) / R, 1);   // of a wave
+  const int part = WB > 1 ? at % WB : 0;                          // of the unit's waves
   const long long room = (long long)p.max_blocks << p.page_shift;
-  // row of pass i: its token, whether there is one (queries have no place in the table)
-  auto pos_of = [&](int i) { return base + i * R + r; };
+  auto pos_of = [&](int i) { return base + (part * NH + i) * R + r; };
+  auto token_of = [&](int i) { return min(max(pos_of(i) - ctx, 0LL), (long long)n - 1); };   // in bounds
+  auto row_of = [&](int i) { return (int)min(max(rp0 + token_of(i), 0LL), (long long)p.rotary_rows - 1); };
+  // (queries have no place in the table)
   auto live = [&](long long pos) { return pos >= ctx && pos < stop && (kind == 2 || pos < room); };
-  auto fetch = [&](int i, float (&x)[2][8]) {
-    const long long pos = pos_of(i), t = pos - ctx;
-    if (live(pos)) {
-      const int rp = (int)min(max(rp0 + t, 0LL), (long long)max(p.rotary_rows - 1, 0));
-      load_row<T>(p, src + t * st.s, ch, rotated, rp, x);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[0][e] = x[1][e] = 0.0f;
-    }
-  };
-  // the page of a position, or -1
+  // the page of a position in the table, or -1
   auto page_of = [&](long long pos) {
     const long long j = pos >> p.page_shift;
     const int blk = p.block_table ? p.block_table[(long long)b * p.max_blocks + j] : (int)(b * (long long)p.max_blocks + j);
     return (unsigned)blk < (unsigned)p.num_blocks ? blk : -1;
   };
 
-  if (kind == 2) {
-    for (int i = 0; i < passes; i++) {
-      const long long pos = pos_of(i);
-      if (!live(pos)) continue;
-      float x[2][8];
-      fetch(i, x);
-      const long long o = (((long long)(p.cu ? c0 : b * (long long)p.n) + pos - ctx) * p.NH + head) * p.HD;
+  if (!Q8 || kind == 2) {
+    // (a wave of queries takes one pass of the tile, whatever the block's length)
+    const int nheads = kind == 2 ? p.NH : p.NKV, per = (nheads + kHeadsPerWave - 1) / kHeadsPerWave;
+    const int mine = unit - kind * p.ukv, i = mine / per, h0 = (mine - i * per) * kHeadsPerWave;
+    const fa_strides cs = kind == 0 ? p.kc : p.vc;
+    T* cache = (T*)(kind == 0 ? p.Kc : p.Vc);
+    const long long pos = pos_of(i);
+    const T* row = src + token_of(i) * st.s;
+    const int rp = rotated ? row_of(i) : 0;
+    Angles an;
+    if (!ANY && rotated) load_angles(p, ch, rp, an);
+    float x[kHeadsPerWave][2][8];
+#pragma unroll
+    for (int g = 0; g < kHeadsPerWave; g++) {
+      const T* q = row + (long long)min(h0 + g, nheads - 1) * st.h;
+      load8(q + 8 * ch.c[0], x[g][0]);
+      load8(q + 8 * ch.c[1], x[g][1]);
+    }
+    bool ok = live(pos);
+    long long o = 0, step = p.HD;
+    T* dst = (T*)p.q_out;
+    if (kind == 2) {
+      o = ((p.cu ? c0 : b * (long long)p.n) + token_of(i)) * p.NH * p.HD;
+    } else if (ok) {
+      const int blk = page_of(pos);
+      ok = blk >= 0;
+      o = (long long)blk * cs.b + (pos & ((1 << p.page_shift) - 1)) * cs.s;
+    }
+    if (kind != 2) {
+      dst = cache;
+      step = cs.h;
+    }
+#pragma unroll
+    for (int g = 0; g < kHeadsPerWave; g++) {
+      const int h = h0 + g;
+      if (rotated) turn<ANY, T>(p, ch, an, row + (long long)min(h, nheads - 1) * st.h, rp, x[g]);
+      if (!ok || h >= nheads) continue;
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         if (!ch.ok[u]) continue;
-        store8((T*)p.q_out + o + 8 * ch.c[u], x[u]);
-        if (p.q_lo) {
+        const long long at = o + h * step + 8 * ch.c[u];
+        store8(dst + at, x[g][u]);
+        if (kind == 2 && p.q_lo) {   // what the rounding left
 #pragma unroll
-          for (int e = 0; e < 8; e++) x[u][e] -= (float)(T)x[u][e];
-          store8((T*)p.q_lo + o + 8 * ch.c[u], x[u]);
+          for (int e = 0; e < 8; e++) x[g][u][e] -= (float)(T)x[g][u][e];
+          store8((T*)p.q_lo + at, x[g][u]);
         }
       }
     }
     return;
   }
-  const fa_strides cs = kind == 0 ? p.kc : p.vc;
-  if constexpr (!Q8) {
-    T* cache = (T*)(kind == 0 ? p.Kc : p.Vc) + (long long)head * cs.h;
-    for (int i = 0; i < passes; i++) {
-      const long long pos = pos_of(i);
-      if (!live(pos)) continue;
-      float x[2][8];
-      fetch(i, x);
-      const int blk = page_of(pos);
-      if (blk < 0) continue;
-      T* dst = cache + (long long)blk * cs.b + (pos & ((1 << p.page_shift) - 1)) * cs.s;
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-        if (ch.ok[u]) store8(dst + 8 * ch.c[u], x[u]);
-    }
-  } else {
-    uint8_t* cache = (uint8_t*)(kind == 0 ? p.Kc : p.Vc) + (long long)head * cs.h;
-    float x[NH][2][8];
-    auto hold = [&](float (&v)[2][8], float& top) {
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          // the largest value a code stands for in T's range (fp16: 65504 would round to 65536)
-          constexpr float kMost = std::is_same<T, _Float16>::value ? 61440.0f : 448.0f * 6.646139978924579e35f /* 2^119 */;
-          if (fabsf(v[u][e]) <= 3.4028234e38f) v[u][e] = fminf(fmaxf(v[u][e], -kMost), kMost);
-          const float a = fabsf(v[u][e]);
-          top = a <= 3.4028234e38f ? fmaxf(top, a) : top;
-        }
-    };
-    float top = 0.0f;
-    if constexpr (NP > 0) {
-#pragma unroll
-      for (int i = 0; i < NP; i++) fetch(i, x[i]);
-#pragma unroll
-      for (int i = 0; i < NP; i++) hold(x[i], top);
-    } else {
-      for (int i = 0; i < passes; i++) {
-        fetch(i, x[0]);
-        hold(x[0], top);
-      }
-    }
-    // the block's lanes: rows of one block in this pass
+  if constexpr (Q8) {
+    const int h0 = (unit - kind * p.ukv) * HB;
+    const fa_strides cs = kind == 0 ? p.kc : p.vc;
+    // this lane's block, its first new row, and what is there already: looked up while the rows come
     const int group = 1 << p.gshift, span = min(group, R) * LPR;
-    for (int m = 1; m < span; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    const long long bs = pos_of(0) & ~(long long)(group - 1), f = max(bs, (long long)ctx);   // the block, its first new row
+    const long long bs = pos_of(0) & ~(long long)(group - 1), f = max(bs, (long long)ctx);
     const bool touched = f < min(min(bs + group, stop), room);
-    const int blk = touched ? page_of(f) : -1;
-    if (blk < 0) return;
+    const int blk = touched && h0 < p.NKV ? page_of(f) : -1;
     const int in = (int)(bs & ((1 << p.page_shift) - 1)), subs = 1 << (p.page_shift - p.gshift);
-    uint8_t* sc = (kind == 0 ? p.k_scale : p.v_scale) + ((long long)blk * p.NKV + head) * subs + (in >> p.gshift);
-    uint8_t* rows = cache + (long long)blk * cs.b + (long long)in * cs.s;
     const long long old = max(bs, (long long)(p.leftpad ? p.leftpad[b] : 0));   // the first row the sequence holds
-    int e = code_exponent(top);
-    if (f > old) {
-      const int was = min((int)*sc, 253) - 127;
-      if (e > was) {   // rows [old, f) under the scale that grew
-        const float down = exp2i(max(was - e, -126));
-        for (int i = 0; i < passes; i++) {
-          const long long pos = pos_of(i);
-          if (pos < old || pos >= f) continue;
-          uint8_t* row = rows + (pos - bs) * cs.s;
+    uint8_t* sc[HB];
+    int was[HB];
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            if (!ch.ok[u]) continue;
-            const u32x2 c = *(const u32x2*)(row + 8 * ch.c[u]);
-            float v[8];
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-              const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[w], true);
-              v[4 * w] = lo[0];
-              v[4 * w + 1] = lo[1];
-              v[4 * w + 2] = hi[0];
-              v[4 * w + 3] = hi[1];
-            }
-            *(u32x2*)(row + 8 * ch.c[u]) = to_codes(v, down);
-          }
-        }
-      } else {
-        e = was;
-      }
+    for (int g = 0; g < HB; g++) {
+      sc[g] = (kind == 0 ? p.k_scale : p.v_scale) + ((long long)max(blk, 0) * p.NKV + min(h0 + g, p.NKV - 1)) * subs + (in >> p.gshift);
+      was[g] = min((int)*sc[g], 253) - 127;
     }
-    const float inv = exp2i(-e);
+    float x[HB][NH][2][8], top[HB];
+    auto fetch = [&](int i, int j) {   // pass i of all heads, to x[.][j]
+      const T* row = src + token_of(i) * st.s;
+      const int rp = rotated ? row_of(i) : 0;
+      Angles an;
+      if (!ANY && rotated) load_angles(p, ch, rp, an);
+#pragma unroll
+      for (int g = 0; g < HB; g++) {
+        const T* q = row + (long long)min(h0 + g, p.NKV - 1) * st.h;
+        load8(q + 8 * ch.c[0], x[g][j][0]);
+        load8(q + 8 * ch.c[1], x[g][j][1]);
+        if (rotated) turn<ANY, T>(p, ch, an, q, rp, x[g][j]);
+      }
+    };
+    auto hold = [&](int i, int j) {
+      const bool ok = live(pos_of(i));
+#pragma unroll
+      for (int g = 0; g < HB; g++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            // the largest value a code stands for in T's range (fp16: 65504 would round to 65536)
+            constexpr float kMost = std::is_same<T, _Float16>::value ? 61440.0f : 448.0f * 6.646139978924579e35f /* 2^119 */;
+            float& v = x[g][j][u][e];
+            if (fabsf(v) <= 3.4028234e38f) v = fminf(fmaxf(v, -kMost), kMost);
+            const float a = fabsf(v);
+            top[g] = ok && ch.ok[u] && a <= 3.4028234e38f ? fmaxf(top[g], a) : top[g];
+          }
+    };
+#pragma unroll
+    for (int g = 0; g < HB; g++) top[g] = 0.0f;
     if constexpr (NP > 0) {
 #pragma unroll
-      for (int i = 0; i < NP; i++) {
-        const long long pos = pos_of(i);
-        if (!live(pos)) continue;
+      for (int i = 0; i < NP; i++) fetch(i, i);
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-          if (ch.ok[u]) *(u32x2*)(rows + (pos - bs) * cs.s + 8 * ch.c[u]) = to_codes(x[i][u], inv);
-      }
+      for (int i = 0; i < NP; i++) hold(i, i);
     } else {
       for (int i = 0; i < passes; i++) {
-        const long long pos = pos_of(i);
-        if (!live(pos)) continue;
-        fetch(i, x[0]);
-        hold(x[0], top);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-          if (ch.ok[u]) *(u32x2*)(rows + (pos - bs) * cs.s + 8 * ch.c[u]) = to_codes(x[0][u], inv);
+        fetch(i, 0);
+        hold(i, 0);
       }
     }
-    if ((lane & (span - 1)) == 0) *sc = (uint8_t)(e + 127);
+#pragma unroll
+    for (int g = 0; g < HB; g++)
+      for (int m = 1; m < span; m <<= 1) top[g] = fmaxf(top[g], __shfl_xor(top[g], m));   // over the block's lanes
+    if constexpr (WB > 1) {   // and its waves
+      __shared__ float tops[4];
+      static_assert(HB == 1, "one head");
+      if (lane == 0) tops[wave] = top[0];
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WB; w++) top[0] = fmaxf(top[0], tops[wave / WB * WB + w]);
+    }
+    if (blk < 0) return;
+#pragma unroll
+    for (int g = 0; g < HB; g++) {
+      if (h0 + g >= p.NKV) break;
+      uint8_t* rows = (uint8_t*)(kind == 0 ? p.Kc : p.Vc) + (long long)(h0 + g) * cs.h + (long long)blk * cs.b + (long long)in * cs.s;
+      int e = code_exponent(top[g]);
+      if (f > old) {
+        if (e > was[g]) {   // rows [old, f) under the scale that grew
+          const float down = exp2i(max(was[g] - e, -126));
+          for (int i = 0; i < passes; i++) {
+            const long long pos = pos_of(i);
+            if (pos < old || pos >= f) continue;
+            uint8_t* row = rows + (pos - bs) * cs.s;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              if (!ch.ok[u]) continue;
+              const u32x2 c = *(const u32x2*)(row + 8 * ch.c[u]);
+              float v[8];
+#pragma unroll
+              for (int w = 0; w < 2; w++) {
+                const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[w], true);
+                v[4 * w] = lo[0];
+                v[4 * w + 1] = lo[1];
+                v[4 * w + 2] = hi[0];
+                v[4 * w + 3] = hi[1];
+              }
+              *(u32x2*)(row + 8 * ch.c[u]) = to_codes(v, down);
+            }
+          }
+        } else {
+          e = was[g];
+        }
+      }
+      const float inv = exp2i(-e);
+      auto put = [&](int i, int j) {
+        const long long pos = pos_of(i);
+        if (!live(pos)) return;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+          if (ch.ok[u]) *(u32x2*)(rows + (pos - bs) * cs.s + 8 * ch.c[u]) = to_codes(x[g][j][u], inv);
+      };
+      if constexpr (NP > 0) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) put(i, i);
+      } else {
+        for (int i = 0; i < passes; i++) {
+          fetch(i, 0);
+          hold(i, 0);
+          put(i, 0);
+        }
+      }
+      if (part == 0 && (lane & (span - 1)) == 0) *sc[g] = (uint8_t)(e + 127);
+    }
   }
 }
 
@@ -305,25 +376,43 @@ template <typename T, bool Q8, int LPR>
 static int launch_append_lpr(AppendArgs& a, hipStream_t st) {
   constexpr int R = 64 / LPR;
   constexpr int rshift = __builtin_ctz(R);
-  // tiles: a pass, or a block that is longer; without scales 4 passes where the tokens fill them
+  // tiles: a pass, or a block that is longer
   a.tshift = Q8 && a.gshift > rshift ? a.gshift : rshift;
-  if (!Q8 && a.n >= 16 * R) a.tshift = rshift + 2;
-  const long long tiles = ((long long)a.n - 1 >> a.tshift) + 2, grid = tiles * a.batch;
-  if (grid > 0x7FFFFFFF || a.nunits > 4 * 65535) return fail(FA_ERR_ARG, "fable_attn_append: grid too large");
-  a.tiles = (int)tiles;
-  const dim3 g((unsigned)grid, (unsigned)((a.nunits + 3) / 4));
-  auto go = [&](auto np) { hipLaunchKernelGGL((append_kernel<T, Q8, decltype(np)::value, LPR>), g, dim3(256), 0, st, a); };
+  const long long tiles = ((a.n - 2LL + (1LL << a.tshift)) >> a.tshift) + 1;   // (wherever the first token is)
+  auto go = [&](auto np, auto hb, auto wb, auto any) -> int {
+    constexpr int NP = decltype(np)::value, HB = decltype(hb)::value, WB = decltype(wb)::value;
+    auto units = [](int heads, int per) { return (heads + per - 1) / per; };
+    a.ukv = a.k ? units(a.NKV, Q8 ? HB : kHeadsPerWave) : 0;
+    a.uq = a.q ? units(a.NH, kHeadsPerWave) << (a.tshift - rshift) : 0;
+    const int waves = (WB > 1 ? (2 * a.ukv * WB + 3) / 4 * 4 : 2 * a.ukv) + a.uq;
+    a.wgs = (waves + 3) / 4;
+    if (tiles > 0x7FFFFFFF / a.batch / a.wgs) return fail(FA_ERR_ARG, "fable_attn_append: grid too large");
+    a.tiles = (int)tiles;
+    hipLaunchKernelGGL((append_kernel<T, Q8, NP, HB, WB, LPR, decltype(any)::value>), dim3((unsigned)(tiles * a.batch * a.wgs)), dim3(256), 0, st, a);
+    return launch_status("fable_attn_append");
+  };
+  using N = std::integral_constant<bool, false>;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I4 = std::integral_constant<int, 4>;
+  using I8 = std::integral_constant<int, 8>;
+  if (a.rot >= kRotHalvesAny) return go(I0{}, I1{}, I1{}, std::integral_constant<bool, true>{});
   if constexpr (Q8) {
+    // (four passes at most, but for the longest blocks: with eight in one wave the instance held 200 registers, and a
+    // prompt of 11400 tokens with 32 query heads, blocks of 64, took 85 us; 74 with four in each of two waves)
     switch (a.tshift - rshift) {
-      case 0: go(std::integral_constant<int, 1>{}); break;
-      case 1: go(std::integral_constant<int, 2>{}); break;
-      case 2: go(std::integral_constant<int, 4>{}); break;
-      default: go(std::integral_constant<int, 0>{}); break;
+      case 0: return go(I1{}, I4{}, I1{}, N{});
+      case 1: return go(I2{}, I2{}, I1{}, N{});
+      case 2: return go(I4{}, I1{}, I1{}, N{});
+      case 3: return go(I4{}, I1{}, I2{}, N{});
+      case 4: return go(I4{}, I1{}, I4{}, N{});
+      case 5: return go(I8{}, I1{}, I4{}, N{});
+      default: return go(I0{}, I1{}, I1{}, N{});   // (blocks of 256 rows wider than 128)
     }
   } else {
-    go(std::integral_constant<int, 0>{});
+    return go(I1{}, I1{}, I1{}, N{});
   }
-  return launch_status("fable_attn_append");
 }
 template <typename T, bool Q8>
 static int launch_append(AppendArgs& a, hipStream_t st) {
@@ -374,8 +463,6 @@ int fa::append_rows(const FableAppendParams& p, int dtype, hipStream_t st) {
   if (p.batch == 0 || p.n == 0) return FA_OK;
   a.page_shift = __builtin_ctz((unsigned)p.page);
   a.gshift = q8 ? __builtin_ctz((unsigned)p.group) : 0;
-  a.nkv = p.k ? p.NKV : 0;
-  a.nunits = 2 * a.nkv + (p.q ? p.NH : 0);
   switch (dtype) {
     case FA_F16: return q8 ? launch_append<_Float16, true>(a, st) : launch_append<_Float16, false>(a, st);
     case FA_BF16: return q8 ? launch_append<__bf16, true>(a, st) : launch_append<__bf16, false>(a, st);

@@ -621,7 +621,8 @@ def fwd_paged8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, m
 def append(k, v, k_cache, v_cache, cache_seqlens, q=None, cu=None, max_seqlen=0, block_table=None, leftpad=None, cos=None,
            sin=None, interleaved=False, rotary_pos=None, k_scale=None, v_scale=None):
     """New tokens k, v (and q, which comes back rotated) [B,N,H,D], or [total,H,D] with cu int32 [batch+1], into the
-    caches at positions cache_seqlens[b] + t. block_table None: a dense cache, sequence b in page b."""
+    caches at positions cache_seqlens[b] + t. block_table None: a dense cache, sequence b in page b. Returns (the
+    launch's parameters and dtype, q rotated or None)."""
     dev = k.device
     packed = cu is not None
     _req(k.is_cuda, "GPU tensors required")
@@ -674,11 +675,12 @@ def append(k, v, k_cache, v_cache, cache_seqlens, q=None, cu=None, max_seqlen=0,
     if k.numel():
         with _on(dev):
             _lib.check(_L.fable_attn_append(p, dt, _stream(k)), "fable_attn_append")
-    return q_out
+    return p, dt, q_out
 
 
 def gather(k_cache, v_cache, cu, total, dtype, block_table=None, k_scale=None, v_scale=None):
-    """The first cu[b+1] - cu[b] cached rows of every sequence as packed k, v [total, Hk, D] in dtype."""
+    """The first cu[b+1] - cu[b] cached rows of every sequence as packed k, v [total, Hk, D] in dtype.
+    Returns (the launch's parameters and dtype, (k, v))."""
     dev = k_cache.device
     kc, vc, group = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev)
     nb, page, Hk, D = k_cache.shape
@@ -702,7 +704,7 @@ def gather(k_cache, v_cache, cu, total, dtype, block_table=None, k_scale=None, v
     if k.numel():
         with _on(dev):
             _lib.check(_L.fable_attn_gather(p, _dt(k), _stream(k)), "fable_attn_gather")
-    return k, v
+    return p, _dt(k), (k, v)
 
 
 def combine(out_partial, lse_partial, out_dtype):

@@ -705,25 +705,27 @@ def _sig(t):
     return None if t is None else (t.shape, t.dtype, t.device, t.is_contiguous())
 
 
-def _decode_key(q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alibi, scale, window, softcap,
+def _decode_key(q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alibi, k_scale, v_scale, scale, window, softcap,
                 interleaved, num_splits):
-    return (_sig(q), _sig(k_cache), _sig(v_cache), _sig(k), _sig(v), _sig(cos), _sig(sin), _sig(lens),
+    return (k_scale is not None and (_sig(k_scale), _sig(v_scale)), _sig(q), _sig(k_cache), _sig(v_cache), _sig(k), _sig(v), _sig(cos), _sig(sin), _sig(lens),
             _sig(leftpad), _sig(table), _sig(alibi), _option_key(scale, window, softcap), bool(interleaved), num_splits)
 
 
-def _decode_plan(q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alibi, scale, window, softcap,
+def _decode_plan(q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alibi, k_scale, v_scale, scale, window, softcap,
                  interleaved, num_splits):
     """The launch parameters of one decode signature that the general path has just served: every
     tensor contiguous, on q's device and of the dtype the kernels read (so the general path passed
     them on as they are). None when some tensor was converted or the call took another shape of the
     problem (a padded or widened head dim, fp32). The result holds no data pointer."""
+    q8 = k_scale is not None
     dev = q.device
     if dev.index is None or lens is None or q.dtype not in (torch.float16, torch.bfloat16):
         return None
     if q.dim() != 4 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or q.shape[3] % 8:
         return None
     if any(t is not None and not (t.is_contiguous() and t.device == dev and t.dtype == dt)
-           for dt, ts in ((q.dtype, (q, k_cache, v_cache, k, v)), (torch.float32, (cos, sin, alibi)),
+           for dt, ts in ((q.dtype, (q, k, v)), (_C.FP8 if q8 else q.dtype, (k_cache, v_cache)),
+                          (_C.E8M0, (k_scale, v_scale)), (torch.float32, (cos, sin, alibi)),
                           (torch.int32, (lens, leftpad, table))) for t in ts):
         return None
     B, NQ, H, D = q.shape
@@ -740,14 +742,20 @@ def _decode_plan(q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alib
     p.softcap, p.nq = float(softcap or 0.0), NQ
     p.rotary_dim = int(cos.shape[-1] * 2) if cos is not None else 0
     dt = _C._dt(q)
-    need = int(_C._L.fable_attn_dec_ws_bytes(p, dt, 1 if k is not None else 0))
-    return None if need < 0 else (p, dt, need)
+    c = None
+    if q8:
+        c = _C._cache8(k_cache, v_cache, k_scale, v_scale, q.dtype, dev, cos.shape[0] if cos is not None else 0)
+        need = int(_C._L.fable_attn_dec8_ws_bytes(p, c, dt, 1 if k is not None else 0))
+        c.k_scale = c.v_scale = None
+    else:
+        need = int(_C._L.fable_attn_dec_ws_bytes(p, dt, 1 if k is not None else 0))
+    return None if need < 0 else (p, dt, need, c)
 
 
-def _decode_fast(plan, q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alibi):
+def _decode_fast(plan, q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alibi, k_scale, v_scale):
     """One call of a planned signature: outputs and workspace allocated, pointers filled, launched.
     None when an address is not aligned or the device is not current (the general path serves it)."""
-    p, dt, need = plan
+    p, dt, need, c = plan
     dev = q.device.index
     ptr = lambda t: t.data_ptr() if t is not None else None
     qp, kp, vp, nkp, nvp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ptr(k), ptr(v)
@@ -757,6 +765,11 @@ def _decode_fast(plan, q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     p.q, p.Kc, p.Vc, p.o, p.ctx_len = qp, kp, vp, out.data_ptr(), lens.data_ptr()
     p.block_table, p.cos, p.sin, p.leftpad, p.alibi = ptr(table), ptr(cos), ptr(sin), ptr(leftpad), ptr(alibi)
+    if c is not None:
+        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        _lib.check(_C._L.fable_attn_dec8(p, c, dt, ptr(ws), need, torch._C._cuda_getCurrentRawStream(dev), nkp, nvp),
+                   "fable_attn_dec8")
+        return out
     _lib.check(_C._L.fable_attn_dec_ws(p, dt, ptr(ws), need, torch._C._cuda_getCurrentRawStream(dev), nkp, nvp),
                "fable_attn_dec")
     return out
@@ -778,13 +791,14 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     of a signature goes through all checks, and the launch parameters it came to are kept per
     thread (without any pointer), so later calls only fill in addresses and launch."""
     key = None
-    if (qv is None and k_scale is None and v_scale is None and cache_batch_idx is None and not attention_chunk and not return_softmax_lse
+    if (qv is None and (k_scale is None) == (v_scale is None) and cache_batch_idx is None and not attention_chunk and not return_softmax_lse
             and q_descale is None and k_descale is None and v_descale is None and cu_seqlens_q is None
             and cu_seqlens_k_new is None and rotary_seqlens is None and (page_table is None or block_table is None)
             and (num_splits is None or type(num_splits) is int) and (pack_gqa is None or type(pack_gqa) is bool)
             and (sm_margin is None or type(sm_margin) is int)):
         table = block_table if block_table is not None else page_table
-        args = (q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, cache_seqlens, cache_leftpad, table, alibi_slopes)
+        args = (q, k_cache, v_cache, k, v, rotary_cos, rotary_sin, cache_seqlens, cache_leftpad, table, alibi_slopes,
+                k_scale, v_scale)
         plans = getattr(_tls, "decode_plans", None)
         if plans is None:
             plans = _tls.decode_plans = {}
@@ -977,6 +991,62 @@ def _kvcache_packed_q(q, k_cache, v_cache, k, qv, cu_seqlens_q, max_seqlen_q, re
 
 
 # ----------------------------------------------------------------------------- append and gather
+# As for decode, the launch parameters that the first call of a signature came to are kept per thread, so that a
+# later one only fills in addresses, sizes that vary (max_seqlen, total_k) and launches.
+def _plans(name):
+    plans = getattr(_tls, name, None)
+    if plans is None:
+        plans = {}
+        setattr(_tls, name, plans)
+    return plans
+
+
+def _remember(plans, key, plan):
+    if len(plans) >= _MAX_PLANS:
+        plans.clear()
+    plans[key] = plan
+
+
+def _place(t):
+    """What a plan depends on of a tensor that may be strided."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _append_fast(plan, k, v, k_cache, v_cache, lens, q, cu, max_seqlen, table, leftpad, cos, sin, rpos, k_scale, v_scale):
+    """One call of a planned signature; (q rotated, or None,), or None when an address is not aligned or the
+    device is not current (the general path serves it)."""
+    p, dt, dev = plan
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    kp, vp, kcp, vcp, qp = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ptr(q)
+    if (kp | vp | kcp | vcp | (qp or 0)) & 15 or dev != torch._C._cuda_getDevice():
+        return None
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
+    p.k, p.v, p.Kc, p.Vc, p.q, p.q_out = kp, vp, kcp, vcp, qp, ptr(q_out)
+    p.ctx_len, p.cu, p.block_table, p.leftpad, p.cos, p.sin = lens.data_ptr(), ptr(cu), ptr(table), ptr(leftpad), ptr(cos), ptr(sin)
+    p.rotary_pos, p.k_scale, p.v_scale = ptr(rpos), ptr(k_scale), ptr(v_scale)
+    if cu is not None:
+        p.n = k.shape[0] if max_seqlen is None else int(max_seqlen)
+    if k.numel():
+        _lib.check(_C._L.fable_attn_append(p, dt, torch._C._cuda_getCurrentRawStream(dev)), "fable_attn_append")
+    return (q_out,)
+
+
+def _gather_fast(plan, k_cache, v_cache, cu, total, table, k_scale, v_scale):
+    """One call of a planned signature, or None (as _append_fast)."""
+    p, dt, dev, shape, dtype = plan
+    kcp, vcp = k_cache.data_ptr(), v_cache.data_ptr()
+    if (kcp | vcp) & 15 or dev != torch._C._cuda_getDevice():
+        return None
+    k, v = (torch.empty((total,) + shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+    p.Kc, p.Vc, p.k_out, p.v_out, p.cu, p.total = kcp, vcp, k.data_ptr(), v.data_ptr(), cu.data_ptr(), total
+    p.block_table = table.data_ptr() if table is not None else None
+    if k_scale is not None:
+        p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    if k.numel():
+        _lib.check(_C._L.fable_attn_gather(p, dt, torch._C._cuda_getCurrentRawStream(dev)), "fable_attn_gather")
+    return k, v
+
+
 def _rows_of_cache(k_cache, block_table, cache_batch_idx, dev):
     """The block table of a paged cache, or of a dense one with chosen rows; None for a dense cache in order."""
     if block_table is not None:
@@ -1010,6 +1080,20 @@ def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, 
     it has, and a scale that grows takes the older codes with it. Values that are not finite become NaN. Two
     sequences of one call must not write to one block of G tokens. Head dims are multiples of 16 up to 256, pages
     have 16 rows at least, k is fp16 or bf16."""
+    key, plans = None, _plans("append_plans")
+    try:
+        key = (_place(k), _place(v), _place(k_cache), _place(v_cache), _place(q), _sig(cache_seqlens), _sig(cu_seqlens), _sig(block_table),
+               _sig(cache_batch_idx), _sig(cache_leftpad), _sig(rotary_cos), _sig(rotary_sin), _sig(rotary_seqlens), _sig(k_scale),
+               _sig(v_scale), bool(rotary_interleaved))
+        plan = plans.get(key)
+    except (AttributeError, TypeError, ValueError, RuntimeError):   # not tensors, or no key
+        key = plan = None
+    if plan is not None:
+        got = _append_fast(plan, k, v, k_cache, v_cache, cache_seqlens, q, cu_seqlens, max_seqlen,
+                           block_table if block_table is not None else cache_batch_idx, cache_leftpad, rotary_cos, rotary_sin,
+                           rotary_seqlens, k_scale, v_scale)
+        if got is not None:
+            return got[0]
     if not k.is_cuda:
         raise ValueError("fable_attn: tensors must be on the GPU (k.is_cuda == False)")
     if k.dtype not in _DTYPES:
@@ -1027,10 +1111,15 @@ def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, 
         cache_seqlens = torch.full((batch,), cache_seqlens, dtype=torch.int32, device=dev)
     idx = lambda t: _as_index(t, dev) if t is not None else None
     f32 = lambda t: t.to(torch.float32).contiguous() if t is not None else None
-    return _C.append(_aligned(k), _aligned(v), k_cache, v_cache, idx(cache_seqlens), _aligned(q) if q is not None else None,
-                     idx(cu_seqlens), k.shape[0] if max_seqlen is None else int(max_seqlen),
-                     _rows_of_cache(k_cache, block_table, cache_batch_idx, dev), idx(cache_leftpad), f32(rotary_cos),
-                     f32(rotary_sin), bool(rotary_interleaved), idx(rotary_seqlens), k_scale, v_scale)
+    args = (_aligned(k), _aligned(v), k_cache, v_cache, idx(cache_seqlens), _aligned(q) if q is not None else None, idx(cu_seqlens))
+    rest = (_rows_of_cache(k_cache, block_table, cache_batch_idx, dev), idx(cache_leftpad), f32(rotary_cos), f32(rotary_sin))
+    rpos = idx(rotary_seqlens)
+    p, dt, q_out = _C.append(*args, k.shape[0] if max_seqlen is None else int(max_seqlen), *rest, bool(rotary_interleaved), rpos,
+                             k_scale, v_scale)
+    given = (k, v, k_cache, v_cache, cache_seqlens, q, cu_seqlens, block_table, cache_leftpad, rotary_cos, rotary_sin, rotary_seqlens)
+    if key is not None and cache_batch_idx is None and all(a is b for a, b in zip(given, args + rest + (rpos,))):
+        _remember(plans, key, (p, dt, dev.index))   # nothing was converted: the next call may fill in its addresses
+    return q_out
 
 
 @torch.no_grad()
@@ -1040,6 +1129,16 @@ def flash_attn_gather_kvcache(k_cache, v_cache, cu_seqlens_k, total_k, *, block_
     d) each: a cache's rows for flash_attn_varlen_func, or to be kept elsewhere. Caches as in
     flash_attn_append_kvcache; dtype: of the result for a cache held in 8 bits (fp16 or bf16, the default), else
     the cache's own. Rows past cu_seqlens_k[-1], and of pages the table does not name, are zeros."""
+    key, plans = None, _plans("gather_plans")
+    try:
+        key = (_place(k_cache), _place(v_cache), _sig(cu_seqlens_k), _sig(block_table), _sig(cache_batch_idx), _sig(k_scale), _sig(v_scale), dtype)
+        plan = plans.get(key)
+    except (AttributeError, TypeError, ValueError, RuntimeError):   # not tensors, or no key
+        key = plan = None
+    if plan is not None:
+        got = _gather_fast(plan, k_cache, v_cache, cu_seqlens_k, int(total_k), block_table, k_scale, v_scale)
+        if got is not None:
+            return got
     if not k_cache.is_cuda:
         raise ValueError("fable_attn: tensors must be on the GPU (k_cache.is_cuda == False)")
     if k_cache.dim() != 4:
@@ -1051,5 +1150,8 @@ def flash_attn_gather_kvcache(k_cache, v_cache, cu_seqlens_k, total_k, *, block_
     elif dtype not in (None, torch.float16, torch.bfloat16):
         raise ValueError(f"fable_attn: a cache in 8 bits comes back in fp16 or bf16, not {dtype}")
     dev = k_cache.device
-    return _C.gather(k_cache, v_cache, _as_index(cu_seqlens_k, dev), int(total_k), dtype or torch.bfloat16,
-                     _rows_of_cache(k_cache, block_table, cache_batch_idx, dev), k_scale, v_scale)
+    cu, table = _as_index(cu_seqlens_k, dev), _rows_of_cache(k_cache, block_table, cache_batch_idx, dev)
+    p, dt, out = _C.gather(k_cache, v_cache, cu, int(total_k), dtype or torch.bfloat16, table, k_scale, v_scale)
+    if key is not None and cache_batch_idx is None and cu is cu_seqlens_k and table is block_table:
+        _remember(plans, key, (p, dt, dev.index, out[0].shape[1:], out[0].dtype))
+    return out
