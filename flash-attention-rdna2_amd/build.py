@@ -29,8 +29,9 @@ FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC",
 
 # per-source extra flags
 def _extra(name):
-    # the fp16/bf16 backward kernels (bwd_dNN.hip) keep MFMA accumulators in VGPR form
-    if name.startswith("bwd_d") and name.endswith(".hip"):
+    # the fp16/bf16 backward kernels (bwd_dNN.hip) and the 8-bit decode (72 of the 480 instructions of its loop
+    # were copies of the accumulators) keep MFMA accumulators in VGPR form
+    if (name.startswith("bwd_d") or name == "decode8.hip") and name.endswith(".hip"):
         return ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
     return []
 

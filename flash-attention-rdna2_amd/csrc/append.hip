@@ -401,9 +401,12 @@ static int launch_append_lpr(AppendArgs& a, hipStream_t st) {
   if constexpr (Q8) {
     // (four passes at most, but for the longest blocks: with eight in one wave the instance held 200 registers, and a
     // prompt of 11400 tokens with 32 query heads, blocks of 64, took 85 us; 74 with four in each of two waves)
+    // Heads share a wave only where there are waves enough without (a chip holds some 2000 of these): 32 tokens of 4
+    // heads of 256 took 10.1 us with four heads to a wave, 5.5 with one.
+    const bool few = tiles * a.batch * 2 * a.NKV <= 2048;
     switch (a.tshift - rshift) {
-      case 0: return go(I1{}, I4{}, I1{}, N{});
-      case 1: return go(I2{}, I2{}, I1{}, N{});
+      case 0: return few ? go(I1{}, I1{}, I1{}, N{}) : go(I1{}, I4{}, I1{}, N{});
+      case 1: return few ? go(I2{}, I1{}, I1{}, N{}) : go(I2{}, I2{}, I1{}, N{});
       case 2: return go(I4{}, I1{}, I1{}, N{});
       case 3: return go(I4{}, I1{}, I2{}, N{});
       case 4: return go(I4{}, I1{}, I4{}, N{});
@@ -437,8 +440,10 @@ int fa::append_rows(const FableAppendParams& p, int dtype, hipStream_t st) {
   if (p.NKV <= 0 || (p.q && p.NH <= 0)) return fail(FA_ERR_ARG, "%s: NKV=%d NH=%d", what, p.NKV, p.NH);
   if (p.batch < 0 || p.n < 0 || p.max_blocks < 0) return fail(FA_ERR_ARG, "%s: batch=%d n=%d max_blocks=%d", what, p.batch, p.n, p.max_blocks);
   if (q8) {
-    const FableCache8 c{p.k_scale, p.v_scale, p.kc, p.vc, p.group, p.num_blocks};
-    if (int rc = cache8_check(what, c, p.HD, p.page)) return rc;
+    for (const fa_strides& s : {p.kc, p.vc}) {
+      const FableCache8 c{p.k_scale, p.v_scale, s, p.group, p.num_blocks, 0};
+      if (int rc = cache8_check(what, c, p.HD, p.page)) return rc;
+    }
   } else {
     if (p.HD <= 0 || p.HD > 256 || p.HD % 8) return fail(FA_ERR_HEADDIM, "%s: head_dim=%d has no kernel (multiples of 8 up to 256)", what, p.HD);
     if (p.page <= 0 || (p.page & (p.page - 1))) return fail(FA_ERR_ARG, "%s: page=%d is not a power of two", what, p.page);
@@ -545,8 +550,10 @@ extern "C" int fable_attn_gather(FableGatherParams p, int dtype, void* stream) {
   if (p.NKV <= 0 || p.batch < 0 || p.total < 0 || p.max_blocks < 0)
     return fail(FA_ERR_ARG, "%s: NKV=%d batch=%d total=%lld max_blocks=%d", what, p.NKV, p.batch, (long long)p.total, p.max_blocks);
   if (q8) {
-    const FableCache8 c{p.k_scale, p.v_scale, p.kc, p.vc, p.group, p.num_blocks};
-    if (int rc = cache8_check(what, c, p.HD, p.page)) return rc;
+    for (const fa_strides& s : {p.kc, p.vc}) {
+      const FableCache8 c{p.k_scale, p.v_scale, s, p.group, p.num_blocks, 0};
+      if (int rc = cache8_check(what, c, p.HD, p.page)) return rc;
+    }
   } else {
     if (p.HD <= 0 || p.HD > 256 || p.HD % 8) return fail(FA_ERR_HEADDIM, "%s: head_dim=%d has no kernel (multiples of 8 up to 256)", what, p.HD);
     if (p.page <= 0 || (p.page & (p.page - 1))) return fail(FA_ERR_ARG, "%s: page=%d is not a power of two", what, p.page);

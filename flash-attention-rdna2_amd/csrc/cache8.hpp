@@ -72,15 +72,13 @@ __device__ __forceinline__ int code_exponent(float amax) {
 
 // whether the caches and scales have a form the kernels take (0: they do)
 inline int cache8_check(const char* what, const FableCache8& c, int HD, int page) {
-  const fa_strides s[2] = {c.k, c.v};
   if (HD <= 0 || HD > 256 || HD % 16) return fail(FA_ERR_HEADDIM, "%s: head_dim=%d (8-bit caches take multiples of 16 up to 256)", what, HD);
   if (page < 16 || (page & (page - 1))) return fail(FA_ERR_ARG, "%s: page=%d (a power of two of at least 16)", what, page);
   if (c.group < 1 || c.group > 256 || c.group > page || (c.group & (c.group - 1)))
     return fail(FA_ERR_ARG, "%s: group=%d (a power of two, at most 256 and the page)", what, c.group);
   if (c.num_blocks < 1) return fail(FA_ERR_ARG, "%s: num_blocks=%d", what, c.num_blocks);
-  for (const fa_strides& x : s)
-    if (x.b < 0 || x.h < 0 || x.s < HD || x.s >= (1 << 26) || (x.b | x.h | x.s) % 16)
-      return fail(FA_ERR_ARG, "%s: cache strides %lld, %lld, %lld", what, (long long)x.b, (long long)x.h, (long long)x.s);
+  if (c.s.b < 0 || c.s.h < 0 || c.s.s < HD || c.s.s >= (1 << 26) || (c.s.b | c.s.h | c.s.s) % 16)
+    return fail(FA_ERR_ARG, "%s: cache strides %lld, %lld, %lld", what, (long long)c.s.b, (long long)c.s.h, (long long)c.s.s);
   return FA_OK;
 }
 

@@ -147,6 +147,20 @@ struct DecShare {
   static constexpr int kSegUnits = 6;
 };
 
+// the kernel's argument (of type A, whole) read again from the kernel argument segment
+template <class A>
+__device__ __forceinline__ A dec_reload() {
+  auto k = (const __attribute__((address_space(4))) uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(k));
+  struct {
+    uint64_t w[sizeof(A) / 8];
+  } raw;
+  static_assert(sizeof(raw) == sizeof(A), "whole words");
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(A) / 8); i++) raw.w[i] = k[i];
+  return __builtin_bit_cast(A, raw);
+}
+
 // floats ahead of the records: two ints per sequence, for the combine
 __host__ __device__ inline long long dec_meta_floats(const FableDecParams& p) { return (2ll * p.batch + 63) / 64 * 64; }
 

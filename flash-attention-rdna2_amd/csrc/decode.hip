@@ -55,18 +55,6 @@ struct DecArgs : FableDecParams {
   int tmask;
   int page_shift, ngrp, flags, parts, nkv;
 };
-__device__ __forceinline__ DecArgs dec_reload() {
-  auto k = (const __attribute__((address_space(4))) uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(k));
-  struct {
-    uint64_t w[sizeof(DecArgs) / 8];
-  } raw;
-  static_assert(sizeof(raw) == sizeof(DecArgs), "whole words");
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(DecArgs) / 8); i++) raw.w[i] = k[i];
-  return __builtin_bit_cast(DecArgs, raw);
-}
-
 // SPT (page >= 16): the block-table entries of a chunk are fetched by scalar loads. A chunk of
 // 16 keys touches at most two pages then, and each lane selects its row's entry from the two.
 // Per-lane table loads share the in-order vector-memory counter with the row loads, so a wave
@@ -114,14 +102,14 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
     return (long long)(b * nq + tok) * NH + kvh * gqa + (r0 + g - tok * gqa);
   };
   auto args = [&]() -> DecArgs {   // (the fixed grid's instances hold them)
-    if constexpr (SHARE) return dec_reload();
+    if constexpr (SHARE) return dec_reload<DecArgs>();
     return p;
   };
   // segments: a stream part's (sequence, run of keys), or the one split of the grid
   DecShare<kUnit> str;
   int at = 0, at_end = 0, sq = 0, first = 0;  // (units; sq: the sequence that holds `at`, first: its first)
   if constexpr (SHARE) {
-    const DecArgs p = dec_reload();
+    const DecArgs p = dec_reload<DecArgs>();
     str.init(p, append, p.parts, lane);
     const int part = blockIdx.y;
     if (str.even) {
@@ -157,7 +145,7 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
   float* rec = nullptr;  // record of row 0 (rows rec_step apart); null: the final output
   long long rec_step = HDr + 2;
   if constexpr (SHARE) {
-    const DecArgs p = dec_reload();
+    const DecArgs p = dec_reload<DecArgs>();
     if (b >= str.base + 64) str.load(p, append, b, lane);
     sp = str.span(b);
     const int units = dec_units<kUnit>(sp), stop = min(at_end, first + units);
@@ -199,7 +187,7 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
   // same bytes. Which calls come here: dec_fuses_append. Several tokens keep the kernel: written here
   // one after another they cost more.)
   if (append && ctx >= start && ctx < end) {
-    const DecArgs p = dec_reload();
+    const DecArgs p = dec_reload<DecArgs>();
     if (p.nk) {
       const int j = ctx >> page_shift, rdim = p.rotary ? (p.rotary_dim > 0 ? p.rotary_dim : HDr) : 0, half = rdim / 2;
       const int blk = p.block_table ? p.block_table[(long long)b * p.max_blocks + j] : b * p.max_blocks + j;

@@ -3,17 +3,23 @@
 // The split of the work, the records and the combine are the 16-bit decode's (decode.hip): one workgroup of
 // four waves per (K/V head, group of 16 rows, run of a sequence's keys), each wave with its own chunks and
 // online softmax, merged in LDS. What differs:
-//  * a chunk is 32 keys, so as many bytes are in flight per wave as there with 16;
+//  * a chunk is 32 keys, so as many bytes are in flight per wave as there with 16. A SIMD has one wave, whose
+//    instructions per chunk are what bounds it next to HBM, so the rest is about having few;
 //  * codes stay codes in LDS (half the LDS traffic) and become fp16/bf16 between the LDS read and the matrix
 //    instruction: K by 16-byte reads of a key's row, V by the transposing 8-bit reads (ds_read_b64_tr_b8: a lane
 //    gets one column of eight rows, the A operand of v_mfma_f32_16x16x32 as it is);
-//  * codes are converted without their scales, which are exact powers of two: a key's K scale multiplies its fp32
+//  * they are converted without their scales, which are exact powers of two: a key's K scale multiplies its fp32
 //    scores, its V scale the fp32 probability ahead of the rounding to 16 bits. The scales of a chunk come
 //    in one byte load per lane and reach the lanes that need them through LDS;
-//  * chunks are aligned to 32 keys, so each half of one lies in one page (of 16 rows at least): a buffer
-//    descriptor per half makes the lanes' offsets loop invariant and rows past the end zero.
+//  * chunks are aligned to 32 keys, so one lies in one page (two of 16 rows): a buffer descriptor for a
+//    page makes the lanes' offsets loop invariant and rows past the end zero;
+//  * the accumulators are rescaled only in chunks that raise a row's maximum, and only chunks that some row does not
+//    see in full are masked (scalar branches).
 // fp16: a scaled probability can leave fp16's range (and V's codes need no more than bf16 holds), so P goes
 // as two bf16 parts, high and low, into two products: 16 bits of it, as many as fp16's own rounding left.
+// Not taken: the products of e4m3 operands with e8m0 scales (v_mfma_scale_f32_16x16x128_f8f6f4), K as it is and q as
+// a sum of e4m3 parts. They need no conversion of K, but add their 128 products aligned to the largest: with one
+// dimension of q and k 30 times the others, scores of size 100 were off by up to 0.1.
 #include "cache8.hpp"
 #include "dec_common.hpp"
 #include "fwd_common.hpp"
@@ -27,7 +33,7 @@ constexpr int kDec8Append = 1, kDec8Final = 2;   // new keys were appended; one 
 struct Dec8Args : FableDecParams {
   FableCache8 c;
   const int* table;   // as DecArgs::table (decode.hip): the block table, or any readable address and tmask 0
-  int tmask, page_shift, gshift, ngrp, flags, parts, nkv;
+  int tmask, page_shift, gshift, ngrp, flags, parts, nkv, bshift;
 };
 
 __device__ __forceinline__ float lane16_max(float x) {
@@ -42,19 +48,27 @@ __device__ __forceinline__ float lane16_sum(float x) {
 template <int HD>
 struct Dec8Lds {
   // rows of codes padded by 16 bytes: the 16-byte K reads of 16 rows and the transposing V reads of 16 rows both
-  // touch every bank once
+  // touch every bank once. Scales: 32 of K, 32 of V, fp32.
   static constexpr int STR = HD + 16;
   static constexpr int WAVE = 2 * kKeys8 * STR + 64 * 4;   // K, V, scales
   static constexpr int ACC = kDecWaves * 16 * HD * 4;       // the merge's accumulators (q staging is smaller)
   static constexpr int BYTES = kDecWaves * WAVE > ACC ? kDecWaves * WAVE : ACC;
 };
 
-template <typename T, int HD, bool FEAT, bool SHARE>
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+// P16: pages of 16 rows (two to a chunk)
+template <typename T, int HD, bool FEAT, bool SHARE, bool P16>
 __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   using V8 = typename Dt<T>::V8;
   using L = Dec8Lds<HD>;
   constexpr bool kTwoP = std::is_same<T, _Float16>::value;   // P in two bf16 parts
-  constexpr int NDS = HD / 32, NDB = HD / 16, RB = HD / 16, NV = kKeys8 * RB / 64;
+  constexpr int NDB = HD / 16, RB = HD / 16, NV = kKeys8 * RB / 64, NDS = HD / 32;
+  constexpr int NPG = P16 ? 2 : 1;
+  // Chunks whose rows are in flight. One left a wave waiting for most of the memory latency (32000 keys of one sequence
+  // in 4 splits, D 128: 78 us, 66 with two; 16 x 32768 keys, D 64: 178 and 119; D 192 96 and 72 in 3 splits); rows of
+  // 256 bytes fill the same bytes with one, and two cost registers (8 x 4000 keys 23.4 and 25.4).
+  constexpr int DEPTH = HD <= 192 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) char raw[L::BYTES];
   __shared__ float red_m[kDecWaves][16], red_l[kDecWaves][16];
   float (*qsh)[HD] = (float (*)[HD])raw;
@@ -63,18 +77,31 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lg = lane >> 4, lh = lane & 15;
   const int NKV = p.nkv, HDr = p.HD, nq = p.nq, gqa = p.gqa, NH = p.NH;
-  const int X = gridDim.x, hgl = blockIdx.x, grp = p.ngrp > 1 ? hgl / NKV : 0, kvh = hgl - grp * NKV;
+  const int X = gridDim.x;
+  int hgl = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
+  if (p.bshift) {   // 2^bshift heads whose rows share 128-byte lines: one after another on one XCD (launch_dec8)
+    const unsigned l = (bz * gridDim.y + by) * X + hgl, k = l / 8, bundle = (k >> p.bshift) * 8 + l % 8, w = bundle / ((unsigned)X >> p.bshift);
+    hgl = (int)(((bundle - w * ((unsigned)X >> p.bshift)) << p.bshift) + (k & ((1u << p.bshift) - 1)));
+    bz = (int)(w / gridDim.y);
+    by = (int)w - bz * gridDim.y;
+  }
+  const int grp = p.ngrp > 1 ? hgl / NKV : 0, kvh = hgl - grp * NKV;
   const int r0 = 16 * grp, hg = min(16, nq * gqa - r0);  // rows of this group
   auto row_tok = [&](int g) { return nq > 1 ? (int)((unsigned)(r0 + g) / (unsigned)gqa) : 0; };
   auto row_of = [&](int b, int g) {
     const int tok = row_tok(g);
     return (long long)(b * nq + tok) * NH + kvh * gqa + (r0 + g - tok * gqa);
   };
+  auto args = [&]() -> Dec8Args {   // (as in decode.hip: the phases that only some workgroups run read it again)
+    if constexpr (SHARE) return dec_reload<Dec8Args>();
+    return p;
+  };
   DecShare<kUnit8, kKeys8> str;
   int at = 0, at_end = 0, sq = 0, first = 0;  // (units; sq: the sequence that holds `at`, first: its first)
   if constexpr (SHARE) {
+    const Dec8Args p = dec_reload<Dec8Args>();
     str.init(p, append, p.parts, lane);
-    const int part = blockIdx.y;
+    const int part = by;
     if (str.even) {
       sq = str.seek(p, append, part, lane, first);
       if (sq >= p.batch) return;
@@ -89,27 +116,31 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     }
   }
   for (bool more = true; more;) {
-    const int b = SHARE ? sq : (int)blockIdx.y;
+    const int b = SHARE ? sq : by;
     // q rows of this group, loaded while the lengths are on their way
     constexpr int RCH = HD / 8, NQI = (16 * RCH + 255) / 256;
     u32x4 qraw[NQI];
+    {
+      const Dec8Args p = args();
 #pragma unroll
-    for (int u = 0; u < NQI; u++) {
-      const int i = min(tid + 256 * u, 16 * RCH - 1), g = i / RCH, c = i % RCH;
-      qraw[u] = *(const u32x4*)((const T*)p.q + row_of(b, min(g, hg - 1)) * HDr + (8 * c < HDr ? 8 * c : 0));
+      for (int u = 0; u < NQI; u++) {
+        const int i = min(tid + 256 * u, 16 * RCH - 1), g = i / RCH, c = i % RCH;
+        qraw[u] = *(const u32x4*)((const T*)p.q + row_of(b, min(g, hg - 1)) * HDr + (8 * c < HDr ? 8 * c : 0));
+      }
     }
     DecSpan sp;
     int start, end;
     float* rec = nullptr;  // record of row 0 (rows rec_step apart); null: the final output
     long long rec_step = HDr + 2;
     if constexpr (SHARE) {
+      const Dec8Args p = dec_reload<Dec8Args>();
       if (b >= str.base + 64) str.load(p, append, b, lane);
       sp = str.span(b);
       const int units = dec_units<kUnit8>(sp), stop = min(at_end, first + units);
       start = sp.lo + (at - first) * kUnit8;
       end = min(sp.lo + (stop - first) * kUnit8, sp.hi);
       const bool begins = at == first;
-      const int part = blockIdx.y;
+      const int part = by;
       if (begins && hgl == 0 && tid == 0) {   // where the combine finds this sequence's records (decode.hip)
         const int n = str.even ? str.items(units) : (int)((unsigned)(first + units - 1) / (unsigned)str.per) - part + 1;
         ((int*)p.scratch)[2 * b] = 2 * part + (str.even ? 0 : 1);
@@ -127,10 +158,10 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
       const int n = max(sp.hi - sp.lo, 0);
       const int share = p.nsplit > 1 ? (int)((unsigned)(n + p.nsplit - 1) / (unsigned)p.nsplit) : n;
       const int chunk = (share + kKeys8 - 1) / kKeys8 * kKeys8;
-      start = sp.lo + (int)blockIdx.z * chunk;
+      start = sp.lo + bz * chunk;
       end = min(start + chunk, sp.hi);
       if (!(p.flags & kDec8Final)) {
-        rec = p.scratch + (long long)blockIdx.z * (HDr + 2);
+        rec = p.scratch + (long long)bz * (HDr + 2);
         rec_step = (long long)p.nsplit * (HDr + 2);   // rows are indexed as in q
       }
       more = false;
@@ -138,8 +169,22 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     const int ctx = sp.ctx;
     start = __builtin_amdgcn_readfirstlane(start);   // a multiple of 32
     end = __builtin_amdgcn_readfirstlane(end);
-    // the first key some row of the call sees: nothing ahead of it is read
-    const int klo = __builtin_amdgcn_readfirstlane(max(append ? max(min(dec_lo(p, b, ctx, 0), ctx), 0) : dec_lo(p, b, ctx, 0), start));
+    // the first key some row of the call sees: nothing ahead of it is read; and the keys that every row sees
+    int klo, slo, shi;
+    int rlo, rspan;   // this lane's row (lh)
+    const int tok = row_tok(min(lh, hg - 1)), qpos = ctx + tok;
+    float slope = 0.0f, c_log2;
+    {
+      const Dec8Args p = args();
+      const int lo0 = dec_lo(p, b, ctx, 0);
+      klo = __builtin_amdgcn_readfirstlane(max(append ? max(min(lo0, ctx), 0) : lo0, start));
+      slo = __builtin_amdgcn_readfirstlane(max(dec_lo(p, b, ctx, nq - 1), start));
+      shi = __builtin_amdgcn_readfirstlane(min(dec_hi(p, ctx, 0, append), end));
+      rlo = max(dec_lo(p, b, ctx, tok), start);
+      rspan = max(min(dec_hi(p, ctx, tok, append), end) - rlo, 0);
+      if (FEAT && p.alibi && lh < hg) slope = p.alibi[kvh * gqa + (r0 + lh - tok * gqa)];
+      c_log2 = p.scale * kLog2e;
+    }
 
     // ---- q rows -> LDS (fp32), rotated; zero columns past the head dim
 #pragma unroll
@@ -152,18 +197,23 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
         for (int e = 0; e < 8; e++) qsh[g][8 * c + e] = g < hg && cok ? (float)v[e] : 0.0f;
     }
     __syncthreads();
-    if (p.rotary) {
-      const int rdim = p.rotary_dim > 0 ? p.rotary_dim : HDr, half = rdim / 2;
-      const int rbase = p.rotary_pos ? p.rotary_pos[b] : ctx;
-      for (int i = tid; i < hg * half; i += 256) {
-        const int g = i / half, j = i % half, rp = min(max(rbase + row_tok(g), 0), p.c.rotary_rows - 1);
-        const float c = p.cos[(long long)rp * half + j], s = p.sin[(long long)rp * half + j];
-        const int ia = p.rotary == 1 ? j : 2 * j, ib = p.rotary == 1 ? j + half : 2 * j + 1;
-        const float x = qsh[g][ia], y = qsh[g][ib];
-        qsh[g][ia] = x * c - y * s;
-        qsh[g][ib] = y * c + x * s;
+    bool qsplit;
+    {
+      const Dec8Args p = args();
+      qsplit = p.rotary != 0;
+      if (p.rotary) {
+        const int rdim = p.rotary_dim > 0 ? p.rotary_dim : HDr, half = rdim / 2;
+        const int rbase = p.rotary_pos ? p.rotary_pos[b] : ctx;
+        for (int i = tid; i < hg * half; i += 256) {
+          const int g = i / half, j = i % half, rp = min(max(rbase + row_tok(g), 0), p.c.rotary_rows - 1);
+          const float c = p.cos[(long long)rp * half + j], s = p.sin[(long long)rp * half + j];
+          const int ia = p.rotary == 1 ? j : 2 * j, ib = p.rotary == 1 ? j + half : 2 * j + 1;
+          const float x = qsh[g][ia], y = qsh[g][ib];
+          qsh[g][ia] = x * c - y * s;
+          qsh[g][ib] = y * c + x * s;
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
     // Q^T as the B operand: a 16-byte read of a K row holds dims 64m + 16lg .. +15 and feeds steps 2m and 2m + 1,
     // so step 2m + s takes dims 64m + 16lg + 8s + e. A rotated q is carried as hi + lo.
@@ -183,16 +233,13 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
 #pragma unroll
     for (int db = 0; db < NDB; db++) oacc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.0f;
-    const float c_log2 = p.scale * kLog2e;
-    const int tok = row_tok(min(lh, hg - 1)), qpos = ctx + tok;  // this lane's row (lh)
-    const int rlo = max(dec_lo(p, b, ctx, tok), start), rspan = max(min(dec_hi(p, ctx, tok, append), end) - rlo, 0);
-    const float slope = (FEAT && p.alibi && lh < hg) ? p.alibi[kvh * gqa + (r0 + lh - tok * gqa)] : 0.0f;
-    const cint_ptr bt = cmem(p.table) + (long long)b * (p.max_blocks & p.tmask);
-    const int blk0 = b * p.max_blocks, pmask = p.page - 1, subs = 1 << (page_shift - p.gshift);
-    const int krow = (int)p.c.k.s, vrow = (int)p.c.v.s;
-    const uint8_t* Kc = (const uint8_t*)p.Kc + (long long)kvh * p.c.k.h;
-    const uint8_t* Vc = (const uint8_t*)p.Vc + (long long)kvh * p.c.v.h;
+    const int* bt = p.table + (long long)b * (p.max_blocks & p.tmask);
+    const int blk0 = b * p.max_blocks, tmask = p.tmask, pmask = p.page - 1, subs = 1 << (page_shift - p.gshift);
+    const unsigned rstep = (unsigned)p.c.s.s, pstep = (unsigned)p.c.s.b, top_blk = (unsigned)p.c.num_blocks - 1;
+    const uint8_t* Kc = (const uint8_t*)p.Kc + (long long)kvh * p.c.s.h;
+    const uint8_t* Vc = (const uint8_t*)p.Vc + (long long)kvh * p.c.s.h;
     const uint8_t* scales = (lane < 32 ? p.c.k_scale : p.c.v_scale) + (long long)kvh * subs;
+    const unsigned sstep = (unsigned)NKV * (unsigned)subs;   // scales of a page
     uint8_t* kb = (uint8_t*)raw + wave * L::WAVE;
     uint8_t* vb = kb + kKeys8 * L::STR;
     float* sb = (float*)(vb + kKeys8 * L::STR);
@@ -201,146 +248,184 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     // lanes on whole rows. K's rows go to the slots that make them the rows of the two S products with eight
     // consecutive keys per lane: row 8a + 4h + r to slot 16h + 4a + r.
     const int last = end - 1;
-    int koff[NV], voff[NV], lk[NV], lv[NV];
+    int off[NV], lk[NV], lv[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int f = 64 * i + lane, row = f / RB, ch = f % RB;
-      const bool cok = 16 * ch < HDr;
-      koff[i] = cok ? (row & 15) * krow + 16 * ch : kBufZero;
-      voff[i] = cok ? (row & 15) * vrow + 16 * ch : kBufZero;
+      off[i] = 16 * ch < HDr ? (P16 ? row & 15 : row) * (int)rstep + 16 * ch : kBufZero;
       lk[i] = (16 * ((row >> 2) & 1) + 4 * (row >> 3) + (row & 3)) * L::STR + 16 * ch;
       lv[i] = row * L::STR + 16 * ch;
     }
-    // pages of the two halves of a chunk, one chunk ahead (raw entries; made pages where the rows are loaded)
-    int ent[2], eidx[2];
-    auto table = [&](int kc0) {
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        eidx[h] = min(max(kc0 + 16 * h, klo), last) >> page_shift;
-        ent[h] = bt[eidx[h] & p.tmask];
-      }
+    // Pages of the wave's chunks, 64 at a time: lane l of `page` has those of chunk c (c % 64 = l), which reach the scalar
+    // unit by a readlane; the next 64 are fetched meanwhile. (By scalar loads, one chunk ahead, an entry
+    // held up the LDS reads it shares a counter with.)
+    const int kfirst = start + kKeys8 * wave;
+    int page[NPG], next[NPG];   // (next: the entries as read)
+    auto index = [&](int c0, int h) {   // lane's page of its sequence, among those with keys of it
+      const unsigned key = (unsigned)kfirst + min((unsigned)(c0 + lane) * kUnit8, (unsigned)end) + 16u * h;
+      return (int)min(max(key, (unsigned)klo), (unsigned)last) >> page_shift;
     };
-    u32x4 kreg[NV], vreg[NV];
-    unsigned sreg = 0;
-    auto load = [&](int kc0, bool front) {
-      __amdgpu_buffer_rsrc_t kr[2], vr[2];
-      unsigned blk[2];
+    auto fetch = [&](int c0) {
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int raw_e = (ent[h] & p.tmask) | ((blk0 + eidx[h]) & ~p.tmask);
-        blk[h] = __builtin_amdgcn_readfirstlane((int)min((unsigned)raw_e, (unsigned)p.c.num_blocks - 1));
-        const int k0 = kc0 + 16 * h, rows = __builtin_amdgcn_readfirstlane(max(min(end - k0, 16), 0)), in = k0 & pmask;
-        kr[h] = buf_rsrc32(Kc + (long long)blk[h] * p.c.k.b + (long long)in * krow, (unsigned)(rows * krow));
-        vr[h] = buf_rsrc32(Vc + (long long)blk[h] * p.c.v.b + (long long)in * vrow, (unsigned)(rows * vrow));
+      for (int h = 0; h < NPG; h++) next[h] = bt[index(c0, h) & tmask];
+    };
+    auto take = [&](int c0) {
+#pragma unroll
+      for (int h = 0; h < NPG; h++) page[h] = (int)min((unsigned)((next[h] & tmask) | ((blk0 + index(c0, h)) & ~tmask)), top_blk);
+    };
+    struct Rows {
+      u32x4 k[NV], v[NV];
+      unsigned s;
+    };
+    Rows set[DEPTH];
+    // (chunks past the end load nothing: their descriptors have no bytes. No condition around the loads, which would
+    // have every wait be for all of them.)
+    auto load = [&](int kc0, int c, bool front, Rows& r) {
+      __amdgpu_buffer_rsrc_t kr[NPG], vr[NPG];
+      unsigned blk[NPG];
+#pragma unroll
+      for (int h = 0; h < NPG; h++) {
+        blk[h] = (unsigned)__builtin_amdgcn_readlane(page[h], c & 63);
+        const int k0 = kc0 + 16 * h;
+        const unsigned bytes = (unsigned)max(min(end - k0, 32 / NPG), 0) * rstep;
+        const uint64_t o = (uint64_t)blk[h] * pstep + (unsigned)(k0 & pmask) * rstep;
+        kr[h] = buf_rsrc32(Kc + o, (unsigned)__builtin_amdgcn_readfirstlane((int)bytes));
+        vr[h] = buf_rsrc32(Vc + o, (unsigned)__builtin_amdgcn_readfirstlane((int)bytes));
       }
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const int f = 64 * i + lane, row = f / RB;
+        const int f = 64 * i + lane;
         // (rows ahead of klo in a run's first chunk: zeros too)
-        const bool hide = front && kc0 + row < klo;
-        const int ko = hide ? kBufZero : koff[i], vo = hide ? kBufZero : voff[i];
-        constexpr int kLo = 16 * RB;   // chunks of the first half
-        if (64 * i + 63 < kLo) {
-          kreg[i] = buf_load16_nt(kr[0], ko);
-          vreg[i] = buf_load16_nt(vr[0], vo);
+        const int o = front && kc0 + f / RB < klo ? kBufZero : off[i];
+        constexpr int kLo = 16 * RB;   // chunks of the first page
+        if (!P16 || 64 * i + 63 < kLo) {
+          r.k[i] = buf_load16_nt(kr[0], o);
+          r.v[i] = buf_load16_nt(vr[0], o);
         } else if (64 * i >= kLo) {
-          kreg[i] = buf_load16_nt(kr[1], ko);
-          vreg[i] = buf_load16_nt(vr[1], vo);
-        } else {   // rows of both halves (head dims over 64 with an odd chunk count): each lane from its own
-          const u32x4 ka = buf_load16_nt(kr[0], f < kLo ? ko : kBufZero), kc = buf_load16_nt(kr[1], f < kLo ? kBufZero : ko);
-          const u32x4 va = buf_load16_nt(vr[0], f < kLo ? vo : kBufZero), vc = buf_load16_nt(vr[1], f < kLo ? kBufZero : vo);
-          kreg[i] = ka | kc;
-          vreg[i] = va | vc;
+          r.k[i] = buf_load16_nt(kr[NPG - 1], o);
+          r.v[i] = buf_load16_nt(vr[NPG - 1], o);
+        } else {   // rows of both pages (width 192): each lane from its own
+          const int o0 = f < kLo ? o : kBufZero, o1 = f < kLo ? kBufZero : o;
+          r.k[i] = buf_load16_nt(kr[0], o0) | buf_load16_nt(kr[NPG - 1], o1);
+          r.v[i] = buf_load16_nt(vr[0], o0) | buf_load16_nt(vr[NPG - 1], o1);
         }
       }
       // scale of key kc0 + (lane & 31): K's for the first 32 lanes, V's for the others
-      const int key = kc0 + (lane & 31);
-      const unsigned pg = (lane & 16) ? blk[1] : blk[0];
-      sreg = scales[(long long)pg * NKV * subs + ((key & pmask) >> p.gshift)];
+      const unsigned pg = P16 && (lane & 16) ? blk[NPG - 1] : blk[0];
+      r.s = scales[(uint64_t)pg * sstep + (unsigned)(((kc0 + (lane & 31)) & pmask) >> p.gshift)];
     };
 
-    const int kfirst = start + kKeys8 * wave;
-    if (kfirst < end) {
-      table(kfirst);
-      load(kfirst, true);
-      table(kfirst + kUnit8);
-    }
-    for (int kc0 = kfirst; kc0 < end; kc0 += kUnit8) {
+    // chunk c at key kc0: its rows from r to LDS, and the loads of the rows DEPTH chunks on to r
+    auto stage = [&](int kc0, int c, Rows& r) {
       // codes and scales -> this wave's own LDS (its operations complete in order: no barrier). A scale of a key
       // that is not there is no number to multiply zeros by.
       const int skey = kc0 + (lane & 31);
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        *(u32x4*)(kb + lk[i]) = kreg[i];
-        *(u32x4*)(vb + lv[i]) = vreg[i];
+        *(u32x4*)(kb + lk[i]) = r.k[i];
+        *(u32x4*)(vb + lv[i]) = r.v[i];
       }
-      sb[lane] = skey >= klo && skey < end ? e8_f32(sreg) : 0.0f;
-      if (kc0 + kUnit8 < end) {   // the next chunk's rows are in flight during this chunk's products
-        load(kc0 + kUnit8, false);
-        table(kc0 + 2 * kUnit8);
+      sb[lane] = skey >= klo && skey < end ? e8_f32(r.s) : 0.0f;
+      if (((c + DEPTH) & 63) == 0) {
+        take(c + DEPTH);
+        fetch(c + DEPTH + 64);
       }
+      load(kc0 + DEPTH * kUnit8, c + DEPTH, false, r);
+    };
+    auto chunk = [&](int kc0) {
       // S^T = K . Q^T of the keys in slots 0..15 and 16..31: lane (lg, lh) gets keys kc0 + 8lg + 4h + r of row lh
       f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      V8 ka[2][NDS];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int m = 0; m < NDS / 2; m++)
 #pragma unroll
-        for (int m = 0; m < NDS / 2; m++) {
+        for (int h = 0; h < 2; h++) {
           const u32x4 c = *(const u32x4*)(kb + (16 * h + lh) * L::STR + 64 * m + 16 * lg);
-          const V8 a0 = codes_to<T>(u32x2{c[0], c[1]}, 1.0f), a1 = codes_to<T>(u32x2{c[2], c[3]}, 1.0f);
-          s[h] = Dt<T>::mma16(a0, qb[2 * m], s[h]);
-          s[h] = Dt<T>::mma16(a1, qb[2 * m + 1], s[h]);
-          if (p.rotary) {
-            s[h] = Dt<T>::mma16(a0, ql[2 * m], s[h]);
-            s[h] = Dt<T>::mma16(a1, ql[2 * m + 1], s[h]);
-          }
+          ka[h][2 * m] = codes_to<T>(u32x2{c[0], c[1]}, 1.0f);
+          ka[h][2 * m + 1] = codes_to<T>(u32x2{c[2], c[3]}, 1.0f);
         }
+#pragma unroll
+      for (int d = 0; d < NDS; d++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) s[h] = Dt<T>::mma16(ka[h][d], qb[d], s[h]);
+      if (qsplit) {
+#pragma unroll
+        for (int d = 0; d < NDS; d++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) s[h] = Dt<T>::mma16(ka[h][d], ql[d], s[h]);
       }
       // logits (log2 domain) and masking
+      const f32x4 ks0 = *(const f32x4*)(sb + 8 * lg), ks1 = *(const f32x4*)(sb + 8 * lg + 4);
       float t[8], mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const int key = kc0 + 8 * lg + e;
-        const float ks = sb[8 * lg + e];
-        float x = s[e >> 2][e & 3];
+        float x = s[e >> 2][e & 3] * (e < 4 ? ks0[e & 3] : ks1[e & 3]);
         if (FEAT) {
-          x = x * ks * p.scale;
+          x = x * p.scale;
           if (p.softcap > 0.0f) x = p.softcap * tanh_exp(x / p.softcap);
-          x += slope * (float)(key - qpos);
-          x *= kLog2e;
+          x += slope * (float)(kc0 + 8 * lg + e - qpos);
+          t[e] = x * kLog2e;
         } else {
-          x = x * ks * c_log2;
+          t[e] = x * c_log2;
         }
-        t[e] = (unsigned)(key - rlo) < (unsigned)rspan ? x : -INFINITY;
-        mx = fmaxf(mx, t[e]);
       }
+      if (kc0 < slo || kc0 + kKeys8 > shi) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) t[e] = (unsigned)(kc0 + 8 * lg + e - rlo) < (unsigned)rspan ? t[e] : -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) mx = fmaxf(mx, t[e]);
       mx = half_max(lane16_max(mx));
       const float m_new = fmaxf(m_run, mx);
       const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-      const float corr = exp2_fast(m_run - m_use);
+      if (__builtin_amdgcn_readfirstlane((int)(__builtin_amdgcn_ballot_w64(m_new > m_run) != 0))) {
+        const float corr = exp2_fast(m_run - m_use);
+        l_run *= corr;
+#pragma unroll
+        for (int db = 0; db < NDB; db++) oacc[db] *= corr;
+        m_run = m_new;
+      }
       float rs = 0.0f;
       bf16x8 pb, pl;     // P^T times V's scales, the B operand: keys 8lg + e, row lh
+      const f32x4 vs0 = *(const f32x4*)(sb + 32 + 8 * lg), vs1 = *(const f32x4*)(sb + 36 + 8 * lg);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float w = exp2_fast(t[e] - m_use), z = w * sb[32 + 8 * lg + e];
+        const float w = exp2_fast(t[e] - m_use), z = w * (e < 4 ? vs0[e & 3] : vs1[e & 3]);
         rs += w;
         pb[e] = (__bf16)z;
         if constexpr (kTwoP) pl[e] = (__bf16)(z - (float)pb[e]);
       }
-      l_run = l_run * corr + rs;
-      m_run = m_new;
-#pragma unroll
-      for (int db = 0; db < NDB; db++) oacc[db] *= corr;
+      l_run += rs;
       // O^T += V^T . P^T: lane lh of group lg addresses row 8lg + lh/2, column 16db + 8(lh%2), and receives
       // column 16db + lh of rows 8lg .. 8lg+7
 #pragma unroll
       for (int db = 0; db < NDB; db++) {
-        typedef int i32x2 __attribute__((ext_vector_type(2)));
         const uint8_t* a = vb + (8 * lg + (lh >> 1)) * L::STR + 16 * db + 8 * (lh & 1);
         const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (__attribute__((address_space(3))) i32x2*)((__attribute__((address_space(3))) uint8_t*)a));
         const bf16x8 av = codes_to<__bf16>(u32x2{(unsigned)c[0], (unsigned)c[1]}, 1.0f);
         oacc[db] = Dt<__bf16>::mma16(av, pb, oacc[db]);
         if constexpr (kTwoP) oacc[db] = Dt<__bf16>::mma16(av, pl, oacc[db]);
+      }
+    };
+    if (kfirst < end) {
+      fetch(0);
+      take(0);
+      fetch(64);
+#pragma unroll
+      for (int d = 0; d < DEPTH; d++) {
+        load(kfirst + d * kUnit8, d, d == 0, set[d]);
+        // (in this order: the loop's waits count the loads behind the ones they need, whichever way it was entered)
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // (no way out in the middle: with one, the compiler's waits at the top of the loop are for every load)
+      for (int kc0 = kfirst, c = 0; kc0 < end; kc0 += DEPTH * kUnit8, c += DEPTH) {
+        stage(kc0, c, set[0]);
+        chunk(kc0);
+        if constexpr (DEPTH == 2) {
+          stage(kc0 + kUnit8, c + 1, set[1]);
+          if (kc0 + kUnit8 < end) chunk(kc0 + kUnit8);
+        }
       }
     }
 
@@ -355,6 +440,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
 #pragma unroll
     for (int db = 0; db < NDB; db++) *(f32x4*)(red_o + (wave * 16 + lh) * HD + 16 * db + 4 * lg) = oacc[db];
     __syncthreads();
+    const Dec8Args pe = args();
     for (int i = tid; i < hg * HDr; i += 256) {
       const int g = i / HDr, d = i % HDr;
       float gm = -INFINITY;
@@ -372,8 +458,8 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
       const long long row = row_of(b, g);
       if (!rec) {
         const bool ok = gm != -INFINITY && l > 0.0f;
-        ((T*)p.o)[row * HDr + d] = (T)(ok ? acc / l : 0.0f);
-        if (p.lse_out && d == 0) p.lse_out[row] = ok ? gm * kLn2 + __logf(l) : -INFINITY;
+        ((T*)pe.o)[row * HDr + d] = (T)(ok ? acc / l : 0.0f);
+        if (pe.lse_out && d == 0) pe.lse_out[row] = ok ? gm * kLn2 + __logf(l) : -INFINITY;
         continue;
       }
       float* out = rec + (SHARE ? g : row) * rec_step;
@@ -403,8 +489,17 @@ static int launch_dec8(const FableDecParams& p, const FableCache8& c, int parts,
   const bool feat = p.softcap > 0.0f || p.alibi != nullptr;
   const unsigned X = (unsigned)(a.nkv * a.ngrp);
   const dim3 grid = parts > 0 ? dim3(X, (unsigned)dec_share_wgs(p, kUnit8)) : dim3(X, (unsigned)p.batch, (unsigned)p.nsplit);
+  // Heads whose rows share 128-byte lines (D 64: two, D 96: four) run one after another on one XCD, whose L2 then
+  // fetches a line once: dealt out like the others, every XCD fetched them for itself (16 x 32768 keys of 8 heads,
+  // D 64: 171 -> 118 us; D 192, 1.1x; at 128 and 256 nothing is shared, and the order measured the same).
+  a.bshift = 0;
+  while ((p.HD << a.bshift) % 128 && a.bshift < 3) a.bshift++;
+  if (a.nkv % (1 << a.bshift) || ((long long)grid.x * grid.y * grid.z >> a.bshift) % 8) a.bshift = 0;
   auto go = [&](auto ft, auto sh) {
-    hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value>), grid, dim3(256), 0, st, a);
+    if (p.page == 16)
+      hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value, true>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value, false>), grid, dim3(256), 0, st, a);
   };
   using Y = std::integral_constant<bool, true>;
   using N = std::integral_constant<bool, false>;
@@ -428,7 +523,7 @@ static int dec8_dispatch(const FableDecParams& p, const FableCache8& c, int part
 // where there are more than kTileStreams (sequence, K/V head, 16 rows): the rule of the 16-bit decode.
 constexpr int kTileRows8 = 64, kTileStreams8 = 16;
 static bool dec8_uses_tiles(const FableDecParams& p, const FableCache8& c) {
-  return c.k.b <= 0x7FFFFFFF && c.v.b <= 0x7FFFFFFF && (long long)p.batch * (p.NH / p.gqa) * dec_groups(p) > kTileStreams8 && (long long)p.nq * p.gqa >= kTileRows8 &&
+  return c.s.b <= 0x7FFFFFFF && (long long)p.batch * (p.NH / p.gqa) * dec_groups(p) > kTileStreams8 && (long long)p.nq * p.gqa >= kTileRows8 &&
          (long long)p.batch * p.max_blocks <= 0x7FFFFFFF && p.max_blocks < (1 << 29) && p.window != 0;
 }
 // Shares worked out on the device for batches that equal splits would not spread evenly, as in decode.hip
@@ -456,8 +551,8 @@ static void dec8_tile_params(const FableDecParams& p, const FableCache8& c, bool
   f.O = p.o;
   f.LSE = p.lse_out;
   f.sQ = f.sO = fa_strides{p.nq * p.NH * D, D, p.NH * D};
-  f.sK = fa_strides{0, c.k.h, c.k.s};
-  f.sV = fa_strides{0, c.v.h, c.v.s};
+  f.sK = fa_strides{0, c.s.h, c.s.s};
+  f.sV = fa_strides{0, c.s.h, c.s.s};
   f.SQ = p.nq;
   const long long room = (long long)p.max_blocks * p.page;
   f.SK = room < 0x7FFFFFFF ? (int)room : 0x7FFFFFFF;
@@ -474,7 +569,7 @@ static void dec8_tile_params(const FableDecParams& p, const FableCache8& c, bool
   f.lse_sb = (int64_t)p.nq * p.NH;
   f.lse_sh = 1;
   (FwdPaged&)pg = FwdPaged{p.block_table ? p.block_table : p.ctx_len, p.block_table ? -1 : 0, p.max_blocks,
-                           __builtin_ctz((unsigned)p.page), c.k.b, c.v.b, p.ctx_len, append ? 1 : 0, p.leftpad, nullptr, p.NH};
+                           __builtin_ctz((unsigned)p.page), c.s.b, c.s.b, p.ctx_len, append ? 1 : 0, p.leftpad, nullptr, p.NH};
   fwd_paged8_scales(pg, c, p.page);
 }
 
@@ -485,11 +580,12 @@ static int dec8_check(FableDecParams& p, const FableCache8& c, int dtype) {
   if (p.NH <= 0 || p.gqa <= 0 || p.NH % p.gqa) return fail(FA_ERR_ARG, "%s: NH=%d gqa=%d", what, p.NH, p.gqa);
   if (p.nq < 1) p.nq = 1;
   if (p.nsplit < 0 || p.nsplit > 512) return fail(FA_ERR_ARG, "%s: nsplit=%d", what, p.nsplit);
-  if (p.max_blocks < 1 || (long long)p.max_blocks * p.page > 0x7FFFFFFF)
+  if (p.max_blocks < 1 || (long long)p.max_blocks * p.page > 0x7FFF0000)
     return fail(FA_ERR_ARG, "%s: max_blocks=%d page=%d", what, p.max_blocks, p.page);
   if (p.batch > 65535 || (long long)p.nq * p.gqa > (1 << 24)) return fail(FA_ERR_ARG, "%s: batch=%d nq=%d", what, p.batch, p.nq);
   if (p.rotary && (p.rotary_dim < 0 || p.rotary_dim > p.HD || p.rotary_dim % 2)) return fail(FA_ERR_ARG, "%s: rotary_dim=%d", what, p.rotary_dim);
   if (p.rotary && (p.rotary > 2 || c.rotary_rows < 1)) return fail(FA_ERR_ARG, "%s: rotary=%d rotary_rows=%d", what, p.rotary, c.rotary_rows);
+  if (c.s.b > 0xFFFFFFFFll) return fail(FA_ERR_ARG, "%s: pages of 4 GiB", what);
   return cache8_check(what, c, p.HD, p.page);
 }
 
@@ -544,8 +640,7 @@ extern "C" int fable_attn_dec8(FableDecParams p, FableCache8 c, int dtype, void*
     a.Vc = const_cast<void*>(p.Vc);
     a.k_scale = const_cast<uint8_t*>(c.k_scale);
     a.v_scale = const_cast<uint8_t*>(c.v_scale);
-    a.kc = c.k;
-    a.vc = c.v;
+    a.kc = a.vc = c.s;
     a.block_table = p.block_table;
     a.ctx_len = p.ctx_len;
     a.leftpad = p.leftpad;

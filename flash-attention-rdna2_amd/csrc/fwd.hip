@@ -243,14 +243,14 @@ static int paged8_run(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtyp
   if (dtype != FA_F16 && dtype != FA_BF16) return fail(FA_ERR_DTYPE, "%s: dtype %d not implemented (fp16/bf16)", what, dtype);
   if (p.dropout_p > 0.0f) return fail(FA_ERR_ARG, "%s: no dropout over a cache", what);
   if (int rc = cache8_check(what, c, p.HD, kv.page)) return rc;
-  if (c.k.b > 0x7FFFFFFF || c.v.b > 0x7FFFFFFF) return fail(FA_ERR_ARG, "%s: pages of 2 GiB", what);
+  if (c.s.b > 0x7FFFFFFF) return fail(FA_ERR_ARG, "%s: pages of 2 GiB", what);
   p.SK = (int)room;
-  p.sK = fa_strides{0, c.k.h, c.k.s};
-  p.sV = fa_strides{0, c.v.h, c.v.s};
+  p.sK = fa_strides{0, c.s.h, c.s.s};
+  p.sV = fa_strides{0, c.s.h, c.s.s};
   int rc;
   if (fwd_check(p, dtype, ws.query, rc)) return rc;
   FwdPaged8 pg;
-  (FwdPaged&)pg = FwdPaged{kv.block_table, -1, kv.max_blocks, __builtin_ctz((unsigned)kv.page), c.k.b, c.v.b, nullptr, 0, nullptr, nullptr, 1};
+  (FwdPaged&)pg = FwdPaged{kv.block_table, -1, kv.max_blocks, __builtin_ctz((unsigned)kv.page), c.s.b, c.s.b, nullptr, 0, nullptr, nullptr, 1};
   fwd_paged8_scales(pg, c, kv.page);
   return launch_fwd_paged8(p, pg, dtype, false, st, ws);
 }

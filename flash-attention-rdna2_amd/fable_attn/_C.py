@@ -504,7 +504,8 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev):
 
 def _cache8(k_cache, v_cache, k_scale, v_scale, dtype, dev, rotary_rows=0):
     ks, vs, group = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev)
-    return _lib.FableCache8(k_scale.data_ptr(), v_scale.data_ptr(), ks, vs, group, k_cache.shape[0], rotary_rows)
+    _req(k_cache.stride() == v_cache.stride(), "8-bit k_cache and v_cache must have the same strides")
+    return _lib.FableCache8(k_scale.data_ptr(), v_scale.data_ptr(), ks, group, k_cache.shape[0], rotary_rows)
 
 
 def _check_table(block_table, batch, dev):

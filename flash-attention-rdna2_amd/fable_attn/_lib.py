@@ -77,7 +77,7 @@ class FablePagedKV(ctypes.Structure):
 
 
 class FableCache8(ctypes.Structure):
-    _fields_ = [("k_scale", c_ptr), ("v_scale", c_ptr), ("k", Strides), ("v", Strides),
+    _fields_ = [("k_scale", c_ptr), ("v_scale", c_ptr), ("s", Strides),
                 ("group", c_i32), ("num_blocks", c_i32), ("rotary_rows", c_i32)]
 
 

@@ -1060,7 +1060,6 @@ def _rows_of_cache(k_cache, block_table, cache_batch_idx, dev):
     return _as_index(cache_batch_idx, dev).view(-1, 1) if cache_batch_idx is not None else None
 
 
-@torch.no_grad()
 def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, cu_seqlens=None, max_seqlen=None,
                               block_table=None, cache_batch_idx=None, cache_leftpad=None, rotary_cos=None,
                               rotary_sin=None, rotary_interleaved=True, rotary_seqlens=None, k_scale=None, v_scale=None):
@@ -1094,6 +1093,14 @@ def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, 
                            rotary_seqlens, k_scale, v_scale)
         if got is not None:
             return got[0]
+    return _append_general(key, plans, k, v, k_cache, v_cache, cache_seqlens, q, cu_seqlens, max_seqlen, block_table, cache_batch_idx,
+                           cache_leftpad, rotary_cos, rotary_sin, rotary_interleaved, rotary_seqlens, k_scale, v_scale)
+
+
+@torch.no_grad()
+def _append_general(key, plans, k, v, k_cache, v_cache, cache_seqlens, q, cu_seqlens, max_seqlen, block_table, cache_batch_idx,
+                    cache_leftpad, rotary_cos, rotary_sin, rotary_interleaved, rotary_seqlens, k_scale, v_scale):
+    """flash_attn_append_kvcache with all checks and conversions; remembers the launch where nothing was converted."""
     if not k.is_cuda:
         raise ValueError("fable_attn: tensors must be on the GPU (k.is_cuda == False)")
     if k.dtype not in _DTYPES:
@@ -1122,7 +1129,6 @@ def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, 
     return q_out
 
 
-@torch.no_grad()
 def flash_attn_gather_kvcache(k_cache, v_cache, cu_seqlens_k, total_k, *, block_table=None, cache_batch_idx=None,
                               k_scale=None, v_scale=None, dtype=None):
     """The first cu_seqlens_k[b+1] - cu_seqlens_k[b] cached rows of every sequence as packed (k, v), (total_k, nheads_k,
@@ -1139,6 +1145,12 @@ def flash_attn_gather_kvcache(k_cache, v_cache, cu_seqlens_k, total_k, *, block_
         got = _gather_fast(plan, k_cache, v_cache, cu_seqlens_k, int(total_k), block_table, k_scale, v_scale)
         if got is not None:
             return got
+    return _gather_general(key, plans, k_cache, v_cache, cu_seqlens_k, total_k, block_table, cache_batch_idx, k_scale, v_scale, dtype)
+
+
+@torch.no_grad()
+def _gather_general(key, plans, k_cache, v_cache, cu_seqlens_k, total_k, block_table, cache_batch_idx, k_scale, v_scale, dtype):
+    """flash_attn_gather_kvcache with all checks; remembers the launch where nothing was converted."""
     if not k_cache.is_cuda:
         raise ValueError("fable_attn: tensors must be on the GPU (k_cache.is_cuda == False)")
     if k_cache.dim() != 4:

@@ -372,7 +372,7 @@ int64_t fable_attn_dec_noalloc_max_floats(void);
 typedef struct FableCache8 {
   const uint8_t* k_scale;
   const uint8_t* v_scale;
-  fa_strides k, v;
+  fa_strides s;          /* of both caches */
   int32_t group, num_blocks;
   int32_t rotary_rows;   /* decode: rows of the rotary tables (positions past them use the last row) */
 } FableCache8;
@@ -385,7 +385,7 @@ int64_t fable_attn_dec8_ws_bytes(FableDecParams p, FableCache8 c, int dtype, int
 int fable_attn_dec8(FableDecParams p, FableCache8 c, int dtype, void* ws, int64_t ws_bytes, void* stream, const void* new_k,
                     const void* new_v);
 
-/* fable_attn_fwd_paged over an 8-bit cache: p.K / p.V are the codes, c.k / c.v their strides (p.sK, p.sV and
+/* fable_attn_fwd_paged over an 8-bit cache: p.K / p.V are the codes, c.s their strides (p.sK, p.sV and
  * the page strides of kv are ignored). Head dims up to 256 in kernels of width 64, 128 and 256. */
 int64_t fable_attn_fwd_paged8_ws_bytes(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype);
 int fable_attn_fwd_paged8(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtype, void* ws, int64_t ws_bytes,

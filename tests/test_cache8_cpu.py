@@ -48,7 +48,7 @@ def _lib():
 
 def _cache(**kw):
     L, _ = _lib()
-    c = L.FableCache8(16, 16, L.Strides(16 * 128, 64, 128), L.Strides(16 * 128, 64, 128), 16, 4, 0)
+    c = L.FableCache8(16, 16, L.Strides(16 * 128, 64, 128), 16, 4, 0)
     for k, v in kw.items():
         setattr(c, k, v)
     return c
@@ -90,7 +90,7 @@ def test_decode_refuses(dec, cache, dtype, code, word):
 def test_decode_refuses_strides_lone_keys_and_small_workspaces():
     L, lib = _lib()
     for s in (L.Strides(16, 8, 128), L.Strides(16, 64, 48), L.Strides(-16, 64, 128), L.Strides(16, 64, 1 << 26)):
-        assert lib.fable_attn_dec8(_dec(), _cache(v=s), 1, None, 0, None, None, None) == ARG
+        assert lib.fable_attn_dec8(_dec(), _cache(s=s), 1, None, 0, None, None, None) == ARG
         assert b"strides" in lib.fable_attn_last_error()
     assert lib.fable_attn_dec8(_dec(), _cache(), 1, None, 0, None, 16, None) == ARG
     need = lib.fable_attn_dec8_ws_bytes(_dec(max_blocks=4096), _cache(), 1, 0)
@@ -170,7 +170,7 @@ def test_prompts_refuse():
     assert call(c=_cache(k_scale=None)) == ARG and call(c=_cache(group=5)) == ARG
     assert call(kv=L.FablePagedKV(None, 4, 16, 0, 0)) == ARG and call(kv=L.FablePagedKV(16, 0, 16, 0, 0)) == ARG
     assert call(kv=L.FablePagedKV(16, 4, 8, 0, 0)) == ARG
-    assert call(c=_cache(k=L.Strides(1 << 31, 64, 128))) == ARG
+    assert call(c=_cache(s=L.Strides(1 << 31, 64, 128))) == ARG
 
 
 # ----------------------------------------------------------------------------- refusals of the Python entry points
