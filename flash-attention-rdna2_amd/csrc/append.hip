@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
   const T* src = (const T*)(kind == 0 ? p.k : (kind == 1 ? p.v : p.q)) + (p.cu ? (long long)c0 * st.s : (long long)b * st.b);
   const long long rp0 = rotated && p.rotary_pos ? p.rotary_pos[b] : ctx;
   const int passes = NP > 0 ? NP : max((1 << p.tshift) / R, 1);   // of a wave
-  const int part = WB > 1 ? at % WB : 0;                          // of the unit's waves
+  const int part = WB > 1 && kind != 2 ? at % WB : 0;             // of the unit's waves (queries: one)
   const long long room = (long long)p.max_blocks << p.page_shift;
   auto pos_of = [&](int i) { return base + (part * NH + i) * R + r; };
   auto token_of = [&](int i) { return min(max(pos_of(i) - ctx, 0LL), (long long)n - 1); };   // in bounds
@@ -499,6 +499,7 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
     else hi = mid;
   }
   const long long j = row - p.cu[lo];
+  if (p.used && (p.batch <= 0 || j < 0 || j >= p.used[lo])) return;
   int blk = -1;
   if (p.batch > 0 && j >= 0 && row < p.cu[lo + 1] && j < ((long long)p.max_blocks << p.page_shift)) {
     const long long at = (long long)lo * p.max_blocks + (j >> p.page_shift);

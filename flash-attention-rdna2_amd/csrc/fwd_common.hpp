@@ -117,6 +117,7 @@ struct FwdPaged8 : FwdPaged {
   const uint8_t *ks, *vs;   // scales [num_blocks][heads][subs]
   int gshift, subs, num_blocks;
 };
+struct FwdPaged8L : FwdPaged8 {};   // pages at least as long as the kernel's key tiles
 inline void fwd_paged8_scales(FwdPaged8& pg, const FableCache8& c, int page) {
   pg.ks = c.k_scale;
   pg.vs = c.v_scale;

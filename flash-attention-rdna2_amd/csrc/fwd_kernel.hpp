@@ -83,7 +83,8 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
   constexpr bool PG = std::is_base_of<FwdPaged, PGT>::value;
   // Q8: the pages hold codes with scales (cache8.hpp); a row's chunk becomes T on its way to LDS, its scale in
   // the conversion, and everything behind LDS is as over 16-bit pages
-  constexpr bool Q8 = std::is_same<PGT, FwdPaged8>::value;
+  constexpr bool Q8 = std::is_base_of<FwdPaged8, PGT>::value;
+  constexpr bool Q8L = std::is_same<PGT, FwdPaged8L>::value;   // a tile of keys lies in one page
   using KT = std::conditional_t<Q8, uint8_t, T>;
   static_assert(!PG || (!CAUSAL && !DROP), "paged instances");
   using V8 = typename Dt<T>::V8;
@@ -329,9 +330,15 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
   // D 128 277 -> 266 us, D 256 746 -> 654; 16 / 4 heads, D 256 1040 -> 899.)
   const int wrow = __builtin_amdgcn_readfirstlane(tid >> 6) * (64 / C::DCH);  // first row of the wave's first load
   constexpr int RW = 64 / C::DCH;                                             // rows of a load
+  // (Q8: see below)
+  constexpr int JQ = Q8L ? C::KJ : (RSTEP > 0 && RSTEP < 16 ? 16 / RSTEP : 1);
+  constexpr int NQ = Q8 ? C::KJ / JQ : 1;
+  static_assert(!Q8 || (C::KJ % JQ == 0 && (JQ == 1 || RSTEP * JQ == 16 || Q8L)), "loads of a page");
+  auto q8_row = [&](int j) { return JQ > 1 || Q8L ? tid / C::DCH + (j % JQ) * RSTEP : lane / C::DCH; };   // of load j, from its page part's first
+  auto q8_key = [&](int q) { return JQ > 1 || Q8L ? q * 16 : wrow + q * RSTEP; };                         // that first row, from the tile's
   auto pg_index = [&](int j) {   // entry of the sequence's row of the table
     if constexpr (PG)
-      return min(max(ekey + wrow + j * RSTEP, FEAT ? bk0 : 0), kvalid - 1) >> pg.page_shift;
+      return min(max(ekey + (Q8 ? q8_key(j) : wrow + j * RSTEP), FEAT ? bk0 : 0), kvalid - 1) >> pg.page_shift;
     else
       return 0;
   };
@@ -339,28 +346,51 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
     if constexpr (PG) {
       const auto r = buf_rsrc32(pg.table + (long long)__builtin_amdgcn_readfirstlane(z) * (pg.max_blocks & pg.tmask), (unsigned)pg.max_blocks * 4u);
 #pragma unroll
-      for (int j = 0; j < NE; j++) ent[j] = __builtin_amdgcn_raw_buffer_load_b32(r, (pg_index(j) & pg.tmask) * 4, 0, 0);
+      for (int j = 0; j < (Q8 ? NQ : NE); j++) ent[j] = __builtin_amdgcn_raw_buffer_load_b32(r, (pg_index(j) & pg.tmask) * 4, 0, 0);
     }
   };
   auto pg_load = [&](bool first, LD (&ld)[C::KJ], const KT* base, int key0, const int (&page)[NE], unsigned spg,
-                     unsigned srow, const int (&off)[C::KJ], unsigned (&lsc)[Q8 ? C::KJ : 1], const uint8_t* scales) {
-    if constexpr (PG) {
+                     unsigned srow, const int (&off)[C::KJ]) {
+    if constexpr (PG && !Q8) {
 #pragma unroll
       for (int j = 0; j < NE; j++) {
         const int key = __builtin_amdgcn_readfirstlane(key0 + wrow + j * RSTEP);
         const unsigned in = key & ((1 << pg.page_shift) - 1);
         const unsigned rows = __builtin_amdgcn_readfirstlane(min(max(kvalid - key, 0), RW));   // (a med3: vector only)
-        const auto r = buf_rsrc32(base + ((uint64_t)(unsigned)page[j] * spg + (uint64_t)in * srow), rows * srow * (unsigned)sizeof(KT));
-        const int row = lane / C::DCH;
-        const bool hide = FEAT && first && key + row < bk0;
-        if constexpr (Q8) {
-          // (rows that are not there get scale 0: their codes are zeros, and no scale's byte may make NaN of them)
-          const auto rs = buf_rsrc32(scales + ((uint64_t)(unsigned)page[j] * nheads + kvh) * pg.subs, (unsigned)pg.subs);
-          lsc[j] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(rs, hide || row >= (int)rows ? kBufZero : (int)(in + row) >> pg.gshift, 0, 0);
-          ld[j] = __builtin_amdgcn_raw_buffer_load_b64(r, hide ? kBufZero : off[j], 0, 0);
-        } else {
-          ld[j] = buf_load16(r, hide ? kBufZero : off[j]);
-        }
+        const auto r = buf_rsrc32(base + ((uint64_t)(unsigned)page[j] * spg + (uint64_t)in * srow), rows * srow * 2u);
+        ld[j] = buf_load16(r, FEAT && first && key + lane / C::DCH < bk0 ? kBufZero : off[j]);
+      }
+    }
+  };
+  // Q8: codes and scales of one tile, whose keys start at key0. K and V have the same strides, so what is worked out for
+  // a page when its K rows are loaded (`at`: the offsets of its rows and scales) serves its V rows a tile later. With a
+  // tile in one page (Q8L) that is once per tile, else once per load, or per 16 rows where loads are 8 rows apart (JQ
+  // loads to a page: the 256-wide kernel).
+  struct Q8At {
+    uint64_t row[NQ];      // of the first row of the tile's (or load's) part of the page, in bytes
+    unsigned scale[NQ];    // of this head's scales of the page
+  };
+  Q8At at_cur, at_prev;
+  auto q8_load = [&](bool first, LD (&ld)[C::KJ], unsigned (&lsc)[Q8 ? C::KJ : 1], const KT* base, const uint8_t* scales, int key0,
+                     const Q8At& at, const int (&off)[C::KJ]) {
+    if constexpr (Q8) {
+      __amdgpu_buffer_rsrc_t r[NQ], rs[NQ];
+      int rows[NQ], in[NQ];
+#pragma unroll
+      for (int j = 0; j < NQ; j++) {
+        const int key = __builtin_amdgcn_readfirstlane(key0 + q8_key(j));
+        in[j] = key & ((1 << pg.page_shift) - 1);
+        rows[j] = __builtin_amdgcn_readfirstlane(min(max(kvalid - key, 0), Q8L ? C::BC : (JQ > 1 ? 16 : RW)));
+        r[j] = buf_rsrc32(base + at.row[j], (unsigned)rows[j] * (unsigned)p.sK.s);
+        rs[j] = buf_rsrc32(scales + at.scale[j], (unsigned)pg.subs);
+      }
+#pragma unroll
+      for (int j = 0; j < C::KJ; j++) {
+        const int q = j / JQ, row = q8_row(j);
+        const bool hide = FEAT && first && key0 + q8_key(q) + row < bk0;
+        // (rows that are not there get scale 0: their codes are zeros, and no scale's byte may make NaN of them)
+        lsc[j] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(rs[q], hide || row >= rows[q] ? kBufZero : (in[q] + row) >> pg.gshift, 0, 0);
+        ld[j] = __builtin_amdgcn_raw_buffer_load_b64(r[q], hide ? kBufZero : off[j], 0, 0);
       }
     }
   };
@@ -368,7 +398,7 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
     // (offsets within the wave's rows: the descriptor starts at the wave's first row)
 #pragma unroll
     for (int j = 0; j < C::KJ; j++) {
-      const int r = lane / C::DCH, c = tid % C::DCH;
+      const int r = Q8 ? q8_row(j) : lane / C::DCH, c = tid % C::DCH;
       constexpr int EL = sizeof(KT);
       koff[j] = 8 * c < HDr ? r * (int)(p.sK.s * EL) + 8 * EL * c : kBufZero;
       voff[j] = 8 * c < HDr ? r * (int)(p.sV.s * EL) + 8 * EL * c : kBufZero;
@@ -376,17 +406,27 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
     if (ntiles > 0) pg_fetch();
   }
   auto gload_k = [&](bool first = false) {
-    if constexpr (PG) {
+    if constexpr (Q8) {
+      at_prev = at_cur;
+#pragma unroll
+      for (int j = 0; j < NQ; j++) {
+        const int raw_e = pg.tmask ? ent[j] : z * pg.max_blocks + pg_index(j);
+        const unsigned page = (unsigned)__builtin_amdgcn_readfirstlane((int)min((unsigned)raw_e, (unsigned)pg.num_blocks - 1));
+        const unsigned in = (unsigned)__builtin_amdgcn_readfirstlane(ekey + q8_key(j)) & ((1u << pg.page_shift) - 1);
+        at_cur.row[j] = (uint64_t)page * (unsigned)pg.kpg + in * (unsigned)p.sK.s;
+        at_cur.scale[j] = (page * (unsigned)nheads + (unsigned)kvh) * (unsigned)pg.subs;
+      }
+      q8_load(first, ldk, lsk, Kg, pg.ks, ekey, at_cur, koff);
+      ekey += C::BC;
+      pg_fetch();
+    } else if constexpr (PG) {
 #pragma unroll
       for (int j = 0; j < NE; j++) {
         pg_prev[j] = pg_cur[j];
         pg_cur[j] = __builtin_amdgcn_readfirstlane(ent[j]);
         if (!pg.tmask) pg_cur[j] = __builtin_amdgcn_readfirstlane(z * pg.max_blocks + pg_index(j));
-        if constexpr (Q8) pg_cur[j] = (int)min((unsigned)pg_cur[j], (unsigned)pg.num_blocks - 1);
       }
-      const uint8_t* ks = nullptr;
-      if constexpr (Q8) ks = pg.ks;
-      pg_load(first, ldk, Kg, ekey, pg_cur, (unsigned)pg.kpg, (unsigned)p.sK.s, koff, lsk, ks);
+      pg_load(first, ldk, Kg, ekey, pg_cur, (unsigned)pg.kpg, (unsigned)p.sK.s, koff);
       ekey += C::BC;
       pg_fetch();
     } else {
@@ -399,10 +439,10 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
   };
   // (PG: `ahead` K tiles have been loaded past this V tile, 0 or 1)
   auto gload_v = [&](int ahead = 1, bool first = false) {
-    if constexpr (PG) {
-      const uint8_t* vs = nullptr;
-      if constexpr (Q8) vs = pg.vs;
-      pg_load(first, ldv, Vg, ekey - (1 + ahead) * C::BC, ahead ? pg_prev : pg_cur, (unsigned)pg.vpg, (unsigned)p.sV.s, voff, lsv, vs);
+    if constexpr (Q8) {
+      q8_load(first, ldv, lsv, Vg, pg.vs, ekey - (1 + ahead) * C::BC, ahead ? at_prev : at_cur, koff);
+    } else if constexpr (PG) {
+      pg_load(first, ldv, Vg, ekey - (1 + ahead) * C::BC, ahead ? pg_prev : pg_cur, (unsigned)pg.vpg, (unsigned)p.sV.s, voff);
     } else {
       const auto r = buf_rsrc(v_cur, v_left);
 #pragma unroll
@@ -985,8 +1025,18 @@ static int launch_fwd_pg(const FableFwdParams& p, const PGT& pg, bool rot, hipSt
     }
     if (ws.query) return FA_OK;
     if (nblk * sp.n > 0x7FFFFFFF) return fail(FA_ERR_ARG, "fable_attn_fwd: grid too large");
-    hipLaunchKernelGGL((fwd_kernel<T, K, false, decltype(ft)::value, false, PGT, decltype(rt)::value>),
-                       dim3((unsigned)(nblk * sp.n)), dim3(K::NT), 0, st, p, nqt, sp, pg);
+    auto launch = [&](const auto& view) {
+      hipLaunchKernelGGL((fwd_kernel<T, K, false, decltype(ft)::value, false, std::decay_t<decltype(view)>, decltype(rt)::value>),
+                         dim3((unsigned)(nblk * sp.n)), dim3(K::NT), 0, st, p, nqt, sp, view);
+    };
+    if constexpr (std::is_same<PGT, FwdPaged8>::value) {
+      if (1 << pg.page_shift >= K::BC)
+        launch(FwdPaged8L{pg});
+      else
+        launch(pg);
+    } else {
+      launch(pg);
+    }
     const int rc = launch_status("fable_attn_fwd (paged)");
     if (rc != FA_OK || sp.n == 1) return rc;
     return launch_fwd_split_combine_paged(p, pg, std::is_same<T, _Float16>::value ? FA_F16 : FA_BF16, sp, st);

@@ -584,7 +584,7 @@ def dec8(q, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, new_
 
 def fwd_paged8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, scale, causal, win_left, win_right,
                softcap, alibi, attn_chunk=0, seqused_q=None, seqused_k=None):
-    """fwd_paged over a cache in 8 bits (as dec8's)."""
+    """fwd_paged over a cache in 8 bits (as dec8's). Returns (out, the launch's parameters)."""
     _req(q.is_cuda, "GPU tensors required")
     _req(q.dtype in (torch.float16, torch.bfloat16), f"8-bit caches take fp16 or bf16 queries, got {q.dtype}")
     _req(q.dim() == 3 and _rows_aligned(q), "q: [total, H, D] with a contiguous head_dim and 16-byte aligned rows expected")
@@ -616,7 +616,7 @@ def fwd_paged8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, m
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
     with _on(q.device):
         _lib.check(_L.fable_attn_fwd_paged8(p, kv, c, _dt(q), _ptr(ws), need, _stream(q)), "fable_attn_fwd_paged8")
-    return out
+    return out, (p, kv, c, _dt(q))
 
 
 def append(k, v, k_cache, v_cache, cache_seqlens, q=None, cu=None, max_seqlen=0, block_table=None, leftpad=None, cos=None,
@@ -679,8 +679,9 @@ def append(k, v, k_cache, v_cache, cache_seqlens, q=None, cu=None, max_seqlen=0,
     return p, dt, q_out
 
 
-def gather(k_cache, v_cache, cu, total, dtype, block_table=None, k_scale=None, v_scale=None):
-    """The first cu[b+1] - cu[b] cached rows of every sequence as packed k, v [total, Hk, D] in dtype.
+def gather(k_cache, v_cache, cu, total, dtype, block_table=None, k_scale=None, v_scale=None, used=None):
+    """The first cu[b+1] - cu[b] cached rows of every sequence as packed k, v [total, Hk, D] in dtype; with used
+    int32 [batch] only that many of them, the others of the result left as they were allocated.
     Returns (the launch's parameters and dtype, (k, v))."""
     dev = k_cache.device
     kc, vc, group = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev)
@@ -700,6 +701,9 @@ def gather(k_cache, v_cache, cu, total, dtype, block_table=None, k_scale=None, v
         p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
     p.block_table = block_table.data_ptr() if block_table is not None else None
     p.cu, p.total, p.batch, p.NKV, p.HD, p.page = cu.data_ptr(), int(total), batch, Hk, D, page
+    if used is not None:
+        _check_index("used", used, dev, batch)
+        p.used = used.data_ptr()
     p.max_blocks = block_table.shape[1] if block_table is not None else 1
     p.num_blocks, p.group = nb, group
     if k.numel():

@@ -95,7 +95,7 @@ class FableAppendParams(ctypes.Structure):
 class FableGatherParams(ctypes.Structure):
     _fields_ = [("Kc", c_ptr), ("Vc", c_ptr), ("k_scale", c_ptr), ("v_scale", c_ptr),
                 ("k_out", c_ptr), ("v_out", c_ptr), ("kc", Strides), ("vc", Strides),
-                ("block_table", c_ptr), ("cu", c_ptr), ("total", c_i64),
+                ("block_table", c_ptr), ("cu", c_ptr), ("used", c_ptr), ("total", c_i64),
                 ("batch", c_i32), ("NKV", c_i32), ("HD", c_i32), ("page", c_i32),
                 ("max_blocks", c_i32), ("num_blocks", c_i32), ("group", c_i32)]
 

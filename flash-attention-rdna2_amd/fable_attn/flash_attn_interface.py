@@ -549,9 +549,38 @@ def _no_grad8(q):
         raise NotImplementedError("fable_attn: attention over an 8-bit cache has no gradient; run it under torch.no_grad()")
 
 
-def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, seqused_q, seqused_k, *,
+# Packed prompts over an 8-bit cache with head dims past 128 have their rows brought to 16 bits first, from this many
+# query-key pairs on (by the longest lengths): one wave per SIMD does the page addresses and conversions of every
+# 32-key tile there by itself. D 256, 16 / 4 heads, pages of 16, times in place / gathered: 1 prompt of 500 rows over
+# 1000 keys (8M pairs) 40 / 48 us, 4 of 500 over 2000 (64M) 119 / 119, 4 of 1000 over 4000 (256M) 374 / 325, 1 of 4000
+# over 16000 (1024M) 1368 / 1038; pages of 64, 6 of 500-4000 over up to 5000 (1920M) 1216 / 1113. A window bounds the
+# keys of a row, not those of a gather (window 512: 430 / 450). Up to head dim 128 in place is the faster (D 128 570 /
+# 620, D 64 404 / 430).
+_GATHER8_PAIRS = 100_000_000
+
+
+def _gather8_pays(batch, heads, max_sq, max_sk, wl, d):
+    """Whether packed prompts over an 8-bit cache are gathered first."""
+    return d > 128 and wl < 0 and batch * heads * max_sq * max_sk > _GATHER8_PAIRS
+
+
+def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, max_sk, seqused_q, seqused_k,
                     descale, hints, **kw):
-    """Packed prompts over a paged cache held in 8 bits, read through the block table."""
+    """Packed prompts over a paged cache held in 8 bits, read through the block table (or gathered: _gather8_pays). As for
+    decode, the launch parameters that the first call of a signature came to are kept per thread."""
+    key, plans = None, _plans("prefill8_plans")
+    try:
+        key = (_place(q), _place(k_cache), _place(v_cache), _sig(k_scale), _sig(v_scale), _sig(block_table), _sig(cu_q), _sig(cu_k),
+               _sig(seqused_q), _sig(seqused_k), kw["alibi_slopes"] is None, bool(kw["causal"]), kw["attention_chunk"],
+               _option_key(kw["softmax_scale"], kw["window_size"], kw["softcap"]), hints)
+        plan = plans.get(key)
+    except (AttributeError, TypeError, ValueError, RuntimeError):   # not tensors, or no key
+        key = plan = None
+    if plan is not None and not (torch.is_grad_enabled() and q.requires_grad) and descale == (None, None, None):
+        out = _prefill8_fast(plan, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, int(max_sq), max_sk, seqused_q,
+                             seqused_k)
+        if out is not None:
+            return out
     _no_grad8(q)
     _reject_fp8(*descale)
     if q.is_cuda and q.dtype not in (torch.float16, torch.bfloat16):
@@ -561,14 +590,49 @@ def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu
                          f"headdim) with q's headdim; got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
     if q.shape[2] % 16:
         raise NotImplementedError(f"fable_attn: 8-bit caches need a head_dim that is a multiple of 16, got {q.shape[2]}")
-    spec = _normalize(q, k_cache[0], v_cache[0], head_axis=1, hints=hints, **kw) if k_cache.shape[0] else None
-    if spec is None:
+    if not k_cache.shape[0]:
         raise ValueError("fable_attn: the cache has no pages")
+    spec = _normalize(q, k_cache[0], v_cache[0], head_axis=1, hints=hints, **kw)
     dev = q.device
     idx = lambda t: _as_index(t, dev) if t is not None else None
-    return _C.fwd_paged8(_aligned(q), k_cache, v_cache, k_scale, v_scale, idx(block_table), idx(cu_q), idx(cu_k), int(max_sq),
-                         spec.scale, bool(spec.causal), spec.wl, spec.wr, spec.softcap, spec.alibi, spec.chunk,
-                         idx(seqused_q), idx(seqused_k))
+    table, cq, ck, uq, uk = (idx(t) for t in (block_table, cu_q, cu_k, seqused_q, seqused_k))
+    scalars = (spec.scale, bool(spec.causal), spec.wl, spec.wr, spec.softcap, spec.alibi)
+    if table.dim() == 2 and max_sk and _gather8_pays(table.shape[0], q.shape[1], int(max_sq), int(max_sk), spec.wl, q.shape[2]):
+        # every sequence's rows at its own multiple of the longest length (no host round trip for their sum)
+        span = min(int(max_sk), table.shape[1] * k_cache.shape[1])
+        cu = torch.arange(0, (table.shape[0] + 1) * span, span, dtype=torch.int32, device=dev)
+        used = (uk if uk is not None else ck[1:] - ck[:-1]).clamp(0, span)
+        _, _, (k, v) = _C.gather(k_cache, v_cache, cu, table.shape[0] * span, q.dtype, table, k_scale, v_scale, used)
+        return _C.fwd_varlen(_aligned(q), k, v, cq, cu, int(max_sq), span, *scalars, 0.0, 0, spec.chunk, uq, used)
+    out, launch = _C.fwd_paged8(_aligned(q), k_cache, v_cache, k_scale, v_scale, table, cq, ck, int(max_sq), *scalars, spec.chunk, uq, uk)
+    if (key is not None and spec.alibi is None and _in_place(q)
+            and all(a is b for a, b in zip((table, cq, ck, uq, uk), (block_table, cu_q, cu_k, seqused_q, seqused_k)))):
+        _remember(plans, key, launch + (dev.index,))
+    return out
+
+
+def _prefill8_fast(plan, q, k_cache, v_cache, k_scale, v_scale, table, cu_q, cu_k, max_sq, max_sk, seqused_q, seqused_k):
+    """One call of a planned signature; None when the rows are gathered first, an address is not aligned or the device is
+    not current (the general path serves it)."""
+    p, kv, c, dt, dev = plan
+    if p.HD > 128 and max_sk and _gather8_pays(p.batch, p.NH, max_sq, int(max_sk), p.win_left, p.HD):
+        return None
+    qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if (qp | kp | vp) & 15 or dev != torch._C._cuda_getDevice():
+        return None
+    out = (torch.empty if seqused_q is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+    p.Q, p.K, p.V, p.O, p.SQ = qp, kp, vp, out.data_ptr(), max_sq
+    p.cu_q, p.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    p.seqused_q = seqused_q.data_ptr() if seqused_q is not None else None
+    p.seqused_k = seqused_k.data_ptr() if seqused_k is not None else None
+    kv.block_table, c.k_scale, c.v_scale = table.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+    need = int(_C._L.fable_attn_fwd_paged8_ws_bytes(p, kv, c, dt))
+    if need < 0:
+        _lib.check(1, "fable_attn_fwd_paged8")
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    _lib.check(_C._L.fable_attn_fwd_paged8(p, kv, c, dt, ws.data_ptr() if ws is not None else None, need,
+                                           torch._C._cuda_getCurrentRawStream(dev)), "fable_attn_fwd_paged8")
+    return out
 
 
 def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
@@ -594,8 +658,8 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
             raise ValueError("fable_attn: k_scale and v_scale belong to a paged cache; pass block_table")
         if dropout_p or qv is not None or return_attn_probs:
             raise NotImplementedError("fable_attn: dropout, qv and return_attn_probs are not supported over an 8-bit cache")
-        return _paged_prefill8(q, k, v, k_scale, v_scale, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, seqused_q,
-                               seqused_k, softmax_scale=softmax_scale, causal=causal, window_size=window_size,
+        return _paged_prefill8(q, k, v, k_scale, v_scale, block_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                               seqused_q, seqused_k, softmax_scale=softmax_scale, causal=causal, window_size=window_size,
                                softcap=softcap, alibi_slopes=alibi_slopes, attention_chunk=attention_chunk,
                                descale=(q_descale, k_descale, v_descale), hints=(num_splits, pack_gqa, sm_margin))
     if block_table is not None:

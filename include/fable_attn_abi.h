@@ -430,7 +430,8 @@ int fable_attn_append(FableAppendParams p, int dtype, void* stream);
 
 /* The first cu[b+1] - cu[b] cached rows of every sequence, packed: rows cu[b].. of the dense k_out / v_out
  * [total][NKV][HD] in dtype (fp16, bf16; fp32 for a cache of that type). k_scale NULL: the caches are of
- * `dtype`. Rows of [0, total) that no sequence has, or whose page the table does not name, become zeros. */
+ * `dtype`. Rows of [0, total) that no sequence has, or whose page the table does not name, become zeros. With
+ * `used` (int32, batch) only the first used[b] rows of sequence b are written, and nothing else. */
 typedef struct FableGatherParams {
   const void* Kc;
   const void* Vc;
@@ -441,6 +442,7 @@ typedef struct FableGatherParams {
   fa_strides kc, vc;
   const int32_t* block_table;
   const int32_t* cu;
+  const int32_t* used;
   int64_t total;
   int32_t batch, NKV, HD, page, max_blocks, num_blocks, group;
 } FableGatherParams;
