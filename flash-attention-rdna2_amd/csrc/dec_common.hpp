@@ -170,8 +170,8 @@ inline int dec_groups(const FableDecParams& p) { return (int)(((long long)p.nq *
 // Parts of a call (DecShare): one workgroup per CU (more in flight per CU read a batch of alike
 // sequences slower: C4 0.96x with two, 0.86x with three), or two where the (K/V head, row group) count
 // leaves more than an eighth of the CUs out of a round of one.
-inline int dec_parts(const FableDecParams& p, int unit) {
-  const long long X = (long long)(p.NH / p.gqa) * dec_groups(p);
+inline int dec_parts(const FableDecParams& p, int unit, int wh = 1) {   // (wh: K/V heads of a workgroup)
+  const long long X = (long long)(p.NH / p.gqa / wh) * dec_groups(p);
   long long parts = 256 / X;
   if (parts * X < 224) parts = (512 + X - 1) / X;
   const long long units = (long long)p.batch * (((long long)p.max_blocks * p.page + unit - 1) / unit + 1);
@@ -179,13 +179,13 @@ inline int dec_parts(const FableDecParams& p, int unit) {
   return parts > 1 ? (int)parts : 1;
 }
 // workgroups per (K/V head, row group) (DecShare::init)
-inline int dec_share_wgs(const FableDecParams& p, int unit) {
-  const int parts = dec_parts(p, unit);
+inline int dec_share_wgs(const FableDecParams& p, int unit, int wh = 1) {
+  const int parts = dec_parts(p, unit, wh);
   return p.batch <= parts ? parts : 2 * parts;
 }
 // scratch: two records of 16 rows per workgroup
-inline long long dec_share_bytes(const FableDecParams& p, int unit) {
-  return (dec_meta_floats(p) + (long long)dec_share_wgs(p, unit) * 2 * (p.NH / p.gqa) * dec_groups(p) * 16 * (p.HD + 2)) * 4;
+inline long long dec_share_bytes(const FableDecParams& p, int unit, int wh = 1) {
+  return (dec_meta_floats(p) + (long long)dec_share_wgs(p, unit, wh) * 2 * (p.NH / p.gqa) * dec_groups(p) * 16 * (p.HD + 2)) * 4;
 }
 
 // merge of the partials in p.scratch into p.o and p.lse_out (fp16/bf16; decode.hip): of p.nsplit splits per

@@ -2,7 +2,7 @@
 //
 // The split of the work, the records and the combine are the 16-bit decode's (decode.hip): one workgroup of
 // four waves per (K/V head, group of 16 rows, run of a sequence's keys), each wave with its own chunks and
-// online softmax, merged in LDS. What differs:
+// online softmax, merged in LDS. Large calls give a workgroup two or four K/V heads, waves and all (dec8_heads). What differs:
 //  * a chunk is 32 keys, so as many bytes are in flight per wave as there with 16. A SIMD has one wave, whose
 //    instructions per chunk are what bounds it next to HBM, so the rest is about having few;
 //  * codes stay codes in LDS (half the LDS traffic) and become fp16/bf16 between the LDS read and the matrix
@@ -27,7 +27,6 @@
 namespace fa {
 
 constexpr int kKeys8 = 32;                       // keys per wave iteration
-constexpr int kUnit8 = kKeys8 * kDecWaves;       // keys of a unit of a share (DecShare)
 constexpr int kDec8Append = 1, kDec8Final = 2;   // new keys were appended; one split, no combine launch
 
 struct Dec8Args : FableDecParams {
@@ -57,14 +56,15 @@ struct Dec8Lds {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
-// P16: pages of 16 rows (two to a chunk)
-template <typename T, int HD, bool FEAT, bool SHARE, bool P16>
+// P16: pages of 16 rows (two to a chunk); WH: heads of a workgroup
+template <typename T, int HD, bool FEAT, bool SHARE, bool P16, int WH>
 __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   using V8 = typename Dt<T>::V8;
   using L = Dec8Lds<HD>;
   constexpr bool kTwoP = std::is_same<T, _Float16>::value;   // P in two bf16 parts
   constexpr int NDB = HD / 16, RB = HD / 16, NV = kKeys8 * RB / 64, NDS = HD / 32;
   constexpr int NPG = P16 ? 2 : 1;
+  constexpr int WR = kDecWaves / WH, kUnit8 = kKeys8 * WR;   // waves on the keys of a head; keys of a unit of a share
   // Chunks whose rows are in flight. One left a wave waiting for most of the memory latency (32000 keys of one sequence
   // in 4 splits, D 128: 78 us, 66 with two; 16 x 32768 keys, D 64: 178 and 119; D 192 96 and 72 in 3 splits); rows of
   // 256 bytes fill the same bytes with one, and two cost registers (8 x 4000 keys 23.4 and 25.4).
@@ -85,12 +85,13 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     bz = (int)(w / gridDim.y);
     by = (int)w - bz * gridDim.y;
   }
-  const int grp = p.ngrp > 1 ? hgl / NKV : 0, kvh = hgl - grp * NKV;
+  const int hw = wave % WH, rw = wave / WH;   // this wave's head of the workgroup's, and place among its waves
+  const int grp = p.ngrp > 1 ? hgl / (NKV / WH) : 0, head0 = (hgl - grp * (NKV / WH)) * WH, kvh = head0 + hw;
   const int r0 = 16 * grp, hg = min(16, nq * gqa - r0);  // rows of this group
   auto row_tok = [&](int g) { return nq > 1 ? (int)((unsigned)(r0 + g) / (unsigned)gqa) : 0; };
-  auto row_of = [&](int b, int g) {
+  auto row_of = [&](int b, int head, int g) {
     const int tok = row_tok(g);
-    return (long long)(b * nq + tok) * NH + kvh * gqa + (r0 + g - tok * gqa);
+    return (long long)(b * nq + tok) * NH + head * gqa + (r0 + g - tok * gqa);
   };
   auto args = [&]() -> Dec8Args {   // (as in decode.hip: the phases that only some workgroups run read it again)
     if constexpr (SHARE) return dec_reload<Dec8Args>();
@@ -118,14 +119,14 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   for (bool more = true; more;) {
     const int b = SHARE ? sq : by;
     // q rows of this group, loaded while the lengths are on their way
-    constexpr int RCH = HD / 8, NQI = (16 * RCH + 255) / 256;
+    constexpr int RCH = HD / 8, NQ = WH * 16 * RCH, NQI = (NQ + 255) / 256;
     u32x4 qraw[NQI];
     {
       const Dec8Args p = args();
 #pragma unroll
       for (int u = 0; u < NQI; u++) {
-        const int i = min(tid + 256 * u, 16 * RCH - 1), g = i / RCH, c = i % RCH;
-        qraw[u] = *(const u32x4*)((const T*)p.q + row_of(b, min(g, hg - 1)) * HDr + (8 * c < HDr ? 8 * c : 0));
+        const int i = min(tid + 256 * u, NQ - 1), g = i / RCH % 16, c = i % RCH;
+        qraw[u] = *(const u32x4*)((const T*)p.q + row_of(b, head0 + i / RCH / 16, min(g, hg - 1)) * HDr + (8 * c < HDr ? 8 * c : 0));
       }
     }
     DecSpan sp;
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
         ((int*)p.scratch)[2 * b + 1] = str.even ? n : -n;
       }
       if (!(begins && stop == first + units))
-        rec = p.scratch + dec_meta_floats(p) + ((2ll * part + (begins && !str.even ? 1 : 0)) * X + hgl) * 16 * (HDr + 2);
+        rec = p.scratch + dec_meta_floats(p) + ((2ll * part + (begins && !str.even ? 1 : 0)) * X * WH + grp * NKV + head0) * 16 * (HDr + 2);
       at = stop;
       first += units;
       sq++;
@@ -192,9 +193,9 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
       const int i = tid + 256 * u, g = i / RCH, c = i % RCH;
       const bool cok = 8 * c < HDr;
       const V8 v = bitcast<V8>(qraw[u]);
-      if (i < 16 * RCH)
+      if (i < NQ)
 #pragma unroll
-        for (int e = 0; e < 8; e++) qsh[g][8 * c + e] = g < hg && cok ? (float)v[e] : 0.0f;
+        for (int e = 0; e < 8; e++) qsh[g][8 * c + e] = g % 16 < hg && cok ? (float)v[e] : 0.0f;
     }
     __syncthreads();
     bool qsplit;
@@ -204,8 +205,10 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
       if (p.rotary) {
         const int rdim = p.rotary_dim > 0 ? p.rotary_dim : HDr, half = rdim / 2;
         const int rbase = p.rotary_pos ? p.rotary_pos[b] : ctx;
-        for (int i = tid; i < hg * half; i += 256) {
-          const int g = i / half, j = i % half, rp = min(max(rbase + row_tok(g), 0), p.c.rotary_rows - 1);
+        for (int i = tid; i < WH * 16 * half; i += 256) {
+          const int g = i / half, j = i % half;
+          if (g % 16 >= hg) continue;
+          const int rp = min(max(rbase + row_tok(g % 16), 0), p.c.rotary_rows - 1);
           const float c = p.cos[(long long)rp * half + j], s = p.sin[(long long)rp * half + j];
           const int ia = p.rotary == 1 ? j : 2 * j, ib = p.rotary == 1 ? j + half : 2 * j + 1;
           const float x = qsh[g][ia], y = qsh[g][ib];
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     for (int ds = 0; ds < NDS; ds++)
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float x = qsh[lh][64 * (ds / 2) + 16 * lg + 8 * (ds % 2) + e];
+        const float x = qsh[16 * hw + lh][64 * (ds / 2) + 16 * lg + 8 * (ds % 2) + e];
         const T hi = (T)x;
         qb[ds][e] = hi;
         ql[ds][e] = (T)(x - (float)hi);
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     // Pages of the wave's chunks, 64 at a time: lane l of `page` has those of chunk c (c % 64 = l), which reach the scalar
     // unit by a readlane; the next 64 are fetched meanwhile. (By scalar loads, one chunk ahead, an entry
     // held up the LDS reads it shares a counter with.)
-    const int kfirst = start + kKeys8 * wave;
+    const int kfirst = start + kKeys8 * rw;
     int page[NPG], next[NPG];   // (next: the entries as read)
     auto index = [&](int c0, int h) {   // lane's page of its sequence, among those with keys of it
       const unsigned key = (unsigned)kfirst + min((unsigned)(c0 + lane) * kUnit8, (unsigned)end) + 16u * h;
@@ -441,28 +444,28 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     for (int db = 0; db < NDB; db++) *(f32x4*)(red_o + (wave * 16 + lh) * HD + 16 * db + 4 * lg) = oacc[db];
     __syncthreads();
     const Dec8Args pe = args();
-    for (int i = tid; i < hg * HDr; i += 256) {
-      const int g = i / HDr, d = i % HDr;
+    for (int i = tid; i < WH * hg * HDr; i += 256) {
+      const int r = i / HDr, d = i % HDr, h = WH > 1 ? r / hg : 0, g = r - h * hg;
       float gm = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kDecWaves; w++) gm = fmaxf(gm, red_m[w][g]);
+      for (int w = 0; w < WR; w++) gm = fmaxf(gm, red_m[WH * w + h][g]);
       float l = 0.0f, acc = 0.0f;
       if (gm != -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < kDecWaves; w++) {
-          const float f = exp2_fast(red_m[w][g] - gm);
-          l += f * red_l[w][g];
-          acc += f * red_o[(w * 16 + g) * HD + d];
+        for (int w = 0; w < WR; w++) {
+          const float f = exp2_fast(red_m[WH * w + h][g] - gm);
+          l += f * red_l[WH * w + h][g];
+          acc += f * red_o[((WH * w + h) * 16 + g) * HD + d];
         }
       }
-      const long long row = row_of(b, g);
+      const long long row = row_of(b, head0 + h, g);
       if (!rec) {
         const bool ok = gm != -INFINITY && l > 0.0f;
         ((T*)pe.o)[row * HDr + d] = (T)(ok ? acc / l : 0.0f);
         if (pe.lse_out && d == 0) pe.lse_out[row] = ok ? gm * kLn2 + __logf(l) : -INFINITY;
         continue;
       }
-      float* out = rec + (SHARE ? g : row) * rec_step;
+      float* out = rec + (SHARE ? 16 * h + g : row) * rec_step;
       if (d == 0) {
         out[0] = gm;
         out[1] = l;
@@ -473,8 +476,26 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   }
 }
 
+// Heads of a workgroup. One wave per head makes what the CUs read at a time runs of 4 * D bytes in place of D, which HBM
+// gives faster (rows of 128 bytes at 1 KiB: 6.24 TB/s alone, 7.1 in fours); but a wave then walks four times the keys, and there
+// are four times the records, so it takes a large call: 16 x 32768 keys of 8 heads, D 128: 185 -> 162 us, 48 of up to 8192 108 -> 85,
+// 16 x 8000 (262 MB) 58 -> 54; 16 x 2000 (67 MB) 20.3 and 21.9, 64 x 1000 (134 MB) 32.4 and 33.0, one of 500 9.5 and 17.
+// The size is the table's: 32 of 3000 keys in tables of 8192 42.8 and 43.6, of 1000 21.1 and 24.7.
+// Two where there are no four (6 heads of 64, 64 x 4000 keys: 69 -> 52), and at D 192 (32 x 4000 keys of 16 heads: 179 -> 161,
+// 157 with four; of 4 heads 46.1 and 47.6, 50.5 with four). Rows of 256 bytes gain nothing (32 x 4000, 8 heads: 99, 103, 105).
+// (Split counts the caller sets are for one head to a workgroup.) A row must not get more than 32 records (one of 64000 keys, 32 heads, 100 -> 96; 16 heads 57.2, 55.7 in twos, 60.1
+// in fours; 8 heads in a table of 131072 35.6, 47.6 in fours).
+constexpr long long kHeadBytes8 = 176LL << 20, kHeadGroups8 = 8;
+static int dec8_heads(const FableDecParams& p) {
+  const int nkv = p.NH / p.gqa;
+  if (p.nsplit > 0 || p.HD > 192 || (long long)p.batch * p.max_blocks * p.page * nkv * p.HD * 2 < kHeadBytes8) return 1;
+  int wh = p.HD <= 128 && nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1;
+  while (wh > 1 && (long long)p.batch * (nkv / wh) * dec_groups(p) < kHeadGroups8) wh /= 2;
+  return wh;
+}
+static int dec8_unit(int wh) { return kKeys8 * (kDecWaves / wh); }   // keys of a unit of a share
 template <typename T, int HD>
-static int launch_dec8(const FableDecParams& p, const FableCache8& c, int parts, hipStream_t st, bool append) {
+static int launch_dec8(const FableDecParams& p, const FableCache8& c, int parts, int wh, hipStream_t st, bool append) {
   Dec8Args a;
   (FableDecParams&)a = p;
   a.c = c;
@@ -487,35 +508,42 @@ static int launch_dec8(const FableDecParams& p, const FableCache8& c, int parts,
   a.parts = parts;
   a.flags = (append ? kDec8Append : 0) | (parts == 0 && p.nsplit == 1 ? kDec8Final : 0);
   const bool feat = p.softcap > 0.0f || p.alibi != nullptr;
-  const unsigned X = (unsigned)(a.nkv * a.ngrp);
-  const dim3 grid = parts > 0 ? dim3(X, (unsigned)dec_share_wgs(p, kUnit8)) : dim3(X, (unsigned)p.batch, (unsigned)p.nsplit);
+  const unsigned X = (unsigned)(a.nkv / wh * a.ngrp);
+  const dim3 grid = parts > 0 ? dim3(X, (unsigned)dec_share_wgs(p, dec8_unit(wh), wh)) : dim3(X, (unsigned)p.batch, (unsigned)p.nsplit);
   // Heads whose rows share 128-byte lines (D 64: two, D 96: four) run one after another on one XCD, whose L2 then
   // fetches a line once: dealt out like the others, every XCD fetched them for itself (16 x 32768 keys of 8 heads,
   // D 64: 171 -> 118 us; D 192, 1.1x; at 128 and 256 nothing is shared, and the order measured the same).
   a.bshift = 0;
-  while ((p.HD << a.bshift) % 128 && a.bshift < 3) a.bshift++;
-  if (a.nkv % (1 << a.bshift) || ((long long)grid.x * grid.y * grid.z >> a.bshift) % 8) a.bshift = 0;
-  auto go = [&](auto ft, auto sh) {
+  while ((p.HD * wh << a.bshift) % 128 && a.bshift < 3) a.bshift++;
+  if (a.nkv / wh % (1 << a.bshift) || ((long long)grid.x * grid.y * grid.z >> a.bshift) % 8) a.bshift = 0;
+  auto go = [&](auto ft, auto sh, auto w) {
     if (p.page == 16)
-      hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value, true>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value, true, decltype(w)::value>), grid, dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value, false>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((dec8_partial_kernel<T, HD, decltype(ft)::value, decltype(sh)::value, false, decltype(w)::value>), grid, dim3(256), 0, st, a);
   };
   using Y = std::integral_constant<bool, true>;
   using N = std::integral_constant<bool, false>;
-  if (parts > 0)
-    feat ? go(Y{}, Y{}) : go(N{}, Y{});
-  else
-    feat ? go(Y{}, N{}) : go(N{}, N{});
+  auto with = [&](auto w) {
+    if (parts > 0)
+      feat ? go(Y{}, Y{}, w) : go(N{}, Y{}, w);
+    else
+      feat ? go(Y{}, N{}, w) : go(N{}, N{}, w);
+  };
+  if constexpr (HD <= 128)
+    if (wh == 4) with(std::integral_constant<int, 4>{});
+  if constexpr (HD <= 192)
+    if (wh == 2) with(std::integral_constant<int, 2>{});
+  if (wh == 1) with(std::integral_constant<int, 1>{});
   return launch_status("fable_attn_dec8 (partial)");
 }
 // kernel widths 64, 128, 192 and 256 (a row of codes is read in 64-byte steps); a head dim below its width runs with zero columns
 template <typename T>
-static int dec8_dispatch(const FableDecParams& p, const FableCache8& c, int parts, hipStream_t st, bool append) {
-  if (p.HD <= 64) return launch_dec8<T, 64>(p, c, parts, st, append);
-  if (p.HD <= 128) return launch_dec8<T, 128>(p, c, parts, st, append);
-  if (p.HD <= 192) return launch_dec8<T, 192>(p, c, parts, st, append);
-  return launch_dec8<T, 256>(p, c, parts, st, append);
+static int dec8_dispatch(const FableDecParams& p, const FableCache8& c, int parts, int wh, hipStream_t st, bool append) {
+  if (p.HD <= 64) return launch_dec8<T, 64>(p, c, parts, wh, st, append);
+  if (p.HD <= 128) return launch_dec8<T, 128>(p, c, parts, wh, st, append);
+  if (p.HD <= 192) return launch_dec8<T, 192>(p, c, parts, wh, st, append);
+  return launch_dec8<T, 256>(p, c, parts, wh, st, append);
 }
 
 // ------------------------------------------------------------------ which path a call takes
@@ -528,14 +556,14 @@ static bool dec8_uses_tiles(const FableDecParams& p, const FableCache8& c) {
 }
 // Shares worked out on the device for batches that equal splits would not spread evenly, as in decode.hip
 constexpr long long kShareBytes8 = 64LL << 20;
-static bool dec8_shares(const FableDecParams& p) {
+static bool dec8_shares(const FableDecParams& p, int wh) {
   if (p.nsplit > 0 || p.batch < 2) return false;
   if ((long long)p.batch * p.max_blocks * p.page * (p.NH / p.gqa) * p.HD * 2 < kShareBytes8) return false;
-  const int parts = dec_parts(p, kUnit8);
+  const int parts = dec_parts(p, dec8_unit(wh), wh);
   return p.batch > parts || parts % p.batch != 0;
 }
-static int dec8_fixed_splits(const FableDecParams& p) {
-  return fa_decode_num_splits(p.batch, dec_groups(p), p.NH / p.gqa, 1, (int64_t)p.max_blocks * p.page, p.nsplit);
+static int dec8_fixed_splits(const FableDecParams& p, int wh) {
+  return fa_decode_num_splits(p.batch, dec_groups(p), p.NH / p.gqa / wh, 1, (int64_t)p.max_blocks * p.page, p.nsplit);
 }
 static long long align256(long long x) { return (x + 255) / 256 * 256; }
 static long long dec8_q_bytes(const FableDecParams& p) {   // one part of a rotated q
@@ -603,8 +631,9 @@ extern "C" int64_t fable_attn_dec8_ws_bytes(FableDecParams p, FableCache8 c, int
     if (launch_fwd_paged8(f, pg, dtype, p.rotary != 0, nullptr, fw) != FA_OK) return -1;
     return 2 * dec8_q_bytes(p) + fw.need;
   }
-  if (dec8_shares(p)) return dec_share_bytes(p, kUnit8);
-  p.nsplit = dec8_fixed_splits(p);
+  const int wh = dec8_heads(p);
+  if (dec8_shares(p, wh)) return dec_share_bytes(p, dec8_unit(wh), wh);
+  p.nsplit = dec8_fixed_splits(p, wh);
   return p.nsplit != 1 ? (int64_t)p.batch * p.nq * p.NH * p.nsplit * (p.HD + 2) * 4 : 0;
 }
 
@@ -675,10 +704,11 @@ extern "C" int fable_attn_dec8(FableDecParams p, FableCache8 c, int dtype, void*
     return launch_fwd_paged8(f, pg, dtype, p.rotary != 0, st, fw);
   }
   p.scratch = (float*)ws;
-  const bool share = dec8_shares(p);
-  const int parts = share ? dec_parts(p, kUnit8) : 0;
-  p.nsplit = share ? 0 : dec8_fixed_splits(p);
-  const int rc = dtype == FA_F16 ? dec8_dispatch<_Float16>(p, c, parts, st, new_k != nullptr) : dec8_dispatch<__bf16>(p, c, parts, st, new_k != nullptr);
+  const int wh = dec8_heads(p);
+  const bool share = dec8_shares(p, wh);
+  const int parts = share ? dec_parts(p, dec8_unit(wh), wh) : 0;
+  p.nsplit = share ? 0 : dec8_fixed_splits(p, wh);
+  const int rc = dtype == FA_F16 ? dec8_dispatch<_Float16>(p, c, parts, wh, st, new_k != nullptr) : dec8_dispatch<__bf16>(p, c, parts, wh, st, new_k != nullptr);
   if (rc != FA_OK || (!share && p.nsplit == 1)) return rc;
   return dec_combine(p, dtype, st, share);
 }

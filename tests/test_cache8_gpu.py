@@ -277,7 +277,8 @@ def test_gather_of_missing_pages_and_dense_rows():
 
 # ----------------------------------------------------------------------------- decode
 def _check_decode(dtype, lens, hq, hk, d, page, group, nq=1, append=False, window=-1, softcap=0.0, alibi=False, leftpad=None,
-                  rotary=0, interleaved=False, dense=False, max_blocks=None, num_splits=0, lse=True, hide=True, seed=0, scale=None):
+                  rotary=0, interleaved=False, dense=False, max_blocks=None, num_splits=0, lse=True, hide=True, seed=0, scale=None,
+                  wide=None):
     """flash_attn_with_kvcache against the plain form, its cache too where the call appends."""
     dt, B = DT[dtype], len(lens)
     new = nq if append else 0
@@ -292,6 +293,8 @@ def _check_decode(dtype, lens, hq, hk, d, page, group, nq=1, append=False, windo
     q = _rand((B, nq, hq, d), dt, 31 + seed)
     k, v = (_rand((B, nq, hk, d), dt, 41 + seed + i) for i in range(2))
     c = pool.cuda()
+    if wide:   # a wider table, as a server keeps one: its further entries are never read for a key
+        c = c[:4] + type(c)([torch.cat((c[4], c[4][:, :1].expand(B, wide - c[4].shape[1])), 1).contiguous()])
     kw = {}
     cos = sin = None
     if rotary:
@@ -371,6 +374,25 @@ def test_decode_long_splits_and_shares(dtype):
     _check_decode(dtype, [3000], 4, 1, 64, 64, 16)
     _check_decode(dtype, [1, 2000, 17, 700, 129], 2, 1, 64, 64, 16, max_blocks=4096)
     _check_decode(dtype, [500, 0, 900], 2, 1, 64, 64, 64, max_blocks=8192, append=True, window=300, hide=False)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("lens,hq,hk,d,page,wide,kw", [
+    # tables of so many keys that a workgroup takes four heads, or two; shares worked out on the device (6
+    # sequences) and splits (8, and one)
+    ([0, 1, 300, 129, 64, 2000], 16, 8, 128, 16, 1024, {}),
+    ([0, 1, 300, 129, 64, 700, 31, 33], 8, 8, 128, 64, 256, {"append": True, "rotary": 64}),
+    ([0, 1, 300, 129, 64, 2000], 8, 8, 64, 64, 512, {"append": True, "window": 100, "hide": False}),
+    ([5, 1, 300, 129, 64, 700, 31, 33], 32, 4, 80, 16, 2048, {"nq": 3, "append": True, "alibi": True, "softcap": 20.0}),
+    ([0, 1, 300, 129, 64, 1000], 6, 6, 128, 16, 2048, {"leftpad": [0, 0, 40, 100, 63, 500], "append": True}),
+    ([0, 1, 300, 129, 64, 700, 31, 33], 12, 6, 64, 32, 1024, {"alibi": True}),
+    ([0, 1, 300, 129, 64, 1000], 4, 2, 192, 16, 3000, {}),
+    ([700, 1, 300, 129, 64, 0, 31, 33], 4, 4, 160, 64, 512, {"append": True, "rotary": 160, "interleaved": True}),
+    ([1500], 64, 32, 128, 64, 512, {}),
+    ([900], 16, 16, 128, 128, 512, {"window": 500}),
+], ids=str)
+def test_decode_heads_of_a_workgroup(lens, hq, hk, d, page, wide, kw, dtype):
+    _check_decode(dtype, lens, hq, hk, d, page, 16, wide=wide, **kw)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
