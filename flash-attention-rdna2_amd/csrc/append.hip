@@ -441,7 +441,7 @@ int fa::append_rows(const FableAppendParams& p, int dtype, hipStream_t st) {
   if (p.batch < 0 || p.n < 0 || p.max_blocks < 0) return fail(FA_ERR_ARG, "%s: batch=%d n=%d max_blocks=%d", what, p.batch, p.n, p.max_blocks);
   if (q8) {
     for (const fa_strides& s : {p.kc, p.vc}) {
-      const FableCache8 c{p.k_scale, p.v_scale, s, p.group, p.num_blocks, 0};
+      const FableCache8 c{p.k_scale, p.v_scale, s, p.group, p.num_blocks, 0, nullptr};
       if (int rc = cache8_check(what, c, p.HD, p.page)) return rc;
     }
   } else {
@@ -552,7 +552,7 @@ extern "C" int fable_attn_gather(FableGatherParams p, int dtype, void* stream) {
     return fail(FA_ERR_ARG, "%s: NKV=%d batch=%d total=%lld max_blocks=%d", what, p.NKV, p.batch, (long long)p.total, p.max_blocks);
   if (q8) {
     for (const fa_strides& s : {p.kc, p.vc}) {
-      const FableCache8 c{p.k_scale, p.v_scale, s, p.group, p.num_blocks, 0};
+      const FableCache8 c{p.k_scale, p.v_scale, s, p.group, p.num_blocks, 0, nullptr};
       if (int rc = cache8_check(what, c, p.HD, p.page)) return rc;
     }
   } else {

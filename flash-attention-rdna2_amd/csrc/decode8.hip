@@ -551,7 +551,8 @@ static int dec8_dispatch(const FableDecParams& p, const FableCache8& c, int part
 // where there are more than kTileStreams (sequence, K/V head, 16 rows): the rule of the 16-bit decode.
 constexpr int kTileRows8 = 64, kTileStreams8 = 16;
 static bool dec8_uses_tiles(const FableDecParams& p, const FableCache8& c) {
-  return c.s.b <= 0x7FFFFFFF && (long long)c.num_blocks * (p.NH / p.gqa) * (p.page / c.group) <= 0x7FFFFFFF && (long long)p.batch * (p.NH / p.gqa) * dec_groups(p) > kTileStreams8 && (long long)p.nq * p.gqa >= kTileRows8 &&
+  return c.s.b <= 0x7FFFFFFF && p.page * c.s.s <= 0x7FFFFFFF && (long long)c.num_blocks * (p.NH / p.gqa) * (p.page / c.group) <= 0x7FFFFFFF &&
+         (long long)p.batch * (p.NH / p.gqa) * dec_groups(p) > kTileStreams8 && (long long)p.nq * p.gqa >= kTileRows8 &&
          (long long)p.batch * p.max_blocks <= 0x7FFFFFFF && p.max_blocks < (1 << 29) && p.window != 0;
 }
 // Shares worked out on the device for batches that equal splits would not spread evenly, as in decode.hip
@@ -613,7 +614,7 @@ static int dec8_check(FableDecParams& p, const FableCache8& c, int dtype) {
   if (p.batch > 65535 || (long long)p.nq * p.gqa > (1 << 24)) return fail(FA_ERR_ARG, "%s: batch=%d nq=%d", what, p.batch, p.nq);
   if (p.rotary && (p.rotary_dim < 0 || p.rotary_dim > p.HD || p.rotary_dim % 2)) return fail(FA_ERR_ARG, "%s: rotary_dim=%d", what, p.rotary_dim);
   if (p.rotary && (p.rotary > 2 || c.rotary_rows < 1)) return fail(FA_ERR_ARG, "%s: rotary=%d rotary_rows=%d", what, p.rotary, c.rotary_rows);
-  if (c.s.b > 0xFFFFFFFFll) return fail(FA_ERR_ARG, "%s: pages of 4 GiB", what);
+  if (c.s.b > 0xFFFFFFFFll || p.page * c.s.s > 0xFFFFFFFFll) return fail(FA_ERR_ARG, "%s: pages of 4 GiB", what);
   return cache8_check(what, c, p.HD, p.page);
 }
 
@@ -672,7 +673,7 @@ extern "C" int fable_attn_dec8(FableDecParams p, FableCache8 c, int dtype, void*
     a.kc = a.vc = c.s;
     a.block_table = p.block_table;
     a.ctx_len = p.ctx_len;
-    a.leftpad = p.leftpad;
+    a.leftpad = c.held;
     a.rotary_pos = p.rotary_pos;
     a.cos = p.cos;
     a.sin = p.sin;

@@ -243,7 +243,7 @@ static int paged8_run(FableFwdParams p, FablePagedKV kv, FableCache8 c, int dtyp
   if (dtype != FA_F16 && dtype != FA_BF16) return fail(FA_ERR_DTYPE, "%s: dtype %d not implemented (fp16/bf16)", what, dtype);
   if (p.dropout_p > 0.0f) return fail(FA_ERR_ARG, "%s: no dropout over a cache", what);
   if (int rc = cache8_check(what, c, p.HD, kv.page)) return rc;
-  if (c.s.b > 0x7FFFFFFF || (long long)c.num_blocks * (p.NH / (p.gqa > 0 ? p.gqa : 1)) * (kv.page / c.group) > 0x7FFFFFFF)
+  if (c.s.b > 0x7FFFFFFF || kv.page * c.s.s > 0x7FFFFFFF || (long long)c.num_blocks * (p.NH / (p.gqa > 0 ? p.gqa : 1)) * (kv.page / c.group) > 0x7FFFFFFF)
     return fail(FA_ERR_ARG, "%s: pages of 2 GiB, or 2^31 scales", what);
   p.SK = (int)room;
   p.sK = fa_strides{0, c.s.h, c.s.s};

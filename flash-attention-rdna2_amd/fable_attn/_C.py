@@ -505,7 +505,7 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev):
 def _cache8(k_cache, v_cache, k_scale, v_scale, dtype, dev, rotary_rows=0):
     ks, vs, group = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, dev)
     _req(k_cache.stride() == v_cache.stride(), "8-bit k_cache and v_cache must have the same strides")
-    return _lib.FableCache8(k_scale.data_ptr(), v_scale.data_ptr(), ks, group, k_cache.shape[0], rotary_rows)
+    return _lib.FableCache8(k_scale.data_ptr(), v_scale.data_ptr(), ks, group, k_cache.shape[0], rotary_rows, None)
 
 
 def _check_table(block_table, batch, dev):
@@ -527,9 +527,10 @@ def _check_rotary(cos, sin, rotary_dim, D, dev):
 
 
 def dec8(q, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, new_k, new_v, cos, sin, interleaved, scale,
-         window, num_splits, leftpad, return_lse, softcap, alibi, rotary_pos):
+         window, num_splits, leftpad, return_lse, softcap, alibi, rotary_pos, held=None):
     """dec over a cache in 8 bits: codes [num_blocks, page, Hk, D] (strided pages, rows and heads), scales
-    [num_blocks, Hk, page / G]. block_table None: a dense cache, sequence b in page b."""
+    [num_blocks, Hk, page / G]. block_table None: a dense cache, sequence b in page b. leftpad: the first row a sequence's
+    queries see; held: the first one it has (an append keeps those of its block under its scale)."""
     _req(q.is_cuda, "GPU tensors required")
     _req(q.dim() == 4 and q.is_contiguous() and q.data_ptr() % 16 == 0, "decode expects contiguous q [B,nq,Hq,D], 16-byte aligned")
     _req(q.dtype in (torch.float16, torch.bfloat16), f"8-bit caches take fp16 or bf16 queries, got {q.dtype}")
@@ -544,9 +545,10 @@ def dec8(q, k_cache, v_cache, k_scale, v_scale, block_table, cache_seqlens, new_
     else:
         _req(nb >= B, f"a dense cache of {nb} rows for a batch of {B}")
     _check_index("cache_seqlens", cache_seqlens, dev, B)
-    for n, t in (("cache_leftpad", leftpad), ("rotary_seqlens", rotary_pos)):
+    for n, t in (("cache_leftpad", leftpad), ("cache_leftpad", held), ("rotary_seqlens", rotary_pos)):
         if t is not None:
             _check_index(n, t, dev, B)
+    c.held = held.data_ptr() if held is not None else None
     if alibi is not None:
         _check_f32("alibi_slopes", alibi, dev, Hq)
     rd = int(cos.shape[-1] * 2) if cos is not None else 0

@@ -78,7 +78,7 @@ class FablePagedKV(ctypes.Structure):
 
 class FableCache8(ctypes.Structure):
     _fields_ = [("k_scale", c_ptr), ("v_scale", c_ptr), ("s", Strides),
-                ("group", c_i32), ("num_blocks", c_i32), ("rotary_rows", c_i32)]
+                ("group", c_i32), ("num_blocks", c_i32), ("rotary_rows", c_i32), ("held", c_ptr)]
 
 
 class FableAppendParams(ctypes.Structure):

@@ -555,13 +555,15 @@ def _no_grad8(q):
 # 1000 keys (8M pairs) 40 / 48 us, 4 of 500 over 2000 (64M) 119 / 119, 4 of 1000 over 4000 (256M) 374 / 325, 1 of 4000
 # over 16000 (1024M) 1368 / 1038; pages of 64, 6 of 500-4000 over up to 5000 (1920M) 1216 / 1113. A window bounds the
 # keys of a row, not those of a gather (window 512: 430 / 450). Up to head dim 128 in place is the faster (D 128 570 /
-# 620, D 64 404 / 430).
-_GATHER8_PAIRS = 100_000_000
+# 620, D 64 404 / 430). The rows are laid out by the longest length, which needs no look at the others: no more than
+# _GATHER8_BYTES of them, however few a batch really holds.
+_GATHER8_PAIRS, _GATHER8_BYTES = 100_000_000, 8 << 30
 
 
-def _gather8_pays(batch, heads, max_sq, max_sk, wl, d):
+def _gather8_pays(batch, heads, heads_k, max_sq, max_sk, wl, d):
     """Whether packed prompts over an 8-bit cache are gathered first."""
-    return d > 128 and wl < 0 and batch * heads * max_sq * max_sk > _GATHER8_PAIRS
+    return (d > 128 and wl < 0 and batch * heads * max_sq * max_sk > _GATHER8_PAIRS
+            and batch * max_sk * heads_k * d * 4 <= _GATHER8_BYTES)
 
 
 def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, max_sk, seqused_q, seqused_k,
@@ -570,9 +572,11 @@ def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu
     decode, the launch parameters that the first call of a signature came to are kept per thread."""
     key, plans = None, _plans("prefill8_plans")
     try:
+        if any(type(x) is not int and type(x) is not bool and x is not None for x in hints + (kw["attention_chunk"],)):
+            raise TypeError("no key")
         key = (_place(q), _place(k_cache), _place(v_cache), _sig(k_scale), _sig(v_scale), _sig(block_table), _sig(cu_q), _sig(cu_k),
                _sig(seqused_q), _sig(seqused_k), kw["alibi_slopes"] is None, bool(kw["causal"]), kw["attention_chunk"],
-               _option_key(kw["softmax_scale"], kw["window_size"], kw["softcap"]), hints)
+               _option_key(kw["softmax_scale"], kw["window_size"], kw["softcap"]), hints, tuple(map(type, hints)))
         plan = plans.get(key)
     except (AttributeError, TypeError, ValueError, RuntimeError):   # not tensors, or no key
         key = plan = None
@@ -597,7 +601,7 @@ def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu
     idx = lambda t: _as_index(t, dev) if t is not None else None
     table, cq, ck, uq, uk = (idx(t) for t in (block_table, cu_q, cu_k, seqused_q, seqused_k))
     scalars = (spec.scale, bool(spec.causal), spec.wl, spec.wr, spec.softcap, spec.alibi)
-    if table.dim() == 2 and max_sk and _gather8_pays(table.shape[0], q.shape[1], int(max_sq), int(max_sk), spec.wl, q.shape[2]):
+    if table.dim() == 2 and max_sk and _gather8_pays(table.shape[0], q.shape[1], k_cache.shape[2], int(max_sq), int(max_sk), spec.wl, q.shape[2]):
         # every sequence's rows at its own multiple of the longest length (no host round trip for their sum)
         span = min(int(max_sk), table.shape[1] * k_cache.shape[1])
         cu = torch.arange(0, (table.shape[0] + 1) * span, span, dtype=torch.int32, device=dev)
@@ -615,7 +619,7 @@ def _prefill8_fast(plan, q, k_cache, v_cache, k_scale, v_scale, table, cu_q, cu_
     """One call of a planned signature; None when the rows are gathered first, an address is not aligned or the device is
     not current (the general path serves it)."""
     p, kv, c, dt, dev = plan
-    if p.HD > 128 and max_sk and _gather8_pays(p.batch, p.NH, max_sq, int(max_sk), p.win_left, p.HD):
+    if p.HD > 128 and max_sk and _gather8_pays(p.batch, p.NH, p.NH // p.gqa, max_sq, int(max_sk), p.win_left, p.HD):
         return None
     qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     if (qp | kp | vp) & 15 or dev != torch._C._cuda_getDevice():
@@ -649,7 +653,8 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
     launch of each backward kernel (the reference loops over the sequences in Python on the
     grad path, :523-540). With return_attn_probs: (out, [lse per sequence], [P per sequence]).
     With block_table, k and v are paged caches; with k_scale and v_scale too, caches held in 8 bits (see
-    flash_attn_append_kvcache), for inference: no gradient, dropout, qv or probabilities."""
+    flash_attn_append_kvcache), for inference: no gradient, dropout, qv or probabilities. max_seqlen_k is then the
+    longest length of the call, or 0 for none known; keys past it may be left out."""
     del deterministic
     if q.dim() != 3:
         raise ValueError(f"fable_attn: varlen expects (total, nheads, headdim), got {tuple(q.shape)}")
@@ -830,7 +835,7 @@ def _decode_fast(plan, q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table
     p.q, p.Kc, p.Vc, p.o, p.ctx_len = qp, kp, vp, out.data_ptr(), lens.data_ptr()
     p.block_table, p.cos, p.sin, p.leftpad, p.alibi = ptr(table), ptr(cos), ptr(sin), ptr(leftpad), ptr(alibi)
     if c is not None:
-        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        c.k_scale, c.v_scale, c.held = k_scale.data_ptr(), v_scale.data_ptr(), p.leftpad
         _lib.check(_C._L.fable_attn_dec8(p, c, dt, ptr(ws), need, torch._C._cuda_getCurrentRawStream(dev), nkp, nvp),
                    "fable_attn_dec8")
         return out
@@ -979,6 +984,7 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     keys_back = wl + 1 if 0 <= wl < 2 ** 31 - 1 else -1   # the kernel's window: keys up to the query
     dev = q.device
     leftpad = _as_index(cache_leftpad, dev) if cache_leftpad is not None else None
+    held = leftpad   # (what a sequence has; a chunk below narrows what its query sees)
     chunk = _check_chunk(attention_chunk)
     if chunk:
         if NQ > 1:
@@ -996,7 +1002,7 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
         out, lse = _C.dec8(_aligned(q, dense=True), k_cache, v_cache, k_scale, v_scale, table, lens,
                            _aligned(k, dense=True) if appending else None, _aligned(v, dense=True) if appending else None,
                            cos, sin, bool(rotary_interleaved), float(softmax_scale), int(keys_back), int(num_splits or 0),
-                           leftpad, bool(return_softmax_lse), float(softcap or 0.0), alibi, rpos)
+                           leftpad, bool(return_softmax_lse), float(softcap or 0.0), alibi, rpos, held)
         return (out, lse.transpose(1, 2).contiguous()) if return_softmax_lse else out
     out, lse = _C.dec(_aligned(q, dense=True), kc.contiguous(), vc.contiguous(), table, lens,
                       _aligned(k, dense=True) if appending else None,
@@ -1131,10 +1137,11 @@ def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, 
     k, v (batch, seqlen_new, nheads_k, d); or packed (total, nheads_k, d) with cu_seqlens int32 (batch+1) and
     max_seqlen, at least the longest sequence's count (a smaller one leaves tokens out; default: total). Token t of
     sequence b goes to position cache_seqlens[b] + t, which the caller then adds to its lengths, and is rotated by row
-    rotary_seqlens[b] + t (default: its position) of the tables. k_cache, v_cache: (num_blocks, page, nheads_k, d) with
+    rotary_seqlens[b] + t (default: its position) of the tables, the last row serving those past it. k_cache, v_cache: (num_blocks, page, nheads_k, d) with
     block_table, or dense (batch, seqlen, nheads_k, d), rows chosen by cache_batch_idx; pages, rows and heads may
     be strided. Positions past the table and table entries that name no page of the cache are dropped. Returns
-    q's tokens (batch, seqlen_new, nheads, d) or (total, nheads, d) rotated, in a new tensor; else None.
+    q's tokens (batch, seqlen_new, nheads, d) or (total, nheads, d) rotated, in a new tensor whose rows behind the last
+    sequence are not set; else None. No gradient passes through.
 
     Caches of k's dtype are written as they are. Caches held in 8 bits are torch.float8_e4m3fn with k_scale, v_scale
     torch.float8_e8m0fnu (num_blocks, nheads_k, page / G): G consecutive tokens of a head share a power of two (G a

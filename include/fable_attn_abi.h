@@ -375,6 +375,8 @@ typedef struct FableCache8 {
   fa_strides s;          /* of both caches */
   int32_t group, num_blocks;
   int32_t rotary_rows;   /* decode: rows of the rotary tables (positions past them use the last row) */
+  const int32_t* held;   /* decode that appends: the first row each sequence holds (FableAppendParams.leftpad; NULL: row 0).
+                            FableDecParams.leftpad says what the queries see, and may lie past it. */
 } FableCache8;
 
 /* fable_attn_dec_ws over an 8-bit cache (p.Kc / p.Vc: the codes): q and o in fp16 or bf16, any number of new

@@ -205,3 +205,17 @@ def test_plain_attention_is_softmax():
     assert torch.allclose(out[0], v[0]) and math.isinf(float(lse[2, 0])) and (out[2] == 0).all()
     w = torch.softmax(torch.einsum("hd,mhd->hm", q[1], k) * 0.25, -1)
     assert torch.allclose(out[1], torch.einsum("hm,mhd->hd", w, v))
+
+
+def test_pages_whose_rows_pass_32_bits_are_refused():
+    """A lone page's stride may be any number: its rows are what the kernels address."""
+    L, lib = _lib()
+    wide = L.Strides(0, 64, 1 << 20)
+    assert lib.fable_attn_dec8(_dec(page=4096), _cache(s=wide, num_blocks=1), 1, None, 0, None, None, None) == ARG
+    assert b"4 GiB" in lib.fable_attn_last_error()
+    p = L.FableFwdParams()
+    p.Q = p.K = p.V = p.O = p.cu_q = p.cu_k = 16
+    p.sQ = p.sO = L.Strides(0, 64, 128)
+    p.SQ, p.HD, p.NH, p.gqa, p.batch, p.win_left, p.win_right = 8, 64, 2, 1, 1, -1, -1
+    assert lib.fable_attn_fwd_paged8(p, L.FablePagedKV(16, 1, 2048, 0, 0), _cache(s=wide, num_blocks=1), 1, None, 0, None) == ARG
+    assert b"2 GiB" in lib.fable_attn_last_error()

@@ -637,3 +637,49 @@ def test_wide_prompts_gathered_first(page, seqused, monkeypatch):
     _check_prompts("bf16", [5, 70, 33], [0, 50, 90], 4, 2, 256, page, 16, seqused=seqused)
     _check_prompts("fp16", [40], [3], 4, 4, 192, page, 8, softcap=10.0)
     assert len(calls) == 2
+
+
+@pytest.mark.parametrize("leftpad", [None, [0, 18]])
+def test_a_chunk_of_attention_leaves_the_rows_before_it_their_scale(leftpad):
+    """attention_chunk ends inside a block of tokens: the new token's block keeps the older rows under its scale, though
+    the query does not see them."""
+    dt, hq, hk, d, page, group, lens, chunk = torch.bfloat16, 4, 2, 128, 32, 16, [30, 29], 24
+    pool = _filled(lens, 1, page, hk, d, group, dt, 77, scale=20.0, leftpad=leftpad)
+    q, k, v = (_rand((2, 1, h, d), dt, 3 + i, 0.01) for i, h in enumerate((hq, hk, hk)))
+    c = pool.cuda()
+    out = _fa().flash_attn_with_kvcache(q.cuda(), c[0], c[1], k=k.cuda(), v=v.cuda(), cache_seqlens=_i32(lens), block_table=c[4],
+                                        k_scale=c[2], v_scale=c[3], attention_chunk=chunk, causal=True,
+                                        cache_leftpad=_i32(leftpad) if leftpad else None)
+    for b, n in enumerate(lens):
+        pool.append(b, n, k[b].double(), v[b].double(), leftpad=leftpad[b] if leftpad else 0)
+    _same_pool(pool, c, exact=True)
+    for b, n in enumerate(lens):
+        kk, vv = pool.values(b, 0, n + 1)
+        want, _, err, weight, _ = ref.attend(q[b].double(), kk, vv, [n // chunk * chunk], [n + 1], [n], d ** -0.5)
+        ref.close(out[b], want, err, weight, dt, ref.HALF[dt], f"sequence {b}")
+
+
+def test_wide_prompts_gather_into_memory_that_held_no_numbers(monkeypatch):
+    from fable_attn import flash_attn_interface as fai
+    monkeypatch.setattr(fai, "_GATHER8_PAIRS", 0)
+    torch.cuda.empty_cache()
+    # (the gathered rows: 3 sequences of the longest length, 140)
+    stale = [torch.full((3 * 140, 2, 256), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    del stale
+    _check_prompts("bf16", [5, 70, 33], [0, 70, 90], 4, 2, 256, 16, 16)
+
+
+def test_a_call_of_a_known_signature_still_checks_its_hints():
+    pool = _filled([20], 2, 16, 2, 64, 16, torch.bfloat16, 9)
+    c = pool.cuda()
+    q = _rand((20, 4, 64), torch.bfloat16, 1).cuda()
+    call = lambda **kw: _fa().flash_attn_varlen_func(q, *c[:2], _cu([20]), _cu([20]), 20, 20, causal=True, block_table=c[4],
+                                                     k_scale=c[2], v_scale=c[3], **kw)
+    want = call(pack_gqa=True)
+    assert torch.equal(call(pack_gqa=True), want)
+    with pytest.raises(TypeError, match="pack_gqa"):
+        call(pack_gqa=1)
+    with pytest.raises(TypeError, match="num_splits"):
+        call(pack_gqa=True, num_splits=1.0)
+    with pytest.raises(ValueError, match="attention_chunk"):
+        call(pack_gqa=True, attention_chunk=0.0)
