@@ -486,18 +486,25 @@ struct GatherArgs : FableGatherParams {
   int page_shift, gshift;
 };
 
-// One wave per row of the output, its keys and values; the row's sequence by bisection of cu.
+// One wave per row of the output, its keys and values, eight per lane and pass. The row's sequence is found by 64
+// entries of cu at a time (a bisection took a memory latency for every doubling of the batch), the loads of kPasses
+// passes are in flight together, and a row that is not there reads page 0. What bounds it: a few rows the launch and
+// four dependent latencies (cu, table, rows and scales); many the bytes.
 template <typename T, bool Q8>
 __global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
+  constexpr int kPasses = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long row = (long long)blockIdx.x * 4 + wave;
   if (row >= p.total) return;
-  int lo = 0, hi = p.batch;   // the last sequence that starts at or before the row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu[mid] <= row) lo = mid;
-    else hi = mid;
+  int lo = 0;   // the last sequence that starts at or before the row
+  for (int n = p.batch; n > 1;) {
+    const int step = (n + 63) / 64, at = lo + lane * step;
+    const bool before = lane * step < n && p.cu[min(at, p.batch)] <= row;
+    const int k = max(__popcll(__builtin_amdgcn_ballot_w64(before)) - 1, 0) * step;
+    lo += k;
+    n = min(step, n - k);
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
   const long long j = row - p.cu[lo];
   if (p.used && (p.batch <= 0 || j < 0 || j >= p.used[lo])) return;
   int blk = -1;
@@ -506,26 +513,41 @@ __global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
     blk = p.block_table ? p.block_table[at] : (int)at;
     if ((unsigned)blk >= (unsigned)p.num_blocks) blk = -1;
   }
-  const int in = (int)(j & ((1 << p.page_shift) - 1));
-  const int per = p.HD / 8, chunks = p.NKV * per;
-  for (int i = lane; i < 2 * chunks; i += 64) {
-    const int kv = i >= chunks, c = i - kv * chunks, h = c / per, d = 8 * (c - h * per);
-    const fa_strides s = kv ? p.vc : p.kc;
-    T* dst = (T*)(kv ? p.v_out : p.k_out) + (row * p.NKV + h) * p.HD + d;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (blk >= 0) {
-      const long long off = (long long)blk * s.b + (long long)in * s.s + (long long)h * s.h + d;
+  const int in = (int)(j & ((1 << p.page_shift) - 1)), in0 = blk >= 0 ? in : 0;
+  const int per = p.HD / 8, chunks = p.NKV * per, subs = Q8 ? 1 << (p.page_shift - p.gshift) : 0;
+  const long long page = max(blk, 0);
+  for (int i0 = lane; i0 < 2 * chunks; i0 += 64 * kPasses) {
+    u32x2 code[kPasses];
+    unsigned scale[kPasses];
+    float x[kPasses][8];
+    int col[kPasses];
+#pragma unroll
+    for (int u = 0; u < kPasses; u++) {
+      const int i = min(i0 + 64 * u, 2 * chunks - 1), kv = i >= chunks, c = i - kv * chunks, h = c / per, d = 8 * (c - h * per);
+      const fa_strides s = kv ? p.vc : p.kc;
+      const long long off = page * s.b + (long long)in0 * s.s + (long long)h * s.h + d;
+      const void* cache = kv ? p.Vc : p.Kc;
+      col[u] = h * p.HD + d;
       if constexpr (Q8) {
-        const int subs = 1 << (p.page_shift - p.gshift);
-        const unsigned e = (kv ? p.v_scale : p.k_scale)[((long long)blk * p.NKV + h) * subs + (in >> p.gshift)];
-        const auto v = codes_to<T>(*(const u32x2*)((const uint8_t*)(kv ? p.Vc : p.Kc) + off), e8_f32(e));
-        *(u32x4*)dst = bitcast<u32x4>(v);
-        continue;
+        scale[u] = (kv ? p.v_scale : p.k_scale)[(page * p.NKV + h) * subs + (in0 >> p.gshift)];
+        code[u] = *(const u32x2*)((const uint8_t*)cache + off);
       } else {
-        load8((const T*)(kv ? p.Vc : p.Kc) + off, x);
+        load8((const T*)cache + off, x[u]);
       }
     }
-    store8(dst, x);
+#pragma unroll
+    for (int u = 0; u < kPasses; u++) {
+      if (i0 + 64 * u >= 2 * chunks) break;
+      T* dst = (T*)(i0 + 64 * u >= chunks ? p.v_out : p.k_out) + row * p.NKV * p.HD + col[u];
+      if constexpr (Q8) {
+        const auto v = codes_to<T>(code[u], e8_f32(scale[u]));
+        *(u32x4*)dst = blk >= 0 ? bitcast<u32x4>(v) : u32x4{0, 0, 0, 0};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[u][e] = blk >= 0 ? x[u][e] : 0.0f;
+        store8(dst, x[u]);
+      }
+    }
   }
 }
 

@@ -275,6 +275,20 @@ def test_gather_of_missing_pages_and_dense_rows():
     assert none.shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("batch", [2, 63, 64, 65, 200, 4100])
+def test_gather_finds_the_sequence_among_many(batch):
+    """Rows of many sequences, empty ones among them, all over the same few pages."""
+    r = random.Random(batch)
+    pool = _filled([16] * 4, 1, 16, 2, 64, 16, torch.bfloat16, 13)
+    c = pool.cuda()
+    lens = [r.choice([0, 0, 1, 2, 5]) for _ in range(batch)]
+    which = [r.randrange(4) for _ in range(batch)]
+    table = c[4][_i32(which).long()].contiguous()
+    k, v = _fa().flash_attn_gather_kvcache(*c[:2], _cu(lens), sum(lens) + 3, block_table=table, k_scale=c[2], v_scale=c[3])
+    want = [torch.cat([pool.values(w, 0, n)[i] for w, n in zip(which, lens)] + [torch.zeros(3, 2, 64, dtype=torch.float64)]) for i in range(2)]
+    assert torch.equal(k.cpu().double(), want[0]) and torch.equal(v.cpu().double(), want[1])
+
+
 # ----------------------------------------------------------------------------- decode
 def _check_decode(dtype, lens, hq, hk, d, page, group, nq=1, append=False, window=-1, softcap=0.0, alibi=False, leftpad=None,
                   rotary=0, interleaved=False, dense=False, max_blocks=None, num_splits=0, lse=True, hide=True, seed=0, scale=None,
