@@ -50,7 +50,9 @@ struct Dec8Lds {
   // touch every bank once. Scales: 32 of K, 32 of V, fp32.
   static constexpr int STR = HD + 16;
   static constexpr int WAVE = 2 * kKeys8 * STR + 64 * 4;   // K, V, scales
-  static constexpr int ACC = kDecWaves * 16 * HD * 4;       // the merge's accumulators (q staging is smaller)
+  // rows of q (fp32) and of the merge's accumulators, padded likewise: 16 lanes write or read a column of them
+  static constexpr int FSTR = HD + 4;
+  static constexpr int ACC = kDecWaves * 16 * FSTR * 4;     // (q's rows are as many at most)
   static constexpr int BYTES = kDecWaves * WAVE > ACC ? kDecWaves * WAVE : ACC;
 };
 
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   constexpr int DEPTH = HD <= 192 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) char raw[L::BYTES];
   __shared__ float red_m[kDecWaves][16], red_l[kDecWaves][16];
-  float (*qsh)[HD] = (float (*)[HD])raw;
+  float (*qsh)[L::FSTR] = (float (*)[L::FSTR])raw;
 
   const int append = p.flags & kDec8Append, page_shift = p.page_shift;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -118,16 +120,15 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
   }
   for (bool more = true; more;) {
     const int b = SHARE ? sq : by;
-    // q rows of this group, loaded while the lengths are on their way
-    constexpr int RCH = HD / 8, NQ = WH * 16 * RCH, NQI = (NQ + 255) / 256;
-    u32x4 qraw[NQI];
+    // Q^T as the B operand, loaded while the lengths are on their way. A 16-byte read of a K row holds dims 64m + 16lg ..
+    // +15 and feeds steps 2m and 2m + 1, so step 2m + s takes dims 64m + 16lg + 8s + e of row lh.
+    auto dim = [&](int ds) { return 64 * (ds / 2) + 16 * lg + 8 * (ds % 2); };
+    u32x4 qraw[NDS];
     {
       const Dec8Args p = args();
+      const T* row = (const T*)p.q + row_of(b, kvh, min(lh, hg - 1)) * HDr;
 #pragma unroll
-      for (int u = 0; u < NQI; u++) {
-        const int i = min(tid + 256 * u, NQ - 1), g = i / RCH % 16, c = i % RCH;
-        qraw[u] = *(const u32x4*)((const T*)p.q + row_of(b, head0 + i / RCH / 16, min(g, hg - 1)) * HDr + (8 * c < HDr ? 8 * c : 0));
-      }
+      for (int ds = 0; ds < NDS; ds++) qraw[ds] = *(const u32x4*)(row + (dim(ds) < HDr ? dim(ds) : 0));
     }
     DecSpan sp;
     int start, end;
@@ -187,22 +188,25 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
       c_log2 = p.scale * kLog2e;
     }
 
-    // ---- q rows -> LDS (fp32), rotated; zero columns past the head dim
+    // ---- zero columns past the head dim; a rotated q goes through LDS in fp32 and is carried as hi + lo
+    V8 qb[NDS], ql[NDS];
 #pragma unroll
-    for (int u = 0; u < NQI; u++) {
-      const int i = tid + 256 * u, g = i / RCH, c = i % RCH;
-      const bool cok = 8 * c < HDr;
-      const V8 v = bitcast<V8>(qraw[u]);
-      if (i < NQ)
-#pragma unroll
-        for (int e = 0; e < 8; e++) qsh[g][8 * c + e] = g % 16 < hg && cok ? (float)v[e] : 0.0f;
+    for (int ds = 0; ds < NDS; ds++) {
+      qb[ds] = bitcast<V8>(dim(ds) < HDr ? qraw[ds] : u32x4{0, 0, 0, 0});
+      ql[ds] = bitcast<V8>(u32x4{0, 0, 0, 0});
     }
-    __syncthreads();
     bool qsplit;
     {
       const Dec8Args p = args();
       qsplit = p.rotary != 0;
       if (p.rotary) {
+        if (rw == 0) {
+#pragma unroll
+          for (int ds = 0; ds < NDS; ds++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) qsh[16 * hw + lh][dim(ds) + e] = (float)qb[ds][e];
+        }
+        __syncthreads();
         const int rdim = p.rotary_dim > 0 ? p.rotary_dim : HDr, half = rdim / 2;
         const int rbase = p.rotary_pos ? p.rotary_pos[b] : ctx;
         for (int i = tid; i < WH * 16 * half; i += 256) {
@@ -216,21 +220,17 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
           qsh[g][ib] = y * c + x * s;
         }
         __syncthreads();
+#pragma unroll
+        for (int ds = 0; ds < NDS; ds++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float x = qsh[16 * hw + lh][dim(ds) + e];
+            qb[ds][e] = (T)x;
+            ql[ds][e] = (T)(x - (float)(T)x);
+          }
+        __syncthreads();  // q staging is dead from here on
       }
     }
-    // Q^T as the B operand: a 16-byte read of a K row holds dims 64m + 16lg .. +15 and feeds steps 2m and 2m + 1,
-    // so step 2m + s takes dims 64m + 16lg + 8s + e. A rotated q is carried as hi + lo.
-    V8 qb[NDS], ql[NDS];
-#pragma unroll
-    for (int ds = 0; ds < NDS; ds++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float x = qsh[16 * hw + lh][64 * (ds / 2) + 16 * lg + 8 * (ds % 2) + e];
-        const T hi = (T)x;
-        qb[ds][e] = hi;
-        ql[ds][e] = (T)(x - (float)hi);
-      }
-    __syncthreads();  // q staging is dead from here on
 
     f32x4 oacc[NDB];
 #pragma unroll
@@ -435,42 +435,46 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     // ---- merge the four waves: per row max, sum and O^T accumulators through LDS
     const float l_grp = half_sum(lane16_sum(l_run));
     __syncthreads();
-    float* red_o = (float*)raw;  // [wave][16 rows][HD]
+    float* red_o = (float*)raw;  // [wave][16 rows][FSTR]
     if (lg == 0) {
       red_m[wave][lh] = m_run;
       red_l[wave][lh] = l_grp;
     }
 #pragma unroll
-    for (int db = 0; db < NDB; db++) *(f32x4*)(red_o + (wave * 16 + lh) * HD + 16 * db + 4 * lg) = oacc[db];
+    for (int db = 0; db < NDB; db++) *(f32x4*)(red_o + (wave * 16 + lh) * L::FSTR + 16 * db + 4 * lg) = oacc[db];
     __syncthreads();
     const Dec8Args pe = args();
-    for (int i = tid; i < WH * hg * HDr; i += 256) {
-      const int r = i / HDr, d = i % HDr, h = WH > 1 ? r / hg : 0, g = r - h * hg;
+    const int quads = HDr / 4;
+    for (int i = tid; i < WH * hg * quads; i += 256) {
+      const int r = i / quads, d = 4 * (i - r * quads), h = WH > 1 ? r / hg : 0, g = r - h * hg;
       float gm = -INFINITY;
 #pragma unroll
       for (int w = 0; w < WR; w++) gm = fmaxf(gm, red_m[WH * w + h][g]);
-      float l = 0.0f, acc = 0.0f;
+      float l = 0.0f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       if (gm != -INFINITY) {
 #pragma unroll
         for (int w = 0; w < WR; w++) {
           const float f = exp2_fast(red_m[WH * w + h][g] - gm);
           l += f * red_l[WH * w + h][g];
-          acc += f * red_o[((WH * w + h) * 16 + g) * HD + d];
+          acc += f * *(const f32x4*)(red_o + ((WH * w + h) * 16 + g) * L::FSTR + d);
         }
       }
       const long long row = row_of(b, head0 + h, g);
       if (!rec) {
         const bool ok = gm != -INFINITY && l > 0.0f;
-        ((T*)pe.o)[row * HDr + d] = (T)(ok ? acc / l : 0.0f);
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        V4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (T)(ok ? acc[e] / l : 0.0f);
+        *(V4*)((T*)pe.o + row * HDr + d) = v;
         if (pe.lse_out && d == 0) pe.lse_out[row] = ok ? gm * kLn2 + __logf(l) : -INFINITY;
         continue;
       }
-      float* out = rec + (SHARE ? 16 * h + g : row) * rec_step;
-      if (d == 0) {
-        out[0] = gm;
-        out[1] = l;
-      }
-      out[2 + d] = acc;
+      float* out = rec + (SHARE ? 16 * h + g : row) * rec_step;   // (8-byte aligned: HDr is even)
+      if (d == 0) *(f32x2*)out = f32x2{gm, l};
+      *(f32x2*)(out + 2 + d) = f32x2{acc[0], acc[1]};
+      *(f32x2*)(out + 4 + d) = f32x2{acc[2], acc[3]};
     }
     if (more) __syncthreads();  // the merge has read the LDS regions before the next segment fills them
   }
