@@ -482,14 +482,15 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
 
 // Heads of a workgroup. One wave per head makes what the CUs read at a time runs of 4 * D bytes in place of D, which HBM
 // gives faster (rows of 128 bytes at 1 KiB: 6.24 TB/s alone, 7.1 in fours); but a wave then walks four times the keys, and there
-// are four times the records, so it takes a large call: 16 x 32768 keys of 8 heads, D 128: 185 -> 162 us, 48 of up to 8192 108 -> 85,
-// 16 x 8000 (262 MB) 58 -> 54; 16 x 2000 (67 MB) 20.3 and 21.9, 64 x 1000 (134 MB) 32.4 and 33.0, one of 500 9.5 and 17.
-// The size is the table's: 32 of 3000 keys in tables of 8192 42.8 and 43.6, of 1000 21.1 and 24.7.
-// Two where there are no four (6 heads of 64, 64 x 4000 keys: 69 -> 52), and at D 192 (32 x 4000 keys of 16 heads: 179 -> 161,
-// 157 with four; of 4 heads 46.1 and 47.6, 50.5 with four). Rows of 256 bytes gain nothing (32 x 4000, 8 heads: 99, 103, 105).
-// (Split counts the caller sets are for one head to a workgroup.) A row must not get more than 32 records (one of 64000 keys, 32 heads, 100 -> 96; 16 heads 57.2, 55.7 in twos, 60.1
-// in fours; 8 heads in a table of 131072 35.6, 47.6 in fours).
-constexpr long long kHeadBytes8 = 176LL << 20, kHeadGroups8 = 8;
+// are four times the records, so it takes a large call: 16 x 32768 keys of 8 heads, D 128: 199 -> 172 us, 48 of up to 8192 98 -> 80,
+// 16 x 8000 (262 MB) 55 -> 49, 64 x 1000 (134 MB) 31 -> 29, 64 x 2000 of 4 heads (134 MB) 26.1 and 27.0; 16 x 2000 (67 MB)
+// 18.6 and 18.3, 64 x 1000 of 4 heads 15.8 and 17.5, one of 500 8.4 and 13.3. The size is the table's, however full: 32 of 300
+// keys in tables of 8192 14.5 and 15.8, of 1000 19.1 and 20.7, of 3000 41.2 and 40.8.
+// Two where there are no four (6 heads of 64, 64 x 4000 keys: 70 -> 53), and at D 192 (32 x 4000 keys of 16 heads: 169 -> 158,
+// 154 with four; of 4 heads 41.7 and 42.7, 45.7 with four). Rows of 256 bytes gain nothing (32 x 4000, 8 heads: 97, 99, 98).
+// (Split counts the caller sets are for one head to a workgroup.) A row must not get more than 32 records (one of 64000
+// keys, 16 heads 54.8, 52.4 in twos, 56.0 in fours; 8 heads in a table of 131072 33.7, 44.3 in fours).
+constexpr long long kHeadBytes8 = 112LL << 20, kHeadGroups8 = 8;
 static int dec8_heads(const FableDecParams& p) {
   const int nkv = p.NH / p.gqa;
   if (p.nsplit > 0 || p.HD > 192 || (long long)p.batch * p.max_blocks * p.page * nkv * p.HD * 2 < kHeadBytes8) return 1;
