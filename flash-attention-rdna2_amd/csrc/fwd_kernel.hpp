@@ -993,7 +993,7 @@ struct CfgTag {
 };
 
 // Launcher of the paged instances: C for the plain masks, CF for the feature masks and for a
-// rotated q. A grid that leaves CUs idle splits the keys of each tile (as fwd_split_count, up
+// rotated q (over 8-bit pages: below). A grid that leaves CUs idle splits the keys of each tile (as fwd_split_count, up
 // to kPagedSplitMax shares of at least kPagedSplitTiles tiles of the longest cache the table holds); a
 // split count of the caller's is taken as it is, up to kPagedSplitMax.
 constexpr int kPagedSplitMax = 32, kPagedSplitTiles = 4;
@@ -1043,6 +1043,18 @@ static int launch_fwd_pg(const FableFwdParams& p, const PGT& pg, bool rot, hipSt
   };
   using Y = std::integral_constant<bool, true>;
   using N = std::integral_constant<bool, false>;
+  if constexpr (std::is_same<PGT, FwdPaged8>::value && !std::is_same<C, CF>::value) {
+    // Over 8-bit pages the plain masks go by the rows of a (sequence, K/V head), a rotated q's too: C's tall tile from more
+    // than half of it on, CF's half as tall below. D 128, us with CF / C: 64 rows (16 sequences of 4000 keys, 16 heads)
+    // 96 / 118, rotated 114 / 157; 128 (1 of 4000, 8 heads) 23.6 / 24.2, 30.4 / 32.7; 256 (4 of 2000) 33.8 / 33.3,
+    // 42.9 / 43.4; 1024 (4 of 4000) 102 / 86, 129 / 118; 4096 (2 of 4000) 165 / 135, 213 / 191. D 64: 128 rows 17.1 / 18.7,
+    // 256 24.5 / 24.0.
+    const bool tall = 2LL * p.SQ * p.gqa > C::BR;
+    if (!feat) {
+      if (rot) return tall ? go(CfgTag<C>{}, N{}, Y{}) : go(CfgTag<CF>{}, N{}, Y{});
+      return tall ? go(CfgTag<C>{}, N{}, N{}) : go(CfgTag<CF>{}, N{}, N{});
+    }
+  }
   if (rot) return feat ? go(CfgTag<CF>{}, Y{}, Y{}) : go(CfgTag<CF>{}, N{}, Y{});
   return feat ? go(CfgTag<CF>{}, Y{}, N{}) : go(CfgTag<C>{}, N{}, N{});
 }

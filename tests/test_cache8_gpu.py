@@ -419,6 +419,15 @@ def test_many_new_tokens(d, kw, dtype):
     _check_decode(dtype, [0, 40, 130], 8, 2, d, 16, 16, nq=17, **kw)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("d,nq,kw", [(128, 70, {"rotary": 128}), (128, 33, {}), (64, 70, {"rotary": 64, "interleaved": True}), (96, 40, {"rotary": 32}),
+                                     (64, 33, {})])
+def test_many_rows_of_a_head(d, nq, kw, page, dtype):
+    """Rows of a K/V head on both sides of the tall tile's half (128 rows), and past one tile."""
+    _check_decode(dtype, [0, 40, 130, 7, 65], 8, 2, d, page, 16, nq=nq, append=True, **kw)
+
+
 def test_decode_reads_strided_caches_and_packed_queries():
     dt, lens, hq, hk, d, page = torch.bfloat16, [40, 7], 4, 2, 64, 16
     pool = _filled(lens, 3, page, hk, d, 16, dt, 1)
