@@ -706,3 +706,56 @@ def test_a_call_of_a_known_signature_still_checks_its_hints():
         call(pack_gqa=True, num_splits=1.0)
     with pytest.raises(ValueError, match="attention_chunk"):
         call(pack_gqa=True, attention_chunk=0.0)
+
+
+def test_two_graphs_over_one_pool(monkeypatch):
+    """A prompt step (packed append, prompts in place and gathered, many new tokens) and a decode step (shared out on the
+    device, four heads to a workgroup) in two graphs over one memory pool, replayed in turn with eager work between."""
+    fa = _fa()
+    from fable_attn import flash_attn_interface as fai
+    monkeypatch.setattr(fai, "_GATHER8_PAIRS", 0)
+    dt, hq, hk, page, new, held = torch.bfloat16, 16, 8, 16, [33, 5, 20, 1, 64], [0, 300, 40, 900, 7]
+    total = [a + b for a, b in zip(new, held)]
+    pools = [(d, _filled(held, 64, page, hk, d, 16, dt, 5)) for d in (128, 256)]
+    mine, eager = ([p.cuda() for _, p in pools] for _ in range(2))
+    wide = [torch.cat((c[4], c[4][:, :1].expand(5, 2048 - 64)), 1).contiguous() for c in mine]
+    cu, cuk, hold, full = _cu(new), _cu(total), _i32(held), _i32(total)
+    cos, sin = (x.cuda() for x in ref.tables(1024, 64))
+    toks = [[_rand((sum(new), h, d), dt, d + i).cuda() for i, h in enumerate((hq, hk, hk))] for d in (128, 256)]
+    qd = [_rand((5, n, hq, 128), dt, n).cuda() for n in (1, 40)]
+
+    def prompts(caches):
+        outs = []
+        for c, (q, k, v) in zip(caches, toks):
+            s = dict(block_table=c[4], k_scale=c[2], v_scale=c[3])
+            rq = fa.flash_attn_append_kvcache(k, v, *c[:2], hold, q=q, cu_seqlens=cu, max_seqlen=64, rotary_cos=cos, rotary_sin=sin, **s)
+            outs += [rq, fa.flash_attn_varlen_func(rq, *c[:2], cu, cuk, 64, 964 if c[0].shape[3] > 128 else 0, causal=True, **s)]
+        return outs
+
+    def decode(caches):
+        c = caches[0]
+        s = dict(k_scale=c[2], v_scale=c[3], cache_seqlens=full)
+        return [fa.flash_attn_with_kvcache(qd[0], *c[:2], block_table=wide[0], **s),
+                fa.flash_attn_with_kvcache(qd[1], *c[:2], block_table=c[4], rotary_cos=cos, rotary_sin=sin, **s)]
+
+    for f in (prompts, decode):   # (warm: the first call of a signature also checks it)
+        f(mine)
+        f(eager)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g, f in zip(graphs, (prompts, decode)):
+        with torch.cuda.graph(g, pool=graphs[0].pool() if outs else None):
+            outs.append(f(mine))
+    for i in range(3):
+        for t in [x for ts in toks for x in ts] + qd:
+            t.copy_(_rand(t.shape, dt, 100 * i + t.shape[-1] + t.shape[-2]).cuda())
+        torch.cuda.synchronize()
+        for g, f, got in zip(graphs, (prompts, decode), outs):
+            g.replay()
+            torch.cuda.synchronize()
+            got = [x.clone() for x in got]   # (the pool's memory is shared: the next graph may write there)
+            for a, b in zip(got, f(eager)):
+                assert torch.equal(a, b), i
+        for a, b in zip(mine, eager):
+            for x, y in zip(a[:4], b[:4]):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
