@@ -759,3 +759,24 @@ def test_two_graphs_over_one_pool(monkeypatch):
         for a, b in zip(mine, eager):
             for x, y in zip(a[:4], b[:4]):
                 assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_append_prompts_and_gather_past_32_bits(d):
+    """A cache of more than 2^32 bytes, its last pages in use: the same bits as in a small one."""
+    fa = _fa()
+    dt, hq, hk, page, n = torch.bfloat16, 16, 8, 256, 300
+    nb = (1 << 32) // (page * hk * d) + 5
+    e4, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    q, k, v = (_rand((n, h, d), dt, 5 + i).cuda() for i, h in enumerate((hq, hk, hk)))
+    got = []
+    for blocks, table in ((2, [1, 0]), (nb, [nb - 1, nb - 2])):
+        kc, vc = (torch.full((blocks, page, hk, d), 0x7F, dtype=torch.uint8, device="cuda").view(e4) for _ in range(2))
+        ks, vs = (torch.full((blocks, hk, page // 16), 255, dtype=torch.uint8, device="cuda").view(e8) for _ in range(2))
+        s = dict(block_table=_i32([table]), k_scale=ks, v_scale=vs)
+        fa.flash_attn_append_kvcache(k, v, kc, vc, _i32([0]), cu_seqlens=_cu([n]), max_seqlen=n, **s)
+        out = fa.flash_attn_varlen_func(q, kc, vc, _cu([n]), _cu([n]), n, n, causal=True, **s)
+        many = fa.flash_attn_with_kvcache(q[None, :100].contiguous(), kc, vc, cache_seqlens=_i32([n]), **s)
+        got.append((*fa.flash_attn_gather_kvcache(kc, vc, _cu([n]), n, **s), out, many))
+    for a, b in zip(*got):
+        assert torch.isfinite(a.float()).all() and torch.equal(a, b)
