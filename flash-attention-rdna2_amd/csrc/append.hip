@@ -157,8 +157,8 @@ __device__ __forceinline__ void turn(const AppendArgs& p, const Chunks& k, const
 // Loads carry no lane condition (a row that is not there reads the sequence's first or last token), so those of a
 // tile are in flight together. What bounds it: a step of few tokens the launch and two dependent
 // memory latencies (lengths, then rows): 48 tokens of 64 + 8 heads of 128, rotated, 7.5-8.7 us; prompts the bytes read and
-// written: 11400 tokens of 32 + 8 heads of 128, rotated, blocks of 64, 75 us for 262 MB (3.5 TB/s: the angles of every
-// head's keys come from L2 beside them); 24 of 64 to 2048 tokens of 8 heads in 16 bits 52 us for 232 MB (4.5 TB/s, a copy's).
+// written: 11400 tokens of 32 + 8 heads of 128, rotated, blocks of 64, 70 us for 262 MB (3.7 TB/s: the angles of every
+// two heads' keys come from L2 beside them); 24 of 64 to 2048 tokens of 8 heads in 16 bits 52 us for 232 MB (4.5 TB/s, a copy's).
 template <typename T, bool Q8, int NP, int HB, int WB, int LPR, bool ANY>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
   constexpr int R = 64 / LPR, NH = NP > 0 ? NP : 1;
@@ -311,12 +311,15 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
     for (int g = 0; g < HB; g++)
       for (int m = 1; m < span; m <<= 1) top[g] = fmaxf(top[g], __shfl_xor(top[g], m));   // over the block's lanes
     if constexpr (WB > 1) {   // and its waves
-      __shared__ float tops[4];
-      static_assert(HB == 1, "one head");
-      if (lane == 0) tops[wave] = top[0];
+      __shared__ float tops[HB][4];
+      if (lane == 0)
+#pragma unroll
+        for (int g = 0; g < HB; g++) tops[g][wave] = top[g];
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < WB; w++) top[0] = fmaxf(top[0], tops[wave / WB * WB + w]);
+      for (int g = 0; g < HB; g++)
+#pragma unroll
+        for (int w = 0; w < WB; w++) top[g] = fmaxf(top[g], tops[g][wave / WB * WB + w]);
     }
     if (blk < 0) return;
 #pragma unroll
@@ -402,7 +405,9 @@ static int launch_append_lpr(AppendArgs& a, hipStream_t st) {
   if (a.rot >= kRotHalvesAny) return go(I0{}, I1{}, I1{}, std::integral_constant<bool, true>{});
   if constexpr (Q8) {
     // (four passes at most, but for the longest blocks: with eight in one wave the instance held 200 registers, and a
-    // prompt of 11400 tokens with 32 query heads, blocks of 64, took 85 us; 74 with four in each of two waves)
+    // prompt of 11400 tokens with 32 query heads of 128, blocks of 64, took 85 us; 67 with four in each of two waves, 62 with two
+    // passes of two heads in each of four, which halves the angles read: eight passes go so. Two of four heads 107, and the
+    // sixteen passes of blocks of 128 as four of two heads 116 for 66, both out of registers.)
     // Heads share a wave only where there are waves enough without (a chip holds some 2000 of these): 32 tokens of 4
     // heads of 256 took 10.1 us with four heads to a wave, 5.5 with one.
     const bool few = tiles * a.batch * 2 * a.NKV <= 2048;
@@ -410,7 +415,7 @@ static int launch_append_lpr(AppendArgs& a, hipStream_t st) {
       case 0: return few ? go(I1{}, I1{}, I1{}, N{}) : go(I1{}, I4{}, I1{}, N{});
       case 1: return few ? go(I2{}, I1{}, I1{}, N{}) : go(I2{}, I2{}, I1{}, N{});
       case 2: return go(I4{}, I1{}, I1{}, N{});
-      case 3: return go(I4{}, I1{}, I2{}, N{});
+      case 3: return go(I2{}, I2{}, I4{}, N{});
       case 4: return go(I4{}, I1{}, I4{}, N{});
       case 5: return go(I8{}, I1{}, I4{}, N{});
       default: return go(I0{}, I1{}, I1{}, N{});   // (blocks of 256 rows wider than 128)
