@@ -812,12 +812,16 @@ def _decode_plan(q, k_cache, v_cache, k, v, cos, sin, lens, leftpad, table, alib
     p.rotary_dim = int(cos.shape[-1] * 2) if cos is not None else 0
     dt = _C._dt(q)
     c = None
+    # (the workspace depends on which optional tensors a call has: the query sees this one's)
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    p.block_table, p.cos, p.sin, p.leftpad, p.alibi = ptr(table), ptr(cos), ptr(sin), ptr(leftpad), ptr(alibi)
     if q8:
         c = _C._cache8(k_cache, v_cache, k_scale, v_scale, q.dtype, dev, cos.shape[0] if cos is not None else 0)
         need = int(_C._L.fable_attn_dec8_ws_bytes(p, c, dt, 1 if k is not None else 0))
         c.k_scale = c.v_scale = None
     else:
         need = int(_C._L.fable_attn_dec_ws_bytes(p, dt, 1 if k is not None else 0))
+    p.block_table = p.cos = p.sin = p.leftpad = p.alibi = None
     return None if need < 0 else (p, dt, need, c)
 
 

@@ -340,7 +340,8 @@ int fable_attn_dec(FableDecParams p, int dtype, void* stream, const void* new_k,
  * split count, 0 for the library's choice (at most 32 splits on the tile path, 512 elsewhere).
  * p.block_table may be NULL in fp16/bf16: sequence b's pages are then b*max_blocks, b*max_blocks+1,
  * ... (a dense cache). fable_attn_dec_ws_bytes gives the bytes to pass (256-byte aligned device memory, scratch per call); `append` tells whether
- * new_k/new_v will be passed. Same results as fable_attn_dec up to fp32 summation order. The tokens of
+ * new_k/new_v will be passed, and the optional pointers of p (leftpad, alibi, cos, block_table) are to be NULL or not as in the call:
+ * the path and its splits depend on it (not on what they point to). Same results as fable_attn_dec up to fp32 summation order. The tokens of
  * a call share the reads of K and V: a V row that is not finite reaches the results of the tokens that
  * do not see it too (as in the forward, whose masked keys meet probabilities of 0). */
 int64_t fable_attn_dec_ws_bytes(FableDecParams p, int dtype, int append);
@@ -381,8 +382,8 @@ typedef struct FableCache8 {
 
 /* fable_attn_dec_ws over an 8-bit cache (p.Kc / p.Vc: the codes): q and o in fp16 or bf16, any number of new
  * tokens, p.block_table NULL for a dense cache. new_k / new_v (of q's type) are quantised into the cache
- * first, as fable_attn_append does. Same arguments, workspace contract and results as there, with the K and
- * V that the codes stand for. */
+ * first, as fable_attn_append does. Same arguments, workspace contract (the query is given the pointers of the call) and results as there, with the K and
+ * V that the codes stand for; a workspace smaller than the call's own query is refused. */
 int64_t fable_attn_dec8_ws_bytes(FableDecParams p, FableCache8 c, int dtype, int append);
 int fable_attn_dec8(FableDecParams p, FableCache8 c, int dtype, void* ws, int64_t ws_bytes, void* stream, const void* new_k,
                     const void* new_v);
