@@ -13,6 +13,12 @@ __device__ __forceinline__ float xor16_max(float x) {
 }
 __device__ __forceinline__ float xor16_sum(float x) { return x + __shfl_xor(x, 16); }
 
+// The maximum that a wave hands on of a row whose weights sum to l. A score that is no number (of a query or key with
+// a NaN, or of infinities) drops out of the running maximum but not out of l, which is then no number either. Such a
+// row goes on with a maximum of +inf: every merge gives it the weight 2^(inf - inf), so its output and LSE are NaN,
+// whatever the row's other waves and splits saw. (Its running maximum may still be -inf, that of a row without keys.)
+__device__ __forceinline__ float dec_row_max(float m, float l) { return l == l ? m : INFINITY; }
+
 // Rows of a (sequence, K/V head): its nq new tokens x the gqa q heads of its group, token first;
 // workgroups take them in groups of 16. The keys of a sequence some row sees are [lo, hi); row
 // masks cut them down (a row of token tk sees [max(leftpad, pos - window + 1), ctx + (append ? tk +

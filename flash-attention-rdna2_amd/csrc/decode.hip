@@ -448,7 +448,7 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
   __syncthreads();  // every wave is done with its V slice: reuse it for the accumulators
   float* red_o = (float*)vraw;  // [wave][16 heads][HD]
   if (lg == 0) {
-    red_m[wave][lh] = m_run;
+    red_m[wave][lh] = dec_row_max(m_run, l_grp);
     red_l[wave][lh] = l_grp;
   }
 #pragma unroll
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256) void dec_partial_kernel(DecArgs p) {
     const long long row = row_of(b, g);
     if (!rec) {
       // what the combine kernel computes from one split (its weight exp2(0) is exactly 1)
-      const bool ok = gm != -INFINITY && l > 0.0f;
+      const bool ok = gm != -INFINITY;
       ((T*)pe.o)[row * HDr + d] = (T)(ok ? acc / l : 0.0f);
       if (pe.lse_out && d == 0) pe.lse_out[row] = ok ? gm * kLn2 + __logf(l) : -INFINITY;
       continue;
@@ -640,7 +640,7 @@ __global__ __launch_bounds__(256) void dec_partial_f32_kernel(FableDecParams p, 
   __syncthreads();  // q staging is dead: the region holds the accumulators
   float* red_o = (float*)raw;  // [wave][16 heads][HD]
   if (lg == 0) {
-    red_m[wave][lh] = m_run;
+    red_m[wave][lh] = dec_row_max(m_run, l_grp);
     red_l[wave][lh] = l_grp;
   }
 #pragma unroll
@@ -735,7 +735,7 @@ __global__ __launch_bounds__(256) void dec_combine_kernel(FableDecParams p, int 
     merge(std::integral_constant<int, 2>{});
   else
     merge(std::integral_constant<int, NC>{});
-  const bool ok = gm != -INFINITY && l > 0.0f;
+  const bool ok = gm != -INFINITY;   // (some key was seen: l is 1 at least, or no number)
   if (d < HDr) ((T*)p.o)[((long long)row * p.NH + h) * HDr + d] = (T)(ok ? acc / l : 0.0f);
   if (p.lse_out && d == 0) p.lse_out[(long long)row * p.NH + h] = ok ? gm * kLn2 + __logf(l) : -INFINITY;
 }

@@ -441,7 +441,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
     __syncthreads();
     float* red_o = (float*)raw;  // [wave][16 rows][FSTR]
     if (lg == 0) {
-      red_m[wave][lh] = m_run;
+      red_m[wave][lh] = dec_row_max(m_run, l_grp);
       red_l[wave][lh] = l_grp;
     }
 #pragma unroll
@@ -466,7 +466,7 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
       }
       const long long row = row_of(b, head0 + h, g);
       if (!rec) {
-        const bool ok = gm != -INFINITY && l > 0.0f;
+        const bool ok = gm != -INFINITY;
         typedef T V4 __attribute__((ext_vector_type(4)));
         V4 v;
 #pragma unroll

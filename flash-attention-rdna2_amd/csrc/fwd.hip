@@ -102,7 +102,8 @@ __global__ __launch_bounds__(256) void fwd_split_combine_kernel(FableFwdParams p
 #pragma unroll
   for (int e = 0; e < 4; e++) o[e] = (T)(acc[e] * inv);
   *(u32x2*)((T*)p.O + orow + 4 * c) = __builtin_bit_cast(u32x2, o);
-  if (c == 0 && p.LSE) p.LSE[lrow] = m != -INFINITY ? m + __logf(wsum) : -INFINITY;
+  // (a row whose scores are no numbers: NaN over a cache, -inf over contiguous keys, as the unsplit kernel writes)
+  if (c == 0 && p.LSE) p.LSE[lrow] = (PG ? m != -INFINITY : wsum > 0.0f) ? m + __logf(wsum) : -INFINITY;
 }
 
 template <typename T, class PGT>

@@ -88,7 +88,7 @@ struct FwdSplit {
   int nqt, br;     // query tiles per (sequence, head) and rows per tile of the launch
   long long rows;  // work items * br
   float* o;        // [n][rows][p.HD]
-  float* lse;      // [n][rows], natural log; -inf where a split saw no key of the row
+  float* lse;      // [n][rows], natural log; -inf where a split saw no key of the row, +inf where a score is no number
 };
 
 // K/V in pages of a cache (fwd_kernel with PGT = FwdPaged): row j of sequence z is row

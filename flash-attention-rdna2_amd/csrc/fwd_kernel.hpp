@@ -975,7 +975,10 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
 #pragma unroll
       for (int db = 0; db < C::NDB; db++)
         store_cblock_f32(sp.o + r * HDr + db * 32, oacc[i][db], inv, hh, qi < SQ, HDr - db * 32);
-      if (qi < SQ && hh == 0) sp.lse[r] = l_tot > 0.0f ? (m_run[i] + m_base) * kLn2 + __logf(l_tot) : -INFINITY;
+      // (a row with a score that is no number, whose sum is none either: +inf, which makes NaN of the merge; the row
+      // of another share, or one without keys, would hide it)
+      if (qi < SQ && hh == 0)
+        sp.lse[r] = l_tot > 0.0f ? (m_run[i] + m_base) * kLn2 + __logf(l_tot) : (l_tot == l_tot ? -INFINITY : INFINITY);
       continue;
     }
     T* orow = Og + (PG ? (long long)ptok * p.sO.s + (long long)phead * p.sO.h : (long long)qi * p.sO.s);
@@ -984,7 +987,8 @@ fwd_kernel(FableFwdParams p, int nqt, FwdSplit sp, PGT pg) {
       store_cblock<T>(orow + db * 32, oacc[i][db], inv, hh, qi < SQ, HDr - db * 32);
     if (qi < SQ) {
       if (p.LSE && hh == 0)
-        p.LSE[PG ? sv.lse0 + (long long)(h + phead) * p.lse_sh + paged_lse(pg, ptok) : sv.lse0 + qi] = l_tot > 0.0f ? (m_run[i] + m_base) * kLn2 + __logf(l_tot) : -INFINITY;
+        p.LSE[PG ? sv.lse0 + (long long)(h + phead) * p.lse_sh + paged_lse(pg, ptok) : sv.lse0 + qi] =
+            l_tot > 0.0f ? (m_run[i] + m_base) * kLn2 + __logf(l_tot) : (PG && l_tot != l_tot ? l_tot : -INFINITY);
     }
   }
 }
