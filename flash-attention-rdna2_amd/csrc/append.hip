@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
 #pragma unroll
     for (int g = 0; g < HB; g++) {
       sc[g] = (kind == 0 ? p.k_scale : p.v_scale) + ((long long)max(blk, 0) * p.NKV + min(h0 + g, p.NKV - 1)) * subs + (in >> p.gshift);
-      was[g] = min((int)*sc[g], 253) - 127;
+      was[g] = min((int)*sc[g], 254) - 127;   // (255 is no number: as the largest)
     }
     float x[HB][NH][2][8], top[HB];
     auto fetch = [&](int i, int j) {   // pass i of all heads, to x[.][j]

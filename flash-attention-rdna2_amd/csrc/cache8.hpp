@@ -20,8 +20,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // the fp32 of an e8m0 byte (byte 0, below every scale an append stores, becomes 0)
 __device__ __forceinline__ float e8_f32(unsigned byte) { return __uint_as_float(byte << 23); }
-// 2^e for e in [-126, 127]
-__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+// 2^e for e in [-127, 127] (2^-127, the inverse of the largest scale, is subnormal)
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(e > -127 ? (unsigned)(e + 127) << 23 : 0x400000u); }
 
 // eight codes times `scale` (a power of two) in T
 template <typename T>
