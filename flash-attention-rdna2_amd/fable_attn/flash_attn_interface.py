@@ -555,15 +555,17 @@ def _no_grad8(q):
 # 1000 keys (8M pairs) 40 / 48 us, 4 of 500 over 2000 (64M) 119 / 119, 4 of 1000 over 4000 (256M) 374 / 325, 1 of 4000
 # over 16000 (1024M) 1368 / 1038; pages of 64, 6 of 500-4000 over up to 5000 (1920M) 1216 / 1113. A window bounds the
 # keys of a row, not those of a gather (window 512: 430 / 450). Up to head dim 128 in place is the faster (D 128 570 /
-# 620, D 64 404 / 430). The rows are laid out by the longest length, which needs no look at the others: no more than
-# _GATHER8_BYTES of them, however few a batch really holds.
+# 620, D 64 404 / 430). A sequence's rows are laid out by the table's width, the only bound
+# that holds for sure without a look at the lengths (max_seqlen_k is the caller's word; rows cut off by one that is too small
+# would move the causal diagonal): no more than _GATHER8_BYTES of them, however few a batch really holds. Rows that no
+# sequence has cost little (1 of 4000 over 16000 under tables 1, 4 and 16 times as wide: 987, 979 and 986, in place 1280).
 _GATHER8_PAIRS, _GATHER8_BYTES = 100_000_000, 8 << 30
 
 
-def _gather8_pays(batch, heads, heads_k, max_sq, max_sk, wl, d):
-    """Whether packed prompts over an 8-bit cache are gathered first."""
-    return (d > 128 and wl < 0 and batch * heads * max_sq * max_sk > _GATHER8_PAIRS
-            and batch * max_sk * heads_k * d * 4 <= _GATHER8_BYTES)
+def _gather8_pays(batch, heads, heads_k, max_sq, max_sk, rows, wl, d):
+    """Whether packed prompts over an 8-bit cache, under a table for `rows` rows of a sequence, are gathered first."""
+    return (d > 128 and wl < 0 and rows > 0 and batch * heads * max_sq * min(max_sk, rows) > _GATHER8_PAIRS
+            and batch * rows * heads_k * d * 4 <= _GATHER8_BYTES)
 
 
 def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu_k, max_sq, max_sk, seqused_q, seqused_k,
@@ -601,9 +603,9 @@ def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu
     idx = lambda t: _as_index(t, dev) if t is not None else None
     table, cq, ck, uq, uk = (idx(t) for t in (block_table, cu_q, cu_k, seqused_q, seqused_k))
     scalars = (spec.scale, bool(spec.causal), spec.wl, spec.wr, spec.softcap, spec.alibi)
-    if table.dim() == 2 and max_sk and _gather8_pays(table.shape[0], q.shape[1], k_cache.shape[2], int(max_sq), int(max_sk), spec.wl, q.shape[2]):
-        # every sequence's rows at its own multiple of the longest length (no host round trip for their sum)
-        span = min(int(max_sk), table.shape[1] * k_cache.shape[1])
+    span = table.shape[1] * k_cache.shape[1] if table.dim() == 2 else 0
+    if max_sk and _gather8_pays(table.shape[0], q.shape[1], k_cache.shape[2], int(max_sq), int(max_sk), span, spec.wl, q.shape[2]):
+        # every sequence's rows at its own multiple of what its table holds (no host round trip for their sum)
         cu = torch.arange(0, (table.shape[0] + 1) * span, span, dtype=torch.int32, device=dev)
         used = (uk if uk is not None else ck[1:] - ck[:-1]).clamp(0, span)
         _, _, (k, v) = _C.gather(k_cache, v_cache, cu, table.shape[0] * span, q.dtype, table, k_scale, v_scale, used)
@@ -619,7 +621,7 @@ def _prefill8_fast(plan, q, k_cache, v_cache, k_scale, v_scale, table, cu_q, cu_
     """One call of a planned signature; None when the rows are gathered first, an address is not aligned or the device is
     not current (the general path serves it)."""
     p, kv, c, dt, dev = plan
-    if p.HD > 128 and max_sk and _gather8_pays(p.batch, p.NH, p.NH // p.gqa, max_sq, int(max_sk), p.win_left, p.HD):
+    if p.HD > 128 and max_sk and _gather8_pays(p.batch, p.NH, p.NH // p.gqa, max_sq, int(max_sk), kv.max_blocks * kv.page, p.win_left, p.HD):
         return None
     qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     if (qp | kp | vp) & 15 or dev != torch._C._cuda_getDevice():
@@ -653,8 +655,8 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, ma
     launch of each backward kernel (the reference loops over the sequences in Python on the
     grad path, :523-540). With return_attn_probs: (out, [lse per sequence], [P per sequence]).
     With block_table, k and v are paged caches; with k_scale and v_scale too, caches held in 8 bits (see
-    flash_attn_append_kvcache), for inference: no gradient, dropout, qv or probabilities. max_seqlen_k is then the
-    longest length of the call, or 0 for none known; keys past it may be left out."""
+    flash_attn_append_kvcache), for inference: no gradient, dropout, qv or probabilities. max_seqlen_k, the
+    longest length of the call or 0 for none known, then only chooses between two ways to read them."""
     del deterministic
     if q.dim() != 3:
         raise ValueError(f"fable_attn: varlen expects (total, nheads, headdim), got {tuple(q.shape)}")
