@@ -559,7 +559,9 @@ def _no_grad8(q):
 # that holds for sure without a look at the lengths (max_seqlen_k is the caller's word; rows cut off by one that is too small
 # would move the causal diagonal): no more than _GATHER8_BYTES of them, however few a batch really holds. Rows that no
 # sequence has cost little (1 of 4000 over 16000 under tables 1, 4 and 16 times as wide: 987, 979 and 986, in place 1280).
-_GATHER8_PAIRS, _GATHER8_BYTES = 100_000_000, 8 << 30
+# The bytes are few because a server gives its memory to the cache, and a gather that finds none of it left is no
+# failure: the pages are read in place then.
+_GATHER8_PAIRS, _GATHER8_BYTES = 100_000_000, 1 << 30
 
 
 def _gather8_pays(batch, heads, heads_k, max_sq, max_sk, rows, wl, d):
@@ -608,8 +610,12 @@ def _paged_prefill8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, cu
         # every sequence's rows at its own multiple of what its table holds (no host round trip for their sum)
         cu = torch.arange(0, (table.shape[0] + 1) * span, span, dtype=torch.int32, device=dev)
         used = (uk if uk is not None else ck[1:] - ck[:-1]).clamp(0, span)
-        _, _, (k, v) = _C.gather(k_cache, v_cache, cu, table.shape[0] * span, q.dtype, table, k_scale, v_scale, used)
-        return _C.fwd_varlen(_aligned(q), k, v, cq, cu, int(max_sq), span, *scalars, 0.0, 0, spec.chunk, uq, used)
+        try:
+            _, _, (k, v) = _C.gather(k_cache, v_cache, cu, table.shape[0] * span, q.dtype, table, k_scale, v_scale, used)
+        except torch.cuda.OutOfMemoryError:
+            k = None
+        if k is not None:
+            return _C.fwd_varlen(_aligned(q), k, v, cq, cu, int(max_sq), span, *scalars, 0.0, 0, spec.chunk, uq, used)
     out, launch = _C.fwd_paged8(_aligned(q), k_cache, v_cache, k_scale, v_scale, table, cq, ck, int(max_sq), *scalars, spec.chunk, uq, uk)
     if (key is not None and spec.alibi is None and _in_place(q)
             and all(a is b for a, b in zip((table, cq, ck, uq, uk), (block_table, cu_q, cu_k, seqused_q, seqused_k)))):

@@ -1,4 +1,5 @@
-"""Packed prompts over an 8-bit cache, read in place or gathered first: one result, whatever max_seqlen_k says."""
+"""Packed prompts over an 8-bit cache, read in place or gathered first: one result, whatever max_seqlen_k says and
+whether there is memory for the gather."""
 import pytest
 import torch
 
@@ -35,3 +36,15 @@ def test_the_longest_length_of_a_prompt_call_moves_no_key(max_sk, monkeypatch):
     got, want = _prompts(max_sk)
     assert len(calls) == 1
     _close(got, want)
+
+
+def test_prompts_that_find_no_memory_to_gather_in(monkeypatch):
+    from fable_attn import flash_attn_interface as fai
+    monkeypatch.setattr(fai, "_GATHER8_PAIRS", 0)
+
+    def full(*a):
+        raise torch.cuda.OutOfMemoryError("no memory")
+
+    monkeypatch.setattr(fai._C, "gather", full)
+    got, want = _prompts(123)
+    assert torch.equal(got, want)   # read in place, both

@@ -86,3 +86,14 @@ def test_the_plan_holds_no_address(q8, kw):
             assert getattr(p, name) is None, name
     if c is not None:
         assert c.k_scale is None and c.v_scale is None and c.held is None
+
+
+def test_prompts_are_gathered_within_bounds():
+    """The route of packed prompts over an 8-bit cache: wide heads, enough pairs, no window, and a temporary copy that is
+    small next to a cache, whatever the caller takes for the longest length."""
+    pays = fai._gather8_pays
+    many = dict(batch=4, heads=16, heads_k=4, max_sq=1000, max_sk=4000, rows=4000, wl=-1, d=256)
+    assert pays(**many)
+    for kw in ({"d": 128}, {"wl": 512}, {"max_sq": 100}, {"max_sk": 10}, {"rows": 0}, {"rows": 1 << 18}, {"batch": 1 << 12}):
+        assert not pays(**dict(many, **kw)), kw
+    assert pays(**dict(many, max_sk=1 << 20)) and not pays(**dict(many, max_sk=1 << 20, rows=16))
