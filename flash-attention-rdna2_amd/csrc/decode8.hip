@@ -304,18 +304,12 @@ __global__ __launch_bounds__(256) void dec8_partial_kernel(Dec8Args p) {
         const int f = 64 * i + lane;
         // (rows ahead of klo in a run's first chunk: zeros too)
         const int o = front && kc0 + f / RB < klo ? kBufZero : off[i];
+        // (a load of the wave lies in one page: 16 rows are HD chunks, whole loads)
+        static_assert(HD % 64 == 0, "loads of a page of 16 rows");
         constexpr int kLo = 16 * RB;   // chunks of the first page
-        if (!P16 || 64 * i + 63 < kLo) {
-          r.k[i] = buf_load16_nt(kr[0], o);
-          r.v[i] = buf_load16_nt(vr[0], o);
-        } else if (64 * i >= kLo) {
-          r.k[i] = buf_load16_nt(kr[NPG - 1], o);
-          r.v[i] = buf_load16_nt(vr[NPG - 1], o);
-        } else {   // rows of both pages (width 192): each lane from its own
-          const int o0 = f < kLo ? o : kBufZero, o1 = f < kLo ? kBufZero : o;
-          r.k[i] = buf_load16_nt(kr[0], o0) | buf_load16_nt(kr[NPG - 1], o1);
-          r.v[i] = buf_load16_nt(vr[0], o0) | buf_load16_nt(vr[NPG - 1], o1);
-        }
+        const int pg = P16 && 64 * i >= kLo ? NPG - 1 : 0;
+        r.k[i] = buf_load16_nt(kr[pg], o);
+        r.v[i] = buf_load16_nt(vr[pg], o);
       }
       // scale of key kc0 + (lane & 31): K's for the first 32 lanes, V's for the others
       const unsigned pg = P16 && (lane & 16) ? blk[NPG - 1] : blk[0];
