@@ -165,12 +165,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bt = blockIdx.x / p.wgs, wg = blockIdx.x - bt * p.wgs;
   const int b = bt / p.tiles, tile = bt - b * p.tiles;
-  // units of K and V, padded to whole workgroups where they are of several waves, then those of q
-  const int kvw = WB > 1 ? (2 * p.ukv * WB + 3) / 4 * 4 : 2 * p.ukv, at = wg * 4 + wave;
+  // units of K and V (of one wave, or of a workgroup's four, which meet at a barrier), then those of q
+  static_assert(WB == 1 || WB == 4, "waves of a unit");
+  const int kvw = 2 * p.ukv * WB, at = wg * 4 + wave;
   const int unit = at < kvw ? at / WB : 2 * p.ukv + at - kvw;
-  if (WB == 1 || at >= kvw) {
-    if (unit >= 2 * p.ukv + p.uq) return;
-  }
+  if (unit >= 2 * p.ukv + p.uq) return;
   const int kind = at >= kvw ? 2 : (unit < p.ukv ? 0 : 1);   // q, K, V
   const int ctx = p.ctx_len[b], c0 = p.cu ? p.cu[b] : 0, n = p.cu ? p.cu[b + 1] - c0 : p.n;
   const long long base = (((long long)max(ctx, 0) >> p.tshift) + tile) << p.tshift, stop = (long long)ctx + n;
@@ -319,7 +318,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
 #pragma unroll
       for (int g = 0; g < HB; g++)
 #pragma unroll
-        for (int w = 0; w < WB; w++) top[g] = fmaxf(top[g], tops[g][wave / WB * WB + w]);
+        for (int w = 0; w < WB; w++) top[g] = fmaxf(top[g], tops[g][w]);
     }
     if (blk < 0) return;
 #pragma unroll
@@ -389,7 +388,7 @@ static int launch_append_lpr(AppendArgs& a, hipStream_t st) {
     auto units = [](int heads, int per) { return (heads + per - 1) / per; };
     a.ukv = a.k ? units(a.NKV, Q8 ? HB : kHeadsPerWave) : 0;
     a.uq = a.q ? units(a.NH, kHeadsPerWave) << (a.tshift - rshift) : 0;
-    const int waves = (WB > 1 ? (2 * a.ukv * WB + 3) / 4 * 4 : 2 * a.ukv) + a.uq;
+    const int waves = 2 * a.ukv * WB + a.uq;
     a.wgs = (waves + 3) / 4;
     if (tiles > 0x7FFFFFFF / a.batch / a.wgs) return fail(FA_ERR_ARG, "fable_attn_append: grid too large");
     a.tiles = (int)tiles;
