@@ -907,6 +907,11 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     return res
 
 
+_RAGGED = ("write the new tokens, and rotate q, with flash_attn_append_kvcache(..., cu_seqlens=...) and attend with "
+           "flash_attn_varlen_func(..., causal=True, block_table=...), or append the same number of tokens to every "
+           "batch element with a 4-D q")
+
+
 @torch.no_grad()
 def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
                   rotary_cos=None, rotary_sin=None,
@@ -933,8 +938,7 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     del scheduler_metadata      # the launcher plans each call itself (fa_decode_num_splits)
     if cu_seqlens_k_new is not None:
         raise NotImplementedError(
-            "fable_attn: cu_seqlens_k_new (ragged append) is not supported; append the same "
-            "number of tokens to every batch element")
+            "fable_attn: cu_seqlens_k_new (ragged append) is not supported here; " + _RAGGED)
     q8 = k_scale is not None or v_scale is not None
     if q8:
         if k_scale is None or v_scale is None:
@@ -1039,8 +1043,7 @@ def _kvcache_packed_q(q, k_cache, v_cache, k, qv, cu_seqlens_q, max_seqlen_q, re
     past it would land in the next sequence's slots."""
     if k is not None:
         raise NotImplementedError(
-            "fable_attn: appending k/v with cu_seqlens_q (a ragged append) is not supported; "
-            "append the same number of tokens to every batch element with a 4-D q")
+            "fable_attn: appending k/v with cu_seqlens_q (a ragged append) is not supported here; " + _RAGGED)
     if q.dim() != 3:
         raise ValueError(f"fable_attn: with cu_seqlens_q, q must be (total_q, nheads, headdim), "
                          f"got {tuple(q.shape)}")
