@@ -614,7 +614,9 @@ static int dec8_check(FableDecParams& p, const FableCache8& c, int dtype) {
   if (p.nsplit < 0 || p.nsplit > 512) return fail(FA_ERR_ARG, "%s: nsplit=%d", what, p.nsplit);
   if (p.max_blocks < 1 || (long long)p.max_blocks * p.page > 0x7FFF0000)
     return fail(FA_ERR_ARG, "%s: max_blocks=%d page=%d", what, p.max_blocks, p.page);
-  if (p.batch > 65535 || (long long)p.nq * p.gqa > (1 << 24)) return fail(FA_ERR_ARG, "%s: batch=%d nq=%d", what, p.batch, p.nq);
+  // (rows of q, and the heads of a sequence's tokens, are counted in 32 bits)
+  if (p.batch > 65535 || (long long)p.nq * p.gqa > (1 << 24) || (long long)p.batch * p.nq > 0x7FFFFFFF || (long long)p.nq * p.NH > 0x7FFFFFFF)
+    return fail(FA_ERR_ARG, "%s: batch=%d nq=%d", what, p.batch, p.nq);
   if (p.rotary && (p.rotary_dim < 0 || p.rotary_dim > p.HD || p.rotary_dim % 2)) return fail(FA_ERR_ARG, "%s: rotary_dim=%d", what, p.rotary_dim);
   if (p.rotary && (p.rotary > 2 || c.rotary_rows < 1)) return fail(FA_ERR_ARG, "%s: rotary=%d rotary_rows=%d", what, p.rotary, c.rotary_rows);
   if (c.s.b > 0xFFFFFFFFll || p.page * c.s.s > 0xFFFFFFFFll) return fail(FA_ERR_ARG, "%s: pages of 4 GiB", what);

@@ -97,3 +97,18 @@ def test_prompts_are_gathered_within_bounds():
     for kw in ({"d": 128}, {"wl": 512}, {"max_sq": 100}, {"max_sk": 10}, {"rows": 0}, {"rows": 1 << 18}, {"batch": 1 << 12}):
         assert not pays(**dict(many, **kw)), kw
     assert pays(**dict(many, max_sk=1 << 20)) and not pays(**dict(many, max_sk=1 << 20, rows=16))
+
+
+@pytest.mark.parametrize("batch,nq,heads,gqa,window", [
+    (128, 1 << 24, 1, 1, 0), (65535, 32769, 1, 1, 0), (1, 1 << 24, 128, 1, -1), (1, 1 << 22, 512, 4, 64)])
+def test_decode_refuses_more_rows_than_32_bits_count(batch, nq, heads, gqa, window):
+    """Tokens of a call, and heads of a sequence's tokens: past 2^31 the kernels' row numbers would wrap around."""
+    lib = _lib.load()
+    p = _lib.FableDecParams()
+    p.q = p.Kc = p.Vc = p.o = p.ctx_len = p.block_table = 16    # never dereferenced
+    p.batch, p.NH, p.gqa, p.HD, p.page, p.max_blocks, p.nq, p.window, p.scale = batch, heads, gqa, 16, 16, 4, nq, window, 0.25
+    c = _lib.FableCache8(16, 16, _lib.Strides(16 * 16 * heads, 16, 16 * heads), 16, 4, 0)
+    assert lib.fable_attn_dec8_ws_bytes(p, c, 1, 0) == -1 and b"nq" in lib.fable_attn_last_error()
+    assert lib.fable_attn_dec8(p, c, 1, None, 0, None, None, None) == 3
+    p.nq = 1
+    assert lib.fable_attn_dec8_ws_bytes(p, c, 1, 0) >= 0
