@@ -151,14 +151,17 @@ __device__ __forceinline__ void turn(const AppendArgs& p, const Chunks& k, const
 // registers between the search for the largest value and the rounding (NP 0: any number of passes, read twice,
 // the second time from L2), and HB heads of the keys or values, which share their angles: a head of 128 has half as many
 // bytes as its angles, which came from L2 for every head before (8192 tokens of 8 heads, blocks of 16: 24.3 us,
-// 17.3 without a rotation). Rows that need no scale (queries, caches of 16 and 32 bits) go four heads to a unit of
+// 17.3 without a rotation, the angles' way through scratch, below, included). Rows that need no scale (queries, caches of 16 and 32 bits) go four heads to a unit of
 // one wave and one pass. The units of a tile follow one another in the grid, so that the heads of a token are
 // read together (rather than the tiles of a head one after another).
-// Loads carry no lane condition (a row that is not there reads the sequence's first or last token), so those of a
-// tile are in flight together. What bounds it: a step of few tokens the launch and two dependent
-// memory latencies (lengths, then rows): 48 tokens of 64 + 8 heads of 128, rotated, 7.5-8.7 us; prompts the bytes read and
-// written: 11400 tokens of 32 + 8 heads of 128, rotated, blocks of 64, 70 us for 262 MB (3.7 TB/s: the angles of every
-// two heads' keys come from L2 beside them); 24 of 64 to 2048 tokens of 8 heads in 16 bits 52 us for 232 MB (4.5 TB/s, a copy's).
+// Loads carry no lane condition (a row that is not there reads the sequence's first or last token). Those of one pass
+// of one head are in flight together; the next pass or head is asked for when this one has been turned. The two forms of
+// load_angles fill one array from different loads, which the compiler joins through memory: 28 bytes of scratch per lane in every
+// instance that takes whole chunks, written and read back between the angles and the rows. What bounds it: a step of few tokens
+// the launch and a chain of latencies (lengths, table, then angles, scratch and rows of each pass and head, and the older codes of a block
+// whose scale grows): 48 tokens of 64 + 8 heads of 128, rotated, 9.0 us (a gather of few rows, four latencies, 3.3); prompts that chain
+// beside the bytes: 11400 tokens of 32 + 8 heads of 128, rotated, blocks of 64, 71 us for 262 MB (3.7 TB/s: the angles of every
+// two heads' keys come from L2 beside them); 24 of 64 to 2048 tokens of 8 heads in 16 bits 50 us for 232 MB (4.6 TB/s, a copy's).
 template <typename T, bool Q8, int NP, int HB, int WB, int LPR, bool ANY>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs p) {
   constexpr int R = 64 / LPR, NH = NP > 0 ? NP : 1;
@@ -495,8 +498,9 @@ struct GatherArgs : FableGatherParams {
 // One wave per row of the output, its keys and values, eight per lane and pass. The row's sequence is found by 64
 // entries of cu at a time (a bisection took a memory latency for every doubling of the batch), the loads of kPasses
 // passes are in flight together, and a row that is not there reads page 0. What bounds it: a few rows the launch and
-// four dependent latencies (cu, table, rows and scales): 300 rows of 8 heads of 64 3.6 us; many the bytes: 16 requests of
-// 500 to 8000 rows, 8 heads of 128, 507 MB in 97 us (5.2 TB/s, written at twice the bytes it is read at).
+// four dependent latencies (cu, table, rows and scales): 300 rows of 8 heads of 64 3.3 us; many the bytes: 16 requests of
+// 500 to 8000 rows, 8 heads of 128, 507 MB in 97 us (5.2 TB/s, written at twice the bytes it is read at); over 16-bit pages 557 MB
+// of as many requests in 109 us, in 32 bits 1114 MB in 217 (5.1 TB/s both).
 template <typename T, bool Q8>
 __global__ __launch_bounds__(256) void gather_kernel(GatherArgs p) {
   constexpr int kPasses = 4;

@@ -21,6 +21,10 @@
 // in this pattern 151), 48 requests of 64 to 8192 keys under pages of 16, 428 MB: 74 and 5.5 (5.4 TB/s; the shares and the prologue
 // of their segments are the rest). Small calls wait for a chain of latencies (lengths, table, rows, merge): 2000 keys 7.2
 // and 3.7 us, 8 x 4 drafted tokens in a window of 512, D 256, 12 and 4.
+// An append is a launch ahead of this one. A share or split starts at a multiple of 32 keys, and a chunk of 32 is one wave's,
+// so with one row group and blocks of at most 32 tokens the wave that reads a new token's block could also write
+// it (where no other sequence names its page); it does not yet. Nor is a row asked for before q has been rotated, though
+// only the lengths and the table are needed for it.
 // Not taken: the products of e4m3 operands with e8m0 scales (v_mfma_scale_f32_16x16x128_f8f6f4), K as it is and q as
 // a sum of e4m3 parts. They need no conversion of K, but add their 128 products aligned to the largest: with one
 // dimension of q and k 30 times the others, scores of size 100 were off by up to 0.1.

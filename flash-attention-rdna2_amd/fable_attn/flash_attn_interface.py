@@ -932,7 +932,8 @@ def _with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None,
     the cache first, and then token t also sees the new keys up to its own. Returns out, or
     (out, softmax_lse (batch, nheads, seqlen_q)). Reference :583-771.
     k_scale and v_scale: the caches are held in 8 bits (flash_attn_append_kvcache says how); q, k and v are fp16
-    or bf16, and new k/v are quantised as that function does."""
+    or bf16, and new k/v are quantised as that function does: two sequences of a call must not append to one block of G
+    tokens (over a 16-bit cache they may share a page, at rows of their own)."""
     _reject_fp8(q_descale, k_descale, v_descale)
     _accept_hints(num_splits, pack_gqa, sm_margin)
     del scheduler_metadata      # the launcher plans each call itself (fa_decode_num_splits)
@@ -1152,7 +1153,8 @@ def flash_attn_append_kvcache(k, v, k_cache, v_cache, cache_seqlens, *, q=None, 
                               rotary_sin=None, rotary_interleaved=True, rotary_seqlens=None, k_scale=None, v_scale=None):
     """Write new keys and values into a cache, the keys (and, if given, the queries) rotated on the way.
     k, v (batch, seqlen_new, nheads_k, d); or packed (total, nheads_k, d) with cu_seqlens int32 (batch+1) and
-    max_seqlen, at least the longest sequence's count (a smaller one leaves tokens out; default: total). Token t of
+    max_seqlen, at least the longest sequence's count (a smaller one leaves tokens out; default: total, for which every
+    sequence gets as many workgroups as all of them need). Token t of
     sequence b goes to position cache_seqlens[b] + t, which the caller then adds to its lengths, and is rotated by row
     rotary_seqlens[b] + t (default: its position) of the tables, the last row serving those past it. k_cache, v_cache: (num_blocks, page, nheads_k, d) with
     block_table, or dense (batch, seqlen, nheads_k, d), rows chosen by cache_batch_idx; pages, rows and heads may
