@@ -48,6 +48,9 @@ extern "C" size_t fable_attn_struct_size(int which) {
     case 8: return sizeof(FableCache8);
     case 9: return sizeof(FableAppendParams);
     case 10: return sizeof(FableGatherParams);
+    case 11: return sizeof(FableLinearParams);
+    case 12: return sizeof(FableRotaryParams);
+    case 13: return sizeof(FableRotaryTableParams);
     default: return 0;
   }
 }

@@ -1,0 +1,301 @@
+// linear.hip — entry points of linear attention: argument checks, the split of long sequences into segments, the three
+// launches of the backward pass, and the kernels between them.
+//
+// Segments. A workgroup per head and 128 columns leaves CUs idle where batch x heads is small, so long sequences are cut:
+// one launch forms what each segment adds to the state (reading y and z), la_scan_kernel turns these
+// into the state before each segment, and the main launch runs all segments side by side.
+#include <string.h>
+
+#include "linear_kernel.hpp"
+#include "status.hpp"
+
+namespace fa {
+
+// ws[sg + 1] holds what segment sg adds to the state; becomes the state before segment sg + 1, and ws[0] the one before the
+// first. A thread carries one element along; its loads of the next segments do not wait for the sum.
+__global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
+  const int n = p.da * p.db, nb = (n + 255) / 256;
+  const int bh = blockIdx.x / nb, b = bh / p.NH, h = bh % p.NH;
+  const int e = (blockIdx.x % nb) * 256 + threadIdx.x;
+  const LaSeq sq = la_seq(p, b);
+  if (e >= n || sq.slot < 0) return;
+  const int nseg = la_segments(p, sq.len);
+  float* const ws = p.ws + (long long)bh * p.nseg * n + e;
+  float cur = p.first ? p.first[((long long)sq.slot * p.NH + h) * n + (e / p.db) * p.sa + (e % p.db) * p.sb] : 0.0f;
+  const float d = la_decay(p, b, h);
+  const float m1 = expm1f(-d * (float)p.seg);
+  ws[0] = cur;
+  for (int s = 1; s < nseg; s += 4) {
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = s + j < nseg ? ws[(long long)(s + j) * n] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float f = p.enter && s + j == 1 ? expm1f(-d * (float)(p.seg - 1)) : m1;
+      cur = fmaf(cur, f, cur) + v[j];
+      if (s + j < nseg) ws[(long long)(s + j) * n] = cur;
+    }
+  }
+}
+
+// The gradients of a head of keys or values that `gqa` heads of queries share: their sum, in the heads' order, rounded once.
+template <typename T>
+__global__ __launch_bounds__(256) void la_group_kernel(const float* part, T* out, fa_strides so, long long rows, int n, int NKV, int gqa, int D) {
+  const int d4 = D / 4;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * NKV * d4) return;
+  const int c = (int)(i % d4), hk = (int)(i / d4 % NKV);
+  const long long row = i / d4 / NKV;
+  const float* from = part + ((row * NKV + hk) * gqa) * (long long)D + 4 * c;
+  f32x4 sum = *(const f32x4*)from;
+  for (int j = 1; j < gqa; j++) sum += *(const f32x4*)(from + (long long)j * D);
+  T* to = out + (row / n) * so.b + (row % n) * so.s + hk * so.h + 4 * c;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 v;
+#pragma unroll
+  for (int j = 0; j < 4; j++) v[j] = (T)sum[j];
+  *(T4*)to = v;
+}
+
+namespace {
+
+int la_elt(int dtype) { return dtype == FA_F32 ? 4 : 2; }
+
+// Segments for a pass of output width db: two workgroups for each of the 256 CUs, but none of fewer than 256 rows.
+void la_split(LaArgs& a) {
+  const int width = a.db <= 64 ? 64 : 128;
+  const long long base = (long long)a.batch * a.NH * ((a.db + width - 1) / width);
+  long long k = base >= 256 ? 1 : (512 + base - 1) / (base > 0 ? base : 1);
+  const long long most = (a.n + 255) / 256;
+  k = k > most ? most : k;
+  k = k < 1 ? 1 : k;
+  const long long seg = ((a.n + k - 1) / k + kLaChunk - 1) / kLaChunk * kLaChunk;
+  a.seg = (int)(seg < kLaChunk ? kLaChunk : seg > (1 << 30) ? (1 << 30) : seg);
+  a.nseg = (int)(((long long)a.n + a.seg - 1) / a.seg);
+  if (a.nseg < 1) a.nseg = 1;
+}
+
+long long la_ws(const LaArgs& a) { return a.nseg > 1 ? (long long)a.batch * a.NH * a.nseg * a.da * a.db * 4 : 0; }
+
+LaArgs la_base(const FableLinearParams& p) {
+  LaArgs a;
+  memset(&a, 0, sizeof(a));
+  a.decay = p.decay;
+  a.decay_b = p.decay_b;
+  a.cu = p.cu;
+  a.total = p.total;
+  a.batch = p.batch;
+  a.n = p.n;
+  a.NH = p.NH;
+  a.pscale = p.scale;
+  a.hx = a.hy = a.hz = 1;
+  return a;
+}
+
+LaArgs la_forward(const FableLinearParams& p) {
+  LaArgs a = la_base(p);
+  a.x = p.q, a.y = p.k, a.z = p.v, a.o = p.o;
+  a.sx = p.sq, a.sy = p.sk, a.sz = p.sv, a.so = p.so;
+  a.hy = a.hz = p.gqa;
+  a.da = p.DK, a.db = p.DV;
+  a.first = p.state_in, a.last = p.state_out;
+  a.sa = p.DV, a.sb = 1;
+  a.slots = p.slots, a.nslots = p.num_slots;
+  a.iscale = p.scale, a.uscale = 1.0f;
+  la_split(a);
+  return a;
+}
+
+// dq_t = scale S_t dout_t
+LaArgs la_dq(const FableLinearParams& p) {
+  LaArgs a = la_base(p);
+  a.x = p.dout, a.y = p.v, a.z = p.k, a.o = p.dq;
+  a.sx = p.sdo, a.sy = p.sv, a.sz = p.sk, a.so = p.sdq;
+  a.hy = a.hz = p.gqa;
+  a.da = p.DV, a.db = p.DK;
+  a.first = p.state_in;
+  a.sa = 1, a.sb = p.DV;
+  a.iscale = p.scale, a.uscale = 1.0f;
+  la_split(a);
+  return a;
+}
+
+// dv_t = G_t^T k_t; G is DK x DV
+LaArgs la_dv(const FableLinearParams& p) {
+  LaArgs a = la_base(p);
+  a.x = p.k, a.y = p.q, a.z = p.dout, a.o = p.dv;
+  a.sx = p.sk, a.sy = p.sq, a.sz = p.sdo, a.so = p.sdv;
+  a.hx = p.gqa;
+  a.da = p.DK, a.db = p.DV;
+  a.first = p.dstate_out, a.last = p.dstate_in;
+  a.sa = p.DV, a.sb = 1;
+  a.iscale = 1.0f, a.uscale = p.scale;
+  a.rev = 1, a.enter = p.dstate_out != nullptr, a.leave = 1;
+  la_split(a);
+  return a;
+}
+
+// dk_t = G_t v_t, on G^T
+LaArgs la_dk(const FableLinearParams& p) {
+  LaArgs a = la_base(p);
+  a.x = p.v, a.y = p.dout, a.z = p.q, a.o = p.dk;
+  a.sx = p.sv, a.sy = p.sdo, a.sz = p.sq, a.so = p.sdk;
+  a.hx = p.gqa;
+  a.da = p.DV, a.db = p.DK;
+  a.first = p.dstate_out;
+  a.sa = 1, a.sb = p.DV;
+  a.iscale = 1.0f, a.uscale = p.scale;
+  a.rev = 1, a.enter = p.dstate_out != nullptr;
+  la_split(a);
+  return a;
+}
+
+int la_go(const LaArgs& a, int dtype, bool state, hipStream_t st) {
+  return dtype == FA_F16 ? la_launch<_Float16>(a, state, st) : dtype == FA_BF16 ? la_launch<__bf16>(a, state, st) : la_launch<float>(a, state, st);
+}
+
+// (nseg is above 1 for fewer than 256 states only, and then at most 512)
+int la_pass(LaArgs a, int dtype, void* ws, hipStream_t st) {
+  a.ws = (float*)ws;
+  if (a.nseg > 1) {
+    la_go(a, dtype, true, st);
+    hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)(a.batch * a.NH * ((a.da * a.db + 255) / 256))), dim3(256), 0, st, a);
+  }
+  la_go(a, dtype, false, st);
+  return launch_status("linear attention");
+}
+
+// What every call has to satisfy; the tensors' own checks follow in the entry points.
+int la_check(const FableLinearParams& p, int dtype, const char* what) {
+  if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return fail(FA_ERR_DTYPE, "%s: unknown dtype %d", what, dtype);
+  if (p.DK < 8 || p.DK > 256 || p.DK % 8 || p.DV < 8 || p.DV > 256 || p.DV % 8)
+    return fail(FA_ERR_HEADDIM, "%s: head dims %d and %d: multiples of 8 up to 256", what, p.DK, p.DV);
+  if (p.batch < 0 || p.n < 0 || p.NH < 1 || p.gqa < 1 || p.NH % p.gqa || p.total < 0 || p.n > (1 << 30))
+    return fail(FA_ERR_ARG, "%s: batch=%d n=%d NH=%d gqa=%d", what, p.batch, p.n, p.NH, p.gqa);
+  // (256 workgroups of the scan for each state, within a grid's 2^32 threads)
+  if ((long long)p.batch * p.NH > 65535) return fail(FA_ERR_ARG, "%s: batch x heads = %lld", what, (long long)p.batch * p.NH);
+  return FA_OK;
+}
+
+int la_tensor(const char* what, const char* name, const void* t, const fa_strides& s, int dtype) {
+  const int e = la_elt(dtype);
+  if (!t) return fail(FA_ERR_ARG, "%s: null %s", what, name);
+  if (((uintptr_t)t | (uintptr_t)(s.b * e) | (uintptr_t)(s.h * e) | (uintptr_t)(s.s * e)) & 15)
+    return fail(FA_ERR_ARG, "%s: %s: rows must be 16-byte aligned", what, name);
+  // (offsets within a chunk are 32 bits wide)
+  if (s.s < 0 || s.s * e * kLaChunk >= (1LL << 31)) return fail(FA_ERR_ARG, "%s: %s: a row stride of %lld values", what, name, (long long)s.s);
+  return FA_OK;
+}
+
+long long la_group_bytes(const FableLinearParams& p) {
+  const long long rows = p.cu ? p.total : (long long)p.batch * p.n;
+  return p.gqa > 1 ? rows * p.NH * (p.DK > p.DV ? p.DK : p.DV) * 4 : 0;
+}
+
+long long la_round(long long x) { return (x + 255) / 256 * 256; }
+
+long long la_need(const FableLinearParams& p, bool backward) {
+  if (!backward) return la_ws(la_forward(p));
+  long long w = la_ws(la_dq(p));
+  const long long b = la_ws(la_dv(p)), c = la_ws(la_dk(p));
+  w = w > b ? w : b;
+  w = w > c ? w : c;
+  return la_round(w) + la_group_bytes(p);
+}
+
+template <typename T>
+void la_group(const float* part, void* out, const fa_strides& so, const FableLinearParams& p, int D, hipStream_t st) {
+  const long long rows = p.cu ? p.total : (long long)p.batch * p.n;
+  const int n = p.cu ? (int)(rows > 0x7fffffff ? 0x7fffffff : rows) : p.n;
+  const long long items = rows * (p.NH / p.gqa) * (D / 4);
+  if (items > 0)
+    hipLaunchKernelGGL(la_group_kernel<T>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, part, (T*)out, so, rows, n, p.NH / p.gqa, p.gqa, D);
+}
+
+}  // namespace
+}  // namespace fa
+
+using namespace fa;
+
+extern "C" int64_t fable_linear_attn_ws_bytes(FableLinearParams p, int dtype, int backward) {
+  if (la_check(p, dtype, "fable_linear_attn_ws_bytes") != FA_OK) return -1;
+  return la_need(p, backward != 0);
+}
+
+extern "C" int fable_linear_attn_fwd(FableLinearParams p, int dtype, void* ws, int64_t ws_bytes, void* stream) {
+  const char* what = "fable_linear_attn_fwd";
+  int rc = la_check(p, dtype, what);
+  if (rc != FA_OK) return rc;
+  if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
+  if (p.slots && (p.num_slots < 0 || (!p.state_in && !p.state_out))) return fail(FA_ERR_ARG, "%s: slots without states", what);
+  if ((p.cu ? p.total : p.n) > 0) {
+    if ((rc = la_tensor(what, "q", p.q, p.sq, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, dtype)) ||
+        (rc = la_tensor(what, "v", p.v, p.sv, dtype)) || (rc = la_tensor(what, "o", p.o, p.so, dtype)))
+      return rc;
+  }
+  const long long need = la_need(p, false);
+  if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+    return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
+  if (p.batch == 0) return FA_OK;
+  return la_pass(la_forward(p), dtype, ws, (hipStream_t)stream);
+}
+
+extern "C" int fable_linear_attn_step(FableLinearParams p, int dtype, void* stream) {
+  const char* what = "fable_linear_attn_step";
+  int rc = la_check(p, dtype, what);
+  if (rc != FA_OK) return rc;
+  if (!p.decay || !p.state_in || !p.state_out) return fail(FA_ERR_ARG, "%s: null decay or state", what);
+  if (((uintptr_t)p.state_in | (uintptr_t)p.state_out) & 15) return fail(FA_ERR_ARG, "%s: states must be 16-byte aligned", what);
+  if (p.slots && p.num_slots < 0) return fail(FA_ERR_ARG, "%s: num_slots=%d", what, p.num_slots);
+  if ((p.cu ? p.total : p.n) > 0) {
+    if ((rc = la_tensor(what, "q", p.q, p.sq, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, dtype)) ||
+        (rc = la_tensor(what, "v", p.v, p.sv, dtype)) || (rc = la_tensor(what, "o", p.o, p.so, dtype)))
+      return rc;
+  }
+  if (p.batch == 0) return FA_OK;
+  la_step(la_forward(p), dtype, (hipStream_t)stream);
+  return launch_status(what);
+}
+
+extern "C" int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, int64_t ws_bytes, void* stream) {
+  const char* what = "fable_linear_attn_bwd";
+  int rc = la_check(p, dtype, what);
+  if (rc != FA_OK) return rc;
+  if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
+  if (p.slots) return fail(FA_ERR_ARG, "%s: states of a pool have no gradient", what);
+  if ((p.cu ? p.total : p.n) > 0) {
+    if ((rc = la_tensor(what, "q", p.q, p.sq, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, dtype)) ||
+        (rc = la_tensor(what, "v", p.v, p.sv, dtype)) || (rc = la_tensor(what, "dout", p.dout, p.sdo, dtype)) ||
+        (rc = la_tensor(what, "dq", p.dq, p.sdq, dtype)) || (rc = la_tensor(what, "dk", p.dk, p.sdk, dtype)) ||
+        (rc = la_tensor(what, "dv", p.dv, p.sdv, dtype)))
+      return rc;
+  }
+  const long long need = la_need(p, true);
+  if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
+    return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
+  if (p.batch == 0) return FA_OK;
+  hipStream_t st = (hipStream_t)stream;
+  if ((rc = la_pass(la_dq(p), dtype, ws, st)) != FA_OK) return rc;
+  LaArgs a[2] = {la_dv(p), la_dk(p)};
+  float* const part = (float*)((char*)ws + (need - la_group_bytes(p)));
+  for (int i = 0; i < 2; i++) {
+    const int D = a[i].db;
+    if (p.gqa > 1) {
+      a[i].o = part;
+      a[i].o32 = 1;
+      a[i].so.b = p.cu ? 0 : (long long)p.n * p.NH * D;
+      a[i].so.s = (long long)p.NH * D;
+      a[i].so.h = D;
+    }
+    if ((rc = la_pass(a[i], dtype, ws, st)) != FA_OK) return rc;
+    if (p.gqa > 1) {
+      void* out = i == 0 ? p.dv : p.dk;
+      const fa_strides so = i == 0 ? p.sdv : p.sdk;
+      if (dtype == FA_F16) la_group<_Float16>(part, out, so, p, D, st);
+      else if (dtype == FA_BF16) la_group<__bf16>(part, out, so, p, D, st);
+      else la_group<float>(part, out, so, p, D, st);
+      if ((rc = launch_status(what)) != FA_OK) return rc;
+    }
+  }
+  return FA_OK;
+}

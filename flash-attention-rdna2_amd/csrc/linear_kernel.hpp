@@ -1,0 +1,530 @@
+// linear_kernel.hpp — causal linear attention with a decay for each head, by chunks.
+//
+// One kernel serves the forward pass and the three products of the backward pass. With lambda = exp(-decay[h])
+//   out_i = pscale sum_{j<=i} lambda^(i-j) (x_i . y_j) z_j + iscale lambda^(i+1) S x_i,
+//   S     = the state before the first row,  S' = lambda^n S + uscale sum_j lambda^(n-1-j) y_j z_j^T,
+// over rows i of the sequence in processing order. The forward pass is x, y, z = q, k, v. With the state's
+// gradient G_t = lambda G_{t+1} + scale q_t dout_t^T, dq is x, y, z = dout, v, k in the same order, and dv
+// (k, q, dout) and dk (v, dout, q) run over the rows from the last one to the first.
+//
+// A workgroup of NW waves takes a segment of one head of one sequence, a chunk of C rows at a time, and a tile of
+// 32 NW columns of z; a wave owns 32 of them. It keeps S (DA x 32 of its columns) in accumulators, in 32 bits, for the
+// whole segment, so a chunk reads its rows of x, y and z once and writes its rows of out once: the kernel is bound by those
+// bytes in 16 bits (some 100 kFLOP per row and head of 128 against 1 KB), by the matrix cores in fp32.
+//   Scores are formed transposed (y x^T), so that a lane holds all keys of one query: weighted and rounded, they are the
+// operand of the product with z as they are. S is DA x 32 with z's columns across the lanes, which is the operand
+// layout of the product with x. x is read from LDS once for both. out is formed transposed too: a lane holds 32 columns of one row.
+//   Roundings to 16 bits: the weighted scores and S once each as operands, as attention rounds its probabilities (each
+// is as large as the rounding of out itself); the weighted z of the state's update not at all: it is split into PIECES parts of
+// T that hold its 24 bits (bf16: 3, fp16: 2, fp32: itself), because S is a result in 32 bits and runs on over
+// the whole sequence. In fp16, whose range is small, S and the weighted z are brought to a power of two of
+// their own before, and scores too large for it likewise.
+//   lambda^n S is S + (lambda^n - 1) S: the factor itself, rounded to 32 bits, would be off by up to 2^-25 in the same
+// direction in each chunk, which adds up over the many chunks that a slow decay remembers.
+//   A chunk with fewer than C rows (the last one of a sequence) sits at the end of the tile, behind rows of zeros, so
+// the weights of scores and update are the same for every chunk.
+#pragma once
+#include "attn_device.hpp"
+
+namespace fa {
+
+// What a launch takes. Strides in elements. Rows of sequence b: [cu[b], cu[b+1]) of [0, total) of the packed tensors, or n of batch element b.
+struct LaArgs {
+  const void *x, *y, *z;
+  void* o;
+  fa_strides sx, sy, sz, so;
+  int hx, hy, hz;            // heads of the item's head h: h / hx, ...
+  int da, db;                // columns of x and y, of z and out
+  const float* decay;
+  long long decay_b;         // stride over the batch
+  const float* first;        // states before the first row in processing order, [slot][NH][da][db] by ...
+  float* last;               // ... and behind the last one; NULL: zeros, not wanted
+  long long sa, sb;          // strides of a state's element (a, b)
+  const int32_t* slots;      // a sequence's state; NULL: its own number. Outside [0, nslots): no sequence
+  int nslots;
+  float* ws;                 // [batch][NH][nseg][da][db]: the states before the segments (nseg > 1)
+  const int32_t* cu;
+  long long total;
+  int batch, n, NH;
+  int nseg, seg;             // segments of `seg` rows, a multiple of C; the last one takes all rows left
+  float pscale, iscale, uscale;
+  int rev;                   // rows from the last to the first
+  int enter;                 // first is not to decay before the first row (the gradient of the final state)
+  int leave;                 // last decays once more behind the last row (the gradient of the initial state)
+  int o32;                   // out is fp32 whatever T
+};
+
+// A fragment: lane (r, g) = (l % 32, l / 32) holds the contraction indices 16 s + 4 g + {0..3} and 16 s + 8 + 4 g + {0..3} of
+// its row or column r, the rows of a 32 x 32 accumulator that its registers 8 (s % 2) .. + 7 hold.
+template <typename T>
+struct La {
+  using F = typename Dt<T>::V8;
+  using H = typename Dt<T>::V4;
+  static constexpr int kPieces = __is_same(T, __bf16) ? 3 : 2;
+  static __device__ __forceinline__ f32x16 mma(F a, F b, f32x16 c) { return Dt<T>::mma32(a, b, c); }
+};
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <>
+struct La<float> {
+  using F = f32x8;
+  using H = f32x4;
+  static constexpr int kPieces = 1;
+  static __device__ __forceinline__ f32x16 mma(F a, F b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// LDS tiles of rows of W values in units of four. A unit's place within its row is turned by the row, so that 32 rows read
+// at one column, and 4 rows x 32 columns read transposed, meet every bank once (16-bit types; 64 banks).
+template <int W>
+__device__ __forceinline__ int la_turn(int row) {
+  if constexpr (W >= 128) return ((row & 3) << 3) | ((row >> 2) & 7);
+  else return (((row >> 1) & 1) << 3) | ((row >> 2) & 7);
+}
+template <int W>
+__device__ __forceinline__ int la_ofs(int row, int unit) { return row * W + 4 * (unit ^ la_turn<W>(row)); }
+
+// rows row (per lane), columns 16 s .. 16 s + 15
+template <typename T, int W>
+__device__ __forceinline__ typename La<T>::F la_rows(const T* tile, int row, int s, int g) {
+  using H = typename La<T>::H;
+  const H a = *(const H*)(tile + la_ofs<W>(row, 4 * s + g)), b = *(const H*)(tile + la_ofs<W>(row, 4 * s + 2 + g));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// column 32 ct + r, rows 16 s .. 16 s + 15
+template <typename T, int W>
+__device__ __forceinline__ typename La<T>::F la_cols(const T* tile, int ct, int s, int lane) {
+  using H = typename La<T>::H;
+  const int g = lane / 32;
+  if constexpr (sizeof(T) == 2) {
+    const int row = 16 * s + 4 * g + (lane % 16) / 4, unit = 8 * ct + 4 * ((lane / 16) % 2) + lane % 4;
+    const H a = lds_read_tr<T>(tile + la_ofs<W>(row, unit)), b = lds_read_tr<T>(tile + la_ofs<W>(row + 8, unit));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    const int r = lane % 32;
+    typename La<T>::F f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[j] = tile[la_ofs<W>(16 * s + 8 * (j / 4) + 4 * g + j % 4, 8 * ct + r / 4) + r % 4];
+    return f;
+  }
+}
+
+__device__ __forceinline__ float la_wave_max(float x) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) x = fmaxf(x, __shfl_xor(x, i));
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+
+// The power of two that brings a largest magnitude m into [2^13, 2^14), its inverse in `inv`; 1 for zero, and for what is no number.
+__device__ __forceinline__ float la_norm(float m, float& inv) {
+  const int e = (int)((__float_as_uint(m) >> 23) & 255);
+  const int k = (e == 0 || e == 255) ? 0 : min(max(140 - e, -120), 120);
+  inv = __uint_as_float((uint32_t)(127 - k) << 23);
+  return __uint_as_float((uint32_t)(127 + k) << 23);
+}
+
+// lambda^k as 2^(-k d log2 e)
+__device__ __forceinline__ float la_pow(float dl2, float k) { return exp2f(-dl2 * k); }
+
+// A decay too large for products with a row count is one that nothing survives; 0 times it has to stay 0.
+__device__ __forceinline__ float la_decay(const LaArgs& p, int b, int h) {
+  const float d = p.decay[b * p.decay_b + h];
+  return d > 1e25f ? 1e25f : d < -1e25f ? -1e25f : d;
+}
+
+struct LaSeq {
+  long long row0;            // first row in the tensors
+  int len;
+  int slot;                  // -1: no sequence
+};
+__device__ __forceinline__ LaSeq la_seq(const LaArgs& p, int b) {
+  LaSeq s;
+  if (p.cu) {
+    const long long lo = min(max((long long)p.cu[b], 0LL), p.total), hi = min(max((long long)p.cu[b + 1], lo), p.total);
+    s.row0 = lo;
+    s.len = (int)(hi - lo);
+  } else {
+    s.row0 = 0;
+    s.len = p.n;
+  }
+  s.slot = p.slots ? p.slots[b] : b;
+  if (p.slots && (s.slot < 0 || s.slot >= p.nslots)) s.slot = -1;
+  return s;
+}
+__device__ __forceinline__ int la_segments(const LaArgs& p, int len) {
+  const int k = (int)(((long long)len + p.seg - 1) / p.seg);
+  return k < 1 ? 1 : k > p.nseg ? p.nseg : k;
+}
+
+// Zeros in rows [lo, hi) of out for the item's columns.
+template <typename T>
+__device__ __forceinline__ void la_zero_rows(const LaArgs& p, long long base, long long lo, long long hi, int c0, int nc, int tid, int nt) {
+  for (long long i = tid; i < (hi - lo) * nc; i += nt) {
+    const long long at = base + (lo + i / nc) * p.so.s + c0 + i % nc;
+    if (p.o32) ((float*)p.o)[at] = 0.0f;
+    else ((T*)p.o)[at] = (T)0.0f;
+  }
+}
+
+template <typename T, int DA, int NW, int C, bool STATE>
+__global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs p) {
+  using F = typename La<T>::F;
+  using H = typename La<T>::H;
+  constexpr int NT = NW * 64, DB = NW * 32, NB = C / 32, KT = DA / 32, E = 16 / sizeof(T);
+  constexpr int CA = DA / E, CB = DB / E;                     // 16-byte chunks of a row
+  constexpr int LA = C * CA / NT, LB = C * CB / NT;           // chunks per thread
+  static_assert(NT % CA == 0 && C * CA % NT == 0 && NT % CB == 0 && C * CB % NT == 0, "tile loads");
+  __shared__ __align__(16) T lds[(STATE ? 0 : C * DA) + C * DA + C * DB];
+  T* const tx = lds;
+  T* const ty = lds + (STATE ? 0 : C * DA);
+  T* const tz = ty + C * DA;
+
+  const int tid = threadIdx.x, lane = tid % 64, r = lane % 32, g = lane / 32;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int ndb = (p.db + DB - 1) / DB;
+  // items in the order (sequence, segment, head, column tile): what shares x and y, and neighbouring heads of the same
+  // rows, run side by side on one XCD
+  const int segs = STATE ? p.nseg - 1 : p.nseg;
+  int w = xcd_remap(blockIdx.x, gridDim.x);
+  const int dbt = w % ndb;
+  w /= ndb;
+  const int h = w % p.NH;
+  w /= p.NH;
+  const int sg = w % segs, b = w / segs;
+  const LaSeq sq = la_seq(p, b);
+  const int nseg = la_segments(p, sq.len);
+  const int col0 = dbt * DB + 32 * wave;                      // the wave's first column
+
+  const long long obase = (p.cu ? 0 : b * p.so.b) + h * p.so.h;
+  if constexpr (!STATE) {
+    // rows of no sequence in front of the first one and behind the last one
+    const int c0 = dbt * DB, nc = min(DB, p.db - c0);
+    if (p.cu && sg == 0 && b == 0) la_zero_rows<T>(p, obase, 0, sq.row0, c0, nc, tid, NT);
+    if (p.cu && sg == 0 && b == p.batch - 1) la_zero_rows<T>(p, obase, sq.row0 + sq.len, p.total, c0, nc, tid, NT);
+    if (sq.slot < 0) {
+      if (sg == 0) la_zero_rows<T>(p, obase, sq.row0, sq.row0 + sq.len, c0, nc, tid, NT);
+      return;
+    }
+  }
+  if (sq.slot < 0 || sg >= nseg || (STATE && sg >= nseg - 1)) return;
+  const bool tail = sg == nseg - 1;
+  // the segment's rows, counted in processing order
+  const int p0 = sg * p.seg, p1 = tail ? sq.len : p0 + p.seg;
+  const int nch = (p1 - p0 + C - 1) / C;
+
+  const float d = la_decay(p, b, h), dl2 = d * kLog2e;
+  // weights of the scores of a block on the diagonal and of one 32 rows below it; of the update within 16 rows
+  float wd[16], wo[NB > 1 ? 16 : 1], wu[8];
+  if constexpr (!STATE) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const int diff = r - (8 * (i / 4) + 4 * g + i % 4);
+      wd[i] = p.pscale * la_pow(dl2, (float)max(diff, 0));
+      if constexpr (NB > 1) wo[i] = p.pscale * la_pow(dl2, (float)(diff + 32));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) wu[j] = la_pow(dl2, (float)(15 - (8 * (j / 4) + 4 * g + j % 4)));
+
+  f32x16 S[KT];
+  const long long state = ((long long)sq.slot * p.NH + h) * p.da * p.db;
+#pragma unroll
+  for (int t = 0; t < KT; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) S[t][i] = 0.0f;
+  if (!STATE) {
+    const float* from = nullptr;
+    long long ra = p.sa, rb = p.sb;
+    if (p.nseg == 1) {
+      if (p.first) from = p.first + state;
+    } else {
+      from = p.ws + (((long long)b * p.NH + h) * p.nseg + sg) * p.da * p.db;
+      ra = p.db;
+      rb = 1;
+    }
+    if (from) {
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int a = 32 * t + 8 * (i / 4) + 4 * g + i % 4;
+          if (a < p.da && col0 + r < p.db) S[t][i] = from[a * ra + (col0 + r) * rb];
+        }
+    }
+  }
+
+  // tile loads: a thread's 16-byte column is the same for all its rows
+  const int xr = tid / CA, xc = tid % CA, zr = tid / CB, zc = tid % CB;
+  const bool xin = xc * E < p.da, zin = dbt * DB + zc * E < p.db;
+  const T* const gx = (const T*)p.x + (p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h + sq.row0 * p.sx.s;
+  const T* const gy = (const T*)p.y + (p.cu ? 0 : b * p.sy.b) + (h / p.hy) * p.sy.h + sq.row0 * p.sy.s;
+  const T* const gz = (const T*)p.z + (p.cu ? 0 : b * p.sz.b) + (h / p.hz) * p.sz.h + sq.row0 * p.sz.s + dbt * DB;
+  u32x4 vx[STATE ? 1 : LA], vy[LA], vz[LB];
+
+  auto rows_of = [&](int c, long long& row) {                 // rows of chunk c, and its first one in the sequence
+    const int q0 = p0 + c * C, n = min(C, p1 - q0);
+    row = p.rev ? sq.len - q0 - n : q0;
+    return n;
+  };
+  auto fetch = [&](int c) {
+    long long row;
+    const int n = rows_of(c, row);
+    const auto rx = buf_rsrc(gx + row * p.sx.s, ((n - 1) * p.sx.s + p.da) * (long long)sizeof(T));
+    const auto ry = buf_rsrc(gy + row * p.sy.s, ((n - 1) * p.sy.s + p.da) * (long long)sizeof(T));
+    const auto rz = buf_rsrc(gz + row * p.sz.s, ((n - 1) * p.sz.s + p.db - dbt * DB) * (long long)sizeof(T));
+#pragma unroll
+    for (int i = 0; i < LA; i++) {
+      const int m = xr + i * (NT / CA);
+      const bool in = xin && m < n;
+      if constexpr (!STATE) vx[i] = buf_load16(rx, in ? m * (int)(p.sx.s * sizeof(T)) + xc * 16 : kBufZero);
+      vy[i] = buf_load16(ry, in ? m * (int)(p.sy.s * sizeof(T)) + xc * 16 : kBufZero);
+    }
+#pragma unroll
+    for (int i = 0; i < LB; i++) {
+      const int m = zr + i * (NT / CB);
+      vz[i] = buf_load16(rz, zin && m < n ? m * (int)(p.sz.s * sizeof(T)) + zc * 16 : kBufZero);
+    }
+  };
+  auto put = [&](T* tile, int W, int row, int c, u32x4 v) {   // 16 bytes as units of four values
+    if constexpr (sizeof(T) == 2) {
+      const int a = W == DA ? la_ofs<DA>(row, 2 * c) : la_ofs<DB>(row, 2 * c);
+      const int e = W == DA ? la_ofs<DA>(row, 2 * c + 1) : la_ofs<DB>(row, 2 * c + 1);
+      *(u32x2*)(tile + a) = u32x2{v[0], v[1]};
+      *(u32x2*)(tile + e) = u32x2{v[2], v[3]};
+    } else {
+      *(u32x4*)(tile + (W == DA ? la_ofs<DA>(row, c) : la_ofs<DB>(row, c))) = v;
+    }
+  };
+
+  if (nch > 0) fetch(0);
+  for (int c = 0; c < nch; c++) {
+    long long row;
+    const int n = rows_of(c, row), shift = C - n;
+    __syncthreads();
+    {
+      const int s = p.rev ? 0 : shift;
+      auto place = [&](int m) { return p.rev ? C - 1 - m : (m + s) & (C - 1); };
+#pragma unroll
+      for (int i = 0; i < LA; i++) {
+        const int at = place(xr + i * (NT / CA));
+        if constexpr (!STATE) put(tx, DA, at, xc, vx[i]);
+        put(ty, DA, at, xc, vy[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < LB; i++) put(tz, DB, place(zr + i * (NT / CB)), zc, vz[i]);
+    }
+    if (c + 1 < nch) fetch(c + 1);
+    __syncthreads();
+
+    // the state enters the first row as it is where it is the final state's gradient
+    const int enter = p.enter && sg == 0 && c == 0;
+    F zf[2 * NB];
+#pragma unroll
+    for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, DB>(tz, wave, s, lane);
+
+    if constexpr (!STATE) {
+      f32x16 sc[NB][NB], o[NB];                                // [key block][query block]
+#pragma unroll
+      for (int q = 0; q < NB; q++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[q][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k <= q; k++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) sc[k][q][i] = 0.0f;
+      }
+      float norm = 1.0f, inv = 1.0f;
+      if constexpr (La<T>::kPieces == 2) {
+        float m = 0.0f;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(S[t][i]));
+        norm = la_norm(la_wave_max(m), inv);
+      }
+#pragma unroll
+      for (int s = 0; s < DA / 16; s++) {
+        F xf[NB], yf[NB], sf;
+#pragma unroll
+        for (int q = 0; q < NB; q++) xf[q] = la_rows<T, DA>(tx, 32 * q + r, s, g);
+#pragma unroll
+        for (int k = 0; k < NB; k++) yf[k] = la_rows<T, DA>(ty, 32 * k + r, s, g);
+#pragma unroll
+        for (int j = 0; j < 8; j++) sf[j] = (T)(S[s / 2][8 * (s % 2) + j] * norm);
+#pragma unroll
+        for (int q = 0; q < NB; q++) {
+#pragma unroll
+          for (int k = 0; k <= q; k++) sc[k][q] = La<T>::mma(yf[k], xf[q], sc[k][q]);
+          o[q] = La<T>::mma(sf, xf[q], o[q]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < NB; q++) {
+        const float lw = p.iscale * inv * la_pow(dl2, (float)max(32 * q + r - shift + 1 - enter, 0));
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[q][i] *= lw;
+#pragma unroll
+        for (int k = 0; k <= q; k++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            float v;
+            if (k == q) v = r >= 8 * (i / 4) + 4 * g + i % 4 ? sc[k][q][i] * wd[i] : 0.0f;
+            else v = sc[k][q][i] * wo[i];
+            sc[k][q][i] = v;
+          }
+        float down = 1.0f;
+        if constexpr (La<T>::kPieces == 2) {
+          float m = 0.0f;
+#pragma unroll
+          for (int k = 0; k <= q; k++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(sc[k][q][i]));
+          if (__builtin_amdgcn_ballot_w64(m >= 32768.0f)) {     // past fp16's range: the wave's own power of two
+            float up;
+            down = la_norm(la_wave_max(m), up);
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[q][i] *= down;
+#pragma unroll
+            for (int k = 0; k <= q; k++)
+#pragma unroll
+              for (int i = 0; i < 16; i++) sc[k][q][i] *= down;
+            down = up;
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < 2 * (q + 1); s++) {
+          F pf;
+#pragma unroll
+          for (int j = 0; j < 8; j++) pf[j] = (T)sc[s / 2][q][8 * (s % 2) + j];
+          o[q] = La<T>::mma(zf[s], pf, o[q]);
+        }
+        const int at = 32 * q + r;
+        const bool ok = at >= shift && col0 < p.db;
+        const long long to = obase + (sq.row0 + row + (p.rev ? C - 1 - at : at - shift)) * p.so.s + col0;
+        if constexpr (sizeof(T) == 4) {
+          store_cblock_f32((float*)p.o + to, o[q], 1.0f, g, ok, p.db - col0);
+        } else {
+          if (p.o32) store_cblock_f32((float*)p.o + to, o[q], down, g, ok, p.db - col0);
+          else store_cblock<T>((T*)p.o + to, o[q], down, g, ok, p.db - col0);
+        }
+      }
+    }
+
+    // the state's update
+    const float m1 = expm1f(-d * (float)(n - enter));
+    if constexpr (La<T>::kPieces == 2) {
+      float m = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2 * NB; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf((float)zf[s][j]));
+      float inv;
+      const float norm = la_norm(la_wave_max(m), inv);
+      F z0[2 * NB], z1[2 * NB];
+#pragma unroll
+      for (int s = 0; s < 2 * NB; s++) {
+        const float ws = norm * la_pow(dl2, (float)(C - 16 - 16 * s));
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          float v = (float)zf[s][j] * (wu[j] * ws);
+          asm("" : "+v"(v));   // (or the product is formed twice, once fused with its rounding, and z1 meets another z0)
+          z0[s][j] = (T)v;
+          z1[s][j] = (T)(v - (float)z0[s][j]);
+        }
+      }
+      inv *= p.uscale;
+#pragma unroll
+      for (int t = 0; t < KT; t++) {
+        f32x16 u;
+#pragma unroll
+        for (int i = 0; i < 16; i++) u[i] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; s++) {
+          const F yt = la_cols<T, DA>(ty, t, s, lane);
+          u = La<T>::mma(yt, z1[s], u);
+          u = La<T>::mma(yt, z0[s], u);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[t][i] = fmaf(u[i], inv, fmaf(S[t][i], m1, S[t][i]));
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[t][i] = fmaf(S[t][i], m1, S[t][i]);
+#pragma unroll
+      for (int s = 0; s < 2 * NB; s++) {
+        const float ws = p.uscale * la_pow(dl2, (float)(C - 16 - 16 * s));
+        F z0, z1, z2;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          float v = (float)zf[s][j] * (wu[j] * ws);
+          asm("" : "+v"(v));
+          z0[j] = (T)v;
+          if constexpr (La<T>::kPieces == 3) {
+            const float v1 = v - (float)z0[j];
+            z1[j] = (T)v1;
+            z2[j] = (T)(v1 - (float)z1[j]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+          const F yt = la_cols<T, DA>(ty, t, s, lane);
+          if constexpr (La<T>::kPieces == 3) {
+            S[t] = La<T>::mma(yt, z2, S[t]);
+            S[t] = La<T>::mma(yt, z1, S[t]);
+          }
+          S[t] = La<T>::mma(yt, z0, S[t]);
+        }
+      }
+    }
+  }
+
+  float* to = nullptr;
+  long long ra = p.sa, rb = p.sb;
+  float f = 1.0f;
+  if constexpr (STATE) {
+    to = p.ws + (((long long)b * p.NH + h) * p.nseg + sg + 1) * p.da * p.db;
+    ra = p.db;
+    rb = 1;
+  } else if (tail && p.last) {
+    to = p.last + state;
+    if (p.leave && sq.len > 0) f = la_pow(dl2, 1.0f);
+  }
+  if (to) {
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int a = 32 * t + 8 * (i / 4) + 4 * g + i % 4;
+        if (a < p.da && col0 + r < p.db) to[a * ra + (col0 + r) * rb] = S[t][i] * f;
+      }
+  }
+}
+
+// one new token or a few of each sequence (linear_step.hip)
+void la_step(const LaArgs& p, int dtype, hipStream_t stream);
+
+template <typename T>
+int la_launch(const LaArgs& p, bool state, hipStream_t stream);
+
+constexpr int kLaChunk = 64;   // the longest chunk of any kernel: segments are multiples of it
+
+template <typename T, int DA, int NW, bool STATE>
+inline int la_run(const LaArgs& p, hipStream_t st) {
+  constexpr int C = sizeof(T) == 2 && DA <= 128 ? 64 : 32;
+  const long long items = (long long)p.batch * (STATE ? p.nseg - 1 : p.nseg) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32));
+  hipLaunchKernelGGL((la_kernel<T, DA, NW, C, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, p);
+  return 0;
+}
+
+template <typename T, bool STATE>
+inline int la_pick(const LaArgs& p, hipStream_t st) {
+  if (p.db <= 64) return p.da <= 64 ? la_run<T, 64, 2, STATE>(p, st) : p.da <= 128 ? la_run<T, 128, 2, STATE>(p, st) : la_run<T, 256, 2, STATE>(p, st);
+  return p.da <= 64 ? la_run<T, 64, 4, STATE>(p, st) : p.da <= 128 ? la_run<T, 128, 4, STATE>(p, st) : la_run<T, 256, 4, STATE>(p, st);
+}
+
+}  // namespace fa

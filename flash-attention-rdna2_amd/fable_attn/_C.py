@@ -736,3 +736,160 @@ def combine(out_partial, lse_partial, out_dtype):
     with _on(out_partial.device):
         _lib.check(_L.fa_combine_launch(c, _stream(out_partial)), "fa_combine_launch")
     return out
+
+
+# ----------------------------------------------------------------------------- linear attention
+def _rows_strides(t, packed):
+    """(b, h, s) strides of a (B,S,H,D) tensor, or of a packed (total,H,D) one."""
+    return Strides(0, t.stride(1), t.stride(0)) if packed else Strides(t.stride(0), t.stride(2), t.stride(1))
+
+
+def _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in=None, slots=None):
+    """FableLinearParams of q [B,S,H,DK], k [B,S,Hk,DK], v [B,S,Hk,DV] (packed [total,H,D] with cu int32 [batch+1]),
+    decay f32 [H] or [batch,H] and states f32 [slots,H,DK,DV]."""
+    packed, dev = cu is not None, q.device
+    _req(q.is_cuda, "GPU tensors required")
+    _req(q.dim() == (3 if packed else 4), "q: [B,S,H,D], or [total,H,D] with cu_seqlens")
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _req(t.dim() == q.dim() and t.dtype == q.dtype and t.device == dev, f"{n}: dims, dtype and device of q")
+        _req(_rows_aligned(t), f"{n}: head_dim must be contiguous with 16-byte aligned rows")
+    H, Hk, DK, DV = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
+    _req(k.shape[:-2] == q.shape[:-2] and k.shape[-1] == DK and v.shape[:-1] == k.shape[:-1],
+         f"q, k, v of one batch expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    _req(Hk > 0 and H > 0 and H % Hk == 0, "nheads must be a multiple of nheads_k (GQA)")
+    p = _lib.FableLinearParams()
+    if packed:
+        _check_index("cu_seqlens", cu, dev)
+        p.batch, p.n, p.total, p.cu = cu.numel() - 1, int(max_seqlen), q.shape[0], cu.data_ptr()
+        _req(p.batch >= 0, "cu_seqlens must have batch+1 entries")
+        _req(p.n >= 0, f"max_seqlen={p.n}")
+    else:
+        p.batch, p.n = q.shape[0], q.shape[1]
+    _check_f32("decay", decay, dev)
+    _req(tuple(decay.shape) in ((H,), (p.batch, H)), f"decay must be [{H}] or [{p.batch}, {H}], got {tuple(decay.shape)}")
+    p.decay, p.decay_b = decay.data_ptr(), H if decay.dim() == 2 else 0
+    p.q, p.k, p.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    p.sq, p.sk, p.sv = _rows_strides(q, packed), _rows_strides(k, packed), _rows_strides(v, packed)
+    p.NH, p.gqa, p.DK, p.DV, p.scale = H, H // Hk, DK, DV, float(scale)
+    if state_in is not None:
+        _check_f32("state", state_in, dev)
+        _req(state_in.dim() == 4 and tuple(state_in.shape[1:]) == (H, DK, DV) and state_in.data_ptr() % 16 == 0,
+             f"states must be [slots, {H}, {DK}, {DV}], 16-byte aligned, got {tuple(state_in.shape)}")
+        p.state_in = state_in.data_ptr()
+        if slots is None:
+            _req(state_in.shape[0] >= p.batch, f"{state_in.shape[0]} states for a batch of {p.batch}")
+    if slots is not None:
+        _check_index("state_idx", slots, dev, p.batch)
+        p.slots, p.num_slots = slots.data_ptr(), state_in.shape[0]
+    return p
+
+
+def _linear_ws(p, dt, backward, dev):
+    need = int(_L.fable_linear_attn_ws_bytes(p, dt, backward))
+    if need < 0:
+        _lib.check(1, "linear attention")
+    return (torch.empty(need, dtype=torch.uint8, device=dev) if need else None), need
+
+
+def linear_fwd(q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, state_out=None, slots=None):
+    """Linear attention by chunks -> out, dense of q's rows and v's width. state_out: where the states behind the last
+    rows go (as state_in; may be it)."""
+    p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in, slots)
+    out = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
+    p.o, p.so = out.data_ptr(), _rows_strides(out, cu is not None)
+    if state_out is not None:
+        p.state_out = state_out.data_ptr()
+    if p.batch == 0:
+        return out.zero_()
+    dt = _dt(q)
+    ws, need = _linear_ws(p, dt, 0, q.device)
+    with _on(q.device):
+        _lib.check(_L.fable_linear_attn_fwd(p, dt, _ptr(ws), need, _stream(q)), "fable_linear_attn_fwd")
+    return out
+
+
+def linear_bwd(dout, q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, dstate_out=None, want_dstate=False):
+    """-> (dq, dk, dv, dstate_in or None)"""
+    p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in)
+    _req(dout.dtype == q.dtype and tuple(dout.shape) == (*q.shape[:-1], v.shape[-1]) and _rows_aligned(dout),
+         "dout: out's shape and dtype, 16-byte aligned rows")
+    packed = cu is not None
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    p.dout, p.dq, p.dk, p.dv = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    p.sdo, p.sdq, p.sdk, p.sdv = (_rows_strides(t, packed) for t in (dout, dq, dk, dv))
+    dstate = None
+    if want_dstate:
+        dstate = torch.empty((p.batch, p.NH, p.DK, p.DV), dtype=torch.float32, device=q.device)
+        p.dstate_in = dstate.data_ptr()
+    if dstate_out is not None:
+        _check_f32("dstate_out", dstate_out, q.device, p.batch * p.NH * p.DK * p.DV)
+        p.dstate_out = dstate_out.data_ptr()
+    if p.batch == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_(), dstate
+    dt = _dt(q)
+    ws, need = _linear_ws(p, dt, 1, q.device)
+    with _on(q.device):
+        _lib.check(_L.fable_linear_attn_bwd(p, dt, _ptr(ws), need, _stream(q)), "fable_linear_attn_bwd")
+    return dq, dk, dv, dstate
+
+
+def linear_step(q, k, v, state, decay, scale, cu=None, max_seqlen=0, slots=None):
+    """A few rows per sequence, token by token; the states of the pool [slots,H,DK,DV] updated in place. Returns (out,
+    the launch's parameters and dtype)."""
+    p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state, slots)
+    out = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
+    p.o, p.so, p.state_out = out.data_ptr(), _rows_strides(out, cu is not None), state.data_ptr()
+    dt = _dt(q)
+    if p.batch == 0:
+        out.zero_()
+    else:
+        with _on(q.device):
+            _lib.check(_L.fable_linear_attn_step(p, dt, _stream(q)), "fable_linear_attn_step")
+    return out, p, dt
+
+
+# ----------------------------------------------------------------------------- rotation
+def rotary(q, k, cos, sin, interleaved, cu=None, start=None, conj=False):
+    """q [B,S,H,D] (or [total,H,D] with cu) and k (may be None) turned by the tables' rows at their positions.
+    Returns (q, k, the launch's parameters and dtype), dense."""
+    packed, dev = cu is not None, q.device
+    _req(q.is_cuda, "GPU tensors required")
+    _req(q.dim() == (3 if packed else 4), "q: [B,S,H,D], or [total,H,D] with cu_seqlens")
+    for n, t in (("q", q),) + ((("k", k),) if k is not None else ()):
+        _req(t.dim() == q.dim() and t.dtype == q.dtype and t.device == dev and t.shape[:-2] == q.shape[:-2] and t.shape[-1] == q.shape[-1],
+             f"{n}: the tokens, head_dim, dtype and device of q")
+        _req(t.stride(-1) == 1 or t.shape[-1] == 1, f"{n}: head_dim must be contiguous")
+        _req(t.shape[-2] > 0, f"{n}: no heads")
+    dt, D = _dt(q), q.shape[-1]
+    rd = int(cos.shape[-1] * 2)
+    _check_rotary(cos, sin, rd, D, dev)
+    p = _lib.FableRotaryParams()
+    if packed:
+        _check_index("cu_seqlens", cu, dev)
+        p.batch, p.total, p.cu = cu.numel() - 1, q.shape[0], cu.data_ptr()
+        _req(p.batch >= 0, "cu_seqlens must have batch+1 entries")
+    else:
+        p.batch, p.n = q.shape[0], q.shape[1]
+    if start is not None:
+        _check_index("rotary_seqlens", start, dev, p.batch)
+        p.start = start.data_ptr()
+    qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=dev) if k is not None else None
+    p.q, p.q_out, p.sq, p.sqo, p.NH = q.data_ptr(), qo.data_ptr(), _rows_strides(q, packed), _rows_strides(qo, packed), q.shape[-2]
+    if k is not None:
+        p.k, p.k_out, p.sk, p.sko, p.NKV = k.data_ptr(), ko.data_ptr(), _rows_strides(k, packed), _rows_strides(ko, packed), k.shape[-2]
+    p.cos, p.sin, p.rotary, p.rotary_dim, p.rotary_rows = cos.data_ptr(), sin.data_ptr(), 2 if interleaved else 1, rd, cos.shape[0]
+    p.HD, p.conj = D, 1 if conj else 0
+    if q.numel():
+        with _on(dev):
+            _lib.check(_L.fable_attn_rotary(p, dt, _stream(q)), "fable_attn_rotary")
+    return qo, ko, p, dt
+
+
+def rotary_tables(rows, first, pairs, base, factor, original, low, high, amplitude, dev):
+    """cos and sin [rows, pairs] in fp32 of positions first, first + 1, ..."""
+    cos, sin = (torch.empty((rows, pairs), dtype=torch.float32, device=dev) for _ in range(2))
+    p = _lib.FableRotaryTableParams(cos.data_ptr(), sin.data_ptr(), rows, first, pairs, base, factor, original, low, high, amplitude)
+    with _on(cos.device):
+        _lib.check(_L.fable_attn_rotary_tables(p, _stream(cos)), "fable_attn_rotary_tables")
+    return cos, sin

@@ -21,6 +21,8 @@ from .flash_attn_interface import (
     flash_attn_varlen_qkvpacked_func,
     flash_attn_with_kvcache,
 )
+from .linear_attn_interface import linear_attn_func, linear_attn_varlen_func, linear_attn_with_state
+from .rotary_interface import flash_attn_rotary_func, flash_attn_rotary_tables
 
 from . import torch_op
 
@@ -32,6 +34,8 @@ __all__ = [
     "flash_attn_varlen_func", "flash_attn_varlen_qkvpacked_func",
     "flash_attn_varlen_kvpacked_func", "flash_attn_combine", "flash_attn_with_kvcache",
     "flash_attn_append_kvcache", "flash_attn_gather_kvcache",
+    "flash_attn_rotary_func", "flash_attn_rotary_tables",
+    "linear_attn_func", "linear_attn_varlen_func", "linear_attn_with_state",
     "install_as_flash_attn",
 ]
 

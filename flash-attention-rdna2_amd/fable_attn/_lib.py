@@ -20,6 +20,7 @@ ABI_VERSION = 5  # FABLE_ATTN_ABI_VERSION of include/fable_attn_abi.h
 
 c_i32, c_i64, c_u64, c_f32, c_ptr = (ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64,
                                      ctypes.c_float, ctypes.c_void_p)
+c_f64 = ctypes.c_double
 c_int, c_ll, c_ull = ctypes.c_int, ctypes.c_longlong, ctypes.c_ulonglong
 
 
@@ -100,6 +101,27 @@ class FableGatherParams(ctypes.Structure):
                 ("max_blocks", c_i32), ("num_blocks", c_i32), ("group", c_i32)]
 
 
+class FableLinearParams(ctypes.Structure):
+    _fields_ = [("q", c_ptr), ("k", c_ptr), ("v", c_ptr), ("o", c_ptr), ("dout", c_ptr), ("dq", c_ptr), ("dk", c_ptr),
+                ("dv", c_ptr), ("sq", Strides), ("sk", Strides), ("sv", Strides), ("so", Strides), ("sdo", Strides),
+                ("sdq", Strides), ("sdk", Strides), ("sdv", Strides), ("decay", c_ptr), ("decay_b", c_i64),
+                ("state_in", c_ptr), ("state_out", c_ptr), ("dstate_out", c_ptr), ("dstate_in", c_ptr), ("cu", c_ptr),
+                ("slots", c_ptr), ("total", c_i64), ("batch", c_i32), ("n", c_i32), ("NH", c_i32), ("gqa", c_i32),
+                ("DK", c_i32), ("DV", c_i32), ("num_slots", c_i32), ("scale", c_f32)]
+
+
+class FableRotaryParams(ctypes.Structure):
+    _fields_ = [("q", c_ptr), ("k", c_ptr), ("q_out", c_ptr), ("k_out", c_ptr), ("sq", Strides), ("sk", Strides),
+                ("sqo", Strides), ("sko", Strides), ("cos", c_ptr), ("sin", c_ptr), ("cu", c_ptr), ("start", c_ptr),
+                ("total", c_i64), ("batch", c_i32), ("n", c_i32), ("NH", c_i32), ("NKV", c_i32), ("HD", c_i32),
+                ("rotary", c_i32), ("rotary_dim", c_i32), ("rotary_rows", c_i32), ("conj", c_i32)]
+
+
+class FableRotaryTableParams(ctypes.Structure):
+    _fields_ = [("cos", c_ptr), ("sin", c_ptr), ("rows", c_i64), ("first", c_i64), ("pairs", c_i32), ("base", c_f64),
+                ("factor", c_f64), ("original", c_f64), ("low", c_f64), ("high", c_f64), ("amplitude", c_f64)]
+
+
 # The reference's layouts (package/csrc/fa_iface.h:9-63), taken by fa_forward_launch,
 # fable_attn_backward_launch and fa_decode_launch.
 class RefStrides(ctypes.Structure):
@@ -144,7 +166,8 @@ class RefDecParams(ctypes.Structure):
 
 STRUCTS = {0: FableFwdParams, 1: FableBwdParams, 2: FableDecParams, 3: CombineParams,
            4: Strides, 5: RefFwdParams, 6: RefBwdParams, 7: RefDecParams,
-           8: FableCache8, 9: FableAppendParams, 10: FableGatherParams}
+           8: FableCache8, 9: FableAppendParams, 10: FableGatherParams,
+           11: FableLinearParams, 12: FableRotaryParams, 13: FableRotaryTableParams}
 
 # exported symbols of libfable_attn_hip.so (the C-ABI surface)
 EXPORTS = ("fa_forward_launch", "fable_attn_backward_launch", "fa_decode_launch",
@@ -153,6 +176,8 @@ EXPORTS = ("fa_forward_launch", "fable_attn_backward_launch", "fa_decode_launch"
            "fable_attn_fwd_paged", "fable_attn_fwd_paged_ws_bytes", "fable_attn_bwd_zero_gaps",
            "fable_attn_dec8", "fable_attn_dec8_ws_bytes", "fable_attn_fwd_paged8",
            "fable_attn_fwd_paged8_ws_bytes", "fable_attn_append", "fable_attn_gather",
+           "fable_linear_attn_ws_bytes", "fable_linear_attn_fwd", "fable_linear_attn_bwd", "fable_linear_attn_step",
+           "fable_attn_rotary", "fable_attn_rotary_tables",
            "fa_decode_num_splits", "fa_combine_launch", "fable_attn_bwd_ds_bytes",
            "fable_attn_abi_version", "fable_attn_struct_size", "fable_attn_last_error")
 
@@ -197,7 +222,14 @@ def load():
     lib.fable_attn_fwd_paged8_ws_bytes.restype = c_i64
     lib.fable_attn_append.argtypes = [FableAppendParams, c_i32, c_ptr]
     lib.fable_attn_gather.argtypes = [FableGatherParams, c_i32, c_ptr]
-    for f in ("fable_attn_dec8", "fable_attn_fwd_paged8", "fable_attn_append", "fable_attn_gather", "fable_attn_bwd_zero_gaps", "fable_attn_dec_ws", "fable_attn_fwd_paged", "fable_attn_fwd", "fable_attn_fwd_ws", "fable_attn_bwd", "fable_attn_dec", "fable_attn_dec_noalloc",
+    lib.fable_linear_attn_ws_bytes.argtypes = [FableLinearParams, c_i32, c_i32]
+    lib.fable_linear_attn_ws_bytes.restype = c_i64
+    lib.fable_linear_attn_fwd.argtypes = [FableLinearParams, c_i32, c_ptr, c_i64, c_ptr]
+    lib.fable_linear_attn_bwd.argtypes = [FableLinearParams, c_i32, c_ptr, c_i64, c_ptr]
+    lib.fable_linear_attn_step.argtypes = [FableLinearParams, c_i32, c_ptr]
+    lib.fable_attn_rotary.argtypes = [FableRotaryParams, c_i32, c_ptr]
+    lib.fable_attn_rotary_tables.argtypes = [FableRotaryTableParams, c_ptr]
+    for f in ("fable_linear_attn_fwd", "fable_linear_attn_bwd", "fable_linear_attn_step", "fable_attn_rotary", "fable_attn_rotary_tables", "fable_attn_dec8", "fable_attn_fwd_paged8", "fable_attn_append", "fable_attn_gather", "fable_attn_bwd_zero_gaps", "fable_attn_dec_ws", "fable_attn_fwd_paged", "fable_attn_fwd", "fable_attn_fwd_ws", "fable_attn_bwd", "fable_attn_dec", "fable_attn_dec_noalloc",
               "fa_forward_launch",
               "fable_attn_backward_launch", "fa_decode_launch",
               "fa_decode_num_splits", "fa_combine_launch", "fable_attn_abi_version"):

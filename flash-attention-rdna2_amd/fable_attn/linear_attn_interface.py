@@ -1,0 +1,137 @@
+"""Causal linear attention with a decay for each head, beside the exact attention of flash_attn_interface: the same
+tensor layouts (batch, seqlen, nheads, headdim) or packed (total, nheads, headdim), shared K/V heads, dtypes and errors.
+
+A head of queries holds a state S of headdim x headdim_v values. With l = exp(-decay[head]),
+    S_t = l S_{t-1} + k_t v_t^T,     o_t = scale q_t^T S_t = scale sum_{s<=t} l^(t-s) (q_t . k_s) v_s.
+
+    linear_attn_func         dense batches, with gradients; states in and out
+    linear_attn_varlen_func  packed batches, with gradients; states in and out
+    linear_attn_with_state   serving: the states of a pool updated in place, one new token or many per sequence
+
+States and sums are kept in fp32. Head dims up to 256 each (values may be wider or narrower than keys; one that is no multiple of 8
+is zero-padded). decay is (nheads) or (batch, nheads), as the slopes that flash_attn_func takes for its biases:
+at least 0, 0 for no decay, infinity for a head that sees only the token itself; like those it gets no gradient.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _C, _lib
+from .flash_attn_interface import MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _kernel_width, _with_width
+
+# rows per sequence up to which linear_attn_with_state goes token by token
+STEP_ROWS = 16
+
+
+def _check(q, k, v, decay, packed, scale):
+    """What every call has to satisfy; (decay in fp32, scale)."""
+    if not q.is_cuda:
+        raise ValueError("fable_attn: tensors must be on the GPU (q.is_cuda == False)")
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"fable_attn: dtype {q.dtype} is not supported; use fp16, bf16 or fp32")
+    dims = 3 if packed else 4
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+        raise ValueError(f"fable_attn: q, k, v must be (batch, seqlen, nheads, headdim), or (total, nheads, headdim) with "
+                         f"cu_seqlens; got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if q.shape[-2] == 0 or k.shape[-2] == 0 or q.shape[-2] % k.shape[-2]:
+        raise ValueError(f"fable_attn: nheads_q={q.shape[-2]} is not a multiple of nheads_k={k.shape[-2]} (GQA)")
+    if max(q.shape[-1], v.shape[-1]) > MAX_HEAD_DIM or min(q.shape[-1], v.shape[-1]) < 1:
+        raise ValueError(f"fable_attn: head_dim={q.shape[-1]} and {v.shape[-1]}: 1 to {MAX_HEAD_DIM}")
+    if not torch.is_tensor(decay):
+        raise TypeError(f"fable_attn: decay must be a tensor (nheads) or (batch, nheads), got {type(decay)}")
+    if decay.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("fable_attn: decay gets no gradient; pass decay.detach()")
+    return decay.detach().to(torch.float32).contiguous(), float(q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+class _LinearAttention(torch.autograd.Function):
+    """Forward and backward of one dense (pack None) or packed (pack = (cu_seqlens, max_seqlen)) batch."""
+
+    @staticmethod
+    def forward(ctx, pack, scale, want, q, k, v, decay, state):
+        cu, most = pack if pack is not None else (None, 0)
+        batch = cu.numel() - 1 if cu is not None else q.shape[0]
+        final = torch.empty((batch, q.shape[-2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=q.device) if want else None
+        out = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
+        ctx.scale, ctx.most = scale, most
+        ctx.save_for_backward(q, k, v, decay, state, cu)
+        ctx.set_materialize_grads(False)
+        return (out, final) if want else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dfinal=None):
+        q, k, v, decay, state, cu = ctx.saved_tensors
+        if dout is None and dfinal is None:
+            return (None,) * 8
+        dout = q.new_zeros((*q.shape[:-1], v.shape[-1])) if dout is None else _aligned(dout)
+        dq, dk, dv, dstate = _C.linear_bwd(dout, q, k, v, decay, ctx.scale, cu, ctx.most, state,
+                                           dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7])
+        return None, None, None, dq, dk, dv, None, dstate
+
+
+def _attend(pack, q, k, v, decay, scale, state, want):
+    batch = pack[0].numel() - 1 if pack is not None else q.shape[0]
+    decay, scale = _check(q, k, v, decay, pack is not None, scale)
+    dk, dv = q.shape[-1], v.shape[-1]
+    if state is not None:
+        if tuple(state.shape) != (batch, q.shape[-2], dk, dv) or state.dtype != torch.float32 or state.device != q.device:
+            raise ValueError(f"fable_attn: initial_state must be float32 {(batch, q.shape[-2], dk, dv)} on q's device, got "
+                             f"{state.dtype} {tuple(state.shape)}")
+    wk, wv = _kernel_width(dk, q.dtype), _kernel_width(dv, q.dtype)
+    if state is not None:
+        state = torch.nn.functional.pad(state, (0, wv - dv, 0, wk - dk)) if (wk, wv) != (dk, dv) else state.contiguous()
+        state = _aligned(state, dense=True)
+    q, k, v = (_aligned(_with_width(t, w)) for t, w in ((q, wk), (k, wk), (v, wv)))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
+        res = _LinearAttention.apply(pack, scale, want, q, k, v, decay, state)
+        out, final = res if want else (res, None)
+    else:
+        cu, most = pack if pack is not None else (None, 0)
+        final = torch.empty((batch, q.shape[-2], wk, wv), dtype=torch.float32, device=q.device) if want else None
+        out = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
+    if wv != dv:
+        out = out[..., :dv].contiguous()
+    if not want:
+        return out
+    return out, (final[..., :dk, :dv].contiguous() if (wk, wv) != (dk, dv) else final)
+
+
+def linear_attn_func(q, k, v, decay, scale=None, initial_state=None, return_final_state=False):
+    """Linear attention of q (batch, seqlen, nheads, d), k (batch, seqlen, nheads_k, d) and v (batch, seqlen, nheads_k, dv),
+    causal, with a decay per head of q. scale: d^-0.5 by default. initial_state: float32 (batch, nheads, d, dv), the state before the first
+    token (zeros by default). Returns out (batch, seqlen, nheads, dv), or (out, final_state) with the state
+    behind the last token, from which the next call goes on. Gradients flow to q, k, v and initial_state, also through
+    final_state; results are reproducible bit for bit."""
+    return _attend(None, q, k, v, decay, scale, initial_state, return_final_state)
+
+
+def linear_attn_varlen_func(q, k, v, cu_seqlens, max_seqlen, decay, scale=None, initial_state=None, return_final_state=False):
+    """linear_attn_func of packed sequences: q (total, nheads, d), k and v (total, nheads_k, ...), cu_seqlens int32 (batch+1);
+    states are (batch, nheads, d, dv). max_seqlen sizes the launch (a longer sequence is served, more
+    slowly). Sequences may be empty: their state passes through. Rows of no sequence come back as zeros, as do their gradients."""
+    cu = _as_index(cu_seqlens, q.device)
+    return _attend((cu, int(max_seqlen)), q, k, v, decay, scale, initial_state, return_final_state)
+
+
+@torch.no_grad()
+def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu_seqlens=None, max_seqlen=None):
+    """Serving: new tokens q, k, v (batch, seqlen_new, nheads, ...), or packed (total, nheads, ...) with cu_seqlens int32 (batch+1) and
+    max_seqlen (default: total), go on from the states of a pool, float32 (num_states, nheads, d, dv), which are
+    updated in place. state_idx int32 (batch): the state of each sequence (default: its own number); an entry outside the pool names
+    no sequence (a padded batch): its rows of out are zeros and no state changes. Two sequences of one call must not name one state; a
+    new request starts from a state that the caller has zeroed. Returns out as linear_attn_func. Up to 16 new tokens per sequence
+    run token by token, each state read and written once; more run by chunks. Head dims are multiples of 8. No gradient passes through."""
+    if not torch.is_tensor(state) or state.dim() != 4 or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError("fable_attn: state must be a contiguous float32 tensor (num_states, nheads, headdim, headdim_v)")
+    packed = cu_seqlens is not None
+    decay, scale = _check(q, k, v, decay, packed, scale)
+    if q.shape[-1] % 8 or v.shape[-1] % 8:
+        raise NotImplementedError(f"fable_attn: states are updated in place for head dims that are multiples of 8, got {q.shape[-1]} and {v.shape[-1]}")
+    dev = q.device
+    cu = _as_index(cu_seqlens, dev) if packed else None
+    most = (q.shape[0] if max_seqlen is None else int(max_seqlen)) if packed else q.shape[1]
+    idx = _as_index(state_idx, dev) if state_idx is not None else None
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    if most <= STEP_ROWS:
+        return _C.linear_step(q, k, v, state, decay, scale, cu, most, idx)[0]
+    return _C.linear_fwd(q, k, v, decay, scale, cu, most, state, state, idx)

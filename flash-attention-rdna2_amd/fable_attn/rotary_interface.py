@@ -1,0 +1,95 @@
+"""Rotary positions outside a cache call: queries and keys turned by the rows of two tables, with gradients, for
+training and for prompts (flash_attn_with_kvcache and flash_attn_append_kvcache turn by the same tables where
+they write a cache), and the tables, scaled for contexts longer than the trained ones.
+
+    flash_attn_rotary_func    q and k of a padded or packed batch
+    flash_attn_rotary_tables  cosines and sines of all positions
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _C
+from .flash_attn_interface import _DTYPES, _as_index
+
+
+def _flat(t):
+    """t with a contiguous head dim."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class _Rotary(torch.autograd.Function):
+    """The rotation is orthogonal but for the tables' amplitude: the gradients go back turned the other way."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, interleaved, cu, start):
+        ctx.save_for_backward(cos, sin, cu, start)
+        ctx.interleaved = interleaved
+        ctx.set_materialize_grads(False)
+        qo, ko, _, _ = _C.rotary(q, k, cos, sin, interleaved, cu, start)
+        return (qo, ko) if k is not None else qo
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        cos, sin, cu, start = ctx.saved_tensors
+        one, two = (dq, dk) if dq is not None else (dk, None)
+        if one is None:
+            return (None,) * 7
+        one, two, _, _ = _C.rotary(_flat(one), _flat(two) if two is not None else None, cos, sin, ctx.interleaved, cu, start, conj=True)
+        return (one, two, *(None,) * 5) if dq is not None else (None, one, *(None,) * 5)
+
+
+def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=True, rotary_seqlens=None, cu_seqlens=None):
+    """q (batch, seqlen, nheads, d) and k (batch, seqlen, nheads_k, d; may be None), or packed (total, nheads, d) with
+    cu_seqlens int32 (batch+1), turned in fp32 and rounded once. rotary_cos, rotary_sin: (rows, rotary_dim / 2), rotary_dim at most d; the
+    columns behind it are copied. Token t of sequence b has row rotary_seqlens[b] + t (an int or int32 (batch); default 0), the last
+    row serving those past it, as in flash_attn_append_kvcache. rotary_interleaved: pairs are columns 2 i and 2 i + 1,
+    else i and i + rotary_dim / 2. Returns (q, k), or q alone without a k, in new tensors; rows of no sequence come back as zeros.
+    Gradients flow to q and k."""
+    if not q.is_cuda:
+        raise ValueError("fable_attn: tensors must be on the GPU (q.is_cuda == False)")
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"fable_attn: dtype {q.dtype} is not supported; use fp16, bf16 or fp32")
+    if q.dim() != (4 if cu_seqlens is None else 3):
+        raise ValueError(f"fable_attn: q must be (batch, seqlen, nheads, headdim), or (total, nheads, headdim) with cu_seqlens; "
+                         f"got {tuple(q.shape)}")
+    grad = torch.is_grad_enabled()
+    if grad and (rotary_cos.requires_grad or rotary_sin.requires_grad):
+        raise NotImplementedError("fable_attn: rotary tables get no gradient; pass them detached")
+    dev = q.device
+    cos, sin = rotary_cos.detach().to(torch.float32).contiguous(), rotary_sin.detach().to(torch.float32).contiguous()
+    cu = _as_index(cu_seqlens, dev) if cu_seqlens is not None else None
+    if isinstance(rotary_seqlens, int):
+        batch = q.shape[0] if cu is None else cu.numel() - 1
+        rotary_seqlens = torch.full((batch,), rotary_seqlens, dtype=torch.int32, device=dev) if rotary_seqlens else None
+    start = _as_index(rotary_seqlens, dev) if rotary_seqlens is not None else None
+    q, k = _flat(q), _flat(k) if k is not None else None
+    if grad and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, cos, sin, bool(rotary_interleaved), cu, start)
+    qo, ko, _, _ = _C.rotary(q, k, cos, sin, bool(rotary_interleaved), cu, start)
+    return (qo, ko) if k is not None else qo
+
+
+@torch.no_grad()
+def flash_attn_rotary_tables(seqlen, rotary_dim, *, base=10000.0, factor=1.0, original_seqlen=None, low_turns=1.0, high_turns=32.0,
+                             amplitude=1.0, start=0, device=None):
+    """(cos, sin) in fp32, (seqlen, rotary_dim / 2), of positions start, start + 1, ...: pair i turns by f_i = base^(-2 i /
+    rotary_dim) per position, angles formed in 64 bits. For a context `factor` times longer than the trained one, f_i becomes f_i
+    (keep + (1 - keep) / factor): without original_seqlen keep is 0 (all positions are divided by the factor); with it
+    a pair that turns r times over that length has keep = (r - low_turns) / (high_turns - low_turns), between 0 and 1. The tables are
+    multiplied by amplitude."""
+    seqlen, rotary_dim, start = int(seqlen), int(rotary_dim), int(start)
+    if seqlen < 0 or start < 0:
+        raise ValueError(f"fable_attn: seqlen={seqlen}, start={start}: at least 0")
+    if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > 8192:
+        raise ValueError(f"fable_attn: rotary_dim={rotary_dim}: an even number of 2 to 8192")
+    if not base > 0 or not factor > 0:
+        raise ValueError(f"fable_attn: base={base}, factor={factor}: above 0")
+    if original_seqlen is not None and not (original_seqlen > 0 and high_turns > low_turns):
+        raise ValueError(f"fable_attn: original_seqlen={original_seqlen}, low_turns={low_turns}, high_turns={high_turns}: "
+                         "a length above 0, high_turns above low_turns")
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"fable_attn: tables are made on the GPU (device={device})")
+    return _C.rotary_tables(seqlen, start, rotary_dim // 2, float(base), float(factor), float(original_seqlen or 0), float(low_turns),
+                            float(high_turns), float(amplitude), device)

@@ -451,6 +451,81 @@ typedef struct FableGatherParams {
 } FableGatherParams;
 int fable_attn_gather(FableGatherParams p, int dtype, void* stream);
 
+/* Causal linear attention with a decay for each head. With l = exp(-decay[b*decay_b + h]), a head h of queries holds a state
+ * S of DK x DV values, and for the rows t of a sequence in order
+ *   S_t = l S_{t-1} + k_t v_t^T,   o_t = scale q_t^T S_t.
+ * NH heads of queries, NH / gqa of keys and values (head h reads head h / gqa); DK and DV are multiples of 8 up to 256.
+ * Padded batches have n rows per sequence (row t of sequence b at b*.b + t*.s elements); with cu (int32, batch+1) sequence b has the
+ * rows cu[b]..cu[b+1] of [0, total) (at row*.s, .b ignored) and n is the most any sequence has, which only sizes the grid: a longer
+ * sequence is served, more slowly. Rows of [0, total) in front of cu[0] and behind cu[batch] become zeros in o and in the gradients.
+ * States are fp32, [slot][NH][DK][DV]; sequence b has slot slots[b] (NULL: b). A slot outside [0, num_slots) names no sequence: its
+ * rows of o become zeros, and no state is read or written. Two sequences of a call must not name one slot.
+ * state_in (NULL: zeros) is S before the first row, state_out (may be NULL, may be state_in) the one behind the last.
+ * Sums and states are kept in 32 bits. A row whose products are not finite may make other rows of its 64 so. */
+typedef struct FableLinearParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const void* dout;          /* fable_linear_attn_bwd: the gradient of o, and where those of q, k and v go */
+  void* dq;
+  void* dk;
+  void* dv;
+  fa_strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  const float* decay;
+  int64_t decay_b;
+  const float* state_in;
+  float* state_out;
+  const float* dstate_out;   /* gradient of state_out (NULL: zeros), and where that of state_in goes (may be NULL) */
+  float* dstate_in;
+  const int32_t* cu;
+  const int32_t* slots;
+  int64_t total;
+  int32_t batch, n, NH, gqa, DK, DV, num_slots;
+  float scale;
+} FableLinearParams;
+/* Workspace of a call in bytes (16-byte aligned; 0: none, -1: invalid call; no tensor is read). */
+int64_t fable_linear_attn_ws_bytes(FableLinearParams p, int dtype, int backward);
+int fable_linear_attn_fwd(FableLinearParams p, int dtype, void* ws, int64_t ws_bytes, void* stream);
+/* dq, dk, dv (and dstate_in) from q, k, v, dout (and state_in, dstate_out); no slots. */
+int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, int64_t ws_bytes, void* stream);
+/* The same as fable_linear_attn_fwd for few rows per sequence (any number is served): token by token, in 32 bits, each state read and
+ * written once. state_in and state_out are required. */
+int fable_linear_attn_step(FableLinearParams p, int dtype, void* stream);
+
+/* Queries and keys turned by their positions: column pair i of a head, (a, b), becomes (a c - b s, b c + a s) with
+ * c = cos[row][i], s = sin[row][i] (conj: s = -sin, the gradient's way back), in fp32, rounded once. rotary 1: pairs are columns i and
+ * i + rotary_dim / 2, 2: columns 2 i and 2 i + 1; columns from rotary_dim on are copied. Token t of sequence b has row
+ * start[b] + t (start NULL: t), at most rotary_rows - 1 and at least 0. Padded (batch, n) or packed (cu, total) as above; rows of no
+ * sequence become zeros. k may be NULL. Outputs must not overlap the inputs. */
+typedef struct FableRotaryParams {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  fa_strides sq, sk, sqo, sko;
+  const float* cos;
+  const float* sin;
+  const int32_t* cu;
+  const int32_t* start;
+  int64_t total;
+  int32_t batch, n, NH, NKV, HD, rotary, rotary_dim, rotary_rows, conj;
+} FableRotaryParams;
+int fable_attn_rotary(FableRotaryParams p, int dtype, void* stream);
+
+/* cos and sin of (row + first) * f_i, i < pairs, times amplitude: [rows][pairs] fp32. f_i = base^(-i / pairs); with a factor
+ * above 1 (or below) it becomes f_i (keep + (1 - keep) / factor), keep = clamp((original f_i / 2 pi - low) / (high - low), 0, 1): a pair
+ * that turns at least `high` times over the `original` positions keeps its frequency, one that turns at most `low` times is
+ * slowed by the factor (original 0: all are). Angles are formed in 64 bits. */
+typedef struct FableRotaryTableParams {
+  float* cos;
+  float* sin;
+  int64_t rows, first;
+  int32_t pairs;
+  double base, factor, original, low, high, amplitude;
+} FableRotaryTableParams;
+int fable_attn_rotary_tables(FableRotaryTableParams p, void* stream);
+
 /* split count chosen for a decode call (reference heuristic: dispatch.cpp:182-200, retuned for
  * 256 CUs); num_splits_hint > 0 is honoured (clamped to [1, 512]). */
 int fa_decode_num_splits(int batch, int nq, int NH, int gqa, int64_t ctx_bound, int num_splits_hint);
@@ -461,8 +536,8 @@ int fa_combine_launch(CombineParams p, void* stream);
 /* introspection for bindings and tests */
 int fable_attn_abi_version(void);
 /* sizeof of a struct: 0 FableFwdParams, 1 FableBwdParams, 2 FableDecParams, 3 CombineParams,
- * 4 fa_strides, 5 FwdParams, 6 BwdParams, 7 DecParams, 8 FableCache8, 9 FableAppendParams, 10 FableGatherParams
- * (0 for any other value) */
+ * 4 fa_strides, 5 FwdParams, 6 BwdParams, 7 DecParams, 8 FableCache8, 9 FableAppendParams, 10 FableGatherParams,
+ * 11 FableLinearParams, 12 FableRotaryParams, 13 FableRotaryTableParams (0 for any other value) */
 size_t fable_attn_struct_size(int which);
 const char* fable_attn_last_error(void);
 
