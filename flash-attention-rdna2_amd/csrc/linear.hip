@@ -61,8 +61,16 @@ namespace {
 
 int la_elt(int dtype) { return dtype == FA_F32 ? 4 : 2; }
 
+// The stride of a single row is anything; the kernel takes it for a distance.
+void la_single(LaArgs& a) {
+  if ((a.cu ? a.total : a.n) > 1) return;
+  a.sx.s = a.sy.s = a.da;
+  a.sz.s = a.db;
+}
+
 // Segments for a pass of output width db: two workgroups for each of the 256 CUs, but none of fewer than 256 rows.
 void la_split(LaArgs& a) {
+  la_single(a);
   const int width = a.db <= 64 ? 64 : 128;
   const long long base = (long long)a.batch * a.NH * ((a.db + width - 1) / width);
   long long k = base >= 256 ? 1 : (512 + base - 1) / (base > 0 ? base : 1);
@@ -177,14 +185,29 @@ int la_check(const FableLinearParams& p, int dtype, const char* what) {
   return FA_OK;
 }
 
-int la_tensor(const char* what, const char* name, const void* t, const fa_strides& s, int dtype) {
+int la_tensor(const char* what, const char* name, const void* t, const fa_strides& s, int width, const FableLinearParams& p, int dtype) {
   const int e = la_elt(dtype);
   if (!t) return fail(FA_ERR_ARG, "%s: null %s", what, name);
   if (((uintptr_t)t | (uintptr_t)(s.b * e) | (uintptr_t)(s.h * e) | (uintptr_t)(s.s * e)) & 15)
     return fail(FA_ERR_ARG, "%s: %s: rows must be 16-byte aligned", what, name);
-  // (offsets within a chunk are 32 bits wide)
-  if (s.s < 0 || s.s * e * kLaChunk >= (1LL << 31)) return fail(FA_ERR_ARG, "%s: %s: a row stride of %lld values", what, name, (long long)s.s);
+  // Offsets within a chunk are 32 bits wide, and its rows must not overlap: a row of no token is known by its offset.
+  if (s.s >= (1LL << 30) / (e * kLaChunk) || ((p.cu ? p.total : p.n) > 1 && s.s < width))
+    return fail(FA_ERR_ARG, "%s: %s: a row stride of %lld values", what, name, (long long)s.s);
   return FA_OK;
+}
+
+// q, k, v and o, or in the backward pass dout and the gradients
+int la_tensors(const char* what, const FableLinearParams& p, int dtype, bool backward) {
+  int rc;
+  if ((p.cu ? p.total : p.n) == 0) return FA_OK;
+  if ((rc = la_tensor(what, "q", p.q, p.sq, p.DK, p, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, p.DK, p, dtype)) ||
+      (rc = la_tensor(what, "v", p.v, p.sv, p.DV, p, dtype)))
+    return rc;
+  if (!backward) return la_tensor(what, "o", p.o, p.so, p.DV, p, dtype);
+  if ((rc = la_tensor(what, "dout", p.dout, p.sdo, p.DV, p, dtype)) || (rc = la_tensor(what, "dq", p.dq, p.sdq, p.DK, p, dtype)) ||
+      (rc = la_tensor(what, "dk", p.dk, p.sdk, p.DK, p, dtype)))
+    return rc;
+  return la_tensor(what, "dv", p.dv, p.sdv, p.DV, p, dtype);
 }
 
 long long la_group_bytes(const FableLinearParams& p) {
@@ -228,11 +251,7 @@ extern "C" int fable_linear_attn_fwd(FableLinearParams p, int dtype, void* ws, i
   if (rc != FA_OK) return rc;
   if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
   if (p.slots && (p.num_slots < 0 || (!p.state_in && !p.state_out))) return fail(FA_ERR_ARG, "%s: slots without states", what);
-  if ((p.cu ? p.total : p.n) > 0) {
-    if ((rc = la_tensor(what, "q", p.q, p.sq, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, dtype)) ||
-        (rc = la_tensor(what, "v", p.v, p.sv, dtype)) || (rc = la_tensor(what, "o", p.o, p.so, dtype)))
-      return rc;
-  }
+  if ((rc = la_tensors(what, p, dtype, false)) != FA_OK) return rc;
   const long long need = la_need(p, false);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
@@ -247,11 +266,7 @@ extern "C" int fable_linear_attn_step(FableLinearParams p, int dtype, void* stre
   if (!p.decay || !p.state_in || !p.state_out) return fail(FA_ERR_ARG, "%s: null decay or state", what);
   if (((uintptr_t)p.state_in | (uintptr_t)p.state_out) & 15) return fail(FA_ERR_ARG, "%s: states must be 16-byte aligned", what);
   if (p.slots && p.num_slots < 0) return fail(FA_ERR_ARG, "%s: num_slots=%d", what, p.num_slots);
-  if ((p.cu ? p.total : p.n) > 0) {
-    if ((rc = la_tensor(what, "q", p.q, p.sq, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, dtype)) ||
-        (rc = la_tensor(what, "v", p.v, p.sv, dtype)) || (rc = la_tensor(what, "o", p.o, p.so, dtype)))
-      return rc;
-  }
+  if ((rc = la_tensors(what, p, dtype, false)) != FA_OK) return rc;
   if (p.batch == 0) return FA_OK;
   la_step(la_forward(p), dtype, (hipStream_t)stream);
   return launch_status(what);
@@ -263,13 +278,7 @@ extern "C" int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, i
   if (rc != FA_OK) return rc;
   if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
   if (p.slots) return fail(FA_ERR_ARG, "%s: states of a pool have no gradient", what);
-  if ((p.cu ? p.total : p.n) > 0) {
-    if ((rc = la_tensor(what, "q", p.q, p.sq, dtype)) || (rc = la_tensor(what, "k", p.k, p.sk, dtype)) ||
-        (rc = la_tensor(what, "v", p.v, p.sv, dtype)) || (rc = la_tensor(what, "dout", p.dout, p.sdo, dtype)) ||
-        (rc = la_tensor(what, "dq", p.dq, p.sdq, dtype)) || (rc = la_tensor(what, "dk", p.dk, p.sdk, dtype)) ||
-        (rc = la_tensor(what, "dv", p.dv, p.sdv, dtype)))
-      return rc;
-  }
+  if ((rc = la_tensors(what, p, dtype, true)) != FA_OK) return rc;
   const long long need = la_need(p, true);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);

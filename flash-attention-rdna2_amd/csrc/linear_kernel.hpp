@@ -76,38 +76,38 @@ struct La<float> {
   }
 };
 
-// LDS tiles of rows of W values in units of four. A unit's place within its row is turned by the row, so that 32 rows read
-// at one column, and 4 rows x 32 columns read transposed, meet every bank once (16-bit types; 64 banks).
-template <int W>
-__device__ __forceinline__ int la_turn(int row) {
-  if constexpr (W >= 128) return ((row & 3) << 3) | ((row >> 2) & 7);
-  else return (((row >> 1) & 1) << 3) | ((row >> 2) & 7);
-}
-template <int W>
-__device__ __forceinline__ int la_ofs(int row, int unit) { return row * W + 4 * (unit ^ la_turn<W>(row)); }
+// LDS tiles, rows of LD values. Rows of x and y are read by 32 lanes at one column (8 bytes each) and y by columns, 4 rows x 32
+// columns at a time: a row is 7 units of 8 bytes longer than a multiple of the 64 banks (or of half of them), so the first meets every bank
+// once and the second nearly so; z is read by columns only and is 8 units longer. (fp32: one unit of 16 bytes.) Padding, not a turned
+// order within the row, because then all addresses are one register and constants.
+template <typename T, int W>
+constexpr int kLaRow = W + (sizeof(T) == 2 ? 28 : 4);
+template <typename T, int W>
+constexpr int kLaRowZ = W + (sizeof(T) == 2 ? 32 : 4);
 
 // rows row (per lane), columns 16 s .. 16 s + 15
-template <typename T, int W>
+template <typename T, int LD>
 __device__ __forceinline__ typename La<T>::F la_rows(const T* tile, int row, int s, int g) {
   using H = typename La<T>::H;
-  const H a = *(const H*)(tile + la_ofs<W>(row, 4 * s + g)), b = *(const H*)(tile + la_ofs<W>(row, 4 * s + 2 + g));
+  const T* at = tile + row * LD + 4 * g + 16 * s;
+  const H a = *(const H*)at, b = *(const H*)(at + 8);
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // column 32 ct + r, rows 16 s .. 16 s + 15
-template <typename T, int W>
+template <typename T, int LD>
 __device__ __forceinline__ typename La<T>::F la_cols(const T* tile, int ct, int s, int lane) {
   using H = typename La<T>::H;
   const int g = lane / 32;
   if constexpr (sizeof(T) == 2) {
-    const int row = 16 * s + 4 * g + (lane % 16) / 4, unit = 8 * ct + 4 * ((lane / 16) % 2) + lane % 4;
-    const H a = lds_read_tr<T>(tile + la_ofs<W>(row, unit)), b = lds_read_tr<T>(tile + la_ofs<W>(row + 8, unit));
+    const T* at = tile + (4 * g + (lane % 16) / 4) * LD + 16 * ((lane / 16) % 2) + 4 * (lane % 4) + 16 * s * LD + 32 * ct;
+    const H a = lds_read_tr<T>(at), b = lds_read_tr<T>(at + 8 * LD);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   } else {
-    const int r = lane % 32;
+    const T* at = tile + 4 * g * LD + lane % 32 + 16 * s * LD + 32 * ct;
     typename La<T>::F f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) f[j] = tile[la_ofs<W>(16 * s + 8 * (j / 4) + 4 * g + j % 4, 8 * ct + r / 4) + r % 4];
+    for (int j = 0; j < 8; j++) f[j] = at[(8 * (j / 4) + j % 4) * LD];
     return f;
   }
 }
@@ -177,10 +177,12 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
   constexpr int CA = DA / E, CB = DB / E;                     // 16-byte chunks of a row
   constexpr int LA = C * CA / NT, LB = C * CB / NT;           // chunks per thread
   static_assert(NT % CA == 0 && C * CA % NT == 0 && NT % CB == 0 && C * CB % NT == 0, "tile loads");
-  __shared__ __align__(16) T lds[(STATE ? 0 : C * DA) + C * DA + C * DB];
+  constexpr int LDA = kLaRow<T, DA>, LDZ = kLaRowZ<T, DB>;
+  __shared__ __align__(16) T lds[(STATE ? 0 : C * LDA) + C * LDA + C * LDZ];
+  __shared__ float pw[STATE ? 1 : C + 32];                    // pscale lambda^k at k + 31; zeros for k < 0
   T* const tx = lds;
-  T* const ty = lds + (STATE ? 0 : C * DA);
-  T* const tz = ty + C * DA;
+  T* const ty = lds + (STATE ? 0 : C * LDA);
+  T* const tz = ty + C * LDA;
 
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 32, g = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -216,16 +218,10 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
   const int nch = (p1 - p0 + C - 1) / C;
 
   const float d = la_decay(p, b, h), dl2 = d * kLog2e;
-  // weights of the scores of a block on the diagonal and of one 32 rows below it; of the update within 16 rows
-  float wd[16], wo[NB > 1 ? 16 : 1], wu[8];
-  if constexpr (!STATE) {
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int diff = r - (8 * (i / 4) + 4 * g + i % 4);
-      wd[i] = p.pscale * la_pow(dl2, (float)max(diff, 0));
-      if constexpr (NB > 1) wo[i] = p.pscale * la_pow(dl2, (float)(diff + 32));
-    }
-  }
+  const float* const weight = pw + 31 + r - 4 * g;
+  if constexpr (!STATE)
+    for (int i = tid; i < C + 32; i += NT) pw[i] = i < 31 ? 0.0f : p.pscale * la_pow(dl2, (float)(i - 31));
+  float wu[8];                                                // weights of the update within 16 rows
 #pragma unroll
   for (int j = 0; j < 8; j++) wu[j] = la_pow(dl2, (float)(15 - (8 * (j / 4) + 4 * g + j % 4)));
 
@@ -256,46 +252,50 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     }
   }
 
-  // tile loads: a thread's 16-byte column is the same for all its rows
+  // Tile loads. A thread's 16-byte column and its rows in LDS are fixed; the row in memory is the row in LDS less `shift`, or counted from the
+  // end. Rows of no token fall outside the buffer descriptor (their offsets are negative, or past its end) and read as zeros;
+  // so do columns past the head dim, from an offset so large that no row brings it back.
   const int xr = tid / CA, xc = tid % CA, zr = tid / CB, zc = tid % CB;
+  constexpr int kOut = (int)0xC0000000u;
+  const int bx = (int)p.sx.s * (int)sizeof(T), by = (int)p.sy.s * (int)sizeof(T), bz = (int)p.sz.s * (int)sizeof(T);
   const bool xin = xc * E < p.da, zin = dbt * DB + zc * E < p.db;
-  const T* const gx = (const T*)p.x + (p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h + sq.row0 * p.sx.s;
-  const T* const gy = (const T*)p.y + (p.cu ? 0 : b * p.sy.b) + (h / p.hy) * p.sy.h + sq.row0 * p.sy.s;
-  const T* const gz = (const T*)p.z + (p.cu ? 0 : b * p.sz.b) + (h / p.hz) * p.sz.h + sq.row0 * p.sz.s + dbt * DB;
+  const char* const gx = (const char*)p.x + ((p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h) * (long long)sizeof(T);
+  const char* const gy = (const char*)p.y + ((p.cu ? 0 : b * p.sy.b) + (h / p.hy) * p.sy.h) * (long long)sizeof(T);
+  const char* const gz = (const char*)p.z + ((p.cu ? 0 : b * p.sz.b) + (h / p.hz) * p.sz.h + dbt * DB) * (long long)sizeof(T);
+  const int wx = p.da * (int)sizeof(T), wz = (p.db - dbt * DB) * (int)sizeof(T);
   u32x4 vx[STATE ? 1 : LA], vy[LA], vz[LB];
 
-  auto rows_of = [&](int c, long long& row) {                 // rows of chunk c, and its first one in the sequence
+  auto rows_of = [&](int c, long long& row) {                 // rows of chunk c, and its first one in memory
     const int q0 = p0 + c * C, n = min(C, p1 - q0);
-    row = p.rev ? sq.len - q0 - n : q0;
+    row = sq.row0 + (p.rev ? sq.len - q0 - n : q0);
     return n;
   };
   auto fetch = [&](int c) {
     long long row;
-    const int n = rows_of(c, row);
-    const auto rx = buf_rsrc(gx + row * p.sx.s, ((n - 1) * p.sx.s + p.da) * (long long)sizeof(T));
-    const auto ry = buf_rsrc(gy + row * p.sy.s, ((n - 1) * p.sy.s + p.da) * (long long)sizeof(T));
-    const auto rz = buf_rsrc(gz + row * p.sz.s, ((n - 1) * p.sz.s + p.db - dbt * DB) * (long long)sizeof(T));
+    const int n = rows_of(c, row), sign = p.rev ? -1 : 1;
+    const auto rx = buf_rsrc32(gx + row * bx, (unsigned)((n - 1) * bx + wx));
+    const auto ry = buf_rsrc32(gy + row * by, (unsigned)((n - 1) * by + wx));
+    const auto rz = buf_rsrc32(gz + row * bz, (unsigned)((n - 1) * bz + wz));
+    const int mx = p.rev ? C - 1 - xr : xr - (C - n), mz = p.rev ? C - 1 - zr : zr - (C - n);
+    const int ox = xin ? mx * bx + xc * 16 : kOut, oy = xin ? mx * by + xc * 16 : kOut, oz = zin ? mz * bz + zc * 16 : kOut;
+    const int ix = sign * (NT / CA) * bx, iy = sign * (NT / CA) * by, iz = sign * (NT / CB) * bz;
 #pragma unroll
     for (int i = 0; i < LA; i++) {
-      const int m = xr + i * (NT / CA);
-      const bool in = xin && m < n;
-      if constexpr (!STATE) vx[i] = buf_load16(rx, in ? m * (int)(p.sx.s * sizeof(T)) + xc * 16 : kBufZero);
-      vy[i] = buf_load16(ry, in ? m * (int)(p.sy.s * sizeof(T)) + xc * 16 : kBufZero);
+      if constexpr (!STATE) vx[i] = buf_load16(rx, ox + i * ix);
+      vy[i] = buf_load16(ry, oy + i * iy);
     }
 #pragma unroll
-    for (int i = 0; i < LB; i++) {
-      const int m = zr + i * (NT / CB);
-      vz[i] = buf_load16(rz, zin && m < n ? m * (int)(p.sz.s * sizeof(T)) + zc * 16 : kBufZero);
-    }
+    for (int i = 0; i < LB; i++) vz[i] = buf_load16(rz, oz + i * iz);
   };
-  auto put = [&](T* tile, int W, int row, int c, u32x4 v) {   // 16 bytes as units of four values
+  T* const px = tx + xr * LDA + xc * E;
+  T* const py = ty + xr * LDA + xc * E;
+  T* const pz = tz + zr * LDZ + zc * E;
+  auto put = [&](T* at, u32x4 v) {                            // rows of x and y are 8-byte aligned in 16 bits
     if constexpr (sizeof(T) == 2) {
-      const int a = W == DA ? la_ofs<DA>(row, 2 * c) : la_ofs<DB>(row, 2 * c);
-      const int e = W == DA ? la_ofs<DA>(row, 2 * c + 1) : la_ofs<DB>(row, 2 * c + 1);
-      *(u32x2*)(tile + a) = u32x2{v[0], v[1]};
-      *(u32x2*)(tile + e) = u32x2{v[2], v[3]};
+      ((u32x2*)at)[0] = u32x2{v[0], v[1]};
+      ((u32x2*)at)[1] = u32x2{v[2], v[3]};
     } else {
-      *(u32x4*)(tile + (W == DA ? la_ofs<DA>(row, c) : la_ofs<DB>(row, c))) = v;
+      *(u32x4*)at = v;
     }
   };
 
@@ -304,18 +304,13 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     long long row;
     const int n = rows_of(c, row), shift = C - n;
     __syncthreads();
-    {
-      const int s = p.rev ? 0 : shift;
-      auto place = [&](int m) { return p.rev ? C - 1 - m : (m + s) & (C - 1); };
 #pragma unroll
-      for (int i = 0; i < LA; i++) {
-        const int at = place(xr + i * (NT / CA));
-        if constexpr (!STATE) put(tx, DA, at, xc, vx[i]);
-        put(ty, DA, at, xc, vy[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < LB; i++) put(tz, DB, place(zr + i * (NT / CB)), zc, vz[i]);
+    for (int i = 0; i < LA; i++) {
+      if constexpr (!STATE) put(px + i * (NT / CA) * LDA, vx[i]);
+      put(py + i * (NT / CA) * LDA, vy[i]);
     }
+#pragma unroll
+    for (int i = 0; i < LB; i++) *(u32x4*)(pz + i * (NT / CB) * LDZ) = vz[i];
     if (c + 1 < nch) fetch(c + 1);
     __syncthreads();
 
@@ -323,7 +318,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     const int enter = p.enter && sg == 0 && c == 0;
     F zf[2 * NB];
 #pragma unroll
-    for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, DB>(tz, wave, s, lane);
+    for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
 
     if constexpr (!STATE) {
       f32x16 sc[NB][NB], o[NB];                                // [key block][query block]
@@ -349,9 +344,9 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
       for (int s = 0; s < DA / 16; s++) {
         F xf[NB], yf[NB], sf;
 #pragma unroll
-        for (int q = 0; q < NB; q++) xf[q] = la_rows<T, DA>(tx, 32 * q + r, s, g);
+        for (int q = 0; q < NB; q++) xf[q] = la_rows<T, LDA>(tx, 32 * q + r, s, g);
 #pragma unroll
-        for (int k = 0; k < NB; k++) yf[k] = la_rows<T, DA>(ty, 32 * k + r, s, g);
+        for (int k = 0; k < NB; k++) yf[k] = la_rows<T, LDA>(ty, 32 * k + r, s, g);
 #pragma unroll
         for (int j = 0; j < 8; j++) sf[j] = (T)(S[s / 2][8 * (s % 2) + j] * norm);
 #pragma unroll
@@ -370,10 +365,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
         for (int k = 0; k <= q; k++)
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            float v;
-            if (k == q) v = r >= 8 * (i / 4) + 4 * g + i % 4 ? sc[k][q][i] * wd[i] : 0.0f;
-            else v = sc[k][q][i] * wo[i];
-            sc[k][q][i] = v;
+            sc[k][q][i] *= weight[32 * (q - k) - (8 * (i / 4) + i % 4)];
           }
         float down = 1.0f;
         if constexpr (La<T>::kPieces == 2) {
@@ -403,7 +395,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
         }
         const int at = 32 * q + r;
         const bool ok = at >= shift && col0 < p.db;
-        const long long to = obase + (sq.row0 + row + (p.rev ? C - 1 - at : at - shift)) * p.so.s + col0;
+        const long long to = obase + (row + (p.rev ? C - 1 - at : at - shift)) * p.so.s + col0;
         if constexpr (sizeof(T) == 4) {
           store_cblock_f32((float*)p.o + to, o[q], 1.0f, g, ok, p.db - col0);
         } else {
@@ -443,7 +435,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
         for (int i = 0; i < 16; i++) u[i] = 0.0f;
 #pragma unroll
         for (int s = 0; s < 2 * NB; s++) {
-          const F yt = la_cols<T, DA>(ty, t, s, lane);
+          const F yt = la_cols<T, LDA>(ty, t, s, lane);
           u = La<T>::mma(yt, z1[s], u);
           u = La<T>::mma(yt, z0[s], u);
         }
@@ -472,7 +464,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
         }
 #pragma unroll
         for (int t = 0; t < KT; t++) {
-          const F yt = la_cols<T, DA>(ty, t, s, lane);
+          const F yt = la_cols<T, LDA>(ty, t, s, lane);
           if constexpr (La<T>::kPieces == 3) {
             S[t] = La<T>::mma(yt, z2, S[t]);
             S[t] = La<T>::mma(yt, z1, S[t]);
@@ -513,9 +505,12 @@ int la_launch(const LaArgs& p, bool state, hipStream_t stream);
 
 constexpr int kLaChunk = 64;   // the longest chunk of any kernel: segments are multiples of it
 
+template <typename T, int DA>
+constexpr int kC = 32;
+
 template <typename T, int DA, int NW, bool STATE>
 inline int la_run(const LaArgs& p, hipStream_t st) {
-  constexpr int C = sizeof(T) == 2 && DA <= 128 ? 64 : 32;
+  constexpr int C = kC<T, DA>;
   const long long items = (long long)p.batch * (STATE ? p.nseg - 1 : p.nseg) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32));
   hipLaunchKernelGGL((la_kernel<T, DA, NW, C, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, p);
   return 0;

@@ -22,6 +22,11 @@ from .flash_attn_interface import MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _k
 STEP_ROWS = 16
 
 
+def _rows(t):
+    """t itself where the kernels can read it in place, else a copy: aligned rows that do not overlap (an expanded sequence)."""
+    return _aligned(t) if t.shape[-3] <= 1 or t.stride(-3) >= t.shape[-1] else t.clone(memory_format=torch.contiguous_format)
+
+
 def _check(q, k, v, decay, packed, scale):
     """What every call has to satisfy; (decay in fp32, scale)."""
     if not q.is_cuda:
@@ -63,7 +68,7 @@ class _LinearAttention(torch.autograd.Function):
         q, k, v, decay, state, cu = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 8
-        dout = q.new_zeros((*q.shape[:-1], v.shape[-1])) if dout is None else _aligned(dout)
+        dout = q.new_zeros((*q.shape[:-1], v.shape[-1])) if dout is None else _rows(dout)
         dq, dk, dv, dstate = _C.linear_bwd(dout, q, k, v, decay, ctx.scale, cu, ctx.most, state,
                                            dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7])
         return None, None, None, dq, dk, dv, None, dstate
@@ -81,7 +86,7 @@ def _attend(pack, q, k, v, decay, scale, state, want):
     if state is not None:
         state = torch.nn.functional.pad(state, (0, wv - dv, 0, wk - dk)) if (wk, wv) != (dk, dv) else state.contiguous()
         state = _aligned(state, dense=True)
-    q, k, v = (_aligned(_with_width(t, w)) for t, w in ((q, wk), (k, wk), (v, wv)))
+    q, k, v = (_rows(_with_width(t, w)) for t, w in ((q, wk), (k, wk), (v, wv)))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         res = _LinearAttention.apply(pack, scale, want, q, k, v, decay, state)
         out, final = res if want else (res, None)
@@ -131,7 +136,7 @@ def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu
     cu = _as_index(cu_seqlens, dev) if packed else None
     most = (q.shape[0] if max_seqlen is None else int(max_seqlen)) if packed else q.shape[1]
     idx = _as_index(state_idx, dev) if state_idx is not None else None
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    q, k, v = _rows(q), _rows(k), _rows(v)
     if most <= STEP_ROWS:
         return _C.linear_step(q, k, v, state, decay, scale, cu, most, idx)[0]
     return _C.linear_fwd(q, k, v, decay, scale, cu, most, state, state, idx)
