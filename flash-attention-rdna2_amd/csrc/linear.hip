@@ -68,19 +68,20 @@ void la_single(LaArgs& a) {
   a.sz.s = a.db;
 }
 
-// Segments for a pass of output width db: two workgroups for each of the 256 CUs, but none of fewer than 256 rows.
-void la_split(LaArgs& a) {
+// Segments of a call, the same for all its passes: two workgroups for each of the 256 CUs, but none of fewer than 256 rows.
+void la_split(LaArgs& a, const FableLinearParams& p) {
   la_single(a);
-  const int width = a.db <= 64 ? 64 : 128;
-  const long long base = (long long)a.batch * a.NH * ((a.db + width - 1) / width);
+  const int D = p.DK > p.DV ? p.DK : p.DV, width = D <= 64 ? 64 : 128;
+  const long long base = (long long)a.batch * a.NH * ((D + width - 1) / width);
   long long k = base >= 256 ? 1 : (512 + base - 1) / (base > 0 ? base : 1);
   const long long most = (a.n + 255) / 256;
   k = k > most ? most : k;
   k = k < 1 ? 1 : k;
   const long long seg = ((a.n + k - 1) / k + kLaChunk - 1) / kLaChunk * kLaChunk;
-  a.seg = (int)(seg < kLaChunk ? kLaChunk : seg > (1 << 30) ? (1 << 30) : seg);
+  a.seg = (int)(seg < kLaChunk ? kLaChunk : seg);
   a.nseg = (int)(((long long)a.n + a.seg - 1) / a.seg);
   if (a.nseg < 1) a.nseg = 1;
+  a.wa = p.DV, a.wb = 1;
 }
 
 long long la_ws(const LaArgs& a) { return a.nseg > 1 ? (long long)a.batch * a.NH * a.nseg * a.da * a.db * 4 : 0; }
@@ -110,7 +111,7 @@ LaArgs la_forward(const FableLinearParams& p) {
   a.sa = p.DV, a.sb = 1;
   a.slots = p.slots, a.nslots = p.num_slots;
   a.iscale = p.scale, a.uscale = 1.0f;
-  la_split(a);
+  la_split(a, p);
   return a;
 }
 
@@ -124,7 +125,8 @@ LaArgs la_dq(const FableLinearParams& p) {
   a.first = p.state_in;
   a.sa = 1, a.sb = p.DV;
   a.iscale = p.scale, a.uscale = 1.0f;
-  la_split(a);
+  la_split(a, p);
+  a.wa = 1, a.wb = p.DV;   // the states as they are for k, v (q, dout)
   return a;
 }
 
@@ -139,7 +141,7 @@ LaArgs la_dv(const FableLinearParams& p) {
   a.sa = p.DV, a.sb = 1;
   a.iscale = 1.0f, a.uscale = p.scale;
   a.rev = 1, a.enter = p.dstate_out != nullptr, a.leave = 1;
-  la_split(a);
+  la_split(a, p);
   return a;
 }
 
@@ -154,23 +156,22 @@ LaArgs la_dk(const FableLinearParams& p) {
   a.sa = 1, a.sb = p.DV;
   a.iscale = 1.0f, a.uscale = p.scale;
   a.rev = 1, a.enter = p.dstate_out != nullptr;
-  la_split(a);
+  la_split(a, p);
+  a.wa = 1, a.wb = p.DV;   // the states as they are for k, v (q, dout)
   return a;
 }
 
-int la_go(const LaArgs& a, int dtype, bool state, hipStream_t st) {
-  return dtype == FA_F16 ? la_launch<_Float16>(a, state, st) : dtype == FA_BF16 ? la_launch<__bf16>(a, state, st) : la_launch<float>(a, state, st);
+void la_go(const LaArgs& a, int dtype, bool state, bool exact, hipStream_t st) {
+  if (dtype == FA_F16) la_launch<_Float16>(a, state, exact, st);
+  else if (dtype == FA_BF16) la_launch<__bf16>(a, state, exact, st);
+  else la_launch<float>(a, state, exact, st);
 }
 
-// (nseg is above 1 for fewer than 256 states only, and then at most 512)
-int la_pass(LaArgs a, int dtype, void* ws, hipStream_t st) {
-  a.ws = (float*)ws;
-  if (a.nseg > 1) {
-    la_go(a, dtype, true, st);
-    hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)(a.batch * a.NH * ((a.da * a.db + 255) / 256))), dim3(256), 0, st, a);
-  }
-  la_go(a, dtype, false, st);
-  return launch_status("linear attention");
+// The states before all segments, into a.ws (nseg is above 1 for fewer than 256 states only, and then at most 512).
+void la_states(const LaArgs& a, int dtype, bool exact, hipStream_t st) {
+  if (a.nseg < 2) return;
+  la_go(a, dtype, true, exact, st);
+  hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)(a.batch * a.NH * ((a.da * a.db + 255) / 256))), dim3(256), 0, st, a);
 }
 
 // What every call has to satisfy; the tensors' own checks follow in the entry points.
@@ -217,13 +218,11 @@ long long la_group_bytes(const FableLinearParams& p) {
 
 long long la_round(long long x) { return (x + 255) / 256 * 256; }
 
+// Forward: the segments' states. Backward: those of q and dout, before them the ones of k and v, if the forward pass's are not
+// given, and behind them the partial gradients of shared heads.
 long long la_need(const FableLinearParams& p, bool backward) {
-  if (!backward) return la_ws(la_forward(p));
-  long long w = la_ws(la_dq(p));
-  const long long b = la_ws(la_dv(p)), c = la_ws(la_dk(p));
-  w = w > b ? w : b;
-  w = w > c ? w : c;
-  return la_round(w) + la_group_bytes(p);
+  const long long w = la_ws(la_forward(p));
+  return backward ? la_round(w) * (p.seg_states ? 1 : 2) + la_group_bytes(p) : w;
 }
 
 template <typename T>
@@ -256,7 +255,12 @@ extern "C" int fable_linear_attn_fwd(FableLinearParams p, int dtype, void* ws, i
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
   if (p.batch == 0) return FA_OK;
-  return la_pass(la_forward(p), dtype, ws, (hipStream_t)stream);
+  LaArgs a = la_forward(p);
+  a.ws = (float*)ws;
+  const bool exact = a.last != nullptr;
+  la_states(a, dtype, exact, (hipStream_t)stream);
+  la_go(a, dtype, false, exact, (hipStream_t)stream);
+  return launch_status(what);
 }
 
 extern "C" int fable_linear_attn_step(FableLinearParams p, int dtype, void* stream) {
@@ -278,33 +282,47 @@ extern "C" int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, i
   if (rc != FA_OK) return rc;
   if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
   if (p.slots) return fail(FA_ERR_ARG, "%s: states of a pool have no gradient", what);
+  if (p.gqa > 1 && (long long)p.NH * (p.DK > p.DV ? p.DK : p.DV) >= (1LL << 30) / (4 * kLaChunk)) return fail(FA_ERR_ARG, "%s: NH=%d", what, p.NH);
   if ((rc = la_tensors(what, p, dtype, true)) != FA_OK) return rc;
   const long long need = la_need(p, true);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
   if (p.batch == 0) return FA_OK;
   hipStream_t st = (hipStream_t)stream;
-  if ((rc = la_pass(la_dq(p), dtype, ws, st)) != FA_OK) return rc;
-  LaArgs a[2] = {la_dv(p), la_dk(p)};
+  // dq over the states of k and v
+  LaArgs a = la_forward(p), dq = la_dq(p);
+  char* at = (char*)ws;
+  if (p.seg_states) {
+    dq.ws = (float*)p.seg_states;
+  } else {
+    a.ws = dq.ws = (float*)at;
+    at += la_round(la_ws(a));
+    la_states(a, dtype, false, st);
+  }
+  la_go(dq, dtype, false, false, st);
+  // dv and dk over those of q and dout, from the last row on
+  LaArgs pass[2] = {la_dv(p), la_dk(p)};
+  const bool exact = pass[0].last != nullptr;
+  pass[0].ws = pass[1].ws = (float*)at;
+  la_states(pass[0], dtype, exact, st);
   float* const part = (float*)((char*)ws + (need - la_group_bytes(p)));
   for (int i = 0; i < 2; i++) {
-    const int D = a[i].db;
+    const int D = pass[i].db;
     if (p.gqa > 1) {
-      a[i].o = part;
-      a[i].o32 = 1;
-      a[i].so.b = p.cu ? 0 : (long long)p.n * p.NH * D;
-      a[i].so.s = (long long)p.NH * D;
-      a[i].so.h = D;
+      pass[i].o = part;
+      pass[i].o32 = 1;
+      pass[i].so.b = p.cu ? 0 : (long long)p.n * p.NH * D;
+      pass[i].so.s = (long long)p.NH * D;
+      pass[i].so.h = D;
     }
-    if ((rc = la_pass(a[i], dtype, ws, st)) != FA_OK) return rc;
+    la_go(pass[i], dtype, false, exact && i == 0, st);
     if (p.gqa > 1) {
       void* out = i == 0 ? p.dv : p.dk;
       const fa_strides so = i == 0 ? p.sdv : p.sdk;
       if (dtype == FA_F16) la_group<_Float16>(part, out, so, p, D, st);
       else if (dtype == FA_BF16) la_group<__bf16>(part, out, so, p, D, st);
       else la_group<float>(part, out, so, p, D, st);
-      if ((rc = launch_status(what)) != FA_OK) return rc;
     }
   }
-  return FA_OK;
+  return launch_status(what);
 }

@@ -1,9 +1,9 @@
-// Linear attention kernels for __bf16 (see linear_kernel.hpp).
+// Linear attention kernels for __bf16.
 #include "linear_kernel.hpp"
 
 namespace fa {
 template <>
-int la_launch<__bf16>(const LaArgs& p, bool state, hipStream_t st) {
-  return state ? la_pick<__bf16, true>(p, st) : la_pick<__bf16, false>(p, st);
+void la_launch<__bf16>(const LaArgs& p, bool state, bool exact, hipStream_t st) {
+  exact ? la_all<__bf16, 3>(p, state, st) : la_all<__bf16, 2>(p, state, st);
 }
 }  // namespace fa

@@ -1,9 +1,9 @@
-// Linear attention kernels for _Float16 (see linear_kernel.hpp).
+// Linear attention kernels for _Float16.
 #include "linear_kernel.hpp"
 
 namespace fa {
 template <>
-int la_launch<_Float16>(const LaArgs& p, bool state, hipStream_t st) {
-  return state ? la_pick<_Float16, true>(p, st) : la_pick<_Float16, false>(p, st);
+void la_launch<_Float16>(const LaArgs& p, bool state, bool, hipStream_t st) {
+  la_all<_Float16, 2>(p, state, st);
 }
 }  // namespace fa

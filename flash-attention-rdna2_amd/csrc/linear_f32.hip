@@ -1,9 +1,9 @@
-// Linear attention kernels for float (see linear_kernel.hpp).
+// Linear attention kernels for float.
 #include "linear_kernel.hpp"
 
 namespace fa {
 template <>
-int la_launch<float>(const LaArgs& p, bool state, hipStream_t st) {
-  return state ? la_pick<float, true>(p, st) : la_pick<float, false>(p, st);
+void la_launch<float>(const LaArgs& p, bool state, bool, hipStream_t st) {
+  la_all<float, 1>(p, state, st);
 }
 }  // namespace fa

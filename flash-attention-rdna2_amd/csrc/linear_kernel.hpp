@@ -39,10 +39,11 @@ struct LaArgs {
   long long decay_b;         // stride over the batch
   const float* first;        // states before the first row in processing order, [slot][NH][da][db] by ...
   float* last;               // ... and behind the last one; NULL: zeros, not wanted
-  long long sa, sb;          // strides of a state's element (a, b)
+  int sa, sb;                // strides of a state's element (a, b)
   const int32_t* slots;      // a sequence's state; NULL: its own number. Outside [0, nslots): no sequence
   int nslots;
-  float* ws;                 // [batch][NH][nseg][da][db]: the states before the segments (nseg > 1)
+  float* ws;                 // [batch][NH][nseg], the states before the segments (nseg > 1) ...
+  int wa, wb;                // ... and the strides of their elements
   const int32_t* cu;
   long long total;
   int batch, n, NH;
@@ -51,7 +52,7 @@ struct LaArgs {
   int rev;                   // rows from the last to the first
   int enter;                 // first is not to decay before the first row (the gradient of the final state)
   int leave;                 // last decays once more behind the last row (the gradient of the initial state)
-  int o32;                   // out is fp32 whatever T
+  int o32;                   // out is fp32 (partial gradients of shared heads)
 };
 
 // A fragment: lane (r, g) = (l % 32, l / 32) holds the contraction indices 16 s + 4 g + {0..3} and 16 s + 8 + 4 g + {0..3} of
@@ -60,7 +61,6 @@ template <typename T>
 struct La {
   using F = typename Dt<T>::V8;
   using H = typename Dt<T>::V4;
-  static constexpr int kPieces = __is_same(T, __bf16) ? 3 : 2;
   static __device__ __forceinline__ f32x16 mma(F a, F b, f32x16 c) { return Dt<T>::mma32(a, b, c); }
 };
 typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -68,7 +68,6 @@ template <>
 struct La<float> {
   using F = f32x8;
   using H = f32x4;
-  static constexpr int kPieces = 1;
   static __device__ __forceinline__ f32x16 mma(F a, F b, f32x16 c) {
 #pragma unroll
     for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
@@ -160,26 +159,61 @@ __device__ __forceinline__ int la_segments(const LaArgs& p, int len) {
 }
 
 // Zeros in rows [lo, hi) of out for the item's columns.
-template <typename T>
+template <typename O>
 __device__ __forceinline__ void la_zero_rows(const LaArgs& p, long long base, long long lo, long long hi, int c0, int nc, int tid, int nt) {
-  for (long long i = tid; i < (hi - lo) * nc; i += nt) {
-    const long long at = base + (lo + i / nc) * p.so.s + c0 + i % nc;
-    if (p.o32) ((float*)p.o)[at] = 0.0f;
-    else ((T*)p.o)[at] = (T)0.0f;
+  for (long long i = tid; i < (hi - lo) * nc; i += nt) ((O*)p.o)[base + (lo + i / nc) * p.so.s + c0 + i % nc] = (O)0.0f;
+}
+
+// An offset past every descriptor of a chunk (those are below 2^30 bytes), also with up to 2^30 added or taken off.
+constexpr int kLaOut = (int)0xC0000000u;
+
+// A 32-column block of a row, laid out as store_cblock's, through a buffer descriptor: `at` is the byte offset of the row's block, kLaOut
+// where nothing is to be stored. No branch around a store: the waits for the loads ahead of it then need not
+// wait for the store as well.
+template <typename O>
+__device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, const f32x16& acc, float scale, int hh, int ncols) {
+  if constexpr (sizeof(O) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int c = 8 * j + 4 * hh;
+      const f32x4 v = {acc[4 * j] * scale, acc[4 * j + 1] * scale, acc[4 * j + 2] * scale, acc[4 * j + 3] * scale};
+      __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(v), to, (c < ncols ? at : kLaOut) + 4 * c, 0, 0);
+    }
+  } else {
+    typedef O O4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      O4 x, y;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        x[c] = (O)(acc[8 * j + c] * scale);
+        y[c] = (O)(acc[8 * j + 4 + c] * scale);
+      }
+      const u32x2 xd = bitcast<u32x2>(x), yd = bitcast<u32x2>(y);
+      const auto r0 = __builtin_amdgcn_permlane32_swap(xd[0], yd[0], false, false);
+      const auto r1 = __builtin_amdgcn_permlane32_swap(xd[1], yd[1], false, false);
+      const int c = 16 * j + 8 * hh;
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{r0[0], r1[0], r0[1], r1[1]}, to, (c < ncols ? at : kLaOut) + 2 * c, 0, 0);
+    }
   }
 }
 
-template <typename T, int DA, int NW, int C, bool STATE>
-__global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs p) {
+// Waves per SIMD that the registers are to allow: S takes DA / 2 of them.
+constexpr int la_waves(int DA, int NW) { return DA <= 64 || (DA <= 128 && NW == 4) ? 3 : DA <= 128 ? 2 : 1; }
+
+template <typename T, typename O, int DA, int NW, int C, int PIECES, bool STATE>
+__global__ __launch_bounds__(NW * 64, la_waves(DA, NW)) void la_kernel(LaArgs p) {
   using F = typename La<T>::F;
   using H = typename La<T>::H;
   constexpr int NT = NW * 64, DB = NW * 32, NB = C / 32, KT = DA / 32, E = 16 / sizeof(T);
   constexpr int CA = DA / E, CB = DB / E;                     // 16-byte chunks of a row
   constexpr int LA = C * CA / NT, LB = C * CB / NT;           // chunks per thread
   static_assert(NT % CA == 0 && C * CA % NT == 0 && NT % CB == 0 && C * CB % NT == 0, "tile loads");
+  constexpr bool HALF = __is_same(T, _Float16);
   constexpr int LDA = kLaRow<T, DA>, LDZ = kLaRowZ<T, DB>;
   __shared__ __align__(16) T lds[(STATE ? 0 : C * LDA) + C * LDA + C * LDZ];
   __shared__ float pw[STATE ? 1 : C + 32];                    // pscale lambda^k at k + 31; zeros for k < 0
+  __shared__ __align__(16) float pu[C];                       // weights of the rows in the update
   T* const tx = lds;
   T* const ty = lds + (STATE ? 0 : C * LDA);
   T* const tz = ty + C * LDA;
@@ -204,10 +238,10 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
   if constexpr (!STATE) {
     // rows of no sequence in front of the first one and behind the last one
     const int c0 = dbt * DB, nc = min(DB, p.db - c0);
-    if (p.cu && sg == 0 && b == 0) la_zero_rows<T>(p, obase, 0, sq.row0, c0, nc, tid, NT);
-    if (p.cu && sg == 0 && b == p.batch - 1) la_zero_rows<T>(p, obase, sq.row0 + sq.len, p.total, c0, nc, tid, NT);
+    if (p.cu && sg == 0 && b == 0) la_zero_rows<O>(p, obase, 0, sq.row0, c0, nc, tid, NT);
+    if (p.cu && sg == 0 && b == p.batch - 1) la_zero_rows<O>(p, obase, sq.row0 + sq.len, p.total, c0, nc, tid, NT);
     if (sq.slot < 0) {
-      if (sg == 0) la_zero_rows<T>(p, obase, sq.row0, sq.row0 + sq.len, c0, nc, tid, NT);
+      if (sg == 0) la_zero_rows<O>(p, obase, sq.row0, sq.row0 + sq.len, c0, nc, tid, NT);
       return;
     }
   }
@@ -221,10 +255,10 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
   const float* const weight = pw + 31 + r - 4 * g;
   if constexpr (!STATE)
     for (int i = tid; i < C + 32; i += NT) pw[i] = i < 31 ? 0.0f : p.pscale * la_pow(dl2, (float)(i - 31));
-  float wu[8];                                                // weights of the update within 16 rows
-#pragma unroll
-  for (int j = 0; j < 8; j++) wu[j] = la_pow(dl2, (float)(15 - (8 * (j / 4) + 4 * g + j % 4)));
+  for (int i = tid; i < C; i += NT) pu[i] = (HALF ? 1.0f : p.uscale) * la_pow(dl2, (float)(C - 1 - i));
 
+  // byte offset of a state's element in the lane's column
+  auto state_at = [&](int a, int ra, int rb) { return a < p.da && col0 + r < p.db ? 4 * (a * ra + (col0 + r) * rb) : kLaOut; };
   f32x16 S[KT];
   const long long state = ((long long)sq.slot * p.NH + h) * p.da * p.db;
 #pragma unroll
@@ -233,22 +267,31 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     for (int i = 0; i < 16; i++) S[t][i] = 0.0f;
   if (!STATE) {
     const float* from = nullptr;
-    long long ra = p.sa, rb = p.sb;
+    int ra = p.sa, rb = p.sb;
     if (p.nseg == 1) {
       if (p.first) from = p.first + state;
     } else {
       from = p.ws + (((long long)b * p.NH + h) * p.nseg + sg) * p.da * p.db;
-      ra = p.db;
-      rb = 1;
+      ra = p.wa;
+      rb = p.wb;
     }
     if (from) {
+      const auto rs = buf_rsrc32(from, (unsigned)(p.da * p.db * 4));
+      if (ra == 1) {                                           // four elements of the lane's side by side
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4 v = bitcast<f32x4>(buf_load16(rs, state_at(32 * t + 2 * i + 4 * g, 1, rb)));
+#pragma unroll
+            for (int j = 0; j < 4; j++) S[t][i + j] = v[j];
+          }
+      } else
 #pragma unroll
       for (int t = 0; t < KT; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int a = 32 * t + 8 * (i / 4) + 4 * g + i % 4;
-          if (a < p.da && col0 + r < p.db) S[t][i] = from[a * ra + (col0 + r) * rb];
-        }
+        for (int i = 0; i < 16; i++)
+          S[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, state_at(32 * t + 8 * (i / 4) + 4 * g + i % 4, ra, rb), 0, 0));
     }
   }
 
@@ -256,7 +299,6 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
   // end. Rows of no token fall outside the buffer descriptor (their offsets are negative, or past its end) and read as zeros;
   // so do columns past the head dim, from an offset so large that no row brings it back.
   const int xr = tid / CA, xc = tid % CA, zr = tid / CB, zc = tid % CB;
-  constexpr int kOut = (int)0xC0000000u;
   const int bx = (int)p.sx.s * (int)sizeof(T), by = (int)p.sy.s * (int)sizeof(T), bz = (int)p.sz.s * (int)sizeof(T);
   const bool xin = xc * E < p.da, zin = dbt * DB + zc * E < p.db;
   const char* const gx = (const char*)p.x + ((p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h) * (long long)sizeof(T);
@@ -265,20 +307,29 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
   const int wx = p.da * (int)sizeof(T), wz = (p.db - dbt * DB) * (int)sizeof(T);
   u32x4 vx[STATE ? 1 : LA], vy[LA], vz[LB];
 
+  // lambda^(i + 1) of the lane's rows and lambda^C - 1: of all chunks but a short one and, with `enter`, the first
+  float full[STATE ? 1 : NB];
+  if constexpr (!STATE)
+#pragma unroll
+    for (int q = 0; q < NB; q++) full[q] = p.iscale * la_pow(dl2, (float)(32 * q + r + 1));
+  const float fade = expm1f(-d * (float)C);
+
   auto rows_of = [&](int c, long long& row) {                 // rows of chunk c, and its first one in memory
     const int q0 = p0 + c * C, n = min(C, p1 - q0);
     row = sq.row0 + (p.rev ? sq.len - q0 - n : q0);
     return n;
   };
+  const int sign = p.rev ? -1 : 1, mx = p.rev ? C - 1 - xr : xr, mz = p.rev ? C - 1 - zr : zr;
+  const int ox0 = xin ? mx * bx + xc * 16 : kLaOut, oy0 = xin ? mx * by + xc * 16 : kLaOut, oz0 = zin ? mz * bz + zc * 16 : kLaOut;
+  const int ix = sign * (NT / CA) * bx, iy = sign * (NT / CA) * by, iz = sign * (NT / CB) * bz;
   auto fetch = [&](int c) {
     long long row;
-    const int n = rows_of(c, row), sign = p.rev ? -1 : 1;
-    const auto rx = buf_rsrc32(gx + row * bx, (unsigned)((n - 1) * bx + wx));
-    const auto ry = buf_rsrc32(gy + row * by, (unsigned)((n - 1) * by + wx));
-    const auto rz = buf_rsrc32(gz + row * bz, (unsigned)((n - 1) * bz + wz));
-    const int mx = p.rev ? C - 1 - xr : xr - (C - n), mz = p.rev ? C - 1 - zr : zr - (C - n);
-    const int ox = xin ? mx * bx + xc * 16 : kOut, oy = xin ? mx * by + xc * 16 : kOut, oz = zin ? mz * bz + zc * 16 : kOut;
-    const int ix = sign * (NT / CA) * bx, iy = sign * (NT / CA) * by, iz = sign * (NT / CB) * bz;
+    const int n = rows_of(c, row), shift = p.rev ? 0 : C - n;
+    // (behind the last chunk nothing is read)
+    const auto rx = buf_rsrc32(gx + row * bx, n > 0 ? (unsigned)((n - 1) * bx + wx) : 0u);
+    const auto ry = buf_rsrc32(gy + row * by, n > 0 ? (unsigned)((n - 1) * by + wx) : 0u);
+    const auto rz = buf_rsrc32(gz + row * bz, n > 0 ? (unsigned)((n - 1) * bz + wz) : 0u);
+    const int ox = ox0 - shift * bx, oy = oy0 - shift * by, oz = oz0 - shift * bz;
 #pragma unroll
     for (int i = 0; i < LA; i++) {
       if constexpr (!STATE) vx[i] = buf_load16(rx, ox + i * ix);
@@ -299,7 +350,17 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     }
   };
 
-  if (nch > 0) fetch(0);
+  fetch(0);
+  if constexpr (!STATE) {
+    // Stores to nowhere, as many as a chunk has behind the next one's loads: a wait for loads counts what was issued since, and the
+    // compiler takes the lowest count of all ways into the loop.
+    f32x16 none;
+#pragma unroll
+    for (int i = 0; i < 16; i++) none[i] = 0.0f;
+    const auto ro = buf_rsrc32(p.o, 0u);
+#pragma unroll
+    for (int q = 0; q < NB; q++) la_store<O>(ro, kLaOut, none, 1.0f, g, 32);
+  }
   for (int c = 0; c < nch; c++) {
     long long row;
     const int n = rows_of(c, row), shift = C - n;
@@ -311,16 +372,19 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     }
 #pragma unroll
     for (int i = 0; i < LB; i++) *(u32x4*)(pz + i * (NT / CB) * LDZ) = vz[i];
-    if (c + 1 < nch) fetch(c + 1);
+    fetch(c + 1);
     __syncthreads();
 
     // the state enters the first row as it is where it is the final state's gradient
     const int enter = p.enter && sg == 0 && c == 0;
+    const bool other = shift || enter;
     F zf[2 * NB];
 #pragma unroll
     for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
 
     if constexpr (!STATE) {
+      const int bo = (int)p.so.s * (int)sizeof(O);
+      const auto ro = buf_rsrc32((const O*)p.o + obase + row * p.so.s + col0, (unsigned)((n - 1) * bo + 32 * (int)sizeof(O)));
       f32x16 sc[NB][NB], o[NB];                                // [key block][query block]
 #pragma unroll
       for (int q = 0; q < NB; q++) {
@@ -332,7 +396,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
           for (int i = 0; i < 16; i++) sc[k][q][i] = 0.0f;
       }
       float norm = 1.0f, inv = 1.0f;
-      if constexpr (La<T>::kPieces == 2) {
+      if constexpr (HALF) {
         float m = 0.0f;
 #pragma unroll
         for (int t = 0; t < KT; t++)
@@ -358,7 +422,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
       }
 #pragma unroll
       for (int q = 0; q < NB; q++) {
-        const float lw = p.iscale * inv * la_pow(dl2, (float)max(32 * q + r - shift + 1 - enter, 0));
+        const float lw = inv * (other ? p.iscale * la_pow(dl2, (float)max(32 * q + r - shift + 1 - enter, 0)) : full[q]);
 #pragma unroll
         for (int i = 0; i < 16; i++) o[q][i] *= lw;
 #pragma unroll
@@ -368,7 +432,7 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
             sc[k][q][i] *= weight[32 * (q - k) - (8 * (i / 4) + i % 4)];
           }
         float down = 1.0f;
-        if constexpr (La<T>::kPieces == 2) {
+        if constexpr (HALF) {
           float m = 0.0f;
 #pragma unroll
           for (int k = 0; k <= q; k++)
@@ -394,20 +458,14 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
           o[q] = La<T>::mma(zf[s], pf, o[q]);
         }
         const int at = 32 * q + r;
-        const bool ok = at >= shift && col0 < p.db;
-        const long long to = obase + (row + (p.rev ? C - 1 - at : at - shift)) * p.so.s + col0;
-        if constexpr (sizeof(T) == 4) {
-          store_cblock_f32((float*)p.o + to, o[q], 1.0f, g, ok, p.db - col0);
-        } else {
-          if (p.o32) store_cblock_f32((float*)p.o + to, o[q], down, g, ok, p.db - col0);
-          else store_cblock<T>((T*)p.o + to, o[q], down, g, ok, p.db - col0);
-        }
+        const int m = p.rev ? C - 1 - at : at - shift;
+        la_store<O>(ro, at >= shift ? m * bo : kLaOut, o[q], down, g, p.db - col0);
       }
     }
 
     // the state's update
-    const float m1 = expm1f(-d * (float)(n - enter));
-    if constexpr (La<T>::kPieces == 2) {
+    const float m1 = other ? expm1f(-d * (float)(n - enter)) : fade;
+    if constexpr (HALF) {
       float m = 0.0f;
 #pragma unroll
       for (int s = 0; s < 2 * NB; s++)
@@ -418,10 +476,10 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
       F z0[2 * NB], z1[2 * NB];
 #pragma unroll
       for (int s = 0; s < 2 * NB; s++) {
-        const float ws = norm * la_pow(dl2, (float)(C - 16 - 16 * s));
+        const f32x8 wu = la_rows<float, 0>(pu, 0, s, g);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          float v = (float)zf[s][j] * (wu[j] * ws);
+          float v = (float)zf[s][j] * (wu[j] * norm);
           asm("" : "+v"(v));   // (or the product is formed twice, once fused with its rounding, and z1 meets another z0)
           z0[s][j] = (T)v;
           z1[s][j] = (T)(v - (float)z0[s][j]);
@@ -449,34 +507,30 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
         for (int i = 0; i < 16; i++) S[t][i] = fmaf(S[t][i], m1, S[t][i]);
 #pragma unroll
       for (int s = 0; s < 2 * NB; s++) {
-        const float ws = p.uscale * la_pow(dl2, (float)(C - 16 - 16 * s));
-        F z0, z1, z2;
+        const f32x8 wu = la_rows<float, 0>(pu, 0, s, g);
+        F z[PIECES];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-          float v = (float)zf[s][j] * (wu[j] * ws);
-          asm("" : "+v"(v));
-          z0[j] = (T)v;
-          if constexpr (La<T>::kPieces == 3) {
-            const float v1 = v - (float)z0[j];
-            z1[j] = (T)v1;
-            z2[j] = (T)(v1 - (float)z1[j]);
+          float v = (float)zf[s][j] * wu[j];
+#pragma unroll
+          for (int i = 0; i < PIECES; i++) {
+            asm("" : "+v"(v));
+            z[i][j] = (T)v;
+            v -= (float)z[i][j];
           }
         }
 #pragma unroll
         for (int t = 0; t < KT; t++) {
           const F yt = la_cols<T, LDA>(ty, t, s, lane);
-          if constexpr (La<T>::kPieces == 3) {
-            S[t] = La<T>::mma(yt, z2, S[t]);
-            S[t] = La<T>::mma(yt, z1, S[t]);
-          }
-          S[t] = La<T>::mma(yt, z0, S[t]);
+#pragma unroll
+          for (int i = PIECES - 1; i >= 0; i--) S[t] = La<T>::mma(yt, z[i], S[t]);
         }
       }
     }
   }
 
   float* to = nullptr;
-  long long ra = p.sa, rb = p.sb;
+  int ra = p.sa, rb = p.sb;
   float f = 1.0f;
   if constexpr (STATE) {
     to = p.ws + (((long long)b * p.NH + h) * p.nseg + sg + 1) * p.da * p.db;
@@ -487,39 +541,42 @@ __global__ __launch_bounds__(NW * 64, (DA <= 128 ? 2 : 1)) void la_kernel(LaArgs
     if (p.leave && sq.len > 0) f = la_pow(dl2, 1.0f);
   }
   if (to) {
+    const auto rs = buf_rsrc32(to, (unsigned)(p.da * p.db * 4));
 #pragma unroll
     for (int t = 0; t < KT; t++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int a = 32 * t + 8 * (i / 4) + 4 * g + i % 4;
-        if (a < p.da && col0 + r < p.db) to[a * ra + (col0 + r) * rb] = S[t][i] * f;
-      }
+      for (int i = 0; i < 16; i++)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[t][i] * f), rs, state_at(32 * t + 8 * (i / 4) + 4 * g + i % 4, ra, rb), 0, 0);
   }
 }
 
 // one new token or a few of each sequence (linear_step.hip)
 void la_step(const LaArgs& p, int dtype, hipStream_t stream);
 
+// the states that the segments add (`state`), or everything; exact: the states are results, or run into such
 template <typename T>
-int la_launch(const LaArgs& p, bool state, hipStream_t stream);
+void la_launch(const LaArgs& p, bool state, bool exact, hipStream_t stream);
 
-constexpr int kLaChunk = 64;   // the longest chunk of any kernel: segments are multiples of it
+constexpr int kLaChunk = 32;   // rows of a chunk; segments are multiples of it
 
-template <typename T, int DA>
-constexpr int kC = 32;
-
-template <typename T, int DA, int NW, bool STATE>
-inline int la_run(const LaArgs& p, hipStream_t st) {
-  constexpr int C = kC<T, DA>;
+template <typename T, typename O, int DA, int NW, int PIECES, bool STATE>
+inline void la_run(const LaArgs& p, hipStream_t st) {
   const long long items = (long long)p.batch * (STATE ? p.nseg - 1 : p.nseg) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32));
-  hipLaunchKernelGGL((la_kernel<T, DA, NW, C, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, p);
-  return 0;
+  hipLaunchKernelGGL((la_kernel<T, O, DA, NW, kLaChunk, PIECES, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, p);
 }
 
-template <typename T, bool STATE>
-inline int la_pick(const LaArgs& p, hipStream_t st) {
-  if (p.db <= 64) return p.da <= 64 ? la_run<T, 64, 2, STATE>(p, st) : p.da <= 128 ? la_run<T, 128, 2, STATE>(p, st) : la_run<T, 256, 2, STATE>(p, st);
-  return p.da <= 64 ? la_run<T, 64, 4, STATE>(p, st) : p.da <= 128 ? la_run<T, 128, 4, STATE>(p, st) : la_run<T, 256, 4, STATE>(p, st);
+template <typename T, typename O, int PIECES, bool STATE>
+inline void la_pick(const LaArgs& p, hipStream_t st) {
+  if (p.db <= 64) p.da <= 64 ? la_run<T, O, 64, 2, PIECES, STATE>(p, st) : p.da <= 128 ? la_run<T, O, 128, 2, PIECES, STATE>(p, st) : la_run<T, O, 256, 2, PIECES, STATE>(p, st);
+  else p.da <= 64 ? la_run<T, O, 64, 4, PIECES, STATE>(p, st) : p.da <= 128 ? la_run<T, O, 128, 4, PIECES, STATE>(p, st) : la_run<T, O, 256, 4, PIECES, STATE>(p, st);
+}
+
+template <typename T, int PIECES>
+inline void la_all(const LaArgs& p, bool state, hipStream_t st) {
+  if (state) return la_pick<T, T, PIECES, true>(p, st);
+  if constexpr (sizeof(T) == 2)
+    if (p.o32) return la_pick<T, float, PIECES, false>(p, st);
+  la_pick<T, T, PIECES, false>(p, st);
 }
 
 }  // namespace fa

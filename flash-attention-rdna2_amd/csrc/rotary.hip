@@ -37,6 +37,10 @@ __device__ __forceinline__ int rot_row(const FableRotaryParams& p, long long tok
   return (int)min(max(row, 0LL), (long long)p.rotary_rows - 1);
 }
 
+// The pair (a, b) turned, its first and second value: one product rounded, the other in the sum, the same in all kernels.
+__device__ __forceinline__ float rot_first(float a, float b, float c, float s) { return fmaf(a, c, -(b * s)); }
+__device__ __forceinline__ float rot_second(float a, float b, float c, float s) { return fmaf(b, c, a * s); }
+
 template <typename T>
 struct RotVec {
   static constexpr int N = 16 / sizeof(T);
@@ -98,16 +102,16 @@ __global__ __launch_bounds__(256) void rot_kernel(RotArgs a) {
 #pragma unroll
             for (int j = 0; j < N; j++) {
               const float e = (float)x[j], f = (float)y[j];
-              x[j] = (T)(e * c[j] - f * s[j]);
-              y[j] = (T)(f * c[j] + e * s[j]);
+              x[j] = (T)rot_first(e, f, c[j], s[j]);
+              y[j] = (T)rot_second(e, f, c[j], s[j]);
             }
           }
         } else if (turn) {
 #pragma unroll
           for (int j = 0; j < N / 2; j++) {
             const float e = (float)x[2 * j], f = (float)x[2 * j + 1];
-            x[2 * j] = (T)(e * c[j] - f * s[j]);
-            x[2 * j + 1] = (T)(f * c[j] + e * s[j]);
+            x[2 * j] = (T)rot_first(e, f, c[j], s[j]);
+            x[2 * j + 1] = (T)rot_second(e, f, c[j], s[j]);
           }
         }
       }
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(256) void rot_any_kernel(RotArgs a) {
       const float c = p.cos[(long long)row * half + pair];
       float s = p.sin[(long long)row * half + pair];
       if (p.conj) s = -s;
-      v = (T)(second ? (float)v * c + o * s : (float)v * c - o * s);
+      v = (T)(second ? rot_second(o, (float)v, c, s) : rot_first((float)v, o, c, s));
     }
   }
   out[col] = v;

@@ -792,23 +792,23 @@ def _linear_ws(p, dt, backward, dev):
 
 
 def linear_fwd(q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, state_out=None, slots=None):
-    """Linear attention by chunks -> out, dense of q's rows and v's width. state_out: where the states behind the last
-    rows go (as state_in; may be it)."""
+    """Linear attention by chunks -> (out, dense of q's rows and v's width; the states before the segments of long sequences for
+    linear_bwd, or None). state_out: where the states behind the last rows go (as state_in; may be it)."""
     p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in, slots)
     out = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
     p.o, p.so = out.data_ptr(), _rows_strides(out, cu is not None)
     if state_out is not None:
         p.state_out = state_out.data_ptr()
     if p.batch == 0:
-        return out.zero_()
+        return out.zero_(), None
     dt = _dt(q)
     ws, need = _linear_ws(p, dt, 0, q.device)
     with _on(q.device):
         _lib.check(_L.fable_linear_attn_fwd(p, dt, _ptr(ws), need, _stream(q)), "fable_linear_attn_fwd")
-    return out
+    return out, ws
 
 
-def linear_bwd(dout, q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, dstate_out=None, want_dstate=False):
+def linear_bwd(dout, q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, dstate_out=None, want_dstate=False, seg_states=None):
     """-> (dq, dk, dv, dstate_in or None)"""
     p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in)
     _req(dout.dtype == q.dtype and tuple(dout.shape) == (*q.shape[:-1], v.shape[-1]) and _rows_aligned(dout),
@@ -824,6 +824,8 @@ def linear_bwd(dout, q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None
     if dstate_out is not None:
         _check_f32("dstate_out", dstate_out, q.device, p.batch * p.NH * p.DK * p.DV)
         p.dstate_out = dstate_out.data_ptr()
+    if seg_states is not None:
+        p.seg_states = seg_states.data_ptr()
     if p.batch == 0:
         return dq.zero_(), dk.zero_(), dv.zero_(), dstate
     dt = _dt(q)

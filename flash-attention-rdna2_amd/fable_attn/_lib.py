@@ -105,7 +105,7 @@ class FableLinearParams(ctypes.Structure):
     _fields_ = [("q", c_ptr), ("k", c_ptr), ("v", c_ptr), ("o", c_ptr), ("dout", c_ptr), ("dq", c_ptr), ("dk", c_ptr),
                 ("dv", c_ptr), ("sq", Strides), ("sk", Strides), ("sv", Strides), ("so", Strides), ("sdo", Strides),
                 ("sdq", Strides), ("sdk", Strides), ("sdv", Strides), ("decay", c_ptr), ("decay_b", c_i64),
-                ("state_in", c_ptr), ("state_out", c_ptr), ("dstate_out", c_ptr), ("dstate_in", c_ptr), ("cu", c_ptr),
+                ("state_in", c_ptr), ("state_out", c_ptr), ("dstate_out", c_ptr), ("dstate_in", c_ptr), ("seg_states", c_ptr), ("cu", c_ptr),
                 ("slots", c_ptr), ("total", c_i64), ("batch", c_i32), ("n", c_i32), ("NH", c_i32), ("gqa", c_i32),
                 ("DK", c_i32), ("DV", c_i32), ("num_slots", c_i32), ("scale", c_f32)]
 

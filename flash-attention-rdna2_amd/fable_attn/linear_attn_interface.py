@@ -56,21 +56,21 @@ class _LinearAttention(torch.autograd.Function):
         cu, most = pack if pack is not None else (None, 0)
         batch = cu.numel() - 1 if cu is not None else q.shape[0]
         final = torch.empty((batch, q.shape[-2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=q.device) if want else None
-        out = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
+        out, seg = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
         ctx.scale, ctx.most = scale, most
-        ctx.save_for_backward(q, k, v, decay, state, cu)
+        ctx.save_for_backward(q, k, v, decay, state, cu, seg)
         ctx.set_materialize_grads(False)
         return (out, final) if want else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dfinal=None):
-        q, k, v, decay, state, cu = ctx.saved_tensors
+        q, k, v, decay, state, cu, seg = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 8
         dout = q.new_zeros((*q.shape[:-1], v.shape[-1])) if dout is None else _rows(dout)
         dq, dk, dv, dstate = _C.linear_bwd(dout, q, k, v, decay, ctx.scale, cu, ctx.most, state,
-                                           dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7])
+                                           dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7], seg)
         return None, None, None, dq, dk, dv, None, dstate
 
 
@@ -93,7 +93,7 @@ def _attend(pack, q, k, v, decay, scale, state, want):
     else:
         cu, most = pack if pack is not None else (None, 0)
         final = torch.empty((batch, q.shape[-2], wk, wv), dtype=torch.float32, device=q.device) if want else None
-        out = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
+        out, _ = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
     if wv != dv:
         out = out[..., :dv].contiguous()
     if not want:
@@ -139,4 +139,4 @@ def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu
     q, k, v = _rows(q), _rows(k), _rows(v)
     if most <= STEP_ROWS:
         return _C.linear_step(q, k, v, state, decay, scale, cu, most, idx)[0]
-    return _C.linear_fwd(q, k, v, decay, scale, cu, most, state, state, idx)
+    return _C.linear_fwd(q, k, v, decay, scale, cu, most, state, state, idx)[0]

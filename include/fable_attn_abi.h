@@ -478,6 +478,8 @@ typedef struct FableLinearParams {
   float* state_out;
   const float* dstate_out;   /* gradient of state_out (NULL: zeros), and where that of state_in goes (may be NULL) */
   float* dstate_in;
+  const float* seg_states;   /* fable_linear_attn_bwd: the workspace that the forward call of the same tensors, decay and state_in left
+                              * (NULL: its states are formed again) */
   const int32_t* cu;
   const int32_t* slots;
   int64_t total;
