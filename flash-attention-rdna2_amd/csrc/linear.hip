@@ -11,8 +11,8 @@
 
 namespace fa {
 
-// ws[sg + 1] holds what segment sg adds to the state; becomes the state before segment sg + 1, and ws[0] the one before the
-// first. A thread carries one element along; its loads of the next segments do not wait for the sum.
+// ws[sg + 1] holds what segment sg adds to the state; becomes the state before segment sg + 1 (and, where the call overwrites it, ws[0]
+// the one before the first). A thread carries one element along; its loads of the next segments do not wait for the sum.
 __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   const int n = p.da * p.db, nb = (n + 255) / 256;
   const int bh = blockIdx.x / nb, b = bh / p.NH, h = bh % p.NH;
@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   float cur = p.first ? p.first[((long long)sq.slot * p.NH + h) * n + (e / p.db) * p.sa + (e % p.db) * p.sb] : 0.0f;
   const float d = la_decay(p, b, h);
   const float m1 = expm1f(-d * (float)p.seg);
-  ws[0] = cur;
+  if (p.inplace) ws[0] = cur;
   for (int s = 1; s < nseg; s += 4) {
     float v[4];
 #pragma unroll
@@ -110,6 +110,7 @@ LaArgs la_forward(const FableLinearParams& p) {
   a.first = p.state_in, a.last = p.state_out;
   a.sa = p.DV, a.sb = 1;
   a.slots = p.slots, a.nslots = p.num_slots;
+  a.inplace = p.state_in && p.state_in == p.state_out;
   a.iscale = p.scale, a.uscale = 1.0f;
   la_split(a, p);
   return a;

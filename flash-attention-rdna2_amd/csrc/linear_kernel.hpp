@@ -24,6 +24,8 @@
 //   A chunk with fewer than C rows (the last one of a sequence) sits at the end of the tile, behind rows of zeros, so
 // the weights of scores and update are the same for every chunk.
 #pragma once
+#include <type_traits>
+
 #include "attn_device.hpp"
 
 namespace fa {
@@ -50,6 +52,7 @@ struct LaArgs {
   int nseg, seg;             // segments of `seg` rows, a multiple of C; the last one takes all rows left
   float pscale, iscale, uscale;
   int rev;                   // rows from the last to the first
+  int inplace;               // last may be first (segments then find the first state in ws)
   int enter;                 // first is not to decay before the first row (the gradient of the final state)
   int leave;                 // last decays once more behind the last row (the gradient of the initial state)
   int o32;                   // out is fp32 (partial gradients of shared heads)
@@ -111,9 +114,17 @@ __device__ __forceinline__ typename La<T>::F la_cols(const T* tile, int ct, int 
   }
 }
 
+// The largest of a wave's values, in a scalar register: within rows of 16 lanes by DPP, across rows by swaps.
 __device__ __forceinline__ float la_wave_max(float x) {
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) x = fmaxf(x, __shfl_xor(x, i));
+  auto dpp = [](float v, auto ctrl) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0xb1>{}));    // quad_perm 1 0 3 2
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x4e>{}));    // quad_perm 2 3 0 1
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x141>{}));   // row_half_mirror
+  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x140>{}));   // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
   return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 
@@ -198,11 +209,12 @@ __device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, cons
   }
 }
 
-// Waves per SIMD that the registers are to allow: S takes DA / 2 of them.
-constexpr int la_waves(int DA, int NW) { return DA <= 64 || (DA <= 128 && NW == 4) ? 3 : DA <= 128 ? 2 : 1; }
+// Waves per SIMD that the registers are to allow (S takes DA / 2 of them); three at DA 128 were slower (B2 S4096 H32 bf16 forward and
+// backward 387 against 371 us): fewer loads of a chunk's operands are in flight.
+constexpr int la_waves(int DA) { return DA <= 128 ? 2 : 1; }
 
 template <typename T, typename O, int DA, int NW, int C, int PIECES, bool STATE>
-__global__ __launch_bounds__(NW * 64, la_waves(DA, NW)) void la_kernel(LaArgs p) {
+__global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
   using F = typename La<T>::F;
   using H = typename La<T>::H;
   constexpr int NT = NW * 64, DB = NW * 32, NB = C / 32, KT = DA / 32, E = 16 / sizeof(T);
@@ -268,7 +280,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA, NW)) void la_kernel(LaArgs p)
   if (!STATE) {
     const float* from = nullptr;
     int ra = p.sa, rb = p.sb;
-    if (p.nseg == 1) {
+    if (p.nseg == 1 || (sg == 0 && !p.inplace)) {              // (one segment has no ws)
       if (p.first) from = p.first + state;
     } else {
       from = p.ws + (((long long)b * p.NH + h) * p.nseg + sg) * p.da * p.db;
