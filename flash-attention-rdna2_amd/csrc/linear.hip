@@ -65,7 +65,7 @@ int la_elt(int dtype) { return dtype == FA_F32 ? 4 : 2; }
 void la_single(LaArgs& a) {
   if ((a.cu ? a.total : a.n) > 1) return;
   a.sx.s = a.sy.s = a.da;
-  a.sz.s = a.db;
+  a.sz.s = a.so.s = a.db;
 }
 
 // Segments of a call, the same for all its passes: two workgroups for each of the 256 CUs, but none of fewer than 256 rows.
@@ -162,7 +162,11 @@ LaArgs la_dk(const FableLinearParams& p) {
   return a;
 }
 
-void la_go(const LaArgs& a, int dtype, bool state, bool exact, hipStream_t st) {
+void la_go(LaArgs a, int dtype, bool state, bool exact, hipStream_t st) {
+  long long row = (state ? 0 : a.so.s * (a.o32 ? 4 : la_elt(dtype)));
+  for (const fa_strides* s : {&a.sx, &a.sy, &a.sz}) row = s->s * la_elt(dtype) > row ? s->s * la_elt(dtype) : row;
+  const long long span = row > 0 ? (1LL << 29) / row / kLaChunk * kLaChunk : kLaChunk;
+  a.span = (int)(span < kLaChunk ? kLaChunk : span > (1 << 29) ? (1 << 29) : span);
   if (dtype == FA_F16) la_launch<_Float16>(a, state, exact, st);
   else if (dtype == FA_BF16) la_launch<__bf16>(a, state, exact, st);
   else la_launch<float>(a, state, exact, st);
@@ -192,8 +196,8 @@ int la_tensor(const char* what, const char* name, const void* t, const fa_stride
   if (!t) return fail(FA_ERR_ARG, "%s: null %s", what, name);
   if (((uintptr_t)t | (uintptr_t)(s.b * e) | (uintptr_t)(s.h * e) | (uintptr_t)(s.s * e)) & 15)
     return fail(FA_ERR_ARG, "%s: %s: rows must be 16-byte aligned", what, name);
-  // Offsets within a chunk are 32 bits wide, and its rows must not overlap: a row of no token is known by its offset.
-  if (s.s >= (1LL << 30) / (e * kLaChunk) || ((p.cu ? p.total : p.n) > 1 && s.s < width))
+  // Offsets within 32 rows or more are 32 bits wide, and rows must not overlap: one of no token is known by its offset.
+  if (s.s >= (1LL << 29) / (e * kLaChunk) || ((p.cu ? p.total : p.n) > 1 && s.s < width))
     return fail(FA_ERR_ARG, "%s: %s: a row stride of %lld values", what, name, (long long)s.s);
   return FA_OK;
 }
@@ -283,7 +287,7 @@ extern "C" int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, i
   if (rc != FA_OK) return rc;
   if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
   if (p.slots) return fail(FA_ERR_ARG, "%s: states of a pool have no gradient", what);
-  if (p.gqa > 1 && (long long)p.NH * (p.DK > p.DV ? p.DK : p.DV) >= (1LL << 30) / (4 * kLaChunk)) return fail(FA_ERR_ARG, "%s: NH=%d", what, p.NH);
+  if (p.gqa > 1 && (long long)p.NH * (p.DK > p.DV ? p.DK : p.DV) >= (1LL << 29) / (4 * kLaChunk)) return fail(FA_ERR_ARG, "%s: NH=%d", what, p.NH);
   if ((rc = la_tensors(what, p, dtype, true)) != FA_OK) return rc;
   const long long need = la_need(p, true);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))

@@ -21,8 +21,6 @@
 // their own before, and scores too large for it likewise.
 //   lambda^n S is S + (lambda^n - 1) S: the factor itself, rounded to 32 bits, would be off by up to 2^-25 in the same
 // direction in each chunk, which adds up over the many chunks that a slow decay remembers.
-//   A chunk with fewer than C rows (the last one of a sequence) sits at the end of the tile, behind rows of zeros, so
-// the weights of scores and update are the same for every chunk.
 #pragma once
 #include <type_traits>
 
@@ -50,6 +48,7 @@ struct LaArgs {
   long long total;
   int batch, n, NH;
   int nseg, seg;             // segments of `seg` rows, a multiple of C; the last one takes all rows left
+  int span;                  // rows, a multiple of C, over which no tensor spans more than 2^29 bytes
   float pscale, iscale, uscale;
   int rev;                   // rows from the last to the first
   int inplace;               // last may be first (segments then find the first state in ws)
@@ -175,7 +174,7 @@ __device__ __forceinline__ void la_zero_rows(const LaArgs& p, long long base, lo
   for (long long i = tid; i < (hi - lo) * nc; i += nt) ((O*)p.o)[base + (lo + i / nc) * p.so.s + c0 + i % nc] = (O)0.0f;
 }
 
-// An offset past every descriptor of a chunk (those are below 2^30 bytes), also with up to 2^30 added or taken off.
+// An offset past every descriptor (those span 2^29 bytes at most), also with up to 2^30 added or taken off.
 constexpr int kLaOut = (int)0xC0000000u;
 
 // A 32-column block of a row, laid out as store_cblock's, through a buffer descriptor: `at` is the byte offset of the row's block, kLaOut
@@ -307,48 +306,56 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     }
   }
 
-  // Tile loads. A thread's 16-byte column and its rows in LDS are fixed; the row in memory is the row in LDS less `shift`, or counted from the
-  // end. Rows of no token fall outside the buffer descriptor (their offsets are negative, or past its end) and read as zeros;
-  // so do columns past the head dim, from an offset so large that no row brings it back.
+  // Tile loads. A thread's 16-byte column and its rows of the tile are fixed. Buffer descriptors span `span` rows of the segment, so that offsets
+  // within them are 32 bits wide and move by the same step from chunk to chunk. Rows behind the segment's last one fall outside
+  // (past the descriptor's end, or in reverse below its start: negative) and read as zeros or are not stored; columns past the head dim
+  // start from an offset so large that no row brings it back.
   const int xr = tid / CA, xc = tid % CA, zr = tid / CB, zc = tid % CB;
-  const int bx = (int)p.sx.s * (int)sizeof(T), by = (int)p.sy.s * (int)sizeof(T), bz = (int)p.sz.s * (int)sizeof(T);
-  const bool xin = xc * E < p.da, zin = dbt * DB + zc * E < p.db;
-  const char* const gx = (const char*)p.x + ((p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h) * (long long)sizeof(T);
-  const char* const gy = (const char*)p.y + ((p.cu ? 0 : b * p.sy.b) + (h / p.hy) * p.sy.h) * (long long)sizeof(T);
-  const char* const gz = (const char*)p.z + ((p.cu ? 0 : b * p.sz.b) + (h / p.hz) * p.sz.h + dbt * DB) * (long long)sizeof(T);
-  const int wx = p.da * (int)sizeof(T), wz = (p.db - dbt * DB) * (int)sizeof(T);
-  u32x4 vx[STATE ? 1 : LA], vy[LA], vz[LB];
-
-  // lambda^(i + 1) of the lane's rows and lambda^C - 1: of all chunks but a short one and, with `enter`, the first
-  float full[STATE ? 1 : NB];
-  if constexpr (!STATE)
-#pragma unroll
-    for (int q = 0; q < NB; q++) full[q] = p.iscale * la_pow(dl2, (float)(32 * q + r + 1));
-  const float fade = expm1f(-d * (float)C);
-
-  auto rows_of = [&](int c, long long& row) {                 // rows of chunk c, and its first one in memory
-    const int q0 = p0 + c * C, n = min(C, p1 - q0);
-    row = sq.row0 + (p.rev ? sq.len - q0 - n : q0);
-    return n;
+  const int bx = (int)p.sx.s * (int)sizeof(T), by = (int)p.sy.s * (int)sizeof(T), bz = (int)p.sz.s * (int)sizeof(T), bo = (int)p.so.s * (int)sizeof(O);
+  const char* const gx = (const char*)p.x + ((p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h + sq.row0 * p.sx.s) * (long long)sizeof(T);
+  const char* const gy = (const char*)p.y + ((p.cu ? 0 : b * p.sy.b) + (h / p.hy) * p.sy.h + sq.row0 * p.sy.s) * (long long)sizeof(T);
+  const char* const gz = (const char*)p.z + ((p.cu ? 0 : b * p.sz.b) + (h / p.hz) * p.sz.h + sq.row0 * p.sz.s + dbt * DB) * (long long)sizeof(T);
+  const char* const go = (const char*)p.o + (obase + sq.row0 * p.so.s + col0) * (long long)sizeof(O);
+  // the lowest row of the span that starts at row q0 in processing order, and its number of rows
+  auto span = [&](int q0, int& rows) -> long long {
+    rows = max(0, min(p.span, p1 - q0));
+    return p.rev ? sq.len - q0 - rows : q0;
   };
-  const int sign = p.rev ? -1 : 1, mx = p.rev ? C - 1 - xr : xr, mz = p.rev ? C - 1 - zr : zr;
-  const int ox0 = xin ? mx * bx + xc * 16 : kLaOut, oy0 = xin ? mx * by + xc * 16 : kLaOut, oz0 = zin ? mz * bz + zc * 16 : kLaOut;
-  const int ix = sign * (NT / CA) * bx, iy = sign * (NT / CA) * by, iz = sign * (NT / CB) * bz;
-  auto fetch = [&](int c) {
-    long long row;
-    const int n = rows_of(c, row), shift = p.rev ? 0 : C - n;
-    // (behind the last chunk nothing is read)
-    const auto rx = buf_rsrc32(gx + row * bx, n > 0 ? (unsigned)((n - 1) * bx + wx) : 0u);
-    const auto ry = buf_rsrc32(gy + row * by, n > 0 ? (unsigned)((n - 1) * by + wx) : 0u);
-    const auto rz = buf_rsrc32(gz + row * bz, n > 0 ? (unsigned)((n - 1) * bz + wz) : 0u);
-    const int ox = ox0 - shift * bx, oy = oy0 - shift * by, oz = oz0 - shift * bz;
+  auto within = [&](const char* base, long long row, int rows, int stride, int width) {
+    return buf_rsrc32(base + row * stride, rows > 0 ? (unsigned)((rows - 1) * stride + width) : 0u);
+  };
+  // the offset of row i of a span
+  auto place = [&](int i, int rows, int stride) { return (p.rev ? rows - 1 - i : i) * stride; };
+  const int sign = p.rev ? -1 : 1, per = p.span / C;                     // chunks of a span
+  const int jx = xc * E < p.da ? xc * 16 : kLaOut, jz = dbt * DB + zc * E < p.db ? zc * 16 : kLaOut;
+  __amdgpu_buffer_rsrc_t rx, ry, rz, ro;
+  int vox = 0, voy = 0, voz = 0, voo[STATE ? 1 : NB];
+  u32x4 vx[STATE ? 1 : LA], vy[LA], vz[LB];
+  int next = p0, left = 0, oleft = 0;                                    // the row to fetch, chunks left of the spans
+  auto fetch = [&]() {
+    if (left == 0) {
+      left = per;
+      int rows;
+      const long long row = span(next, rows);
+      if constexpr (!STATE) rx = within(gx, row, rows, bx, p.da * (int)sizeof(T));
+      ry = within(gy, row, rows, by, p.da * (int)sizeof(T));
+      rz = within(gz, row, rows, bz, (p.db - dbt * DB) * (int)sizeof(T));
+      vox = jx + place(xr, rows, bx);
+      voy = jx + place(xr, rows, by);
+      voz = jz + place(zr, rows, bz);
+    }
+    left--;
+    next += C;
 #pragma unroll
     for (int i = 0; i < LA; i++) {
-      if constexpr (!STATE) vx[i] = buf_load16(rx, ox + i * ix);
-      vy[i] = buf_load16(ry, oy + i * iy);
+      if constexpr (!STATE) vx[i] = buf_load16(rx, vox + i * (sign * (NT / CA) * bx));
+      vy[i] = buf_load16(ry, voy + i * (sign * (NT / CA) * by));
     }
 #pragma unroll
-    for (int i = 0; i < LB; i++) vz[i] = buf_load16(rz, oz + i * iz);
+    for (int i = 0; i < LB; i++) vz[i] = buf_load16(rz, voz + i * (sign * (NT / CB) * bz));
+    vox += sign * C * bx;
+    voy += sign * C * by;
+    voz += sign * C * bz;
   };
   T* const px = tx + xr * LDA + xc * E;
   T* const py = ty + xr * LDA + xc * E;
@@ -362,20 +369,26 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     }
   };
 
-  fetch(0);
+  // lambda^(i + 1) of the lane's rows and lambda^C - 1: of all chunks but, with `enter`, the first and a short one
+  float full[STATE ? 1 : NB];
+  if constexpr (!STATE)
+#pragma unroll
+    for (int q = 0; q < NB; q++) full[q] = p.iscale * la_pow(dl2, (float)(32 * q + r + 1));
+  const float fade = expm1f(-d * (float)C);
+
+  fetch();
   if constexpr (!STATE) {
     // Stores to nowhere, as many as a chunk has behind the next one's loads: a wait for loads counts what was issued since, and the
     // compiler takes the lowest count of all ways into the loop.
     f32x16 none;
 #pragma unroll
     for (int i = 0; i < 16; i++) none[i] = 0.0f;
-    const auto ro = buf_rsrc32(p.o, 0u);
+    ro = buf_rsrc32(p.o, 0u);
 #pragma unroll
     for (int q = 0; q < NB; q++) la_store<O>(ro, kLaOut, none, 1.0f, g, 32);
   }
   for (int c = 0; c < nch; c++) {
-    long long row;
-    const int n = rows_of(c, row), shift = C - n;
+    const int n = min(C, p1 - p0 - c * C);                    // rows of the chunk; zeros behind them
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < LA; i++) {
@@ -384,19 +397,27 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     }
 #pragma unroll
     for (int i = 0; i < LB; i++) *(u32x4*)(pz + i * (NT / CB) * LDZ) = vz[i];
-    fetch(c + 1);
+    if (n < C && tid < C) pu[tid] = (HALF ? 1.0f : p.uscale) * la_pow(dl2, (float)max(n - 1 - tid, 0));
+    fetch();
     __syncthreads();
 
     // the state enters the first row as it is where it is the final state's gradient
     const int enter = p.enter && sg == 0 && c == 0;
-    const bool other = shift || enter;
+    const bool other = n < C || enter;
     F zf[2 * NB];
 #pragma unroll
     for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
 
     if constexpr (!STATE) {
-      const int bo = (int)p.so.s * (int)sizeof(O);
-      const auto ro = buf_rsrc32((const O*)p.o + obase + row * p.so.s + col0, (unsigned)((n - 1) * bo + 32 * (int)sizeof(O)));
+      if (oleft == 0) {
+        oleft = per;
+        int rows;
+        const long long row = span(p0 + c * C, rows);
+        ro = within(go, row, rows, bo, min(32, max(p.db - col0, 0)) * (int)sizeof(O));
+#pragma unroll
+        for (int q = 0; q < NB; q++) voo[q] = place(32 * q + r, rows, bo);
+      }
+      oleft--;
       f32x16 sc[NB][NB], o[NB];                                // [key block][query block]
 #pragma unroll
       for (int q = 0; q < NB; q++) {
@@ -434,7 +455,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
       }
 #pragma unroll
       for (int q = 0; q < NB; q++) {
-        const float lw = inv * (other ? p.iscale * la_pow(dl2, (float)max(32 * q + r - shift + 1 - enter, 0)) : full[q]);
+        const float lw = inv * (enter ? p.iscale * la_pow(dl2, (float)(32 * q + r)) : full[q]);
 #pragma unroll
         for (int i = 0; i < 16; i++) o[q][i] *= lw;
 #pragma unroll
@@ -469,9 +490,8 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
           for (int j = 0; j < 8; j++) pf[j] = (T)sc[s / 2][q][8 * (s % 2) + j];
           o[q] = La<T>::mma(zf[s], pf, o[q]);
         }
-        const int at = 32 * q + r;
-        const int m = p.rev ? C - 1 - at : at - shift;
-        la_store<O>(ro, at >= shift ? m * bo : kLaOut, o[q], down, g, p.db - col0);
+        la_store<O>(ro, voo[q], o[q], down, g, p.db - col0);
+        voo[q] += sign * C * bo;
       }
     }
 
