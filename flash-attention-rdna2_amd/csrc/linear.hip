@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   float* const ws = p.ws + (long long)bh * p.nseg * n + e;
   float cur = p.first ? p.first[((long long)sq.slot * p.NH + h) * n + (e / p.db) * p.sa + (e % p.db) * p.sb] : 0.0f;
   const float d = la_decay(p, b, h);
-  const float m1 = expm1f(-d * (float)p.seg);
+  const LaFade whole(d, (float)p.seg), first(d, (float)(p.seg - 1));
   if (p.inplace) ws[0] = cur;
   for (int s = 1; s < nseg; s += 4) {
     float v[4];
@@ -31,8 +31,7 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
     for (int j = 0; j < 4; j++) v[j] = s + j < nseg ? ws[(long long)(s + j) * n] : 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float f = p.enter && s + j == 1 ? expm1f(-d * (float)(p.seg - 1)) : m1;
-      cur = fmaf(cur, f, cur) + v[j];
+      cur = (p.enter && s + j == 1 ? first(cur) : whole(cur)) + v[j];
       if (s + j < nseg) ws[(long long)(s + j) * n] = cur;
     }
   }

@@ -19,8 +19,10 @@
 // T that hold its 24 bits (bf16: 3, fp16: 2, fp32: itself), because S is a result in 32 bits and runs on over
 // the whole sequence. In fp16, whose range is small, S and the weighted z are brought to a power of two of
 // their own before, and scores too large for it likewise.
-//   lambda^n S is S + (lambda^n - 1) S: the factor itself, rounded to 32 bits, would be off by up to 2^-25 in the same
-// direction in each chunk, which adds up over the many chunks that a slow decay remembers.
+//   The decay of S is put off: the accumulators hold S lambda^-lag, `lag` the rows since they were last brought up to date, and what a chunk adds is
+// weighted up by as much, until lambda^lag leaves 2^+-kLaLag. Each rounding of such a factor then touches what is about to be forgotten only, where one for each
+// chunk would add up over all that a slow decay remembers; and for all but fast decays that spares most of the DA / 2 multiplications
+// per lane and chunk (the kernel's time is its vector and matrix instructions together as much as its bytes).
 #pragma once
 #include <type_traits>
 
@@ -135,6 +137,49 @@ __device__ __forceinline__ float la_norm(float m, float& inv) {
   return __uint_as_float((uint32_t)(127 + k) << 23);
 }
 
+constexpr float kLaLag = 8.0f;
+
+// Two values split into parts of T, each the rounding of what the ones before left.
+template <typename T, int PIECES, typename F>
+__device__ __forceinline__ void la_split2(float a, float b, F* parts, int j) {
+  if constexpr (sizeof(T) == 4) {
+    parts[0][j] = a;
+    parts[0][j + 1] = b;
+  } else {
+    using V2 = typename Dt<T>::V2;
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+      // (The empty asm keeps the compiler from forming a product twice, once fused with its rounding, and from converting a value
+      // once for the operand and once for the difference.)
+      asm("" : "+v"(a), "+v"(b));
+      uint32_t u = bitcast<uint32_t>(V2{(T)a, (T)b});
+      asm("" : "+v"(u));
+      const V2 h = bitcast<V2>(u);
+      parts[i][j] = h[0];
+      parts[i][j + 1] = h[1];
+      if (i + 1 < PIECES) {
+        a -= (float)h[0];
+        b -= (float)h[1];
+      }
+    }
+  }
+}
+
+// A state carried over `rows` rows, S <- keep S + by S: keep 1 and by = lambda^rows - 1 where that is near 1 (the factor itself, rounded
+// to 32 bits, is off by up to 2^-25 in the same direction each time), else 0 and the factor.
+struct LaFade {
+  float by, keep;
+  __device__ __forceinline__ LaFade(float d, float rows) {
+    by = expm1f(-d * rows);
+    keep = 1.0f;
+    if (by < -0.5f) {
+      by = expf(-d * rows);
+      keep = 0.0f;
+    }
+  }
+  __device__ __forceinline__ float operator()(float s) const { return fmaf(s, by, keep * s); }
+};
+
 // lambda^k as 2^(-k d log2 e)
 __device__ __forceinline__ float la_pow(float dl2, float k) { return exp2f(-dl2 * k); }
 
@@ -143,6 +188,14 @@ __device__ __forceinline__ float la_decay(const LaArgs& p, int b, int h) {
   const float d = p.decay[b * p.decay_b + h];
   return d > 1e25f ? 1e25f : d < -1e25f ? -1e25f : d;
 }
+
+// A value that all lanes have, in scalar registers.
+__device__ __forceinline__ const char* la_uniform(const char* at) {
+  const unsigned long long u = (unsigned long long)at;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+  return (const char*)(((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ unsigned la_uniform(unsigned n) { return __builtin_amdgcn_readfirstlane(n); }
 
 struct LaSeq {
   long long row0;            // first row in the tensors
@@ -321,14 +374,14 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     rows = max(0, min(p.span, p1 - q0));
     return p.rev ? sq.len - q0 - rows : q0;
   };
-  auto within = [&](const char* base, long long row, int rows, int stride, int width) {
-    return buf_rsrc32(base + row * stride, rows > 0 ? (unsigned)((rows - 1) * stride + width) : 0u);
-  };
+  auto bytes = [&](int rows, int stride, int width) { return rows > 0 ? (unsigned)((rows - 1) * stride + width) : 0u; };
   // the offset of row i of a span
   auto place = [&](int i, int rows, int stride) { return (p.rev ? rows - 1 - i : i) * stride; };
   const int sign = p.rev ? -1 : 1, per = p.span / C;                     // chunks of a span
   const int jx = xc * E < p.da ? xc * 16 : kLaOut, jz = dbt * DB + zc * E < p.db ? zc * 16 : kLaOut;
-  __amdgpu_buffer_rsrc_t rx, ry, rz, ro;
+  // (start and size, not descriptors: those went through vector registers and a loop around each store)
+  const char *fx = nullptr, *fy = nullptr, *fz = nullptr, *fo = nullptr;
+  unsigned nx = 0, ny = 0, nz = 0, no = 0;
   int vox = 0, voy = 0, voz = 0, voo[STATE ? 1 : NB];
   u32x4 vx[STATE ? 1 : LA], vy[LA], vz[LB];
   int next = p0, left = 0, oleft = 0;                                    // the row to fetch, chunks left of the spans
@@ -337,15 +390,16 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
       left = per;
       int rows;
       const long long row = span(next, rows);
-      if constexpr (!STATE) rx = within(gx, row, rows, bx, p.da * (int)sizeof(T));
-      ry = within(gy, row, rows, by, p.da * (int)sizeof(T));
-      rz = within(gz, row, rows, bz, (p.db - dbt * DB) * (int)sizeof(T));
+      fx = la_uniform(gx + row * bx), nx = la_uniform(bytes(rows, bx, p.da * (int)sizeof(T)));
+      fy = la_uniform(gy + row * by), ny = la_uniform(bytes(rows, by, p.da * (int)sizeof(T)));
+      fz = la_uniform(gz + row * bz), nz = la_uniform(bytes(rows, bz, (p.db - dbt * DB) * (int)sizeof(T)));
       vox = jx + place(xr, rows, bx);
       voy = jx + place(xr, rows, by);
       voz = jz + place(zr, rows, bz);
     }
     left--;
     next += C;
+    const auto rx = buf_rsrc32(fx, nx), ry = buf_rsrc32(fy, ny), rz = buf_rsrc32(fz, nz);
 #pragma unroll
     for (int i = 0; i < LA; i++) {
       if constexpr (!STATE) vx[i] = buf_load16(rx, vox + i * (sign * (NT / CA) * bx));
@@ -369,12 +423,8 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     }
   };
 
-  // lambda^(i + 1) of the lane's rows and lambda^C - 1: of all chunks but, with `enter`, the first and a short one
-  float full[STATE ? 1 : NB];
-  if constexpr (!STATE)
-#pragma unroll
-    for (int q = 0; q < NB; q++) full[q] = p.iscale * la_pow(dl2, (float)(32 * q + r + 1));
-  const float fade = expm1f(-d * (float)C);
+  // the state's gradient enters the first row as it is, any other state decayed once
+  int lag = p.enter && sg == 0 ? -1 : 0;
 
   fetch();
   if constexpr (!STATE) {
@@ -383,7 +433,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     f32x16 none;
 #pragma unroll
     for (int i = 0; i < 16; i++) none[i] = 0.0f;
-    ro = buf_rsrc32(p.o, 0u);
+    const auto ro = buf_rsrc32(p.o, 0u);
 #pragma unroll
     for (int q = 0; q < NB; q++) la_store<O>(ro, kLaOut, none, 1.0f, g, 32);
   }
@@ -401,9 +451,6 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     fetch();
     __syncthreads();
 
-    // the state enters the first row as it is where it is the final state's gradient
-    const int enter = p.enter && sg == 0 && c == 0;
-    const bool other = n < C || enter;
     F zf[2 * NB];
 #pragma unroll
     for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
@@ -413,11 +460,12 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
         oleft = per;
         int rows;
         const long long row = span(p0 + c * C, rows);
-        ro = within(go, row, rows, bo, min(32, max(p.db - col0, 0)) * (int)sizeof(O));
+        fo = la_uniform(go + row * bo), no = la_uniform(bytes(rows, bo, min(32, max(p.db - col0, 0)) * (int)sizeof(O)));
 #pragma unroll
         for (int q = 0; q < NB; q++) voo[q] = place(32 * q + r, rows, bo);
       }
       oleft--;
+      const auto ro = buf_rsrc32(fo, no);
       f32x16 sc[NB][NB], o[NB];                                // [key block][query block]
 #pragma unroll
       for (int q = 0; q < NB; q++) {
@@ -455,7 +503,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
       }
 #pragma unroll
       for (int q = 0; q < NB; q++) {
-        const float lw = inv * (enter ? p.iscale * la_pow(dl2, (float)(32 * q + r)) : full[q]);
+        const float lw = p.iscale * inv * exp2_fast(-dl2 * (float)(32 * q + r + 1 + lag));
 #pragma unroll
         for (int i = 0; i < 16; i++) o[q][i] *= lw;
 #pragma unroll
@@ -496,7 +544,18 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     }
 
     // the state's update
-    const float m1 = other ? expm1f(-d * (float)(n - enter)) : fade;
+    lag += n;
+    float late = 1.0f;
+    if (fabsf(dl2 * (float)lag) > kLaLag) {
+      const float f = exp2_fast(-dl2 * (float)lag);
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[t][i] *= f;
+      lag = 0;
+    } else {
+      late = exp2_fast(dl2 * (float)lag);
+    }
     if constexpr (HALF) {
       float m = 0.0f;
 #pragma unroll
@@ -505,19 +564,15 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
         for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf((float)zf[s][j]));
       float inv;
       const float norm = la_norm(la_wave_max(m), inv);
-      F z0[2 * NB], z1[2 * NB];
+      F z[2 * NB][PIECES];
 #pragma unroll
       for (int s = 0; s < 2 * NB; s++) {
         const f32x8 wu = la_rows<float, 0>(pu, 0, s, g);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          float v = (float)zf[s][j] * (wu[j] * norm);
-          asm("" : "+v"(v));   // (or the product is formed twice, once fused with its rounding, and z1 meets another z0)
-          z0[s][j] = (T)v;
-          z1[s][j] = (T)(v - (float)z0[s][j]);
-        }
+        for (int j = 0; j < 8; j += 2)
+          la_split2<T, PIECES>((float)zf[s][j] * (wu[j] * norm), (float)zf[s][j + 1] * (wu[j + 1] * norm), z[s], j);
       }
-      inv *= p.uscale;
+      inv *= p.uscale * late;
 #pragma unroll
       for (int t = 0; t < KT; t++) {
         f32x16 u;
@@ -526,31 +581,20 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
 #pragma unroll
         for (int s = 0; s < 2 * NB; s++) {
           const F yt = la_cols<T, LDA>(ty, t, s, lane);
-          u = La<T>::mma(yt, z1[s], u);
-          u = La<T>::mma(yt, z0[s], u);
+#pragma unroll
+          for (int i = PIECES - 1; i >= 0; i--) u = La<T>::mma(yt, z[s][i], u);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++) S[t][i] = fmaf(u[i], inv, fmaf(S[t][i], m1, S[t][i]));
+        for (int i = 0; i < 16; i++) S[t][i] = fmaf(u[i], inv, S[t][i]);
       }
     } else {
-#pragma unroll
-      for (int t = 0; t < KT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) S[t][i] = fmaf(S[t][i], m1, S[t][i]);
 #pragma unroll
       for (int s = 0; s < 2 * NB; s++) {
         const f32x8 wu = la_rows<float, 0>(pu, 0, s, g);
         F z[PIECES];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          float v = (float)zf[s][j] * wu[j];
-#pragma unroll
-          for (int i = 0; i < PIECES; i++) {
-            asm("" : "+v"(v));
-            z[i][j] = (T)v;
-            v -= (float)z[i][j];
-          }
-        }
+        for (int j = 0; j < 8; j += 2)
+          la_split2<T, PIECES>((float)zf[s][j] * (wu[j] * late), (float)zf[s][j + 1] * (wu[j + 1] * late), z, j);
 #pragma unroll
         for (int t = 0; t < KT; t++) {
           const F yt = la_cols<T, LDA>(ty, t, s, lane);
@@ -573,6 +617,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     if (p.leave && sq.len > 0) f = la_pow(dl2, 1.0f);
   }
   if (to) {
+    if (nch > 0) f *= exp2_fast(-dl2 * (float)lag);
     const auto rs = buf_rsrc32(to, (unsigned)(p.da * p.db * 4));
 #pragma unroll
     for (int t = 0; t < KT; t++)

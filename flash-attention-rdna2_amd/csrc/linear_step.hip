@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaArgs p) {
     const int a = rg * R + i;
     S[i] = cin && a < p.da ? *(const f32x4*)(p.first + state + (long long)a * p.db) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  const float m1 = expm1f(-la_decay(p, b, h));
+  const LaFade fade(la_decay(p, b, h), 1.0f);
   const T* const gq = (const T*)p.x + (p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h + sq.row0 * p.sx.s;
   const T* const gk = (const T*)p.y + (p.cu ? 0 : b * p.sy.b) + (h / p.hy) * p.sy.h + sq.row0 * p.sy.s;
   const T* const gv = (const T*)p.z + (p.cu ? 0 : b * p.sz.b) + (h / p.hz) * p.sz.h + sq.row0 * p.sz.s + c0;
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaArgs p) {
         const float k = ks[t][rg * R + i], q = qs[t][rg * R + i];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          S[i][j] = fmaf(k, v[j], fmaf(S[i][j], m1, S[i][j]));
+          S[i][j] = fmaf(k, v[j], fade(S[i][j]));
           acc[j] = fmaf(q, S[i][j], acc[j]);
         }
       }
