@@ -224,7 +224,8 @@ __device__ __forceinline__ int la_segments(const LaArgs& p, int len) {
 // Zeros in rows [lo, hi) of out for the item's columns.
 template <typename O>
 __device__ __forceinline__ void la_zero_rows(const LaArgs& p, long long base, long long lo, long long hi, int c0, int nc, int tid, int nt) {
-  for (long long i = tid; i < (hi - lo) * nc; i += nt) ((O*)p.o)[base + (lo + i / nc) * p.so.s + c0 + i % nc] = (O)0.0f;
+  for (long long row = lo; row < hi; row++)
+    for (int c = tid; c < nc; c += nt) ((O*)p.o)[base + row * p.so.s + c0 + c] = (O)0.0f;
 }
 
 // An offset past every descriptor (those span 2^29 bytes at most), also with up to 2^30 added or taken off.
@@ -451,22 +452,38 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     fetch();
     __syncthreads();
 
-    F zf[2 * NB];
+    // What follows alternates matrix and vector instructions that do not wait for one another: the scores and the product with S beside the
+    // splitting of z, the state's update beside the weighting of the scores.
+    F zf[2 * NB], z[2 * NB][PIECES];
+    f32x8 wu[2 * NB];
 #pragma unroll
-    for (int s = 0; s < 2 * NB; s++) zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
+    for (int s = 0; s < 2 * NB; s++) {
+      zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
+      wu[s] = la_rows<float, 0>(pu, 0, s, g);
+    }
+    // the decay that S is behind by, and whether it is made up for now
+    const int behind = lag + n;
+    const bool due = fabsf(dl2 * (float)behind) > kLaLag;
+    float weigh = due ? 1.0f : exp2_fast(dl2 * (float)behind), undo = 1.0f;
+    if constexpr (HALF) {
+      float m = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2 * NB; s++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf((float)zf[s][j]));
+      undo = p.uscale * weigh;
+      float inv;
+      weigh = la_norm(la_wave_max(m), inv);
+      undo *= inv;
+    }
+    auto split = [&](int k) {                                  // the k-th of 8 NB pairs of weighted z
+      const int s = k / 4, j = 2 * (k % 4);
+      la_split2<T, PIECES>((float)zf[s][j] * (wu[s][j] * weigh), (float)zf[s][j + 1] * (wu[s][j + 1] * weigh), z[s], j);
+    };
 
+    f32x16 sc[NB][NB], o[NB];                                  // [key block][query block], transposed
+    float norm = 1.0f, inv = 1.0f;
     if constexpr (!STATE) {
-      if (oleft == 0) {
-        oleft = per;
-        int rows;
-        const long long row = span(p0 + c * C, rows);
-        fo = la_uniform(go + row * bo), no = la_uniform(bytes(rows, bo, min(32, max(p.db - col0, 0)) * (int)sizeof(O)));
-#pragma unroll
-        for (int q = 0; q < NB; q++) voo[q] = place(32 * q + r, rows, bo);
-      }
-      oleft--;
-      const auto ro = buf_rsrc32(fo, no);
-      f32x16 sc[NB][NB], o[NB];                                // [key block][query block]
 #pragma unroll
       for (int q = 0; q < NB; q++) {
 #pragma unroll
@@ -476,7 +493,6 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
 #pragma unroll
           for (int i = 0; i < 16; i++) sc[k][q][i] = 0.0f;
       }
-      float norm = 1.0f, inv = 1.0f;
       if constexpr (HALF) {
         float m = 0.0f;
 #pragma unroll
@@ -500,18 +516,90 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
           for (int k = 0; k <= q; k++) sc[k][q] = La<T>::mma(yf[k], xf[q], sc[k][q]);
           o[q] = La<T>::mma(sf, xf[q], o[q]);
         }
+#pragma unroll
+        for (int k = s * 8 * NB / (DA / 16); k < (s + 1) * 8 * NB / (DA / 16); k++) split(k);
       }
+    }
+
+    // the state's update
+    if (due) {
+      const float f = exp2_fast(-dl2 * (float)behind);
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[t][i] *= f;
+    }
+    if constexpr (STATE)
+#pragma unroll
+      for (int k = 0; k < 4; k++) split(k);
+    // the lane's rows of the scores and of the product with S, a quarter for each quarter of the tiles
+    float lw[NB];
+    if constexpr (!STATE)
+#pragma unroll
+      for (int q = 0; q < NB; q++) lw[q] = p.iscale * inv * exp2_fast(-dl2 * (float)(32 * q + r + 1 + lag));
+    auto weighted = [&](int part, int parts) {
+#pragma unroll
+      for (int q = 0; q < NB; q++)
+#pragma unroll
+        for (int i = 16 * part / parts; i < 16 * (part + 1) / parts; i++) {
+          o[q][i] *= lw[q];
+#pragma unroll
+          for (int k = 0; k <= q; k++) sc[k][q][i] *= weight[32 * (q - k) - (8 * (i / 4) + i % 4)];
+        }
+    };
+    if constexpr (HALF) {
+#pragma unroll
+      for (int t = 0; t < KT; t++) {
+        f32x16 u;
+#pragma unroll
+        for (int i = 0; i < 16; i++) u[i] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; s++) {
+          const F yt = la_cols<T, LDA>(ty, t, s, lane);
+#pragma unroll
+          for (int i = PIECES - 1; i >= 0; i--) u = La<T>::mma(yt, z[s][i], u);
+          if constexpr (STATE)
+            if (t == 0 && s + 1 < 2 * NB)
+#pragma unroll
+              for (int k = 0; k < 4; k++) split(4 * (s + 1) + k);
+        }
+        if constexpr (!STATE) weighted(t, KT);
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[t][i] = fmaf(u[i], undo, S[t][i]);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2 * NB; s++) {
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+          const F yt = la_cols<T, LDA>(ty, t, s, lane);
+#pragma unroll
+          for (int i = PIECES - 1; i >= 0; i--) S[t] = La<T>::mma(yt, z[s][i], S[t]);
+          if constexpr (STATE) {
+            if (s + 1 < 2 * NB)
+#pragma unroll
+              for (int k = 4 * t / KT; k < 4 * (t + 1) / KT; k++) split(4 * (s + 1) + k);
+          } else {
+            weighted(s * KT + t, 2 * NB * KT);
+          }
+        }
+      }
+    }
+    lag = due ? 0 : behind;
+
+    if constexpr (!STATE) {
+      if (oleft == 0) {
+        oleft = per;
+        int rows;
+        const long long row = span(p0 + c * C, rows);
+        fo = la_uniform(go + row * bo), no = la_uniform(bytes(rows, bo, min(32, max(p.db - col0, 0)) * (int)sizeof(O)));
+#pragma unroll
+        for (int q = 0; q < NB; q++) voo[q] = place(32 * q + r, rows, bo);
+      }
+      oleft--;
+      const auto ro = buf_rsrc32(fo, no);
 #pragma unroll
       for (int q = 0; q < NB; q++) {
-        const float lw = p.iscale * inv * exp2_fast(-dl2 * (float)(32 * q + r + 1 + lag));
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[q][i] *= lw;
-#pragma unroll
-        for (int k = 0; k <= q; k++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            sc[k][q][i] *= weight[32 * (q - k) - (8 * (i / 4) + i % 4)];
-          }
         float down = 1.0f;
         if constexpr (HALF) {
           float m = 0.0f;
@@ -540,67 +628,6 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
         }
         la_store<O>(ro, voo[q], o[q], down, g, p.db - col0);
         voo[q] += sign * C * bo;
-      }
-    }
-
-    // the state's update
-    lag += n;
-    float late = 1.0f;
-    if (fabsf(dl2 * (float)lag) > kLaLag) {
-      const float f = exp2_fast(-dl2 * (float)lag);
-#pragma unroll
-      for (int t = 0; t < KT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) S[t][i] *= f;
-      lag = 0;
-    } else {
-      late = exp2_fast(dl2 * (float)lag);
-    }
-    if constexpr (HALF) {
-      float m = 0.0f;
-#pragma unroll
-      for (int s = 0; s < 2 * NB; s++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf((float)zf[s][j]));
-      float inv;
-      const float norm = la_norm(la_wave_max(m), inv);
-      F z[2 * NB][PIECES];
-#pragma unroll
-      for (int s = 0; s < 2 * NB; s++) {
-        const f32x8 wu = la_rows<float, 0>(pu, 0, s, g);
-#pragma unroll
-        for (int j = 0; j < 8; j += 2)
-          la_split2<T, PIECES>((float)zf[s][j] * (wu[j] * norm), (float)zf[s][j + 1] * (wu[j + 1] * norm), z[s], j);
-      }
-      inv *= p.uscale * late;
-#pragma unroll
-      for (int t = 0; t < KT; t++) {
-        f32x16 u;
-#pragma unroll
-        for (int i = 0; i < 16; i++) u[i] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 2 * NB; s++) {
-          const F yt = la_cols<T, LDA>(ty, t, s, lane);
-#pragma unroll
-          for (int i = PIECES - 1; i >= 0; i--) u = La<T>::mma(yt, z[s][i], u);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i++) S[t][i] = fmaf(u[i], inv, S[t][i]);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 2 * NB; s++) {
-        const f32x8 wu = la_rows<float, 0>(pu, 0, s, g);
-        F z[PIECES];
-#pragma unroll
-        for (int j = 0; j < 8; j += 2)
-          la_split2<T, PIECES>((float)zf[s][j] * (wu[j] * late), (float)zf[s][j + 1] * (wu[j + 1] * late), z, j);
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
-          const F yt = la_cols<T, LDA>(ty, t, s, lane);
-#pragma unroll
-          for (int i = PIECES - 1; i >= 0; i--) S[t] = La<T>::mma(yt, z[i], S[t]);
-        }
       }
     }
   }

@@ -3,6 +3,8 @@
 // The rotation reads and writes every value once: bound by HBM, by latency for a few tokens. A wave takes one token; its lanes
 // are (head, unit of columns) and walk over the token's heads, so a lane loads its cosines and sines once for all of them. A unit is
 // 16 bytes of a head and, where pairs are half the rotated columns apart, the 16 bytes it is paired with. Few tokens spread their heads over several waves.
+#include <math.h>
+
 #include "attn_device.hpp"
 #include "status.hpp"
 
@@ -176,34 +178,47 @@ void rot_launch(RotArgs a, bool wide, hipStream_t st) {
 }
 
 // Angles are counted in turns, in 64 bits, and reduced to half a turn; what rounding that to fp32 leaves goes into the first order of
-// sine and cosine, so the tables are exact to about their own rounding at any position. Bound by the bytes written at
-// lengths of 10^5; a workgroup forms its pairs' frequencies once, in LDS.
-__global__ __launch_bounds__(256) void rot_table_kernel(FableRotaryTableParams p, int rows_per) {
-  extern __shared__ double freq[];
-  for (int i = threadIdx.x; i < p.pairs; i += 256) {
-    const double f = exp(-(double)i / p.pairs * log(p.base)) * 0.15915494309189533577;   // turns per position
-    double g = f;
-    if (p.factor != 1.0) {
-      double keep = p.original > 0.0 ? (p.original * f - p.low) / (p.high - p.low) : 0.0;
-      keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
-      g = f * (keep + (1.0 - keep) / p.factor);
-    }
-    freq[i] = g;
-  }
-  __syncthreads();
-  const long long r0 = (long long)blockIdx.x * rows_per;
-  const long long rows = min((long long)rows_per, p.rows - r0);
+// sine and cosine, so the tables are exact to about their own rounding at any position. A thread keeps V neighbouring pairs, forms
+// their frequencies once, and walks over the rows: bound by the bytes written at 10^5 rows.
+struct RotTable {
+  FableRotaryTableParams p;
+  double step;            // log2(base) / pairs
+  int columns;            // threads of a row: pairs / V, at most 256; the others of a workgroup take further rows
+};
+template <int V>
+__global__ __launch_bounds__(256) void rot_table_kernel(RotTable a) {
+  const FableRotaryTableParams& p = a.p;
+  const int rows = 256 / a.columns, sub = threadIdx.x / a.columns;
+  if (sub >= rows) return;
   const float amp = (float)p.amplitude;
-  for (long long i = threadIdx.x; i < rows * p.pairs; i += 256) {
-    const int c = (int)(i % p.pairs);
-    const long long row = r0 + i / p.pairs;
-    double x = (double)(row + p.first) * freq[c];
-    x = 2.0 * (x - rint(x));
-    const float hi = (float)x, lo = (float)(x - (double)hi) * 3.14159265358979f;
-    float s, k;
-    sincospif(hi, &s, &k);
-    p.cos[row * p.pairs + c] = amp * fmaf(-lo, s, k);
-    p.sin[row * p.pairs + c] = amp * fmaf(lo, k, s);
+  for (int c = V * (threadIdx.x % a.columns); c < p.pairs; c += V * a.columns) {
+    double freq[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const double f = exp2(-(double)(c + j) * a.step) * 0.15915494309189533577;   // turns per position
+      freq[j] = f;
+      if (p.factor != 1.0) {
+        double keep = p.original > 0.0 ? (p.original * f - p.low) / (p.high - p.low) : 0.0;
+        keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+        freq[j] = f * (keep + (1.0 - keep) / p.factor);
+      }
+    }
+    typedef float FV __attribute__((ext_vector_type(V)));
+    for (long long row = (long long)blockIdx.x * rows + sub; row < p.rows; row += (long long)gridDim.x * rows) {
+      FV co, si;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        double x = (double)(row + p.first) * freq[j];
+        x = 2.0 * (x - rint(x));
+        const float hi = (float)x, lo = (float)(x - (double)hi) * 3.14159265358979f;
+        float s, k;
+        sincospif(hi, &s, &k);
+        co[j] = amp * fmaf(-lo, s, k);
+        si[j] = amp * fmaf(lo, k, s);
+      }
+      *(FV*)(p.cos + row * p.pairs + c) = co;
+      *(FV*)(p.sin + row * p.pairs + c) = si;
+    }
   }
 }
 
@@ -249,9 +264,16 @@ extern "C" int fable_attn_rotary_tables(FableRotaryTableParams p, void* stream) 
     return fail(FA_ERR_ARG, "%s: base=%g factor=%g original=%g low=%g high=%g", what, p.base, p.factor, p.original, p.low, p.high);
   if (p.rows == 0) return FA_OK;
   if (!p.cos || !p.sin) return fail(FA_ERR_ARG, "%s: null tensor", what);
-  const int per = p.pairs >= 2048 ? 1 : 2048 / p.pairs;
-  const long long blocks = (p.rows + per - 1) / per;
-  if (blocks >= (1LL << 24)) return fail(FA_ERR_ARG, "%s: rows=%lld", what, (long long)p.rows);
-  hipLaunchKernelGGL(rot_table_kernel, dim3((unsigned)blocks), dim3(256), p.pairs * sizeof(double), (hipStream_t)stream, p, per);
+  const bool wide = p.pairs % 4 == 0 && (((uintptr_t)p.cos | (uintptr_t)p.sin) & 15) == 0;
+  RotTable a;
+  a.p = p;
+  a.step = log2(p.base) / p.pairs;
+  const int columns = wide ? p.pairs / 4 : p.pairs;
+  a.columns = columns < 256 ? columns : 256;
+  // eight rows a thread at least where there are enough of them to fill the chip
+  const long long groups = (p.rows + 256 / a.columns - 1) / (256 / a.columns);
+  const unsigned grid = (unsigned)(groups < 1024 ? groups : groups / 8 < 1024 ? 1024 : groups / 8 < 4096 ? groups / 8 : 4096);
+  if (wide) hipLaunchKernelGGL(rot_table_kernel<4>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(rot_table_kernel<1>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
   return launch_status(what);
 }

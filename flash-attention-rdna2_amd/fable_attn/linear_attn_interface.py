@@ -16,7 +16,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _C, _lib
-from .flash_attn_interface import MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _kernel_width, _with_width
+from .flash_attn_interface import (MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _kernel_width, _place, _plans, _remember, _sig,
+                                   _with_width)
 
 # rows per sequence up to which linear_attn_with_state goes token by token
 STEP_ROWS = 16
@@ -118,7 +119,23 @@ def linear_attn_varlen_func(q, k, v, cu_seqlens, max_seqlen, decay, scale=None, 
     return _attend((cu, int(max_seqlen)), q, k, v, decay, scale, initial_state, return_final_state)
 
 
-@torch.no_grad()
+def _step_fast(plan, q, k, v, state, decay, idx, cu):
+    """One call of a planned signature, or None when an address is not aligned or the device is not current (the general path
+    serves it)."""
+    p, dt, dev, shape, strides = plan
+    qp, kp, vp, sp = q.data_ptr(), k.data_ptr(), v.data_ptr(), state.data_ptr()
+    if (qp | kp | vp | sp) & 15 or dev != torch._C._cuda_getDevice():
+        return None
+    out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
+    p.q, p.k, p.v, p.o, p.state_in, p.state_out, p.decay = qp, kp, vp, out.data_ptr(), sp, sp, decay.data_ptr()
+    if idx is not None:
+        p.slots = idx.data_ptr()
+    if cu is not None:
+        p.cu = cu.data_ptr()
+    _lib.check(_C._L.fable_linear_attn_step(p, dt, torch._C._cuda_getCurrentRawStream(dev)), "fable_linear_attn_step")
+    return out
+
+
 def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu_seqlens=None, max_seqlen=None):
     """Serving: new tokens q, k, v (batch, seqlen_new, nheads, ...), or packed (total, nheads, ...) with cu_seqlens int32 (batch+1) and
     max_seqlen (default: total), go on from the states of a pool, float32 (num_states, nheads, d, dv), which are
@@ -126,17 +143,39 @@ def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu
     no sequence (a padded batch): its rows of out are zeros and no state changes. Two sequences of one call must not name one state; a
     new request starts from a state that the caller has zeroed. Returns out as linear_attn_func. Up to 16 new tokens per sequence
     run token by token, each state read and written once; more run by chunks. Head dims are multiples of 8. No gradient passes through."""
+    key, plans = None, _plans("linear_step_plans")
+    try:
+        key = (_place(q), _place(k), _place(v), _place(state), _sig(decay), _sig(state_idx), _sig(cu_seqlens), scale, max_seqlen)
+        plan = plans.get(key)
+    except (AttributeError, TypeError, ValueError, RuntimeError):   # not tensors, or no key
+        key = plan = None
+    if plan is not None:
+        out = _step_fast(plan, q, k, v, state, decay, state_idx, cu_seqlens)
+        if out is not None:
+            return out
+    return _with_state(key, plans, q, k, v, state, decay, state_idx, scale, cu_seqlens, max_seqlen)
+
+
+@torch.no_grad()
+def _with_state(key, plans, q, k, v, state, decay, state_idx, scale, cu_seqlens, max_seqlen):
+    """linear_attn_with_state with all checks and conversions; remembers the launch where nothing was converted."""
     if not torch.is_tensor(state) or state.dim() != 4 or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("fable_attn: state must be a contiguous float32 tensor (num_states, nheads, headdim, headdim_v)")
     packed = cu_seqlens is not None
-    decay, scale = _check(q, k, v, decay, packed, scale)
+    fp32, scale = _check(q, k, v, decay, packed, scale)
     if q.shape[-1] % 8 or v.shape[-1] % 8:
         raise NotImplementedError(f"fable_attn: states are updated in place for head dims that are multiples of 8, got {q.shape[-1]} and {v.shape[-1]}")
     dev = q.device
     cu = _as_index(cu_seqlens, dev) if packed else None
     most = (q.shape[0] if max_seqlen is None else int(max_seqlen)) if packed else q.shape[1]
     idx = _as_index(state_idx, dev) if state_idx is not None else None
+    given = (q, k, v, decay, cu_seqlens, state_idx)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if most <= STEP_ROWS:
-        return _C.linear_step(q, k, v, state, decay, scale, cu, most, idx)[0]
-    return _C.linear_fwd(q, k, v, decay, scale, cu, most, state, state, idx)[0]
+    if most > STEP_ROWS:
+        return _C.linear_fwd(q, k, v, fp32, scale, cu, most, state, state, idx)[0]
+    out, p, dt = _C.linear_step(q, k, v, state, fp32, scale, cu, most, idx)
+    # (decay: the same values where they are, whether or not it records gradients)
+    used = (q, k, v, decay if fp32.data_ptr() == decay.data_ptr() else fp32, cu, idx)
+    if key is not None and p.batch and all(a is b for a, b in zip(given, used)):
+        _remember(plans, key, (p, dt, dev.index, out.shape, out.stride()))   # nothing was converted: the next call may fill in its addresses
+    return out

@@ -8,13 +8,40 @@ they write a cache), and the tables, scaled for contexts longer than the trained
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _C
-from .flash_attn_interface import _DTYPES, _as_index
+from . import _C, _lib
+from .flash_attn_interface import _DTYPES, _as_index, _place, _plans, _remember, _sig
 
 
 def _flat(t):
     """t with a contiguous head dim."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _turn(q, k, cos, sin, interleaved, cu, start, conj):
+    """One launch; the parameters that the first one of a signature came to are kept per thread, and later ones fill in addresses."""
+    key = (_place(q), _place(k), _sig(cos), _sig(sin), _sig(cu), _sig(start), interleaved, conj)
+    plans = _plans("rotary_plans")
+    plan = plans.get(key)
+    dev = q.get_device()
+    qp, kp = q.data_ptr(), k.data_ptr() if k is not None else 0
+    if plan is None or (qp | kp) & 15 != plan[4] or dev != torch._C._cuda_getDevice():
+        qo, ko, p, dt = _C.rotary(q, k, cos, sin, interleaved, cu, start, conj)
+        if q.numel():
+            _remember(plans, key, (p, dt, qo.stride(), ko.stride() if ko is not None else None, (qp | kp) & 15))
+        return qo, ko
+    p, dt, qs, ks, _ = plan
+    qo = torch.empty_strided(q.shape, qs, dtype=q.dtype, device=q.device)
+    p.q, p.q_out, p.cos, p.sin = qp, qo.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    ko = None
+    if k is not None:
+        ko = torch.empty_strided(k.shape, ks, dtype=k.dtype, device=k.device)
+        p.k, p.k_out = kp, ko.data_ptr()
+    if cu is not None:
+        p.cu = cu.data_ptr()
+    if start is not None:
+        p.start = start.data_ptr()
+    _lib.check(_C._L.fable_attn_rotary(p, dt, torch._C._cuda_getCurrentRawStream(dev)), "fable_attn_rotary")
+    return qo, ko
 
 
 class _Rotary(torch.autograd.Function):
@@ -25,7 +52,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(cos, sin, cu, start)
         ctx.interleaved = interleaved
         ctx.set_materialize_grads(False)
-        qo, ko, _, _ = _C.rotary(q, k, cos, sin, interleaved, cu, start)
+        qo, ko = _turn(q, k, cos, sin, interleaved, cu, start, False)
         return (qo, ko) if k is not None else qo
 
     @staticmethod
@@ -35,8 +62,8 @@ class _Rotary(torch.autograd.Function):
         one, two = (dq, dk) if dq is not None else (dk, None)
         if one is None:
             return (None,) * 7
-        one, two, _, _ = _C.rotary(_flat(one), _flat(two) if two is not None else None, cos, sin, ctx.interleaved, cu, start, conj=True)
-        return (one, two, *(None,) * 5) if dq is not None else (None, one, *(None,) * 5)
+        one, two = _turn(_flat(one), _flat(two) if two is not None else None, cos, sin, ctx.interleaved, cu, start, True)
+        return (one, two, None, None, None, None, None) if dq is not None else (None, one, None, None, None, None, None)
 
 
 def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=True, rotary_seqlens=None, cu_seqlens=None):
@@ -57,16 +84,20 @@ def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=T
     if grad and (rotary_cos.requires_grad or rotary_sin.requires_grad):
         raise NotImplementedError("fable_attn: rotary tables get no gradient; pass them detached")
     dev = q.device
-    cos, sin = rotary_cos.detach().to(torch.float32).contiguous(), rotary_sin.detach().to(torch.float32).contiguous()
-    cu = _as_index(cu_seqlens, dev) if cu_seqlens is not None else None
-    if isinstance(rotary_seqlens, int):
+    cos, sin, cu, start = rotary_cos, rotary_sin, cu_seqlens, rotary_seqlens
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        cos, sin = cos.detach().to(torch.float32).contiguous(), sin.detach().to(torch.float32).contiguous()
+    if cu is not None:
+        cu = _as_index(cu, dev)
+    if isinstance(start, int):
         batch = q.shape[0] if cu is None else cu.numel() - 1
-        rotary_seqlens = torch.full((batch,), rotary_seqlens, dtype=torch.int32, device=dev) if rotary_seqlens else None
-    start = _as_index(rotary_seqlens, dev) if rotary_seqlens is not None else None
+        start = torch.full((batch,), start, dtype=torch.int32, device=dev) if start else None
+    elif start is not None:
+        start = _as_index(start, dev)
     q, k = _flat(q), _flat(k) if k is not None else None
     if grad and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, cos, sin, bool(rotary_interleaved), cu, start)
-    qo, ko, _, _ = _C.rotary(q, k, cos, sin, bool(rotary_interleaved), cu, start)
+    qo, ko = _turn(q, k, cos, sin, bool(rotary_interleaved), cu, start, False)
     return (qo, ko) if k is not None else qo
 
 
