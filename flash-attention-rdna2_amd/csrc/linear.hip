@@ -12,27 +12,30 @@
 namespace fa {
 
 // ws[sg + 1] holds what segment sg adds to the state; becomes the state before segment sg + 1 (and, where the call overwrites it, ws[0]
-// the one before the first). A thread carries one element along; its loads of the next segments do not wait for the sum.
+// the one before the first). A thread carries four elements along; its loads of the next segments do not wait for the sum.
 __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
-  const int n = p.da * p.db, nb = (n + 255) / 256;
+  const int n = p.da * p.db, nb = (n / 4 + 255) / 256;
   const int bh = blockIdx.x / nb, b = bh / p.NH, h = bh % p.NH;
-  const int e = (blockIdx.x % nb) * 256 + threadIdx.x;
+  const int e = 4 * ((blockIdx.x % nb) * 256 + threadIdx.x);
   const LaSeq sq = la_seq(p, b);
   if (e >= n || sq.slot < 0) return;
   const int nseg = la_segments(p, sq.len);
   float* const ws = p.ws + (long long)bh * p.nseg * n + e;
-  float cur = p.first ? p.first[((long long)sq.slot * p.NH + h) * n + (e / p.db) * p.sa + (e % p.db) * p.sb] : 0.0f;
+  f32x4 cur = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (p.first) cur = *(const f32x4*)(p.first + ((long long)sq.slot * p.NH + h) * n + e);
   const float d = la_decay(p, b, h);
   const LaFade whole(d, (float)p.seg), first(d, (float)(p.seg - 1));
-  if (p.inplace) ws[0] = cur;
+  if (p.inplace) *(f32x4*)ws = cur;
   for (int s = 1; s < nseg; s += 4) {
-    float v[4];
+    f32x4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = s + j < nseg ? ws[(long long)(s + j) * n] : 0.0f;
+    for (int j = 0; j < 4; j++) v[j] = *(const f32x4*)(ws + (long long)min(s + j, nseg - 1) * n);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      cur = (p.enter && s + j == 1 ? first(cur) : whole(cur)) + v[j];
-      if (s + j < nseg) ws[(long long)(s + j) * n] = cur;
+      const LaFade& fade = p.enter && s + j == 1 ? first : whole;
+#pragma unroll
+      for (int i = 0; i < 4; i++) cur[i] = fade(cur[i]) + v[j][i];
+      if (s + j < nseg) *(f32x4*)(ws + (long long)(s + j) * n) = cur;
     }
   }
 }
@@ -67,17 +70,22 @@ void la_single(LaArgs& a) {
   a.sz.s = a.so.s = a.db;
 }
 
-// Segments of a call, the same for all its passes: two workgroups for each of the 256 CUs, but none of fewer than 256 rows.
-void la_split(LaArgs& a, const FableLinearParams& p) {
+// Segments of a call, the same for all its passes. A wave per 32 columns of a head has a row's work in about 60 ns, whatever the others do, so
+// the longest sequence takes n of those; spread evenly over the 1024 SIMDs the rows of all heads take n * 1024 / (waves' rows) times
+// less. Below 1.8 that does not pay for a second reading of k and v and the states' traffic (8 prompts of up to 2048 rows, 32 heads
+// of 128, ratio 1.44: 131 us in one piece, 190 cut; 24 documents H16 D64, ratio 2.6: forward and backward 448 against 365). Two waves per
+// SIMD then, but no segment under `least` rows.
+void la_split(LaArgs& a, const FableLinearParams& p, int dtype) {
   la_single(a);
-  const int D = p.DK > p.DV ? p.DK : p.DV, width = D <= 64 ? 64 : 128;
-  const long long base = (long long)a.batch * a.NH * ((D + width - 1) / width);
-  long long k = base >= 256 ? 1 : (512 + base - 1) / (base > 0 ? base : 1);
-  const long long most = (a.n + 255) / 256;
-  k = k > most ? most : k;
-  k = k < 1 ? 1 : k;
-  const long long seg = ((a.n + k - 1) / k + kLaChunk - 1) / kLaChunk * kLaChunk;
-  a.seg = (int)(seg < kLaChunk ? kLaChunk : seg);
+  const int D = p.DK > p.DV ? p.DK : p.DV;
+  const long long rows = p.cu ? p.total : (long long)a.batch * a.n;
+  const long long work = rows * a.NH * ((D + 31) / 32);
+  const long long least = dtype == FA_F32 ? 64 : 256;
+  long long seg = a.n;
+  if ((long long)a.n * 10240 > 18 * work) seg = (work + 2047) / 2048;
+  seg = seg < least ? least : seg;
+  seg = (seg + kLaChunk - 1) / kLaChunk * kLaChunk;
+  a.seg = (int)(seg < (1 << 30) ? seg : (1 << 30));
   a.nseg = (int)(((long long)a.n + a.seg - 1) / a.seg);
   if (a.nseg < 1) a.nseg = 1;
   a.wa = p.DV, a.wb = 1;
@@ -100,7 +108,7 @@ LaArgs la_base(const FableLinearParams& p) {
   return a;
 }
 
-LaArgs la_forward(const FableLinearParams& p) {
+LaArgs la_forward(const FableLinearParams& p, int dtype) {
   LaArgs a = la_base(p);
   a.x = p.q, a.y = p.k, a.z = p.v, a.o = p.o;
   a.sx = p.sq, a.sy = p.sk, a.sz = p.sv, a.so = p.so;
@@ -111,12 +119,12 @@ LaArgs la_forward(const FableLinearParams& p) {
   a.slots = p.slots, a.nslots = p.num_slots;
   a.inplace = p.state_in && p.state_in == p.state_out;
   a.iscale = p.scale, a.uscale = 1.0f;
-  la_split(a, p);
+  la_split(a, p, dtype);
   return a;
 }
 
 // dq_t = scale S_t dout_t
-LaArgs la_dq(const FableLinearParams& p) {
+LaArgs la_dq(const FableLinearParams& p, int dtype) {
   LaArgs a = la_base(p);
   a.x = p.dout, a.y = p.v, a.z = p.k, a.o = p.dq;
   a.sx = p.sdo, a.sy = p.sv, a.sz = p.sk, a.so = p.sdq;
@@ -125,13 +133,13 @@ LaArgs la_dq(const FableLinearParams& p) {
   a.first = p.state_in;
   a.sa = 1, a.sb = p.DV;
   a.iscale = p.scale, a.uscale = 1.0f;
-  la_split(a, p);
+  la_split(a, p, dtype);
   a.wa = 1, a.wb = p.DV;   // the states as they are for k, v (q, dout)
   return a;
 }
 
 // dv_t = G_t^T k_t; G is DK x DV
-LaArgs la_dv(const FableLinearParams& p) {
+LaArgs la_dv(const FableLinearParams& p, int dtype) {
   LaArgs a = la_base(p);
   a.x = p.k, a.y = p.q, a.z = p.dout, a.o = p.dv;
   a.sx = p.sk, a.sy = p.sq, a.sz = p.sdo, a.so = p.sdv;
@@ -141,12 +149,12 @@ LaArgs la_dv(const FableLinearParams& p) {
   a.sa = p.DV, a.sb = 1;
   a.iscale = 1.0f, a.uscale = p.scale;
   a.rev = 1, a.enter = p.dstate_out != nullptr, a.leave = 1;
-  la_split(a, p);
+  la_split(a, p, dtype);
   return a;
 }
 
 // dk_t = G_t v_t, on G^T
-LaArgs la_dk(const FableLinearParams& p) {
+LaArgs la_dk(const FableLinearParams& p, int dtype) {
   LaArgs a = la_base(p);
   a.x = p.v, a.y = p.dout, a.z = p.q, a.o = p.dk;
   a.sx = p.sv, a.sy = p.sdo, a.sz = p.sq, a.so = p.sdk;
@@ -156,7 +164,7 @@ LaArgs la_dk(const FableLinearParams& p) {
   a.sa = 1, a.sb = p.DV;
   a.iscale = 1.0f, a.uscale = p.scale;
   a.rev = 1, a.enter = p.dstate_out != nullptr;
-  la_split(a, p);
+  la_split(a, p, dtype);
   a.wa = 1, a.wb = p.DV;   // the states as they are for k, v (q, dout)
   return a;
 }
@@ -171,11 +179,11 @@ void la_go(LaArgs a, int dtype, bool state, bool exact, hipStream_t st) {
   else la_launch<float>(a, state, exact, st);
 }
 
-// The states before all segments, into a.ws (nseg is above 1 for fewer than 256 states only, and then at most 512).
+// The states before all segments, into a.ws, for arguments whose states are as the caller has them (DK x DV).
 void la_states(const LaArgs& a, int dtype, bool exact, hipStream_t st) {
   if (a.nseg < 2) return;
   la_go(a, dtype, true, exact, st);
-  hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)(a.batch * a.NH * ((a.da * a.db + 255) / 256))), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)(a.batch * a.NH * ((a.da * a.db / 4 + 255) / 256))), dim3(256), 0, st, a);
 }
 
 // What every call has to satisfy; the tensors' own checks follow in the entry points.
@@ -185,7 +193,7 @@ int la_check(const FableLinearParams& p, int dtype, const char* what) {
     return fail(FA_ERR_HEADDIM, "%s: head dims %d and %d: multiples of 8 up to 256", what, p.DK, p.DV);
   if (p.batch < 0 || p.n < 0 || p.NH < 1 || p.gqa < 1 || p.NH % p.gqa || p.total < 0 || p.n > (1 << 30))
     return fail(FA_ERR_ARG, "%s: batch=%d n=%d NH=%d gqa=%d", what, p.batch, p.n, p.NH, p.gqa);
-  // (256 workgroups of the scan for each state, within a grid's 2^32 threads)
+  // (64 workgroups of the scan for each state, within a grid's 2^32 threads)
   if ((long long)p.batch * p.NH > 65535) return fail(FA_ERR_ARG, "%s: batch x heads = %lld", what, (long long)p.batch * p.NH);
   return FA_OK;
 }
@@ -224,8 +232,8 @@ long long la_round(long long x) { return (x + 255) / 256 * 256; }
 
 // Forward: the segments' states. Backward: those of q and dout, before them the ones of k and v, if the forward pass's are not
 // given, and behind them the partial gradients of shared heads.
-long long la_need(const FableLinearParams& p, bool backward) {
-  const long long w = la_ws(la_forward(p));
+long long la_need(const FableLinearParams& p, int dtype, bool backward) {
+  const long long w = la_ws(la_forward(p, dtype));
   return backward ? la_round(w) * (p.seg_states ? 1 : 2) + la_group_bytes(p) : w;
 }
 
@@ -245,7 +253,7 @@ using namespace fa;
 
 extern "C" int64_t fable_linear_attn_ws_bytes(FableLinearParams p, int dtype, int backward) {
   if (la_check(p, dtype, "fable_linear_attn_ws_bytes") != FA_OK) return -1;
-  return la_need(p, backward != 0);
+  return la_need(p, dtype, backward != 0);
 }
 
 extern "C" int fable_linear_attn_fwd(FableLinearParams p, int dtype, void* ws, int64_t ws_bytes, void* stream) {
@@ -255,11 +263,11 @@ extern "C" int fable_linear_attn_fwd(FableLinearParams p, int dtype, void* ws, i
   if (!p.decay) return fail(FA_ERR_ARG, "%s: null decay", what);
   if (p.slots && (p.num_slots < 0 || (!p.state_in && !p.state_out))) return fail(FA_ERR_ARG, "%s: slots without states", what);
   if ((rc = la_tensors(what, p, dtype, false)) != FA_OK) return rc;
-  const long long need = la_need(p, false);
+  const long long need = la_need(p, dtype, false);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
   if (p.batch == 0) return FA_OK;
-  LaArgs a = la_forward(p);
+  LaArgs a = la_forward(p, dtype);
   a.ws = (float*)ws;
   const bool exact = a.last != nullptr;
   la_states(a, dtype, exact, (hipStream_t)stream);
@@ -276,7 +284,7 @@ extern "C" int fable_linear_attn_step(FableLinearParams p, int dtype, void* stre
   if (p.slots && p.num_slots < 0) return fail(FA_ERR_ARG, "%s: num_slots=%d", what, p.num_slots);
   if ((rc = la_tensors(what, p, dtype, false)) != FA_OK) return rc;
   if (p.batch == 0) return FA_OK;
-  la_step(la_forward(p), dtype, (hipStream_t)stream);
+  la_step(la_forward(p, dtype), dtype, (hipStream_t)stream);
   return launch_status(what);
 }
 
@@ -288,13 +296,13 @@ extern "C" int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, i
   if (p.slots) return fail(FA_ERR_ARG, "%s: states of a pool have no gradient", what);
   if (p.gqa > 1 && (long long)p.NH * (p.DK > p.DV ? p.DK : p.DV) >= (1LL << 29) / (4 * kLaChunk)) return fail(FA_ERR_ARG, "%s: NH=%d", what, p.NH);
   if ((rc = la_tensors(what, p, dtype, true)) != FA_OK) return rc;
-  const long long need = la_need(p, true);
+  const long long need = la_need(p, dtype, true);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     return fail(FA_ERR_ARG, "%s: a workspace of %lld bytes is needed, %lld given", what, need, (long long)ws_bytes);
   if (p.batch == 0) return FA_OK;
   hipStream_t st = (hipStream_t)stream;
   // dq over the states of k and v
-  LaArgs a = la_forward(p), dq = la_dq(p);
+  LaArgs a = la_forward(p, dtype), dq = la_dq(p, dtype);
   char* at = (char*)ws;
   if (p.seg_states) {
     dq.ws = (float*)p.seg_states;
@@ -305,7 +313,7 @@ extern "C" int fable_linear_attn_bwd(FableLinearParams p, int dtype, void* ws, i
   }
   la_go(dq, dtype, false, false, st);
   // dv and dk over those of q and dout, from the last row on
-  LaArgs pass[2] = {la_dv(p), la_dk(p)};
+  LaArgs pass[2] = {la_dv(p, dtype), la_dk(p, dtype)};
   const bool exact = pass[0].last != nullptr;
   pass[0].ws = pass[1].ws = (float*)at;
   la_states(pass[0], dtype, exact, st);

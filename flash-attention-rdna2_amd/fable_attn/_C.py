@@ -793,23 +793,24 @@ def _linear_ws(p, dt, backward, dev):
 
 def linear_fwd(q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, state_out=None, slots=None):
     """Linear attention by chunks -> (out, dense of q's rows and v's width; the states before the segments of long sequences for
-    linear_bwd, or None). state_out: where the states behind the last rows go (as state_in; may be it)."""
+    linear_bwd, or None; the launch's parameters, dtype and workspace size). state_out: where the states behind the last rows go
+    (as state_in; may be it)."""
     p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in, slots)
     out = torch.empty((*q.shape[:-1], v.shape[-1]), dtype=q.dtype, device=q.device)
     p.o, p.so = out.data_ptr(), _rows_strides(out, cu is not None)
     if state_out is not None:
         p.state_out = state_out.data_ptr()
     if p.batch == 0:
-        return out.zero_(), None
+        return out.zero_(), None, p, _dt(q), 0
     dt = _dt(q)
     ws, need = _linear_ws(p, dt, 0, q.device)
     with _on(q.device):
         _lib.check(_L.fable_linear_attn_fwd(p, dt, _ptr(ws), need, _stream(q)), "fable_linear_attn_fwd")
-    return out, ws
+    return out, ws, p, dt, need
 
 
 def linear_bwd(dout, q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None, dstate_out=None, want_dstate=False, seg_states=None):
-    """-> (dq, dk, dv, dstate_in or None)"""
+    """-> (dq, dk, dv, dstate_in or None, the launch's parameters, dtype and workspace size)"""
     p = _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in)
     _req(dout.dtype == q.dtype and tuple(dout.shape) == (*q.shape[:-1], v.shape[-1]) and _rows_aligned(dout),
          "dout: out's shape and dtype, 16-byte aligned rows")
@@ -827,12 +828,12 @@ def linear_bwd(dout, q, k, v, decay, scale, cu=None, max_seqlen=0, state_in=None
     if seg_states is not None:
         p.seg_states = seg_states.data_ptr()
     if p.batch == 0:
-        return dq.zero_(), dk.zero_(), dv.zero_(), dstate
+        return dq.zero_(), dk.zero_(), dv.zero_(), dstate, p, _dt(q), 0
     dt = _dt(q)
     ws, need = _linear_ws(p, dt, 1, q.device)
     with _on(q.device):
         _lib.check(_L.fable_linear_attn_bwd(p, dt, _ptr(ws), need, _stream(q)), "fable_linear_attn_bwd")
-    return dq, dk, dv, dstate
+    return dq, dk, dv, dstate, p, dt, need
 
 
 def linear_step(q, k, v, state, decay, scale, cu=None, max_seqlen=0, slots=None):

@@ -46,7 +46,60 @@ def _check(q, k, v, decay, packed, scale):
         raise TypeError(f"fable_attn: decay must be a tensor (nheads) or (batch, nheads), got {type(decay)}")
     if decay.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("fable_attn: decay gets no gradient; pass decay.detach()")
-    return decay.detach().to(torch.float32).contiguous(), float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if decay.dtype != torch.float32 or decay.requires_grad or not decay.is_contiguous():
+        decay = decay.detach().to(torch.float32).contiguous()
+    return decay, float(q.shape[-1] ** -0.5 if scale is None else scale)
+
+
+def _forward(q, k, v, decay, scale, cu, most, state, final, idx=None):
+    """_C.linear_fwd; the parameters that the first call of a signature came to are kept per thread, and later ones fill in
+    addresses."""
+    key = (_place(q), _place(k), _place(v), _sig(decay), scale, _sig(cu), most, _sig(state), _sig(final), _sig(idx))
+    plans = _plans("linear_plans")
+    plan = plans.get(key)
+    qp, kp, vp, sp, dev = q.data_ptr(), k.data_ptr(), v.data_ptr(), state.data_ptr() if state is not None else 0, q.get_device()
+    if plan is None or (qp | kp | vp | sp) & 15 or dev != torch._C._cuda_getDevice():
+        out, ws, p, dt, need = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final, idx)
+        if p.batch:
+            _remember(plans, key, (p, dt, need, out.shape, out.stride()))
+        return out, ws
+    p, dt, need, shape, strides = plan
+    out = torch.empty_strided(shape, strides, dtype=q.dtype, device=q.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    p.q, p.k, p.v, p.o, p.decay = qp, kp, vp, out.data_ptr(), decay.data_ptr()
+    p.state_in, p.state_out = sp or None, final.data_ptr() if final is not None else None
+    if cu is not None:
+        p.cu = cu.data_ptr()
+    if idx is not None:
+        p.slots = idx.data_ptr()
+    _lib.check(_C._L.fable_linear_attn_fwd(p, dt, ws.data_ptr() if need else None, need, torch._C._cuda_getCurrentRawStream(dev)),
+               "fable_linear_attn_fwd")
+    return out, ws
+
+
+def _backward(dout, q, k, v, decay, scale, cu, most, state, dfinal, want, seg):
+    """_C.linear_bwd, planned as _forward."""
+    key = (_place(dout), _place(q), _place(k), _place(v), _sig(decay), scale, _sig(cu), most, _sig(state), _sig(dfinal), want, seg is None)
+    plans = _plans("linear_bwd_plans")
+    plan = plans.get(key)
+    dp, qp, kp, vp, dev = dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), q.get_device()
+    if plan is None or (dp | qp | kp | vp) & 15 or dev != torch._C._cuda_getDevice():
+        dq, dk, dv, dstate, p, dt, need = _C.linear_bwd(dout, q, k, v, decay, scale, cu, most, state, dfinal, want, seg)
+        if p.batch:
+            _remember(plans, key, (p, dt, need, dq.stride(), dk.stride(), dv.stride()))
+        return dq, dk, dv, dstate
+    p, dt, need, qs, ks, vs = plan
+    device = q.device
+    dq = torch.empty_strided(q.shape, qs, dtype=q.dtype, device=device)
+    dk = torch.empty_strided(k.shape, ks, dtype=q.dtype, device=device)
+    dv = torch.empty_strided(v.shape, vs, dtype=q.dtype, device=device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    dstate = torch.empty((p.batch, p.NH, p.DK, p.DV), dtype=torch.float32, device=device) if want else None
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    p.dout, p.q, p.k, p.v, p.dq, p.dk, p.dv, p.decay = dp, qp, kp, vp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), decay.data_ptr()
+    p.state_in, p.dstate_out, p.dstate_in, p.seg_states, p.cu = ptr(state), ptr(dfinal), ptr(dstate), ptr(seg), ptr(cu)
+    _lib.check(_C._L.fable_linear_attn_bwd(p, dt, ptr(ws), need, torch._C._cuda_getCurrentRawStream(dev)), "fable_linear_attn_bwd")
+    return dq, dk, dv, dstate
 
 
 class _LinearAttention(torch.autograd.Function):
@@ -57,7 +110,7 @@ class _LinearAttention(torch.autograd.Function):
         cu, most = pack if pack is not None else (None, 0)
         batch = cu.numel() - 1 if cu is not None else q.shape[0]
         final = torch.empty((batch, q.shape[-2], q.shape[-1], v.shape[-1]), dtype=torch.float32, device=q.device) if want else None
-        out, seg = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
+        out, seg = _forward(q, k, v, decay, scale, cu, most, state, final)
         ctx.scale, ctx.most = scale, most
         ctx.save_for_backward(q, k, v, decay, state, cu, seg)
         ctx.set_materialize_grads(False)
@@ -68,10 +121,10 @@ class _LinearAttention(torch.autograd.Function):
     def backward(ctx, dout, dfinal=None):
         q, k, v, decay, state, cu, seg = ctx.saved_tensors
         if dout is None and dfinal is None:
-            return (None,) * 8
+            return None, None, None, None, None, None, None, None
         dout = q.new_zeros((*q.shape[:-1], v.shape[-1])) if dout is None else _rows(dout)
-        dq, dk, dv, dstate = _C.linear_bwd(dout, q, k, v, decay, ctx.scale, cu, ctx.most, state,
-                                           dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7], seg)
+        dq, dk, dv, dstate = _backward(dout, q, k, v, decay, ctx.scale, cu, ctx.most, state,
+                                       dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7], seg)
         return None, None, None, dq, dk, dv, None, dstate
 
 
@@ -84,22 +137,22 @@ def _attend(pack, q, k, v, decay, scale, state, want):
             raise ValueError(f"fable_attn: initial_state must be float32 {(batch, q.shape[-2], dk, dv)} on q's device, got "
                              f"{state.dtype} {tuple(state.shape)}")
     wk, wv = _kernel_width(dk, q.dtype), _kernel_width(dv, q.dtype)
+    padded = wk != dk or wv != dv
     if state is not None:
-        state = torch.nn.functional.pad(state, (0, wv - dv, 0, wk - dk)) if (wk, wv) != (dk, dv) else state.contiguous()
-        state = _aligned(state, dense=True)
-    q, k, v = (_rows(_with_width(t, w)) for t, w in ((q, wk), (k, wk), (v, wv)))
+        state = _aligned(torch.nn.functional.pad(state, (0, wv - dv, 0, wk - dk)) if padded else state, dense=True)
+    q, k, v = _rows(_with_width(q, wk)), _rows(_with_width(k, wk)), _rows(_with_width(v, wv))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (state is not None and state.requires_grad)):
         res = _LinearAttention.apply(pack, scale, want, q, k, v, decay, state)
         out, final = res if want else (res, None)
     else:
         cu, most = pack if pack is not None else (None, 0)
         final = torch.empty((batch, q.shape[-2], wk, wv), dtype=torch.float32, device=q.device) if want else None
-        out, _ = _C.linear_fwd(q, k, v, decay, scale, cu, most, state, final)
+        out, _ = _forward(q, k, v, decay, scale, cu, most, state, final)
     if wv != dv:
         out = out[..., :dv].contiguous()
     if not want:
         return out
-    return out, (final[..., :dk, :dv].contiguous() if (wk, wv) != (dk, dv) else final)
+    return out, (final[..., :dk, :dv].contiguous() if padded else final)
 
 
 def linear_attn_func(q, k, v, decay, scale=None, initial_state=None, return_final_state=False):
@@ -172,10 +225,9 @@ def _with_state(key, plans, q, k, v, state, decay, state_idx, scale, cu_seqlens,
     given = (q, k, v, decay, cu_seqlens, state_idx)
     q, k, v = _rows(q), _rows(k), _rows(v)
     if most > STEP_ROWS:
-        return _C.linear_fwd(q, k, v, fp32, scale, cu, most, state, state, idx)[0]
+        return _forward(q, k, v, fp32, scale, cu, most, state, state, idx)[0]
     out, p, dt = _C.linear_step(q, k, v, state, fp32, scale, cu, most, idx)
-    # (decay: the same values where they are, whether or not it records gradients)
-    used = (q, k, v, decay if fp32.data_ptr() == decay.data_ptr() else fp32, cu, idx)
+    used = (q, k, v, fp32, cu, idx)
     if key is not None and p.batch and all(a is b for a, b in zip(given, used)):
         _remember(plans, key, (p, dt, dev.index, out.shape, out.stride()))   # nothing was converted: the next call may fill in its addresses
     return out
