@@ -891,7 +891,8 @@ def rotary(q, k, cos, sin, interleaved, cu=None, start=None, conj=False):
 
 def rotary_tables(rows, first, pairs, base, factor, original, low, high, amplitude, dev):
     """cos and sin [rows, pairs] in fp32 of positions first, first + 1, ..."""
-    cos, sin = (torch.empty((rows, pairs), dtype=torch.float32, device=dev) for _ in range(2))
+    cos = torch.empty((rows, pairs), dtype=torch.float32, device=dev)
+    sin = torch.empty_like(cos)
     p = _lib.FableRotaryTableParams(cos.data_ptr(), sin.data_ptr(), rows, first, pairs, base, factor, original, low, high, amplitude)
     with _on(cos.device):
         _lib.check(_L.fable_attn_rotary_tables(p, _stream(cos)), "fable_attn_rotary_tables")

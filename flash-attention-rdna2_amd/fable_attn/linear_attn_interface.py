@@ -168,7 +168,7 @@ def linear_attn_varlen_func(q, k, v, cu_seqlens, max_seqlen, decay, scale=None, 
     """linear_attn_func of packed sequences: q (total, nheads, d), k and v (total, nheads_k, ...), cu_seqlens int32 (batch+1);
     states are (batch, nheads, d, dv). max_seqlen sizes the launch (a longer sequence is served, more
     slowly). Sequences may be empty: their state passes through. Rows of no sequence come back as zeros, as do their gradients."""
-    cu = _as_index(cu_seqlens, q.device)
+    cu = cu_seqlens if cu_seqlens.dtype == torch.int32 and cu_seqlens.device == q.device and cu_seqlens.is_contiguous() else _as_index(cu_seqlens, q.device)
     return _attend((cu, int(max_seqlen)), q, k, v, decay, scale, initial_state, return_final_state)
 
 

@@ -17,6 +17,11 @@ def _flat(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _index(t, dev):
+    """t as the kernels read it: int32, contiguous, on dev."""
+    return t if t.dtype == torch.int32 and t.device == dev and t.is_contiguous() else _as_index(t, dev)
+
+
 def _turn(q, k, cos, sin, interleaved, cu, start, conj):
     """One launch; the parameters that the first one of a signature came to are kept per thread, and later ones fill in addresses."""
     key = (_place(q), _place(k), _sig(cos), _sig(sin), _sig(cu), _sig(start), interleaved, conj)
@@ -88,12 +93,12 @@ def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=T
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
         cos, sin = cos.detach().to(torch.float32).contiguous(), sin.detach().to(torch.float32).contiguous()
     if cu is not None:
-        cu = _as_index(cu, dev)
+        cu = _index(cu, dev)
     if isinstance(start, int):
         batch = q.shape[0] if cu is None else cu.numel() - 1
         start = torch.full((batch,), start, dtype=torch.int32, device=dev) if start else None
     elif start is not None:
-        start = _as_index(start, dev)
+        start = _index(start, dev)
     q, k = _flat(q), _flat(k) if k is not None else None
     if grad and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, cos, sin, bool(rotary_interleaved), cu, start)
@@ -101,7 +106,6 @@ def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=T
     return (qo, ko) if k is not None else qo
 
 
-@torch.no_grad()
 def flash_attn_rotary_tables(seqlen, rotary_dim, *, base=10000.0, factor=1.0, original_seqlen=None, low_turns=1.0, high_turns=32.0,
                              amplitude=1.0, start=0, device=None):
     """(cos, sin) in fp32, (seqlen, rotary_dim / 2), of positions start, start + 1, ...: pair i turns by f_i = base^(-2 i /
@@ -119,8 +123,11 @@ def flash_attn_rotary_tables(seqlen, rotary_dim, *, base=10000.0, factor=1.0, or
     if original_seqlen is not None and not (original_seqlen > 0 and high_turns > low_turns):
         raise ValueError(f"fable_attn: original_seqlen={original_seqlen}, low_turns={low_turns}, high_turns={high_turns}: "
                          "a length above 0, high_turns above low_turns")
-    device = torch.device("cuda" if device is None else device)
-    if device.type != "cuda":
-        raise ValueError(f"fable_attn: tables are made on the GPU (device={device})")
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    else:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"fable_attn: tables are made on the GPU (device={device})")
     return _C.rotary_tables(seqlen, start, rotary_dim // 2, float(base), float(factor), float(original_seqlen or 0), float(low_turns),
                             float(high_turns), float(amplitude), device)
