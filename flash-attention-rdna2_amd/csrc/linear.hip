@@ -11,16 +11,31 @@
 
 namespace fa {
 
-// ws[sg + 1] holds what segment sg adds to the state; becomes the state before segment sg + 1 (and, where the call overwrites it, ws[0]
-// the one before the first). A thread carries four elements along; its loads of the next segments do not wait for the sum.
+// Segment sg's addition to the state stands where the state before segment sg + 1 is to be; that of the first is written where the call
+// overwrites it. A thread carries four elements along; its loads of the next segments do not wait for the sum.
 __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   const int n = p.da * p.db, nb = (n / 4 + 255) / 256;
-  const int bh = blockIdx.x / nb, b = bh / p.NH, h = bh % p.NH;
   const int e = 4 * ((blockIdx.x % nb) * 256 + threadIdx.x);
+  const int i = blockIdx.x / nb / p.NH, h = blockIdx.x / nb % p.NH;
+  int b = i;
+  if (p.cu) {
+    // item i: the one sequence of several segments that starts in rows [i seg, (i + 1) seg)
+    __shared__ int found;
+    if (threadIdx.x == 0) found = -1;
+    __syncthreads();
+    for (int j = threadIdx.x; j < p.batch; j += 256) {
+      const LaSeq sq = la_seq(p, j);
+      if (sq.row0 / p.seg == i && la_segments(p, sq.len) > 1) found = j;
+    }
+    __syncthreads();
+    b = found;
+    if (b < 0) return;
+  }
   const LaSeq sq = la_seq(p, b);
   if (e >= n || sq.slot < 0) return;
   const int nseg = la_segments(p, sq.len);
-  float* const ws = p.ws + (long long)bh * p.nseg * n + e;
+  const long long step = (long long)p.NH * n;
+  float* const ws = p.ws + (la_ws_row(p, b, sq) * p.NH + h) * n + e;
   f32x4 cur = {0.0f, 0.0f, 0.0f, 0.0f};
   if (p.first) cur = *(const f32x4*)(p.first + ((long long)sq.slot * p.NH + h) * n + e);
   const float d = la_decay(p, b, h);
@@ -29,13 +44,13 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   for (int s = 1; s < nseg; s += 4) {
     f32x4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = *(const f32x4*)(ws + (long long)min(s + j, nseg - 1) * n);
+    for (int j = 0; j < 4; j++) v[j] = *(const f32x4*)(ws + min(s + j, nseg - 1) * step);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const LaFade& fade = p.enter && s + j == 1 ? first : whole;
 #pragma unroll
-      for (int i = 0; i < 4; i++) cur[i] = fade(cur[i]) + v[j][i];
-      if (s + j < nseg) *(f32x4*)(ws + (long long)(s + j) * n) = cur;
+      for (int k = 0; k < 4; k++) cur[k] = fade(cur[k]) + v[j][k];
+      if (s + j < nseg) *(f32x4*)(ws + (s + j) * step) = cur;
     }
   }
 }
@@ -91,7 +106,11 @@ void la_split(LaArgs& a, const FableLinearParams& p, int dtype) {
   a.wa = p.DV, a.wb = 1;
 }
 
-long long la_ws(const LaArgs& a) { return a.nseg > 1 ? (long long)a.batch * a.NH * a.nseg * a.da * a.db * 4 : 0; }
+// the rows that la_ws_row() counts on
+long long la_ws(const LaArgs& a) {
+  const long long rows = a.cu ? 2 * (a.total / a.seg + 2) : (long long)a.batch * a.nseg;
+  return a.nseg > 1 ? rows * a.NH * a.da * a.db * 4 : 0;
+}
 
 LaArgs la_base(const FableLinearParams& p) {
   LaArgs a;
@@ -101,7 +120,7 @@ LaArgs la_base(const FableLinearParams& p) {
   a.cu = p.cu;
   a.total = p.total;
   a.batch = p.batch;
-  a.n = p.n;
+  a.n = p.cu && p.n > p.total ? (int)p.total : p.n;
   a.NH = p.NH;
   a.pscale = p.scale;
   a.hx = a.hy = a.hz = 1;
@@ -183,7 +202,8 @@ void la_go(LaArgs a, int dtype, bool state, bool exact, hipStream_t st) {
 void la_states(const LaArgs& a, int dtype, bool exact, hipStream_t st) {
   if (a.nseg < 2) return;
   la_go(a, dtype, true, exact, st);
-  hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)(a.batch * a.NH * ((a.da * a.db / 4 + 255) / 256))), dim3(256), 0, st, a);
+  const long long items = (a.cu ? a.total / a.seg + 1 : a.batch) * a.NH * ((a.da * a.db / 4 + 255) / 256);
+  hipLaunchKernelGGL(la_scan_kernel, dim3((unsigned)items), dim3(256), 0, st, a);
 }
 
 // What every call has to satisfy; the tensors' own checks follow in the entry points.

@@ -44,7 +44,7 @@ struct LaArgs {
   int sa, sb;                // strides of a state's element (a, b)
   const int32_t* slots;      // a sequence's state; NULL: its own number. Outside [0, nslots): no sequence
   int nslots;
-  float* ws;                 // [batch][NH][nseg], the states before the segments (nseg > 1) ...
+  float* ws;                 // the states before the segments (nseg > 1), [la_ws_row() + segment][NH] ...
   int wa, wb;                // ... and the strides of their elements
   const int32_t* cu;
   long long total;
@@ -220,6 +220,32 @@ __device__ __forceinline__ int la_segments(const LaArgs& p, int len) {
   const int k = (int)(((long long)len + p.seg - 1) / p.seg);
   return k < 1 ? 1 : k > p.nseg ? p.nseg : k;
 }
+// Where the states of a sequence's segments start in ws. A packed sequence of more than one segment ends at least one multiple of `seg` rows further
+// than it starts, so twice that count leaves room for its segments ahead of the next such sequence's.
+__device__ __forceinline__ long long la_ws_row(const LaArgs& p, int b, const LaSeq& sq) {
+  return p.cu ? 2 * (sq.row0 / p.seg) : (long long)b * p.nseg;
+}
+// (sequence, segment) of an item. Packed sequence b has its items from cu[b] / seg + b on, which leaves room for all its segments without
+// a grid of the longest sequence's count for each: the threads of a workgroup look for it side by side.
+__device__ __forceinline__ void la_item(const LaArgs& p, int i, int segs, int tid, int nt, int& b, int& sg) {
+  if (!p.cu || p.nseg == 1) {
+    b = i / segs;
+    sg = i % segs;
+    return;
+  }
+  int at = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += nt) {
+    const int j = b0 + tid;
+    at += __syncthreads_count(j < p.batch && min(max((long long)p.cu[j], 0LL), p.total) / p.seg + j <= i);
+  }
+  b = __builtin_amdgcn_readfirstlane(max(at - 1, 0));
+  sg = __builtin_amdgcn_readfirstlane(i - b - (int)(min(max((long long)p.cu[b], 0LL), p.total) / p.seg));
+}
+// how many items a launch has
+inline long long la_items(const LaArgs& p, bool state) {
+  if (p.nseg == 1) return p.batch;
+  return p.cu ? p.total / p.seg + p.batch : (long long)p.batch * (state ? p.nseg - 1 : p.nseg);
+}
 
 // Zeros in rows [lo, hi) of out for the item's columns.
 template <typename O>
@@ -286,15 +312,19 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 32, g = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int ndb = (p.db + DB - 1) / DB;
-  // items in the order (sequence, segment, head, column tile): what shares x and y, and neighbouring heads of the same
-  // rows, run side by side on one XCD
+  // Items in the order (sequence, segment, head, column tile). What shares rows (the tiles of a head, the heads of a group) runs on one XCD; such
+  // groups are dealt to the XCDs in turn, because neighbours may differ in length (in contiguous ranges a prompt of 32768 rows beside 255
+  // single tokens ran on one XCD: 1958 us, 675 dealt).
   const int segs = STATE ? p.nseg - 1 : p.nseg;
-  int w = xcd_remap(blockIdx.x, gridDim.x);
+  const int G = ndb * max(p.hx, max(p.hy, p.hz));
+  int w = blockIdx.x;
+  if (w < (int)(gridDim.x / G / 8) * 8 * G) w = ((w / 8) / G * 8 + w % 8) * G + (w / 8) % G;
   const int dbt = w % ndb;
   w /= ndb;
   const int h = w % p.NH;
-  w /= p.NH;
-  const int sg = w % segs, b = w / segs;
+  int b, sg;
+  la_item(p, w / p.NH, segs, tid, NT, b, sg);
+  if (sg < 0) return;
   const LaSeq sq = la_seq(p, b);
   const int nseg = la_segments(p, sq.len);
   const int col0 = dbt * DB + 32 * wave;                      // the wave's first column
@@ -333,10 +363,10 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
   if (!STATE) {
     const float* from = nullptr;
     int ra = p.sa, rb = p.sb;
-    if (p.nseg == 1 || (sg == 0 && !p.inplace)) {              // (one segment has no ws)
+    if (nseg == 1 || (sg == 0 && !p.inplace)) {                // (one segment has no ws)
       if (p.first) from = p.first + state;
     } else {
-      from = p.ws + (((long long)b * p.NH + h) * p.nseg + sg) * p.da * p.db;
+      from = p.ws + ((la_ws_row(p, b, sq) + sg) * p.NH + h) * p.da * p.db;
       ra = p.wa;
       rb = p.wb;
     }
@@ -636,7 +666,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
   int ra = p.sa, rb = p.sb;
   float f = 1.0f;
   if constexpr (STATE) {
-    to = p.ws + (((long long)b * p.NH + h) * p.nseg + sg + 1) * p.da * p.db;
+    to = p.ws + ((la_ws_row(p, b, sq) + sg + 1) * p.NH + h) * p.da * p.db;
     ra = p.db;
     rb = 1;
   } else if (tail && p.last) {
@@ -665,7 +695,7 @@ constexpr int kLaChunk = 32;   // rows of a chunk; segments are multiples of it
 
 template <typename T, typename O, int DA, int NW, int PIECES, bool STATE>
 inline void la_run(const LaArgs& p, hipStream_t st) {
-  const long long items = (long long)p.batch * (STATE ? p.nseg - 1 : p.nseg) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32));
+  const long long items = la_items(p, STATE) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32));
   hipLaunchKernelGGL((la_kernel<T, O, DA, NW, kLaChunk, PIECES, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, p);
 }
 

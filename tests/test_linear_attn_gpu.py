@@ -176,7 +176,7 @@ def test_segments(dtype, packed):
     _run(dtype, [1500, 1500] if not packed else [2000, 3, 900, 0], 2, 2, 64, 64, packed=packed, grad=True, carry=True, decay="slow", seed=6)
 
 
-@pytest.mark.parametrize("most", [1, 100, 5000])
+@pytest.mark.parametrize("most", [1, 100, 5000, 10 ** 9])
 def test_max_seqlen_only_sizes_the_launch(most):
     _run("bf16", [700, 90], 2, 1, 64, 64, grad=True, carry=True, seed=8, most=most)
 
@@ -377,3 +377,125 @@ def test_refusals():
     (g,) = torch.autograd.grad(fa.linear_attn_func(a, k.float(), v.float(), dec).sum(), a, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_many_short_sequences_and_a_long_one(dtype):
+    """More sequences than a workgroup has threads, most of one or two rows, a few of several segments, rows in front and behind."""
+    lens = [1] * 281 + [700] + [0, 2] * 20 + [513, 256, 257] + [1] * 30
+    _run(dtype, lens, 2, 1, 64, 64, front=3, tail=2, grad=True, carry=True, decay="slow", seed=12)
+
+
+def test_mixed_batch_of_a_pool():
+    """The same kind of batch over a pool in place, some of its entries naming no state."""
+    fa = _fa()
+    lens = [1] * 260 + [900, 0, 1, 600]
+    cu = _cu(lens)
+    q, k, v, g = _inputs("bf16", (cu[-1],), 2, 2, 64, 64, 1)
+    slots = torch.randperm(300, generator=g)[:len(lens)].tolist()
+    slots[5], slots[262] = -1, 300
+    pool, dec = torch.randn(300, 2, 64, 64, generator=g), _decay(2, "slow")
+    got = pool.cuda()
+    out = fa.linear_attn_with_state(q.cuda(), k.cuda(), v.cuda(), got, dec.cuda(), state_idx=_i32(slots), cu_seqlens=_i32(cu), max_seqlen=900).cpu()
+    want, tol = pool.double().clone(), torch.zeros(pool.shape, dtype=torch.float64)
+    for b, s in enumerate(slots):
+        rows = slice(cu[b], cu[b + 1])
+        if not 0 <= s < 300:
+            assert not out[rows].any()
+            continue
+        args = (q[rows].double(), k[rows].double(), v[rows].double(), dec.double(), 0.125)
+        eo, es = ref.one(*args, pool[s].double())
+        mo, ms = ref.one(*(x.abs() for x in args[:3]), *args[3:], pool[s].double().abs())
+        ref.check(out[rows], eo, ref.bound(eo, mo, torch.bfloat16, lens[b], 64), "out")
+        want[s], tol[s] = es, ref.state_bound(ms, torch.bfloat16, lens[b], 64)
+    ref.check(got, want, tol + 1e-300, "pool")
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_nothing_new_behind_old_rows(dtype):
+    """Padding by rows whose keys are zeros: the state is only what is left of the earlier rows, exact to its own size. An
+    exponent k d is off by two roundings, so is what it weighs, relatively."""
+    fa = _fa()
+    q, k, v, _ = _inputs(dtype, (1, 700), 4, 4, 64, 64, 5, "plus")
+    k[:, 400:] = 0
+    dec = torch.tensor([0.0, 0.003, 0.05, 0.2])
+    out, last = fa.linear_attn_func(q.cuda(), k.cuda(), v.cuda(), dec.cuda(), return_final_state=True)
+    wide = [x.double() for x in (q, k, v)]
+    eo, es = ref.batch(*wide, dec.double(), 0.125)
+    tol = ref.state_bound(es, DT[dtype], 700, 64) + 2.0 ** -22 * 700 * dec.double()[None, :, None, None] * es
+    ref.check(last, es, tol, "state")
+    more = ref.bound(eo, eo, DT[dtype], 700, 64) + 2.0 ** -22 * 700 * dec.double()[None, None, :, None] * eo
+    ref.check(out, eo, more, "out")
+    # and one by one
+    state = last.clone()
+    zero = torch.zeros(1, 8, 4, 64, device="cuda", dtype=DT[dtype])
+    fa.linear_attn_with_state(zero, zero, zero, state, dec.cuda())
+    assert torch.allclose(state.cpu().double(), last.cpu().double() * torch.exp(-8 * dec.double())[None, :, None, None], rtol=16 * 2.0 ** -24, atol=0)
+
+
+def test_rows_far_apart():
+    """Rows 8 MiB apart: offsets past 32 bits over the sequence, buffer descriptors of 64 rows, in both directions."""
+    fa = _fa()
+    big = torch.empty(600, 1 << 22, device="cuda", dtype=torch.bfloat16)
+    dense = [torch.randn(600, 1, 64, device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    far = []
+    for i, x in enumerate(dense):
+        view = big[:, 64 * i:64 * i + 64].unsqueeze(1)
+        view.copy_(x)
+        far.append(view)
+    dec = torch.tensor([0.01], device="cuda")
+    cu = _i32([0, 600])
+    assert torch.equal(fa.linear_attn_varlen_func(*far[:3], cu, 600, dec), fa.linear_attn_varlen_func(*dense[:3], cu, 600, dec))
+    for x, y in zip(fa._C.linear_bwd(far[3], *far[:3], dec, 0.125, cu, 600)[:3], fa._C.linear_bwd(dense[3], *dense[:3], dec, 0.125, cu, 600)[:3]):
+        assert torch.equal(x, y)
+    del big, far
+
+
+def test_empty_batches():
+    fa = _fa()
+    dec = torch.zeros(2, device="cuda")
+    mk = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.bfloat16)
+    out, last = fa.linear_attn_func(mk(0, 5, 2, 64), mk(0, 5, 2, 64), mk(0, 5, 2, 64), dec, return_final_state=True)
+    assert out.shape == (0, 5, 2, 64) and last.shape == (0, 2, 64, 64)
+    first = torch.randn(3, 2, 64, 64, device="cuda")
+    out, last = fa.linear_attn_func(mk(3, 0, 2, 64), mk(3, 0, 2, 64), mk(3, 0, 2, 64), dec, initial_state=first, return_final_state=True)
+    assert out.shape == (3, 0, 2, 64) and torch.equal(last, first)
+    out = fa.linear_attn_varlen_func(mk(4, 2, 64) + 1, mk(4, 2, 64) + 1, mk(4, 2, 64) + 1, _i32([0]), 0, dec)
+    assert out.shape == (4, 2, 64) and not out.any()
+    assert fa.linear_attn_with_state(mk(0, 1, 2, 64), mk(0, 1, 2, 64), mk(0, 1, 2, 64), first, dec).shape == (0, 1, 2, 64)
+
+
+def test_bad_lengths_stay_in_bounds():
+    """Offsets past the rows, or not in order, are not refused (they are on the GPU), but nothing outside the tensors is touched."""
+    fa = _fa()
+    big = torch.full((64, 2, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+    q, k, v = big[16:48].clone(), big[16:48].clone(), big[16:48].clone()
+    dec = torch.zeros(2, device="cuda")
+    for cu in ([0, 100], [-5, 10, 32], [20, 10, 32], [0, 40, 20, 90]):
+        for most in (4, 32):
+            assert fa.linear_attn_varlen_func(q, k, v, _i32(cu), most, dec).shape == q.shape
+            pool = torch.zeros(len(cu) - 1, 2, 64, 64, device="cuda")
+            fa.linear_attn_with_state(q, k, v, pool, dec, cu_seqlens=_i32(cu), max_seqlen=most)
+            fa.flash_attn_rotary_func(q, k, torch.ones(8, 32, device="cuda"), torch.zeros(8, 32, device="cuda"), cu_seqlens=_i32(cu))
+    torch.cuda.synchronize()
+
+
+def test_calls_of_a_known_signature():
+    """Later calls of a signature fill in addresses only: other tensors, tables and lengths, the same results as first calls."""
+    fa = _fa()
+    dec = _decay(4, "slopes").cuda()
+    for seed in range(3):
+        q, k, v, g = (x.cuda() if torch.is_tensor(x) else x for x in _inputs("bf16", (2, 300), 4, 2, 64, 64, seed))
+        first = torch.randn(2, 4, 64, 64, generator=g).cuda()
+        q.requires_grad_()
+        got = fa.linear_attn_func(q, k, v, dec, initial_state=first, return_final_state=True)
+        (dq,) = torch.autograd.grad(got[0], q, got[0].detach())
+        fresh, seg = fa._C.linear_fwd(q.detach(), k, v, dec, 0.125, None, 0, first, torch.empty_like(first))[:2]
+        assert torch.equal(got[0], fresh)
+        # (over the forward pass's states: with a final state wanted they have a part more than those the backward pass would form)
+        assert torch.equal(dq, fa._C.linear_bwd(got[0].detach(), q.detach(), k, v, dec, 0.125, None, 0, first, seg_states=seg)[0])
+        step, pool = [x[:, :1].detach().contiguous() for x in (q, k, v)], first.clone()
+        idx = _i32([seed % 2, 1 - seed % 2])
+        out = fa.linear_attn_with_state(*step, pool, dec, state_idx=idx)
+        other = first.clone()
+        assert torch.equal(out, fa._C.linear_step(*step, other, dec, 0.125, None, 1, idx)[0]) and torch.equal(pool, other)
