@@ -214,6 +214,8 @@ int la_check(const FableLinearParams& p, int dtype, const char* what) {
   if (p.batch < 0 || p.n < 0 || p.NH < 1 || p.gqa < 1 || p.NH % p.gqa || p.total < 0 || p.n > (1 << 30))
     return fail(FA_ERR_ARG, "%s: batch=%d n=%d NH=%d gqa=%d", what, p.batch, p.n, p.NH, p.gqa);
   // (64 workgroups of the scan for each state, within a grid's 2^32 threads)
+  if (((uintptr_t)p.state_in | (uintptr_t)p.state_out | (uintptr_t)p.dstate_out | (uintptr_t)p.dstate_in | (uintptr_t)p.seg_states) & 15)
+    return fail(FA_ERR_ARG, "%s: states must be 16-byte aligned", what);
   if ((long long)p.batch * p.NH > 65535) return fail(FA_ERR_ARG, "%s: batch x heads = %lld", what, (long long)p.batch * p.NH);
   return FA_OK;
 }
@@ -300,7 +302,6 @@ extern "C" int fable_linear_attn_step(FableLinearParams p, int dtype, void* stre
   int rc = la_check(p, dtype, what);
   if (rc != FA_OK) return rc;
   if (!p.decay || !p.state_in || !p.state_out) return fail(FA_ERR_ARG, "%s: null decay or state", what);
-  if (((uintptr_t)p.state_in | (uintptr_t)p.state_out) & 15) return fail(FA_ERR_ARG, "%s: states must be 16-byte aligned", what);
   if (p.slots && p.num_slots < 0) return fail(FA_ERR_ARG, "%s: num_slots=%d", what, p.num_slots);
   if ((rc = la_tensors(what, p, dtype, false)) != FA_OK) return rc;
   if (p.batch == 0) return FA_OK;

@@ -198,16 +198,17 @@ __device__ __forceinline__ const char* la_uniform(const char* at) {
 __device__ __forceinline__ unsigned la_uniform(unsigned n) { return __builtin_amdgcn_readfirstlane(n); }
 
 struct LaSeq {
-  long long row0;            // first row in the tensors
+  int row0;                  // first row in the tensors
   int len;
   int slot;                  // -1: no sequence
 };
+// cu[b], kept within the rows that there are
+__device__ __forceinline__ int la_row(const LaArgs& p, int b) { return (int)min((long long)max(p.cu[b], 0), p.total); }
 __device__ __forceinline__ LaSeq la_seq(const LaArgs& p, int b) {
   LaSeq s;
   if (p.cu) {
-    const long long lo = min(max((long long)p.cu[b], 0LL), p.total), hi = min(max((long long)p.cu[b + 1], lo), p.total);
-    s.row0 = lo;
-    s.len = (int)(hi - lo);
+    s.row0 = la_row(p, b);
+    s.len = max(la_row(p, b + 1), s.row0) - s.row0;
   } else {
     s.row0 = 0;
     s.len = p.n;
@@ -223,7 +224,7 @@ __device__ __forceinline__ int la_segments(const LaArgs& p, int len) {
 // Where the states of a sequence's segments start in ws. A packed sequence of more than one segment ends at least one multiple of `seg` rows further
 // than it starts, so twice that count leaves room for its segments ahead of the next such sequence's.
 __device__ __forceinline__ long long la_ws_row(const LaArgs& p, int b, const LaSeq& sq) {
-  return p.cu ? 2 * (sq.row0 / p.seg) : (long long)b * p.nseg;
+  return p.cu ? 2LL * (sq.row0 / p.seg) : (long long)b * p.nseg;
 }
 // (sequence, segment) of an item. Packed sequence b has its items from cu[b] / seg + b on, which leaves room for all its segments without
 // a grid of the longest sequence's count for each: the threads of a workgroup look for it side by side.
@@ -236,10 +237,10 @@ __device__ __forceinline__ void la_item(const LaArgs& p, int i, int segs, int ti
   int at = 0;
   for (int b0 = 0; b0 < p.batch; b0 += nt) {
     const int j = b0 + tid;
-    at += __syncthreads_count(j < p.batch && min(max((long long)p.cu[j], 0LL), p.total) / p.seg + j <= i);
+    at += __syncthreads_count(j < p.batch && la_row(p, j) / p.seg + j <= i);
   }
   b = __builtin_amdgcn_readfirstlane(max(at - 1, 0));
-  sg = __builtin_amdgcn_readfirstlane(i - b - (int)(min(max((long long)p.cu[b], 0LL), p.total) / p.seg));
+  sg = __builtin_amdgcn_readfirstlane(i - b - la_row(p, b) / p.seg);
 }
 // how many items a launch has
 inline long long la_items(const LaArgs& p, bool state) {
@@ -574,7 +575,10 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
         for (int i = 16 * part / parts; i < 16 * (part + 1) / parts; i++) {
           o[q][i] *= lw[q];
 #pragma unroll
-          for (int k = 0; k <= q; k++) sc[k][q][i] *= weight[32 * (q - k) - (8 * (i / 4) + i % 4)];
+          for (int k = 0; k <= q; k++) {
+            const float w = weight[32 * (q - k) - (8 * (i / 4) + i % 4)];
+            sc[k][q][i] = w == 0.0f ? 0.0f : sc[k][q][i] * w;  // (a masked score that is no number stays out)
+          }
         }
     };
     if constexpr (HALF) {
@@ -637,9 +641,10 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
           for (int k = 0; k <= q; k++)
 #pragma unroll
             for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(sc[k][q][i]));
-          if (__builtin_amdgcn_ballot_w64(m >= 32768.0f)) {     // past fp16's range: the wave's own power of two
-            float up;
-            down = la_norm(la_wave_max(m), up);
+          m = half_max(m);
+          if (__builtin_amdgcn_ballot_w64(m >= 32768.0f)) {     // past fp16's range: the query's own power of two
+            float up = 1.0f;
+            if (m >= 32768.0f) down = la_norm(m, up);
 #pragma unroll
             for (int i = 0; i < 16; i++) o[q][i] *= down;
 #pragma unroll

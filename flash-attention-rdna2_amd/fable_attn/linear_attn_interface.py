@@ -11,6 +11,7 @@ A head of queries holds a state S of headdim x headdim_v values. With l = exp(-d
 States and sums are kept in fp32. Head dims up to 256 each (values may be wider or narrower than keys; one that is no multiple of 8
 is zero-padded). decay is (nheads) or (batch, nheads), as the slopes that flash_attn_func takes for its biases:
 at least 0, 0 for no decay, infinity for a head that sees only the token itself; like those it gets no gradient.
+A value that is not finite makes every later output of its head so; one of v also the earlier ones of the 32 rows that are worked on together.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -124,7 +125,7 @@ class _LinearAttention(torch.autograd.Function):
             return None, None, None, None, None, None, None, None
         dout = q.new_zeros((*q.shape[:-1], v.shape[-1])) if dout is None else _rows(dout)
         dq, dk, dv, dstate = _backward(dout, q, k, v, decay, ctx.scale, cu, ctx.most, state,
-                                       dfinal.contiguous() if dfinal is not None else None, ctx.needs_input_grad[7], seg)
+                                       _aligned(dfinal, dense=True) if dfinal is not None else None, ctx.needs_input_grad[7], seg)
         return None, None, None, dq, dk, dv, None, dstate
 
 

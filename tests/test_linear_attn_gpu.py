@@ -499,3 +499,22 @@ def test_calls_of_a_known_signature():
         out = fa.linear_attn_with_state(*step, pool, dec, state_idx=idx)
         other = first.clone()
         assert torch.equal(out, fa._C.linear_step(*step, other, dec, 0.125, None, 1, idx)[0]) and torch.equal(pool, other)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_keys_and_queries_that_are_no_numbers(dtype, bad):
+    """A query reaches its own row only, a key its row and later ones, in another sequence nothing."""
+    fa = _fa()
+    q, k, v, _ = (x.cuda() if torch.is_tensor(x) else x for x in _inputs(dtype, (120,), 2, 2, 64, 64, 1))
+    dec, cu = torch.tensor([0.0, 0.01], device="cuda"), _i32([0, 70, 120])
+    want = fa.linear_attn_varlen_func(q, k, v, cu, 70, dec)
+    q2, k2 = q.clone(), k.clone()
+    q2[20, 0, 3] = bad
+    k2[40, 1, 5] = bad
+    out = fa.linear_attn_varlen_func(q2, k2, v, cu, 70, dec)
+    keep = torch.ones(120, 2, dtype=torch.bool, device="cuda")
+    keep[20, 0] = False
+    keep[40:70, 1] = False
+    assert torch.equal(out[keep], want[keep])
+    assert not torch.isfinite(out[20, 0]).any() and not torch.isfinite(out[40:70, 1]).any()
