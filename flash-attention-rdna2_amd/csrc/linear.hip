@@ -1,9 +1,10 @@
-// linear.hip — entry points of linear attention: argument checks, the split of long sequences into segments, the three
-// launches of the backward pass, and the kernels between them.
+// linear.hip — entry points of linear attention: argument checks, the split of long sequences into segments, the passes of
+// forward and backward, and the kernels between them.
 //
 // Segments. A workgroup per head and 128 columns leaves CUs idle where batch x heads is small, so long sequences are cut:
-// one launch forms what each segment adds to the state (reading y and z), la_scan_kernel turns these
-// into the state before each segment, and the main launch runs all segments side by side.
+// one launch forms what each segment adds to the state (reading y and z), la_scan_kernel turns these into the state before
+// each segment, and the main launch runs all segments side by side. The backward pass takes the forward pass's states
+// for dq; dv and dk share theirs.
 #include <string.h>
 
 #include "linear_kernel.hpp"
@@ -11,8 +12,9 @@
 
 namespace fa {
 
-// Segment sg's addition to the state stands where the state before segment sg + 1 is to be; that of the first is written where the call
-// overwrites it. A thread carries four elements along; its loads of the next segments do not wait for the sum.
+// Segment sg's addition to the state stands where the state before segment sg + 1 is to be; the state before the first is written
+// where the call overwrites it. A thread carries four elements along; its loads of the next four segments do not wait for
+// the sum (B2 S4096 H32 D128, 8 segments: 10 us, 64 MB).
 __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   const int n = p.da * p.db, nb = (n / 4 + 255) / 256;
   const int e = 4 * ((blockIdx.x % nb) * 256 + threadIdx.x);
@@ -211,12 +213,12 @@ int la_check(const FableLinearParams& p, int dtype, const char* what) {
   if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return fail(FA_ERR_DTYPE, "%s: unknown dtype %d", what, dtype);
   if (p.DK < 8 || p.DK > 256 || p.DK % 8 || p.DV < 8 || p.DV > 256 || p.DV % 8)
     return fail(FA_ERR_HEADDIM, "%s: head dims %d and %d: multiples of 8 up to 256", what, p.DK, p.DV);
-  if (p.batch < 0 || p.n < 0 || p.NH < 1 || p.gqa < 1 || p.NH % p.gqa || p.total < 0 || p.n > (1 << 30))
-    return fail(FA_ERR_ARG, "%s: batch=%d n=%d NH=%d gqa=%d", what, p.batch, p.n, p.NH, p.gqa);
-  // (64 workgroups of the scan for each state, within a grid's 2^32 threads)
+  if (p.batch < 0 || p.n < 0 || p.NH < 1 || p.gqa < 1 || p.NH % p.gqa || p.total < 0 || p.n > (1 << 30) || p.total > (1 << 30))
+    return fail(FA_ERR_ARG, "%s: batch=%d n=%d total=%lld NH=%d gqa=%d", what, p.batch, p.n, (long long)p.total, p.NH, p.gqa);
   if (((uintptr_t)p.state_in | (uintptr_t)p.state_out | (uintptr_t)p.dstate_out | (uintptr_t)p.dstate_in | (uintptr_t)p.seg_states) & 15)
     return fail(FA_ERR_ARG, "%s: states must be 16-byte aligned", what);
-  if ((long long)p.batch * p.NH > 65535) return fail(FA_ERR_ARG, "%s: batch x heads = %lld", what, (long long)p.batch * p.NH);
+  // (64 workgroups of 256 threads for each state in the scan; a grid has fewer than 2^32 threads)
+  if ((long long)p.batch * p.NH >= (1 << 18)) return fail(FA_ERR_ARG, "%s: batch x heads = %lld", what, (long long)p.batch * p.NH);
   return FA_OK;
 }
 
@@ -226,7 +228,7 @@ int la_tensor(const char* what, const char* name, const void* t, const fa_stride
   if (((uintptr_t)t | (uintptr_t)(s.b * e) | (uintptr_t)(s.h * e) | (uintptr_t)(s.s * e)) & 15)
     return fail(FA_ERR_ARG, "%s: %s: rows must be 16-byte aligned", what, name);
   // Offsets within 32 rows or more are 32 bits wide, and rows must not overlap: one of no token is known by its offset.
-  if (s.s >= (1LL << 29) / (e * kLaChunk) || ((p.cu ? p.total : p.n) > 1 && s.s < width))
+  if ((p.cu ? p.total : p.n) > 1 && (s.s >= (1LL << 29) / (e * kLaChunk) || s.s < width))
     return fail(FA_ERR_ARG, "%s: %s: a row stride of %lld values", what, name, (long long)s.s);
   return FA_OK;
 }

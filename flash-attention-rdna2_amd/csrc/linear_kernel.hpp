@@ -9,20 +9,29 @@
 //
 // A workgroup of NW waves takes a segment of one head of one sequence, a chunk of C rows at a time, and a tile of
 // 32 NW columns of z; a wave owns 32 of them. It keeps S (DA x 32 of its columns) in accumulators, in 32 bits, for the
-// whole segment, so a chunk reads its rows of x, y and z once and writes its rows of out once: the kernel is bound by those
-// bytes in 16 bits (some 100 kFLOP per row and head of 128 against 1 KB), by the matrix cores in fp32.
+// whole segment, so a chunk reads its rows of x, y and z once and writes its rows of out once: 1 KB per row and head of
+// 128 in 16 bits against some 100 kFLOP.
 //   Scores are formed transposed (y x^T), so that a lane holds all keys of one query: weighted and rounded, they are the
 // operand of the product with z as they are. S is DA x 32 with z's columns across the lanes, which is the operand
-// layout of the product with x. x is read from LDS once for both. out is formed transposed too: a lane holds 32 columns of one row.
+// layout of the product with x. x is read from LDS once for both. out is formed transposed too: a lane holds 32 columns
+// of one row.
 //   Roundings to 16 bits: the weighted scores and S once each as operands, as attention rounds its probabilities (each
-// is as large as the rounding of out itself); the weighted z of the state's update not at all: it is split into PIECES parts of
-// T that hold its 24 bits (bf16: 3, fp16: 2, fp32: itself), because S is a result in 32 bits and runs on over
-// the whole sequence. In fp16, whose range is small, S and the weighted z are brought to a power of two of
-// their own before, and scores too large for it likewise.
-//   The decay of S is put off: the accumulators hold S lambda^-lag, `lag` the rows since they were last brought up to date, and what a chunk adds is
-// weighted up by as much, until lambda^lag leaves 2^+-kLaLag. Each rounding of such a factor then touches what is about to be forgotten only, where one for each
-// chunk would add up over all that a slow decay remembers; and for all but fast decays that spares most of the DA / 2 multiplications
-// per lane and chunk (the kernel's time is its vector and matrix instructions together as much as its bytes).
+// is as large as the rounding of out itself). The weighted z of the state's update is split into PIECES parts of T, each
+// the rounding of what the ones before left: in bf16 three parts, which hold its 24 bits, where a state is a result or
+// runs into one, and two (16 bits) where only rounded outputs follow; in fp16 two (22 bits); in fp32 it is itself. In fp16,
+// whose range is small, S and the weighted z are brought to a power of two of their own before, and scores too large for
+// the type likewise.
+//   The decay of S is put off: the accumulators hold S lambda^-lag, `lag` the rows since they were last brought up to
+// date, and what a chunk adds is weighted up by as much, until lambda^lag leaves 2^+-kLaLag. Each rounding of such a factor
+// then touches what is about to be forgotten only, where one for each chunk would add up over all that a slow decay
+// remembers; and for all but fast decays that spares most of the DA / 2 multiplications per lane and chunk.
+//
+// Measured, bf16, heads of 128: B2 S4096 H32 (268 MB) 54 to 60 us, 4.5 to 5.0 TB/s, of the 5.2 that a large copy reaches
+// here; the states of its segments beside that 33 us. What bounds it is the bytes and, as much, the issue of vector and
+// matrix instructions, which are busy 80% of a CU's cycles together. Where a SIMD has one wave, the chain of a chunk's steps
+// does: 1.9 us per chunk, 60 ns per row. Not kept, because slower or no faster: three waves per SIMD (387 against 371 us forward
+// and backward: fewer loads of operands in flight), two chunks' tiles ahead in registers, two LDS buffers, the operands of
+// four steps read ahead, C = 64 (registers spill).
 #pragma once
 #include <type_traits>
 
@@ -79,10 +88,10 @@ struct La<float> {
   }
 };
 
-// LDS tiles, rows of LD values. Rows of x and y are read by 32 lanes at one column (8 bytes each) and y by columns, 4 rows x 32
-// columns at a time: a row is 7 units of 8 bytes longer than a multiple of the 64 banks (or of half of them), so the first meets every bank
-// once and the second nearly so; z is read by columns only and is 8 units longer. (fp32: one unit of 16 bytes.) Padding, not a turned
-// order within the row, because then all addresses are one register and constants.
+// LDS tiles, rows of LD values. Rows of x and y are read by 32 lanes at one column (8 bytes each) and y by columns, 4 rows
+// x 32 columns at a time: a row is 7 units of 8 bytes longer than a multiple of the 64 banks (or of half of them), so the
+// first meets every bank once and the second nearly so; z is read by columns only and is 8 units longer. (fp32: one unit of
+// 16 bytes.) Padding, not a turned order within the row, because then all addresses are one register and constants.
 template <typename T, int W>
 constexpr int kLaRow = W + (sizeof(T) == 2 ? 28 : 4);
 template <typename T, int W>
@@ -221,13 +230,14 @@ __device__ __forceinline__ int la_segments(const LaArgs& p, int len) {
   const int k = (int)(((long long)len + p.seg - 1) / p.seg);
   return k < 1 ? 1 : k > p.nseg ? p.nseg : k;
 }
-// Where the states of a sequence's segments start in ws. A packed sequence of more than one segment ends at least one multiple of `seg` rows further
-// than it starts, so twice that count leaves room for its segments ahead of the next such sequence's.
+// Where the states of a sequence's segments start in ws. A packed sequence of more than one segment ends at least one
+// multiple of `seg` rows further than it starts, so twice that count leaves room for its segments ahead of the next such
+// sequence's.
 __device__ __forceinline__ long long la_ws_row(const LaArgs& p, int b, const LaSeq& sq) {
   return p.cu ? 2LL * (sq.row0 / p.seg) : (long long)b * p.nseg;
 }
-// (sequence, segment) of an item. Packed sequence b has its items from cu[b] / seg + b on, which leaves room for all its segments without
-// a grid of the longest sequence's count for each: the threads of a workgroup look for it side by side.
+// (sequence, segment) of an item. Packed sequence b has its items from cu[b] / seg + b on, which leaves room for all its
+// segments without a grid of the longest sequence's count for each: the threads of a workgroup look for it side by side.
 __device__ __forceinline__ void la_item(const LaArgs& p, int i, int segs, int tid, int nt, int& b, int& sg) {
   if (!p.cu || p.nseg == 1) {
     b = i / segs;
@@ -248,11 +258,13 @@ inline long long la_items(const LaArgs& p, bool state) {
   return p.cu ? p.total / p.seg + p.batch : (long long)p.batch * (state ? p.nseg - 1 : p.nseg);
 }
 
-// Zeros in rows [lo, hi) of out for the item's columns.
+// Zeros in rows [lo, hi) of out for the item's columns (at most 512 bytes of a row), 32 threads to a row.
 template <typename O>
 __device__ __forceinline__ void la_zero_rows(const LaArgs& p, long long base, long long lo, long long hi, int c0, int nc, int tid, int nt) {
-  for (long long row = lo; row < hi; row++)
-    for (int c = tid; c < nc; c += nt) ((O*)p.o)[base + row * p.so.s + c0 + c] = (O)0.0f;
+  constexpr int E = 16 / sizeof(O);
+  const int c = E * (tid % 32);
+  if (c >= nc) return;
+  for (long long row = lo + tid / 32; row < hi; row += nt / 32) *(u32x4*)((O*)p.o + base + row * p.so.s + c0 + c) = u32x4{0, 0, 0, 0};
 }
 
 // An offset past every descriptor (those span 2^29 bytes at most), also with up to 2^30 added or taken off.
@@ -289,14 +301,12 @@ __device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, cons
   }
 }
 
-// Waves per SIMD that the registers are to allow (S takes DA / 2 of them); three at DA 128 were slower (B2 S4096 H32 bf16 forward and
-// backward 387 against 371 us): fewer loads of a chunk's operands are in flight.
+// Waves per SIMD that the registers are to allow; S takes DA / 2 of them.
 constexpr int la_waves(int DA) { return DA <= 128 ? 2 : 1; }
 
 template <typename T, typename O, int DA, int NW, int C, int PIECES, bool STATE>
 __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
   using F = typename La<T>::F;
-  using H = typename La<T>::H;
   constexpr int NT = NW * 64, DB = NW * 32, NB = C / 32, KT = DA / 32, E = 16 / sizeof(T);
   constexpr int CA = DA / E, CB = DB / E;                     // 16-byte chunks of a row
   constexpr int LA = C * CA / NT, LB = C * CB / NT;           // chunks per thread
@@ -313,9 +323,9 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 32, g = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int ndb = (p.db + DB - 1) / DB;
-  // Items in the order (sequence, segment, head, column tile). What shares rows (the tiles of a head, the heads of a group) runs on one XCD; such
-  // groups are dealt to the XCDs in turn, because neighbours may differ in length (in contiguous ranges a prompt of 32768 rows beside 255
-  // single tokens ran on one XCD: 1958 us, 675 dealt).
+  // Items in the order (sequence, segment, head, column tile). What shares rows (the tiles of a head, the heads of a
+  // group) runs on one XCD; such groups are dealt to the XCDs in turn, because neighbours may differ in length (in contiguous
+  // ranges a prompt of 32768 rows beside 255 single tokens ran on one XCD: 1958 us, 675 dealt).
   const int segs = STATE ? p.nseg - 1 : p.nseg;
   const int G = ndb * max(p.hx, max(p.hy, p.hz));
   int w = blockIdx.x;
@@ -391,10 +401,10 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     }
   }
 
-  // Tile loads. A thread's 16-byte column and its rows of the tile are fixed. Buffer descriptors span `span` rows of the segment, so that offsets
-  // within them are 32 bits wide and move by the same step from chunk to chunk. Rows behind the segment's last one fall outside
-  // (past the descriptor's end, or in reverse below its start: negative) and read as zeros or are not stored; columns past the head dim
-  // start from an offset so large that no row brings it back.
+  // Tile loads. A thread's 16-byte column and its rows of the tile are fixed. Buffer descriptors span `span` rows of the
+  // segment, so that offsets within them are 32 bits wide and move by the same step from chunk to chunk. Rows behind the
+  // segment's last one fall outside (past the descriptor's end, or in reverse below its start: negative) and read as zeros or
+  // are not stored; columns past the head dim start from an offset so large that no row brings it back.
   const int xr = tid / CA, xc = tid % CA, zr = tid / CB, zc = tid % CB;
   const int bx = (int)p.sx.s * (int)sizeof(T), by = (int)p.sy.s * (int)sizeof(T), bz = (int)p.sz.s * (int)sizeof(T), bo = (int)p.so.s * (int)sizeof(O);
   const char* const gx = (const char*)p.x + ((p.cu ? 0 : b * p.sx.b) + (h / p.hx) * p.sx.h + sq.row0 * p.sx.s) * (long long)sizeof(T);
@@ -483,8 +493,8 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
     fetch();
     __syncthreads();
 
-    // What follows alternates matrix and vector instructions that do not wait for one another: the scores and the product with S beside the
-    // splitting of z, the state's update beside the weighting of the scores.
+    // What follows alternates matrix and vector instructions that do not wait for one another: the scores and the product
+    // with S beside the splitting of z, the state's update beside the weighting of the scores.
     F zf[2 * NB], z[2 * NB][PIECES];
     f32x8 wu[2 * NB];
 #pragma unroll

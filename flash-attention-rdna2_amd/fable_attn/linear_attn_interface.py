@@ -11,7 +11,8 @@ A head of queries holds a state S of headdim x headdim_v values. With l = exp(-d
 States and sums are kept in fp32. Head dims up to 256 each (values may be wider or narrower than keys; one that is no multiple of 8
 is zero-padded). decay is (nheads) or (batch, nheads), as the slopes that flash_attn_func takes for its biases:
 at least 0, 0 for no decay, infinity for a head that sees only the token itself; like those it gets no gradient.
-A value that is not finite makes every later output of its head so; one of v also the earlier ones of the 32 rows that are worked on together.
+What is not finite in a row of k or v makes the outputs of its heads so from that row on, in a row of q that row's only; in v also the
+earlier ones of the 32 rows that are worked on together.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -198,6 +199,8 @@ def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu
     new request starts from a state that the caller has zeroed. Returns out as linear_attn_func. Up to 16 new tokens per sequence
     run token by token, each state read and written once; more run by chunks. Head dims are multiples of 8. No gradient passes through."""
     key, plans = None, _plans("linear_step_plans")
+    scale = None if scale is None else float(scale)
+    max_seqlen = None if max_seqlen is None else int(max_seqlen)
     try:
         key = (_place(q), _place(k), _place(v), _place(state), _sig(decay), _sig(state_idx), _sig(cu_seqlens), scale, max_seqlen)
         plan = plans.get(key)
@@ -221,7 +224,7 @@ def _with_state(key, plans, q, k, v, state, decay, state_idx, scale, cu_seqlens,
         raise NotImplementedError(f"fable_attn: states are updated in place for head dims that are multiples of 8, got {q.shape[-1]} and {v.shape[-1]}")
     dev = q.device
     cu = _as_index(cu_seqlens, dev) if packed else None
-    most = (q.shape[0] if max_seqlen is None else int(max_seqlen)) if packed else q.shape[1]
+    most = (q.shape[0] if max_seqlen is None else max_seqlen) if packed else q.shape[1]
     idx = _as_index(state_idx, dev) if state_idx is not None else None
     given = (q, k, v, decay, cu_seqlens, state_idx)
     q, k, v = _rows(q), _rows(k), _rows(v)

@@ -118,8 +118,8 @@ def flash_attn_rotary_tables(seqlen, rotary_dim, *, base=10000.0, factor=1.0, or
         raise ValueError(f"fable_attn: seqlen={seqlen}, start={start}: at least 0")
     if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > 8192:
         raise ValueError(f"fable_attn: rotary_dim={rotary_dim}: an even number of 2 to 8192")
-    if not base > 0 or not factor > 0:
-        raise ValueError(f"fable_attn: base={base}, factor={factor}: above 0")
+    if not 0 < base < float("inf") or not factor > 0:
+        raise ValueError(f"fable_attn: base={base}, factor={factor}: above 0, the base finite")
     if original_seqlen is not None and not (original_seqlen > 0 and high_turns > low_turns):
         raise ValueError(f"fable_attn: original_seqlen={original_seqlen}, low_turns={low_turns}, high_turns={high_turns}: "
                          "a length above 0, high_turns above low_turns")

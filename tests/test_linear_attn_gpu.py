@@ -518,3 +518,72 @@ def test_keys_and_queries_that_are_no_numbers(dtype, bad):
     keep[40:70, 1] = False
     assert torch.equal(out[keep], want[keep])
     assert not torch.isfinite(out[20, 0]).any() and not torch.isfinite(out[40:70, 1]).any()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_more_states_than_sixteen_bits_count(packed):
+    """2100 sequences x 32 heads: steps, and packed prompts with gradients, against the same in two halves."""
+    fa = _fa()
+    B, H, D = 2100, 32, 8
+    q, k, v, _ = _inputs("bf16", (3 * B,) if packed else (B, 1), H, H, D, D, 3)
+    q, k, v = (x.cuda() for x in (q, k, v))
+    dec = torch.linspace(0.0, 1.0, H, device="cuda")
+    if not packed:
+        pool = torch.randn(B, H, D, D, device="cuda")
+        halves = [pool[i:i + B // 2].clone() for i in (0, B // 2)]
+        out = fa.linear_attn_with_state(q, k, v, pool, dec)
+        parts = [fa.linear_attn_with_state(q[i:i + B // 2], k[i:i + B // 2], v[i:i + B // 2], s, dec) for i, s in zip((0, B // 2), halves)]
+        assert torch.equal(out, torch.cat(parts)) and torch.equal(pool, torch.cat(halves))
+        return
+    cu = torch.arange(0, 3 * B + 1, 3, dtype=torch.int32, device="cuda")
+    def run(a, b):
+        x = [t[3 * a:3 * b].detach().requires_grad_() for t in (q, k, v)]
+        out = fa.linear_attn_varlen_func(*x, cu[a:b + 1] - 3 * a, 3, dec)
+        out.float().square().sum().backward()
+        return [out] + [t.grad for t in x]
+    for whole, one, two in zip(run(0, B), run(0, B // 2), run(B // 2, B)):
+        assert torch.equal(whole, torch.cat([one, two]))
+
+
+def test_a_single_row_has_any_stride():
+    """A token per sequence out of a layout whose row stride is past what several rows may have."""
+    fa = _fa()
+    D = 64
+    base = torch.randn(2, 4, D, device="cuda", dtype=torch.bfloat16)
+    q = torch.as_strided(base, (2, 1, 4, D), (4 * D, 1 << 25, D, 1))
+    pool = torch.zeros(2, 4, D, D, device="cuda")
+    dec = torch.zeros(4, device="cuda")
+    out = fa.linear_attn_with_state(q, q, q, pool, dec)
+    want = fa.linear_attn_func(base[:, None], base[:, None], base[:, None], dec)
+    assert torch.equal(fa.linear_attn_func(q, q, q, dec), want)
+    # (two roundings on the way of the chunks, one on the steps')
+    ref = (base.double() * base.double()).sum(-1, keepdim=True) * D ** -0.5 * base.double()
+    assert torch.allclose(out[:, 0].double(), ref, rtol=2.0 ** -7, atol=0)
+
+
+def test_scale_and_lengths_given_as_tensors():
+    """A plan is known by their values, not by the objects."""
+    fa = _fa()
+    x = torch.randn(2, 1, 2, 32, device="cuda", dtype=torch.float32)
+    dec, scale = torch.zeros(2, device="cuda"), torch.tensor(0.5)
+    run = lambda s: fa.linear_attn_with_state(x, x, x, torch.zeros(2, 2, 32, 32, device="cuda"), dec, scale=s)
+    first = run(scale)
+    assert torch.equal(run(scale), first)
+    scale.fill_(0.25)
+    assert torch.equal(run(scale), run(0.25)) and torch.equal(2 * run(scale), first)
+    p = x[:, 0]
+    cu, most = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), torch.tensor(1)
+    assert torch.equal(fa.linear_attn_varlen_func(p, p, p, cu, most, dec, scale=0.5), fa.linear_attn_varlen_func(p, p, p, cu, 1, dec, scale=0.5))
+
+
+def test_long_gaps_are_zeroed():
+    fa = _fa()
+    q, k, v, _ = _inputs("fp16", (20011,), 2, 1, 40, 72, 5)
+    q, k, v = (x.cuda() for x in (q, k, v))
+    cu, dec = _i32([9000, 9010]), torch.zeros(2, device="cuda")
+    torch.full((20011, 2, 72), 7.0, device="cuda", dtype=torch.float16)   # (freed: what the outputs may be laid over)
+    for out in (fa.linear_attn_varlen_func(q, k, v, cu, 10, dec),
+                fa.linear_attn_with_state(q, k, v, torch.zeros(1, 2, 40, 72, device="cuda"), dec, cu_seqlens=cu, max_seqlen=10),
+                fa.linear_attn_with_state(q, k, v, torch.zeros(1, 2, 40, 72, device="cuda"), dec, cu_seqlens=cu, max_seqlen=100),
+                fa.linear_attn_with_state(q, k, v, torch.zeros(1, 2, 40, 72, device="cuda"), dec, _i32([-1]), cu_seqlens=cu, max_seqlen=10)):
+        assert not out[:9000].any() and not out[9010:].any()
