@@ -3,7 +3,7 @@
 
 namespace fa {
 template <>
-void la_launch<__bf16>(const LaArgs& p, bool state, bool exact, hipStream_t st) {
+void la_launch<__bf16>(const LaPasses& p, bool state, bool exact, hipStream_t st) {
   exact ? la_all<__bf16, 3>(p, state, st) : la_all<__bf16, 2>(p, state, st);
 }
 }  // namespace fa

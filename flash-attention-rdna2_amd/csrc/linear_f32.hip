@@ -3,7 +3,7 @@
 
 namespace fa {
 template <>
-void la_launch<float>(const LaArgs& p, bool state, bool, hipStream_t st) {
+void la_launch<float>(const LaPasses& p, bool state, bool, hipStream_t st) {
   la_all<float, 1>(p, state, st);
 }
 }  // namespace fa

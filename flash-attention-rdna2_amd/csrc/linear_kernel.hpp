@@ -68,6 +68,12 @@ struct LaArgs {
   int o32;                   // out is fp32 (partial gradients of shared heads)
 };
 
+// Passes of one launch over the same rows: the backward pass's three, that share the reading of theirs through the caches.
+struct LaPasses {
+  LaArgs p[3];
+  int n;
+};
+
 // A fragment: lane (r, g) = (l % 32, l / 32) holds the contraction indices 16 s + 4 g + {0..3} and 16 s + 8 + 4 g + {0..3} of
 // its row or column r, the rows of a 32 x 32 accumulator that its registers 8 (s % 2) .. + 7 hold.
 template <typename T>
@@ -305,7 +311,7 @@ __device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, cons
 constexpr int la_waves(int DA) { return DA <= 128 ? 2 : 1; }
 
 template <typename T, typename O, int DA, int NW, int C, int PIECES, bool STATE>
-__global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
+__global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
   using F = typename La<T>::F;
   constexpr int NT = NW * 64, DB = NW * 32, NB = C / 32, KT = DA / 32, E = 16 / sizeof(T);
   constexpr int CA = DA / E, CB = DB / E;                     // 16-byte chunks of a row
@@ -322,14 +328,18 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
 
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 32, g = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  const int ndb = (p.db + DB - 1) / DB;
-  // Items in the order (sequence, segment, head, column tile). What shares rows (the tiles of a head, the heads of a
-  // group) runs on one XCD; such groups are dealt to the XCDs in turn, because neighbours may differ in length (in contiguous
-  // ranges a prompt of 32768 rows beside 255 single tokens ran on one XCD: 1958 us, 675 dealt).
-  const int segs = STATE ? p.nseg - 1 : p.nseg;
-  const int G = ndb * max(p.hx, max(p.hy, p.hz));
+  // The argument, where it lies: one of its passes is picked by a scalar, which no copy of it in registers allows.
+  const LaPasses& all = *(const LaPasses*)(const __attribute__((address_space(4))) LaPasses*)__builtin_amdgcn_kernarg_segment_ptr();
+  const int ndb = (all.p[0].db + DB - 1) / DB;
+  // Items in the order (sequence, segment, head, column tile, pass). What shares rows (the passes and tiles of a head, the
+  // heads of a group) runs on one XCD; such groups are dealt to the XCDs in turn, because neighbours may differ in length (in
+  // contiguous ranges a prompt of 32768 rows beside 255 single tokens ran on one XCD: 1958 us, 675 dealt).
+  const int G = all.n * ndb * max(all.p[0].hx, max(all.p[0].hy, all.p[0].hz));
   int w = blockIdx.x;
   if (w < (int)(gridDim.x / G / 8) * 8 * G) w = ((w / 8) / G * 8 + w % 8) * G + (w / 8) % G;
+  const LaArgs& p = all.p[w % all.n];
+  w /= all.n;
+  const int segs = STATE ? p.nseg - 1 : p.nseg;
   const int dbt = w % ndb;
   w /= ndb;
   const int h = w % p.NH;
@@ -702,30 +712,40 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaArgs p) {
 // one new token or a few of each sequence (linear_step.hip)
 void la_step(const LaArgs& p, int dtype, hipStream_t stream);
 
-// the states that the segments add (`state`), or everything; exact: the states are results, or run into such
+// The states that the segments add (`state`), or everything; exact: the states are results, or run into such. The passes of a
+// launch have da, db and o32 in common, and all that makes their items.
 template <typename T>
-void la_launch(const LaArgs& p, bool state, bool exact, hipStream_t stream);
+void la_launch(const LaPasses& p, bool state, bool exact, hipStream_t stream);
 
 constexpr int kLaChunk = 32;   // rows of a chunk; segments are multiples of it
 
 template <typename T, typename O, int DA, int NW, int PIECES, bool STATE>
-inline void la_run(const LaArgs& p, hipStream_t st) {
-  const long long items = la_items(p, STATE) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32));
-  hipLaunchKernelGGL((la_kernel<T, O, DA, NW, kLaChunk, PIECES, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, p);
+inline void la_run(const LaPasses& a, hipStream_t st) {
+  const LaArgs& p = a.p[0];
+  const long long items = la_items(p, STATE) * p.NH * ((p.db + NW * 32 - 1) / (NW * 32)) * a.n;
+  hipLaunchKernelGGL((la_kernel<T, O, DA, NW, kLaChunk, PIECES, STATE>), dim3((unsigned)items), dim3(NW * 64), 0, st, a);
+}
+
+template <typename T, typename O, int NW, int PIECES, bool STATE>
+inline void la_depth(const LaPasses& a, hipStream_t st) {
+  const int da = a.p[0].da;
+  if (da <= 64) la_run<T, O, 64, NW, PIECES, STATE>(a, st);
+  else if (da <= 128) la_run<T, O, 128, NW, PIECES, STATE>(a, st);
+  else la_run<T, O, 256, NW, PIECES, STATE>(a, st);
 }
 
 template <typename T, typename O, int PIECES, bool STATE>
-inline void la_pick(const LaArgs& p, hipStream_t st) {
-  if (p.db <= 64) p.da <= 64 ? la_run<T, O, 64, 2, PIECES, STATE>(p, st) : p.da <= 128 ? la_run<T, O, 128, 2, PIECES, STATE>(p, st) : la_run<T, O, 256, 2, PIECES, STATE>(p, st);
-  else p.da <= 64 ? la_run<T, O, 64, 4, PIECES, STATE>(p, st) : p.da <= 128 ? la_run<T, O, 128, 4, PIECES, STATE>(p, st) : la_run<T, O, 256, 4, PIECES, STATE>(p, st);
+inline void la_pick(const LaPasses& a, hipStream_t st) {
+  if (a.p[0].db <= 64) la_depth<T, O, 2, PIECES, STATE>(a, st);
+  else la_depth<T, O, 4, PIECES, STATE>(a, st);
 }
 
 template <typename T, int PIECES>
-inline void la_all(const LaArgs& p, bool state, hipStream_t st) {
-  if (state) return la_pick<T, T, PIECES, true>(p, st);
+inline void la_all(const LaPasses& a, bool state, hipStream_t st) {
+  if (state) return la_pick<T, T, PIECES, true>(a, st);
   if constexpr (sizeof(T) == 2)
-    if (p.o32) return la_pick<T, float, PIECES, false>(p, st);
-  la_pick<T, T, PIECES, false>(p, st);
+    if (a.p[0].o32) return la_pick<T, float, PIECES, false>(a, st);
+  la_pick<T, T, PIECES, false>(a, st);
 }
 
 }  // namespace fa
