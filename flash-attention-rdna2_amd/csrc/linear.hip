@@ -101,13 +101,14 @@ void la_single(LaArgs& a) {
 // the longest sequence takes n of those; spread evenly over the 1024 SIMDs the rows of all heads take n * 1024 / (waves' rows) times
 // less. Below 1.8 that does not pay for a second reading of k and v and the states' traffic (8 prompts of up to 2048 rows, 32 heads
 // of 128, ratio 1.44: 131 us in one piece, 190 cut; 24 documents H16 D64, ratio 2.6: forward and backward 448 against 365). Two waves per
-// SIMD then, but no segment under `least` rows.
+// SIMD then, but no segment under `least` rows (fp32, B2 S1000 H16 of 64 and 128 wide, forward and backward: 64 rows 165 us,
+// 128 rows 153; 16 bits, heads of 256: 128 rows 93, 256 rows 71).
 void la_split(LaArgs& a, const FableLinearParams& p, int dtype) {
   la_single(a);
   const int D = p.DK > p.DV ? p.DK : p.DV;
   const long long rows = p.cu ? p.total : (long long)a.batch * a.n;
   const long long work = rows * a.NH * ((D + 31) / 32);
-  const long long least = dtype == FA_F32 ? 64 : 256;
+  const long long least = dtype == FA_F32 ? 128 : 256;
   long long seg = a.n;
   if ((long long)a.n * 10240 > 18 * work) seg = (work + 2047) / 2048;
   seg = seg < least ? least : seg;
