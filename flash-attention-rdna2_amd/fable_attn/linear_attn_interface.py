@@ -13,6 +13,8 @@ is zero-padded). decay is (nheads) or (batch, nheads), as the slopes that flash_
 at least 0, 0 for no decay, infinity for a head that sees only the token itself; like those it gets no gradient.
 What is not finite in a row of k or v makes the outputs of its heads so from that row on, in a row of q that row's only; in v also the
 earlier ones of the 32 rows that are worked on together.
+All calls capture into HIP graphs; a captured backward pass wants leaves that no eager graph still holds, because torch's own
+accumulation would run on that graph's stream.
 """
 import torch
 from torch.autograd.function import once_differentiable

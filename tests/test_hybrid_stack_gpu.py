@@ -122,3 +122,84 @@ def test_serving_goes_on_from_a_prompt():
         y = run(torch.stack([full[b][lens[b] + t] for b in range(2)]), [1, 1])
         assert near(y[0], want[0][lens[0] + t]) and near(y[1], want[1][lens[1] + t]), t
     assert not pool[[0, 2, 4]].any()
+
+
+def test_captured_training_pass():
+    """Rotation, linear attention of packed sequences and the gradients of both in one graph, on leaves that no other graph holds:
+    replays on new inputs give an eager pass's bits."""
+    fa = _fa()
+    g = torch.Generator().manual_seed(3)
+    n = 1500
+    make = lambda heads: torch.randn(n, heads, D, generator=g).to(torch.bfloat16)
+    new = lambda: [make(H), make(HK), make(HK), make(H)]
+    cos, sin = fa.flash_attn_rotary_tables(n, D)
+    cu, decay = torch.tensor([0, 1100, 1101, 1400], dtype=torch.int32, device="cuda"), DECAY.float().cuda()
+    *leaves, dout = (t.cuda() for t in new())
+    for t in leaves:
+        t.requires_grad_()
+
+    def step(leaves, dout):
+        q, k = fa.flash_attn_rotary_func(leaves[0], leaves[1], cos, sin, cu_seqlens=cu)
+        out = fa.linear_attn_varlen_func(q, k, leaves[2], cu, 1100, decay)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaves, dout)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step(leaves, dout)
+    for _ in range(4):
+        fresh = [t.cuda() for t in new()]
+        with torch.no_grad():
+            for x, y in zip((*leaves, dout), fresh):
+                x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in kept]
+        want = step([t.requires_grad_() for t in fresh[:3]], fresh[3])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_threads():
+    """Two threads, each on a stream of its own, train and step at once: plans are a thread's own."""
+    import threading
+    fa = _fa()
+    g = torch.Generator().manual_seed(4)
+    cos, sin = fa.flash_attn_rotary_tables(ROWS, D)
+    decay = DECAY.float().cuda()
+    data = [[torch.randn(2, 50, heads, D, generator=g).half().cuda() for heads in (H, HK, HK, H)] for _ in range(2)]
+
+    def work(t):
+        *leaves, dout = (x.clone() for x in data[t])
+        for x in leaves:
+            x.requires_grad_()
+        pool = torch.zeros(2, H, D, D, device="cuda")
+        res = []
+        for i in range(8):
+            q, k = fa.flash_attn_rotary_func(leaves[0], leaves[1], cos, sin, rotary_seqlens=i)
+            out = fa.linear_attn_func(q, k, leaves[2], decay)
+            res += [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+            q, k, v = (x.detach()[:, :1] for x in (q, k, leaves[2]))
+            res.append(fa.linear_attn_with_state(q, k, v, pool, decay))
+        return [*res, pool]
+
+    want = [work(t) for t in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(t):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[t] = work(t)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
