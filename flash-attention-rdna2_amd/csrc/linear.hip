@@ -102,7 +102,8 @@ void la_single(LaArgs& a) {
 // less. Below 1.8 that does not pay for a second reading of k and v and the states' traffic (8 prompts of up to 2048 rows, 32 heads
 // of 128, ratio 1.44: 131 us in one piece, 190 cut; 24 documents H16 D64, ratio 2.6: forward and backward 448 against 365). Two waves per
 // SIMD then, but no segment under `least` rows (fp32, B2 S1000 H16 of 64 and 128 wide, forward and backward: 64 rows 165 us,
-// 128 rows 153; 16 bits, heads of 256: 128 rows 93, 256 rows 71).
+// 128 rows 153; 16 bits, heads of 256: 128 rows 93, 256 rows 71). Packed sequences leave parts of segments at their ends: with them
+// counted the 24 documents take 295 us, 303 without, prompts of 8 such documents H16 D128 93 and 113.
 void la_split(LaArgs& a, const FableLinearParams& p, int dtype) {
   la_single(a);
   const int D = p.DK > p.DV ? p.DK : p.DV;
@@ -110,7 +111,12 @@ void la_split(LaArgs& a, const FableLinearParams& p, int dtype) {
   const long long work = rows * a.NH * ((D + 31) / 32);
   const long long least = dtype == FA_F32 ? 128 : 256;
   long long seg = a.n;
-  if ((long long)a.n * 10240 > 18 * work) seg = (work + 2047) / 2048;
+  long long waves = 2048;
+  if (p.cu) {                                                  // each packed sequence ends in a part of a segment, half of one on average
+    waves -= (long long)a.batch * a.NH * ((D + 31) / 32) / 2;
+    if (waves < 1024) waves = 1024;
+  }
+  if ((long long)a.n * 10240 > 18 * work) seg = (work + waves - 1) / waves;
   seg = seg < least ? least : seg;
   seg = (seg + kLaChunk - 1) / kLaChunk * kLaChunk;
   a.seg = (int)(seg < (1 << 30) ? seg : (1 << 30));
