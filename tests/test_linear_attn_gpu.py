@@ -587,3 +587,54 @@ def test_long_gaps_are_zeroed():
                 fa.linear_attn_with_state(q, k, v, torch.zeros(1, 2, 40, 72, device="cuda"), dec, cu_seqlens=cu, max_seqlen=100),
                 fa.linear_attn_with_state(q, k, v, torch.zeros(1, 2, 40, 72, device="cuda"), dec, _i32([-1]), cu_seqlens=cu, max_seqlen=10)):
         assert not out[:9000].any() and not out[9010:].any()
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_sweep(seed):
+    """Seeded calls over the whole range of what the fixed cases above list one by one."""
+    import random
+    r = random.Random(1000 + seed)
+    packed = r.random() < 0.6
+    B = r.choice([1, 2, 3, 7])
+    lens = [r.choice([0, 1, 2, 31, 32, 33, 64, 65, 127, 300, 700]) for _ in range(B)] if packed else [r.choice([1, 5, 32, 100, 257, 640])] * B
+    hk = r.choice([1, 2, 3])
+    hq = hk * r.choice([1, 1, 2, 4])
+    dk, dv = r.choice([8, 24, 64, 72, 128, 136, 256]), r.choice([8, 32, 40, 64, 96, 128, 200, 256])
+    _run(r.choice(ALL), lens, hq, hk, dk, dv, packed=packed, decay=r.choice(["slopes", "slow", "none", "mixed"]), carry=r.random() < 0.5,
+         want=r.random() < 0.5, grad=r.random() < 0.7, seed=seed, front=r.choice([0, 0, 3, 40]) if packed else 0,
+         tail=r.choice([0, 0, 5, 70]) if packed else 0, scale=r.choice([None, 1.0, -0.3]), most=r.choice([None, 1, 4096]) if packed else None,
+         per_batch=r.random() < 0.3)
+
+
+def test_gradients_of_some_inputs_only():
+    """One of q, k, v and the state asking for a gradient, a gradient of the final state alone, of broadcast heads and states: the
+    bits (or, summed by torch, the sums) of the call that asks for all."""
+    fa = _fa()
+    q, k, v, g = _inputs("bf16", (2, 90), 4, 2, 32, 64, 9)
+    dec = _decay(4, "slopes").cuda()
+    data = [q.cuda(), k.cuda(), v.cuda(), _rand(g, (2, 4, 32, 64), "fp32", "any").cuda()]
+    dout, dlast = _rand(g, (2, 90, 4, 64), "bf16", "any").cuda(), _rand(g, (2, 4, 32, 64), "fp32", "any").cuda()
+
+    def grads(which, outs):
+        x = [t.clone().requires_grad_(i in which) for i, t in enumerate(data)]
+        out, last = fa.linear_attn_func(*x[:3], dec, initial_state=x[3], return_final_state=True)
+        given = [(out, dout), (last, dlast)]
+        return torch.autograd.grad([given[i][0] for i in outs], [x[i] for i in which], [given[i][1] for i in outs], allow_unused=True)
+
+    for outs in ((0, 1), (0,), (1,)):
+        every = grads(range(4), outs)
+        # (v's is formed on the way to the state's, which keeps more bits where it is asked for)
+        for which in ([0], [1], [3], [2, 3], [0, 2, 3], [1, 3]):
+            for i, x in zip(which, grads(which, outs)):
+                assert torch.equal(x, every[i]), (outs, which, i)
+    # q does not reach the final state
+    assert not grads([0], (1,))[0].any()
+    # one state for all sequences, one head of k repeated by an expand
+    one = data[3][:1].clone().requires_grad_()
+    kk = data[1][:, :, :1].clone().requires_grad_()
+    out = fa.linear_attn_func(data[0], kk.expand(-1, -1, 2, -1), data[2], dec, initial_state=one.expand(2, -1, -1, -1))
+    dk, ds = torch.autograd.grad(out, [kk, one], dout)
+    x = [data[0], kk.detach().repeat(1, 1, 2, 1).requires_grad_(), data[2], one.detach().repeat(2, 1, 1, 1).requires_grad_()]
+    dk2, ds2 = torch.autograd.grad(fa.linear_attn_func(*x[:3], dec, initial_state=x[3]), [x[1], x[3]], dout)
+    # (torch sums the parts in the type: two terms, one rounding each side)
+    assert torch.equal(dk, dk2.sum(2, keepdim=True)) and torch.equal(ds, ds2.sum(0, keepdim=True))
