@@ -152,6 +152,30 @@ __device__ __forceinline__ float la_norm(float m, float& inv) {
   return __uint_as_float((uint32_t)(127 + k) << 23);
 }
 
+// The larger magnitude, as bits, of `top` (0 at first) and a fragment's values; what is no number is above all that are.
+template <typename F>
+__device__ __forceinline__ uint32_t la_top(uint32_t top, F f) {
+  if constexpr (sizeof(f[0]) == 2) {
+    typedef unsigned short U2 __attribute__((ext_vector_type(2)));
+    U2 t = bitcast<U2>(top);
+    const u32x4 w = bitcast<u32x4>(f);
+#pragma unroll
+    for (int j = 0; j < 4; j++) t = __builtin_elementwise_max(t, bitcast<U2>(w[j] & 0x7fff7fffu));
+    return bitcast<uint32_t>(t);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+    return top;
+  }
+}
+// the magnitude that la_top() came to, in the lane; the bits from which on it is no number
+template <typename T>
+__device__ __forceinline__ uint32_t la_top_bits(uint32_t top) {
+  return sizeof(T) == 2 ? max(top & 0xffffu, top >> 16) : top;
+}
+template <typename T>
+constexpr uint32_t kLaNone = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+
 constexpr float kLaLag = 8.0f;
 
 // Two values split into parts of T, each the rounding of what the ones before left.
@@ -516,12 +540,28 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
     const int behind = lag + n;
     const bool due = fabsf(dl2 * (float)behind) > kLaLag;
     float weigh = due ? 1.0f : exp2_fast(dl2 * (float)behind), undo = 1.0f;
+    // A value of z that is no number reaches the rows that see it, not those whose weight for it is 0: a wave that has one (rare)
+    // leaves it out of the product and sets those rows after.
+    bool none = false;
+    uint32_t top = 0;
+    if constexpr (HALF || !STATE) {
+#pragma unroll
+      for (int s = 0; s < 2 * NB; s++) top = la_top(top, zf[s]);
+      top = la_top_bits<T>(top);
+      none = __builtin_amdgcn_ballot_w64(top >= kLaNone<T>) != 0;
+    }
     if constexpr (HALF) {
-      float m = 0.0f;
+      float m = (float)bitcast<_Float16>((unsigned short)top);
+      if (none) {
+        m = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 2 * NB; s++)
+        for (int s = 0; s < 2 * NB; s++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf((float)zf[s][j]));
+          for (int j = 0; j < 8; j++) {
+            const float v = fabsf((float)zf[s][j]);
+            m = v < 1e30f ? fmaxf(m, v) : m;
+          }
+      }
       undo = p.uscale * weigh;
       float inv;
       weigh = la_norm(la_wave_max(m), inv);
@@ -674,6 +714,12 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
             down = up;
           }
         }
+        if (none) {
+#pragma unroll
+          for (int s = 0; s < 2 * NB; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) zf[s][j] = fabsf((float)zf[s][j]) < __builtin_inff() ? zf[s][j] : (T)0.0f;
+        }
 #pragma unroll
         for (int s = 0; s < 2 * (q + 1); s++) {
           F pf;
@@ -681,6 +727,13 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
           for (int j = 0; j < 8; j++) pf[j] = (T)sc[s / 2][q][8 * (s % 2) + j];
           o[q] = La<T>::mma(zf[s], pf, o[q]);
         }
+        if (none)
+          for (int j = 0; j <= 32 * q + r && j < n; j++) {
+            const T* const row = tz + j * LDZ + 32 * wave + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+              if (!(fabsf((float)row[8 * (i / 4) + i % 4]) < __builtin_inff())) o[q][i] = __builtin_nanf("");
+          }
         la_store<O>(ro, voo[q], o[q], down, g, p.db - col0);
         voo[q] += sign * C * bo;
       }

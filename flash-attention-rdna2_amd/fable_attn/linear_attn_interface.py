@@ -11,8 +11,8 @@ A head of queries holds a state S of headdim x headdim_v values. With l = exp(-d
 States and sums are kept in fp32. Head dims up to 256 each (values may be wider or narrower than keys; one that is no multiple of 8
 is zero-padded). decay is (nheads) or (batch, nheads), as the slopes that flash_attn_func takes for its biases:
 at least 0, 0 for no decay, infinity for a head that sees only the token itself; like those it gets no gradient.
-What is not finite in a row of k or v makes the outputs of its heads so from that row on, in a row of q that row's only; in v also the
-earlier ones of the 32 rows that are worked on together.
+What is no number (or infinite) in a row of k or v makes the outputs of its heads so (in v: of its column) from that row on, in a row
+of q that row's only; rows before it and other sequences keep their bits.
 All calls capture into HIP graphs; a captured backward pass wants leaves that no eager graph still holds, because torch's own
 accumulation would run on that graph's stream.
 """

@@ -461,8 +461,8 @@ int fable_attn_gather(FableGatherParams p, int dtype, void* stream);
  * States are fp32, [slot][NH][DK][DV]; sequence b has slot slots[b] (NULL: b). A slot outside [0, num_slots) names no sequence: its
  * rows of o become zeros, and no state is read or written. Two sequences of a call must not name one slot.
  * state_in (NULL: zeros) is S before the first row, state_out (may be NULL, may be state_in) the one behind the last.
- * Sums and states are kept in 32 bits. A value of v that is not finite reaches all of the 32 rows of o that are worked on together with its own,
- * one of q or k only rows that see it. All states are 16-byte aligned. */
+ * Sums and states are kept in 32 bits. A value that is not finite reaches only rows
+ * that see it. All states are 16-byte aligned. */
 typedef struct FableLinearParams {
   const void* q;
   const void* k;

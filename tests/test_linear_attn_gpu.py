@@ -638,3 +638,35 @@ def test_gradients_of_some_inputs_only():
     dk2, ds2 = torch.autograd.grad(fa.linear_attn_func(*x[:3], dec, initial_state=x[3]), [x[1], x[3]], dout)
     # (torch sums the parts in the type: two terms, one rounding each side)
     assert torch.equal(dk, dk2.sum(2, keepdim=True)) and torch.equal(ds, ds2.sum(0, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dk,dv,n", [(64, 64, 70), (128, 128, 70), (32, 256, 1500)])
+def test_values_that_are_no_numbers(dtype, bad, dk, dv, n):
+    """A value makes its column so from its row on; rows before it, other columns, heads and sequences keep their bits. In reverse
+    too: the gradient of v where dout has one. (The column is small, so that it sets no power of two for the others.)"""
+    fa = _fa()
+    q, k, v, g = _inputs(dtype, (n + 50,), 2, 2, dk, dv, 1)
+    dout = _rand(g, (n + 50, 2, dv), dtype, "any")
+    c, row = dv - 11, n - 27
+    v[..., c] *= 2.0 ** -6
+    dout[..., c] *= 2.0 ** -6
+    q, k, v, dout = (x.cuda() for x in (q, k, v, dout))
+    dec, cu = torch.tensor([0.0, 0.01], device="cuda"), _i32([0, n, n + 50])
+
+    def run(v, dout):
+        x = v.clone().requires_grad_()
+        out = fa.linear_attn_varlen_func(q, k, x, cu, n, dec)
+        return out.detach(), torch.autograd.grad(out, x, dout)[0]
+
+    want, wgrad = run(v, dout)
+    v2, d2 = v.clone(), dout.clone()
+    v2[row, 1, c] = d2[row, 1, c] = bad
+    out, grad = run(v2, d2)
+    hit = torch.zeros(n + 50, 2, dv, dtype=torch.bool, device="cuda")
+    hit[row:n, 1, c] = True
+    assert not torch.isfinite(out[hit]).any() and torch.equal(out[~hit], want[~hit])
+    hit = torch.zeros_like(hit)
+    hit[:row + 1, 1, c] = True
+    assert not torch.isfinite(grad[hit]).any() and torch.equal(grad[~hit], wgrad[~hit])
