@@ -18,6 +18,7 @@ accumulation would run on that graph's stream.
 """
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _C, _lib
 from .flash_attn_interface import (MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _kernel_width, _place, _plans, _remember, _sig,
@@ -189,6 +190,7 @@ def _step_fast(plan, q, k, v, state, decay, idx, cu):
         p.slots = idx.data_ptr()
     if cu is not None:
         p.cu = cu.data_ptr()
+    increment_version(state)                   # (a graph that holds the pool for its backward pass sees that it changed)
     _lib.check(_C._L.fable_linear_attn_step(p, dt, torch._C._cuda_getCurrentRawStream(dev)), "fable_linear_attn_step")
     return out
 
@@ -196,7 +198,7 @@ def _step_fast(plan, q, k, v, state, decay, idx, cu):
 def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu_seqlens=None, max_seqlen=None):
     """Serving: new tokens q, k, v (batch, seqlen_new, nheads, ...), or packed (total, nheads, ...) with cu_seqlens int32 (batch+1) and
     max_seqlen (default: total), go on from the states of a pool, float32 (num_states, nheads, d, dv), which are
-    updated in place. state_idx int32 (batch): the state of each sequence (default: its own number); an entry outside the pool names
+    updated in place (which autograd sees as it sees any change in place). state_idx int32 (batch): the state of each sequence (default: its own number); an entry outside the pool names
     no sequence (a padded batch): its rows of out are zeros and no state changes. Two sequences of one call must not name one state; a
     new request starts from a state that the caller has zeroed. Returns out as linear_attn_func. Up to 16 new tokens per sequence
     run token by token, each state read and written once; more run by chunks. Head dims are multiples of 8. No gradient passes through."""
@@ -231,8 +233,11 @@ def _with_state(key, plans, q, k, v, state, decay, state_idx, scale, cu_seqlens,
     given = (q, k, v, decay, cu_seqlens, state_idx)
     q, k, v = _rows(q), _rows(k), _rows(v)
     if most > STEP_ROWS:
-        return _forward(q, k, v, fp32, scale, cu, most, state, state, idx)[0]
+        out = _forward(q, k, v, fp32, scale, cu, most, state, state, idx)[0]
+        increment_version(state)
+        return out
     out, p, dt = _C.linear_step(q, k, v, state, fp32, scale, cu, most, idx)
+    increment_version(state)
     used = (q, k, v, fp32, cu, idx)
     if key is not None and p.batch and all(a is b for a, b in zip(given, used)):
         _remember(plans, key, (p, dt, dev.index, out.shape, out.stride()))   # nothing was converted: the next call may fill in its addresses
