@@ -15,12 +15,13 @@
 // operand of the product with z as they are. S is DA x 32 with z's columns across the lanes, which is the operand
 // layout of the product with x. x is read from LDS once for both. out is formed transposed too: a lane holds 32 columns
 // of one row.
-//   Roundings to 16 bits: the weighted scores and S once each as operands, as attention rounds its probabilities (each
-// is as large as the rounding of out itself). The weighted z of the state's update is split into PIECES parts of T, each
+//   Roundings to 16 bits: the weighted scores (bf16) and S once each as operands, as attention rounds its probabilities (each
+// is as large as the rounding of out itself). In fp16, where a score of 2^-24 may meet a value of 2^15 and their product is an ordinary
+// output (in the backward pass scores are products of dout and v), each weighted score and each z is two parts in bf16
+// instead, whose range is fp32's: 16 bits of the score, all of z. The weighted z of the state's update is split into PIECES parts of T, each
 // the rounding of what the ones before left: in bf16 three parts, which hold its 24 bits, where a state is a result or
 // runs into one, and two (16 bits) where only rounded outputs follow; in fp16 two (22 bits); in fp32 it is itself. In fp16,
-// whose range is small, S and the weighted z are brought to a power of two of their own before, and scores too large for
-// the type likewise.
+// whose range is small, S and the weighted z are brought to a power of two of their own before.
 //   The decay of S is put off: the accumulators hold S lambda^-lag, `lag` the rows since they were last brought up to
 // date, and what a chunk adds is weighted up by as much, until lambda^lag leaves 2^+-kLaLag. Each rounding of such a factor
 // then touches what is about to be forgotten only, where one for each chunk would add up over all that a slow decay
@@ -304,12 +305,12 @@ constexpr int kLaOut = (int)0xC0000000u;
 // where nothing is to be stored. No branch around a store: the waits for the loads ahead of it then need not
 // wait for the store as well.
 template <typename O>
-__device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, const f32x16& acc, float scale, int hh, int ncols) {
+__device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, const f32x16& acc, int hh, int ncols) {
   if constexpr (sizeof(O) == 4) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int c = 8 * j + 4 * hh;
-      const f32x4 v = {acc[4 * j] * scale, acc[4 * j + 1] * scale, acc[4 * j + 2] * scale, acc[4 * j + 3] * scale};
+      const f32x4 v = {acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]};
       __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(v), to, (c < ncols ? at : kLaOut) + 4 * c, 0, 0);
     }
   } else {
@@ -319,8 +320,8 @@ __device__ __forceinline__ void la_store(__amdgpu_buffer_rsrc_t to, int at, cons
       O4 x, y;
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        x[c] = (O)(acc[8 * j + c] * scale);
-        y[c] = (O)(acc[8 * j + 4 + c] * scale);
+        x[c] = (O)acc[8 * j + c];
+        y[c] = (O)acc[8 * j + 4 + c];
       }
       const u32x2 xd = bitcast<u32x2>(x), yd = bitcast<u32x2>(y);
       const auto r0 = __builtin_amdgcn_permlane32_swap(xd[0], yd[0], false, false);
@@ -511,7 +512,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
     for (int i = 0; i < 16; i++) none[i] = 0.0f;
     const auto ro = buf_rsrc32(p.o, 0u);
 #pragma unroll
-    for (int q = 0; q < NB; q++) la_store<O>(ro, kLaOut, none, 1.0f, g, 32);
+    for (int q = 0; q < NB; q++) la_store<O>(ro, kLaOut, none, g, 32);
   }
   for (int c = 0; c < nch; c++) {
     const int n = min(C, p1 - p0 - c * C);                    // rows of the chunk; zeros behind them
@@ -694,26 +695,6 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
       const auto ro = buf_rsrc32(fo, no);
 #pragma unroll
       for (int q = 0; q < NB; q++) {
-        float down = 1.0f;
-        if constexpr (HALF) {
-          float m = 0.0f;
-#pragma unroll
-          for (int k = 0; k <= q; k++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(sc[k][q][i]));
-          m = half_max(m);
-          if (__builtin_amdgcn_ballot_w64(m >= 32768.0f)) {     // past fp16's range: the query's own power of two
-            float up = 1.0f;
-            if (m >= 32768.0f) down = la_norm(m, up);
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[q][i] *= down;
-#pragma unroll
-            for (int k = 0; k <= q; k++)
-#pragma unroll
-              for (int i = 0; i < 16; i++) sc[k][q][i] *= down;
-            down = up;
-          }
-        }
         if (none) {
 #pragma unroll
           for (int s = 0; s < 2 * NB; s++)
@@ -722,10 +703,26 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
         }
 #pragma unroll
         for (int s = 0; s < 2 * (q + 1); s++) {
-          F pf;
+          if constexpr (HALF) {                                // two parts in bf16 of each: 16 bits of the score, in any range
+            using B = La<__bf16>;
+            typename B::F pf[2], vf[2];
+            u32x4 w = bitcast<u32x4>(zf[s]);
+            asm("" : "+v"(w));                                 // (else the conversions for the update stay in registers until here)
+            const F zs = bitcast<F>(w);
 #pragma unroll
-          for (int j = 0; j < 8; j++) pf[j] = (T)sc[s / 2][q][8 * (s % 2) + j];
-          o[q] = La<T>::mma(zf[s], pf, o[q]);
+            for (int j = 0; j < 8; j += 2) {
+              la_split2<__bf16, 2>(sc[s / 2][q][8 * (s % 2) + j], sc[s / 2][q][8 * (s % 2) + j + 1], pf, j);
+              la_split2<__bf16, 2>((float)zs[j], (float)zs[j + 1], vf, j);
+            }
+            o[q] = B::mma(vf[1], pf[0], o[q]);
+            o[q] = B::mma(vf[0], pf[1], o[q]);
+            o[q] = B::mma(vf[0], pf[0], o[q]);
+          } else {
+            F pf;
+#pragma unroll
+            for (int j = 0; j < 8; j++) pf[j] = (T)sc[s / 2][q][8 * (s % 2) + j];
+            o[q] = La<T>::mma(zf[s], pf, o[q]);
+          }
         }
         if (none)
           for (int j = 0; j <= 32 * q + r && j < n; j++) {
@@ -734,7 +731,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
             for (int i = 0; i < 16; i++)
               if (!(fabsf((float)row[8 * (i / 4) + i % 4]) < __builtin_inff())) o[q][i] = __builtin_nanf("");
           }
-        la_store<O>(ro, voo[q], o[q], down, g, p.db - col0);
+        la_store<O>(ro, voo[q], o[q], g, p.db - col0);
         voo[q] += sign * C * bo;
       }
     }

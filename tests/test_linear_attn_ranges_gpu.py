@@ -1,0 +1,74 @@
+"""Linear attention where values differ in size by more than a 16-bit type's range holds: small scores against large values, fast decays over rows
+that add nothing, columns and rows far apart in size.
+
+Bounds are those of linear_ref, whose terms are relative to each product's own size, and for fp16 2^-15 of that size: a weighted score
+and a weighted row of the state's update are taken as two parts of 8 bits each (2^-16 left over), and the product of both second parts
+(2^-8 of each factor) is left out. A weight l^n is off by its exponent's two roundings, 2^-23 of n d, relatively."""
+import pytest
+import torch
+
+from tests import linear_ref as ref
+from tests.linear_ref import DT
+
+pytestmark = pytest.mark.gpu
+ALL = ["bf16", "fp16", "fp32"]
+
+
+def _fa():
+    import fable_attn
+    return fable_attn
+
+
+def _bound(want, size, dtype, rows, dk, far=0.0):
+    more = (2.0 ** -15 if dtype == "fp16" else 0.0) + 2.0 ** -22 * far
+    return ref.bound(want, size, DT[dtype], rows, dk) + more * size
+
+
+def _against(dtype, q, k, v, dec, scale, state=None, dout=None, far=0.0, hk=None):
+    """(rows, heads, d) of one sequence, forward and with dout backward, against the definition."""
+    fa = _fa()
+    n, dk, dv = q.shape[0], q.shape[2], v.shape[2]
+    grad = dout is not None
+    wide = [x.double()[None].requires_grad_(grad) for x in (q, k, v)]
+    first = None if state is None else state.double()[None]
+    eo, es = ref.batch(*wide, dec.double(), scale, None, first)
+    mag = [x.detach().abs().requires_grad_(grad) for x in wide]
+    mo, ms = ref.batch(*mag, dec.double(), abs(scale), None, None if first is None else first.abs())
+    dev = [x.cuda()[None].requires_grad_(grad) for x in (q, k, v)]
+    out = fa.linear_attn_func(*dev, dec.cuda(), scale=scale, initial_state=None if state is None else state.cuda()[None])
+    worst = ref.check(out, eo.detach(), _bound(eo.detach(), mo.detach(), dtype, n, dk, far), "out")
+    if grad:
+        want = torch.autograd.grad(eo, wide, dout.double()[None])
+        size = torch.autograd.grad(mo, mag, dout.double().abs()[None])
+        got = torch.autograd.grad(out, dev, dout.cuda()[None])
+        for name, x, e, m in zip(("dq", "dk", "dv"), got, want, size):
+            worst = max(worst, ref.check(x, e, _bound(e, m, dtype, n, max(dk, dv), far), name))
+    else:
+        out, last = fa.linear_attn_func(*dev, dec.cuda(), scale=scale, initial_state=None if state is None else state.cuda()[None], return_final_state=True)
+        worst = max(worst, ref.check(out, eo, _bound(eo, mo, dtype, n, dk, far), "out with a state"))
+        worst = max(worst, ref.check(last, es, ref.state_bound(ms, DT[dtype], n, dk) + 2.0 ** -22 * far * ms, "state"))
+    print(f"[ranges]   worst {worst:.3f} of its bound", flush=True)
+
+
+def _of(g, rows, heads, d, size, dtype, plus=True):
+    x = torch.randn(rows, heads, d, generator=g)
+    return ((x.abs() + 2.0 ** -6 if plus else x) * size).to(DT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("scale,sv", [(2.0 ** -28, 2.0 ** 14), (2.0 ** -34, 2.0 ** 13), (2.0 ** -18, 1.0)])
+@pytest.mark.parametrize("n", [5, 80])
+def test_small_scores_against_large_values(dtype, scale, sv, n):
+    g = torch.Generator().manual_seed(1)
+    q, k, v = _of(g, n, 2, 64, 2.0, dtype), _of(g, n, 1, 64, 4.0, dtype), _of(g, n, 1, 64, sv, dtype)
+    _against(dtype, q, k, v, torch.tensor([0.0, 0.05]), scale, far=n * 0.05)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("sd,sv,sk,sq", [(1e-5, 1.0, 8.0, 1.0), (1e-6, 1.0, 8.0, 1.0), (1e-3, 1e-2, 10.0, 1.0), (1e-3, 1e-3, 30.0, 5.0)])
+@pytest.mark.parametrize("hk,plus", [(2, True), (2, False), (1, True)])
+def test_gradients_of_small_dout(dtype, sd, sv, sk, sq, hk, plus):
+    """The gradients' scores are products of dout and v."""
+    g = torch.Generator().manual_seed(2)
+    q, k, v = _of(g, 70, 2, 64, sq, dtype, plus), _of(g, 70, hk, 64, sk, dtype, plus), _of(g, 70, hk, 64, sv, dtype, plus)
+    _against(dtype, q, k, v, torch.tensor([0.003, 0.05]), 0.125, dout=_of(g, 70, 2, 64, sd, dtype, plus), far=70 * 0.05)
