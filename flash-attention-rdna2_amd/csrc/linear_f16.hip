@@ -3,7 +3,7 @@
 
 namespace fa {
 template <>
-void la_launch<_Float16>(const LaPasses& p, bool state, bool, hipStream_t st) {
-  la_all<_Float16, 2>(p, state, st);
+void la_launch<_Float16>(const LaPasses& p, bool state, bool exact, hipStream_t st) {
+  exact ? la_all<_Float16, 3>(p, state, st) : la_all<_Float16, 2>(p, state, st);
 }
 }  // namespace fa

@@ -15,13 +15,15 @@
 // operand of the product with z as they are. S is DA x 32 with z's columns across the lanes, which is the operand
 // layout of the product with x. x is read from LDS once for both. out is formed transposed too: a lane holds 32 columns
 // of one row.
-//   Roundings to 16 bits: the weighted scores (bf16) and S once each as operands, as attention rounds its probabilities (each
-// is as large as the rounding of out itself). In fp16, where a score of 2^-24 may meet a value of 2^15 and their product is an ordinary
-// output (in the backward pass scores are products of dout and v), each weighted score and each z is two parts in bf16
-// instead, whose range is fp32's: 16 bits of the score, all of z. The weighted z of the state's update is split into PIECES parts of T, each
+//   Roundings to 16 bits: the weighted scores and S once each as operands, as attention rounds its probabilities (each
+// is as large as the rounding of out itself). The weighted z of the state's update is split into PIECES parts, each
 // the rounding of what the ones before left: in bf16 three parts, which hold its 24 bits, where a state is a result or
-// runs into one, and two (16 bits) where only rounded outputs follow; in fp16 two (22 bits); in fp32 it is itself. In fp16,
-// whose range is small, S and the weighted z are brought to a power of two of their own before.
+// runs into one, and two (16 bits) where only rounded outputs follow; in fp32 it is itself.
+//   fp16 has too few exponents for what a chunk puts together: a score of 2^-24 may meet a value of 2^15 (in the backward pass scores
+// are products of dout and v), a row weighted by 2^-40 may be all that there is, columns may be 2^24 apart. There every operand
+// that carries a weight is taken in bf16, whose range is fp32's: the rows of y, weighted as they are put into LDS (once for all waves), in PIECES
+// parts, z in two (all of its 11 bits), a weighted score in two. Products of parts that the result does not resolve are left out: three a
+// product remain, five where a state is a result. S alone is an fp16 operand, brought to a power of two of its own before.
 //   The decay of S is put off: the accumulators hold S lambda^-lag, `lag` the rows since they were last brought up to
 // date, and what a chunk adds is weighted up by as much, until lambda^lag leaves 2^+-kLaLag. Each rounding of such a factor
 // then touches what is about to be forgotten only, where one for each chunk would add up over all that a slow decay
@@ -205,6 +207,17 @@ __device__ __forceinline__ void la_split2(float a, float b, F* parts, int j) {
   }
 }
 
+// Eight values of fp16 times w, in PARTS tiles `part` values apart of their parts in bf16.
+template <int PARTS, int part>
+__device__ __forceinline__ void la_put(__bf16* at, u32x4 v, float w) {
+  const f16x8 h = bitcast<f16x8>(v);
+  bf16x8 parts[PARTS];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) la_split2<__bf16, PARTS>((float)h[j] * w, (float)h[j + 1] * w, parts, j);
+#pragma unroll
+  for (int i = 0; i < PARTS; i++) *(bf16x8*)(at + i * part) = parts[i];
+}
+
 // A state carried over `rows` rows, S <- keep S + by S: keep 1 and by = lambda^rows - 1 where that is near 1 (the factor itself, rounded
 // to 32 bits, is off by up to 2^-25 in the same direction each time), else 0 and the factor.
 struct LaFade {
@@ -342,14 +355,20 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
   constexpr int CA = DA / E, CB = DB / E;                     // 16-byte chunks of a row
   constexpr int LA = C * CA / NT, LB = C * CB / NT;           // chunks per thread
   static_assert(NT % CA == 0 && C * CA % NT == 0 && NT % CB == 0 && C * CB % NT == 0, "tile loads");
+  // fp16: y with its rows weighted, in PIECES parts, and z, in two, lie beside x and y in tiles of their own
   constexpr bool HALF = __is_same(T, _Float16);
-  constexpr int LDA = kLaRow<T, DA>, LDZ = kLaRowZ<T, DB>;
-  __shared__ __align__(16) T lds[(STATE ? 0 : C * LDA) + C * LDA + C * LDZ];
+  using U = typename std::conditional<HALF, __bf16, T>::type;
+  using FU = typename La<U>::F;
+  constexpr int PZ = HALF ? 2 : PIECES;
+  constexpr int LDA = kLaRow<T, DA>, LDW = kLaRowZ<U, DA>, LDZ = kLaRowZ<U, DB>;
+  constexpr int NX = STATE ? 0 : C * LDA, NY = HALF && STATE ? 0 : C * LDA, NV = HALF ? C * LDW : 0, NZ = C * LDZ;
+  __shared__ __align__(16) T lds[NX + NY + PIECES * NV + (HALF ? 2 : 1) * NZ];
   __shared__ float pw[STATE ? 1 : C + 32];                    // pscale lambda^k at k + 31; zeros for k < 0
-  __shared__ __align__(16) float pu[C];                       // weights of the rows in the update
+  __shared__ __align__(16) float pu[HALF ? 4 : C];            // weights of the rows in the update
   T* const tx = lds;
-  T* const ty = lds + (STATE ? 0 : C * LDA);
-  T* const tz = ty + C * LDA;
+  T* const ty = lds + NX;
+  U* const tw = (U*)(ty + NY);
+  U* const tz = tw + PIECES * NV;
 
   const int tid = threadIdx.x, lane = tid % 64, r = lane % 32, g = lane / 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -396,7 +415,8 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
   const float* const weight = pw + 31 + r - 4 * g;
   if constexpr (!STATE)
     for (int i = tid; i < C + 32; i += NT) pw[i] = i < 31 ? 0.0f : p.pscale * la_pow(dl2, (float)(i - 31));
-  for (int i = tid; i < C; i += NT) pu[i] = (HALF ? 1.0f : p.uscale) * la_pow(dl2, (float)(C - 1 - i));
+  if constexpr (!HALF)
+    for (int i = tid; i < C; i += NT) pu[i] = p.uscale * la_pow(dl2, (float)(C - 1 - i));
 
   // byte offset of a state's element in the lane's column
   auto state_at = [&](int a, int ra, int rb) { return a < p.da && col0 + r < p.db ? 4 * (a * ra + (col0 + r) * rb) : kLaOut; };
@@ -490,7 +510,11 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
   };
   T* const px = tx + xr * LDA + xc * E;
   T* const py = ty + xr * LDA + xc * E;
-  T* const pz = tz + zr * LDZ + zc * E;
+  U* const py2 = tw + xr * LDW + xc * E;
+  U* const pz = tz + zr * LDZ + zc * E;
+  float wy[LA];                                               // fp16: the weights of the thread's rows of y
+#pragma unroll
+  for (int i = 0; i < LA; i++) wy[i] = HALF ? p.uscale * la_pow(dl2, (float)(C - 1 - xr - i * (NT / CA))) : 0.0f;
   auto put = [&](T* at, u32x4 v) {                            // rows of x and y are 8-byte aligned in 16 bits
     if constexpr (sizeof(T) == 2) {
       ((u32x2*)at)[0] = u32x2{v[0], v[1]};
@@ -516,61 +540,59 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
   }
   for (int c = 0; c < nch; c++) {
     const int n = min(C, p1 - p0 - c * C);                    // rows of the chunk; zeros behind them
+    // the decay that S is behind by, and whether it is made up for now
+    const int behind = lag + n;
+    const bool due = fabsf(dl2 * (float)behind) > kLaLag;
+    const float weigh = due ? 1.0f : exp2_fast(dl2 * (float)behind);
+    if constexpr (HALF)
+      if (n < C)
+#pragma unroll
+        for (int i = 0; i < LA; i++) wy[i] = p.uscale * la_pow(dl2, (float)max(n - 1 - xr - i * (NT / CA), 0));
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < LA; i++) {
       if constexpr (!STATE) put(px + i * (NT / CA) * LDA, vx[i]);
-      put(py + i * (NT / CA) * LDA, vy[i]);
+      if constexpr (!STATE || !HALF) put(py + i * (NT / CA) * LDA, vy[i]);
+      if constexpr (HALF) la_put<PIECES, NV>(py2 + i * (NT / CA) * LDW, vy[i], wy[i] * weigh);
     }
 #pragma unroll
-    for (int i = 0; i < LB; i++) *(u32x4*)(pz + i * (NT / CB) * LDZ) = vz[i];
-    if (n < C && tid < C) pu[tid] = (HALF ? 1.0f : p.uscale) * la_pow(dl2, (float)max(n - 1 - tid, 0));
+    for (int i = 0; i < LB; i++) {
+      if constexpr (HALF) la_put<2, NZ>(pz + i * (NT / CB) * LDZ, vz[i], 1.0f);
+      else *(u32x4*)(pz + i * (NT / CB) * LDZ) = vz[i];
+    }
+    if constexpr (!HALF)
+      if (n < C && tid < C) pu[tid] = p.uscale * la_pow(dl2, (float)max(n - 1 - tid, 0));
     fetch();
     __syncthreads();
 
     // What follows alternates matrix and vector instructions that do not wait for one another: the scores and the product
     // with S beside the splitting of z, the state's update beside the weighting of the scores.
-    F zf[2 * NB], z[2 * NB][PIECES];
+    FU zf[2 * NB], z[2 * NB][PZ];                              // fp16: z is its two parts, and zf the first
     f32x8 wu[2 * NB];
 #pragma unroll
     for (int s = 0; s < 2 * NB; s++) {
-      zf[s] = la_cols<T, LDZ>(tz, wave, s, lane);
-      wu[s] = la_rows<float, 0>(pu, 0, s, g);
+      zf[s] = la_cols<U, LDZ>(tz, wave, s, lane);
+      if constexpr (HALF) {
+        z[s][0] = zf[s];
+        z[s][1] = la_cols<U, LDZ>(tz + NZ, wave, s, lane);
+      } else {
+        wu[s] = la_rows<float, 0>(pu, 0, s, g);
+      }
     }
-    // the decay that S is behind by, and whether it is made up for now
-    const int behind = lag + n;
-    const bool due = fabsf(dl2 * (float)behind) > kLaLag;
-    float weigh = due ? 1.0f : exp2_fast(dl2 * (float)behind), undo = 1.0f;
     // A value of z that is no number reaches the rows that see it, not those whose weight for it is 0: a wave that has one (rare)
     // leaves it out of the product and sets those rows after.
     bool none = false;
-    uint32_t top = 0;
-    if constexpr (HALF || !STATE) {
+    if constexpr (!STATE) {
+      uint32_t top = 0;
 #pragma unroll
       for (int s = 0; s < 2 * NB; s++) top = la_top(top, zf[s]);
-      top = la_top_bits<T>(top);
-      none = __builtin_amdgcn_ballot_w64(top >= kLaNone<T>) != 0;
-    }
-    if constexpr (HALF) {
-      float m = (float)bitcast<_Float16>((unsigned short)top);
-      if (none) {
-        m = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 2 * NB; s++)
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float v = fabsf((float)zf[s][j]);
-            m = v < 1e30f ? fmaxf(m, v) : m;
-          }
-      }
-      undo = p.uscale * weigh;
-      float inv;
-      weigh = la_norm(la_wave_max(m), inv);
-      undo *= inv;
+      none = __builtin_amdgcn_ballot_w64(la_top_bits<U>(top) >= kLaNone<U>) != 0;
     }
     auto split = [&](int k) {                                  // the k-th of 8 NB pairs of weighted z
-      const int s = k / 4, j = 2 * (k % 4);
-      la_split2<T, PIECES>((float)zf[s][j] * (wu[s][j] * weigh), (float)zf[s][j + 1] * (wu[s][j + 1] * weigh), z[s], j);
+      if constexpr (!HALF) {
+        const int s = k / 4, j = 2 * (k % 4);
+        la_split2<T, PIECES>((float)zf[s][j] * (wu[s][j] * weigh), (float)zf[s][j + 1] * (wu[s][j + 1] * weigh), z[s], j);
+      }
     };
 
     f32x16 sc[NB][NB], o[NB];                                  // [key block][query block], transposed
@@ -642,41 +664,33 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
           }
         }
     };
-    if constexpr (HALF) {
+#pragma unroll
+    for (int s = 0; s < 2 * NB; s++) {
 #pragma unroll
       for (int t = 0; t < KT; t++) {
-        f32x16 u;
+        if constexpr (HALF) {
+          FU y[PIECES];
 #pragma unroll
-        for (int i = 0; i < 16; i++) u[i] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < 2 * NB; s++) {
-          const F yt = la_cols<T, LDA>(ty, t, s, lane);
-#pragma unroll
-          for (int i = PIECES - 1; i >= 0; i--) u = La<T>::mma(yt, z[s][i], u);
-          if constexpr (STATE)
-            if (t == 0 && s + 1 < 2 * NB)
-#pragma unroll
-              for (int k = 0; k < 4; k++) split(4 * (s + 1) + k);
-        }
-        if constexpr (!STATE) weighted(t, KT);
-#pragma unroll
-        for (int i = 0; i < 16; i++) S[t][i] = fmaf(u[i], undo, S[t][i]);
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 2 * NB; s++) {
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
+          for (int i = 0; i < PIECES; i++) y[i] = la_cols<U, LDW>(tw + i * NV, t, s, lane);
+          // from the smallest on; left out are 2^-16 of the product for two parts of y, 2^-24 for three
+          if constexpr (PIECES == 3) {
+            S[t] = La<U>::mma(y[2], z[s][0], S[t]);
+            S[t] = La<U>::mma(y[1], z[s][1], S[t]);
+          }
+          S[t] = La<U>::mma(y[1], z[s][0], S[t]);
+          S[t] = La<U>::mma(y[0], z[s][1], S[t]);
+          S[t] = La<U>::mma(y[0], z[s][0], S[t]);
+        } else {
           const F yt = la_cols<T, LDA>(ty, t, s, lane);
 #pragma unroll
           for (int i = PIECES - 1; i >= 0; i--) S[t] = La<T>::mma(yt, z[s][i], S[t]);
-          if constexpr (STATE) {
-            if (s + 1 < 2 * NB)
+        }
+        if constexpr (STATE) {
+          if (s + 1 < 2 * NB)
 #pragma unroll
-              for (int k = 4 * t / KT; k < 4 * (t + 1) / KT; k++) split(4 * (s + 1) + k);
-          } else {
-            weighted(s * KT + t, 2 * NB * KT);
-          }
+            for (int k = 4 * t / KT; k < 4 * (t + 1) / KT; k++) split(4 * (s + 1) + k);
+        } else {
+          weighted(s * KT + t, 2 * NB * KT);
         }
       }
     }
@@ -699,24 +713,21 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
 #pragma unroll
           for (int s = 0; s < 2 * NB; s++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) zf[s][j] = fabsf((float)zf[s][j]) < __builtin_inff() ? zf[s][j] : (T)0.0f;
+            for (int j = 0; j < 8; j++) {
+              const bool ok = fabsf((float)zf[s][j]) < __builtin_inff();
+              zf[s][j] = ok ? zf[s][j] : (U)0.0f;
+              if constexpr (HALF) z[s][1][j] = ok ? z[s][1][j] : (U)0.0f;
+            }
         }
 #pragma unroll
         for (int s = 0; s < 2 * (q + 1); s++) {
-          if constexpr (HALF) {                                // two parts in bf16 of each: 16 bits of the score, in any range
-            using B = La<__bf16>;
-            typename B::F pf[2], vf[2];
-            u32x4 w = bitcast<u32x4>(zf[s]);
-            asm("" : "+v"(w));                                 // (else the conversions for the update stay in registers until here)
-            const F zs = bitcast<F>(w);
+          if constexpr (HALF) {                                // 16 bits of the score, in any range
+            FU pf[2];
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              la_split2<__bf16, 2>(sc[s / 2][q][8 * (s % 2) + j], sc[s / 2][q][8 * (s % 2) + j + 1], pf, j);
-              la_split2<__bf16, 2>((float)zs[j], (float)zs[j + 1], vf, j);
-            }
-            o[q] = B::mma(vf[1], pf[0], o[q]);
-            o[q] = B::mma(vf[0], pf[1], o[q]);
-            o[q] = B::mma(vf[0], pf[0], o[q]);
+            for (int j = 0; j < 8; j += 2) la_split2<U, 2>(sc[s / 2][q][8 * (s % 2) + j], sc[s / 2][q][8 * (s % 2) + j + 1], pf, j);
+            o[q] = La<U>::mma(z[s][1], pf[0], o[q]);
+            o[q] = La<U>::mma(zf[s], pf[1], o[q]);
+            o[q] = La<U>::mma(zf[s], pf[0], o[q]);
           } else {
             F pf;
 #pragma unroll
@@ -726,7 +737,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
         }
         if (none)
           for (int j = 0; j <= 32 * q + r && j < n; j++) {
-            const T* const row = tz + j * LDZ + 32 * wave + 4 * g;
+            const U* const row = tz + j * LDZ + 32 * wave + 4 * g;
 #pragma unroll
             for (int i = 0; i < 16; i++)
               if (!(fabsf((float)row[8 * (i / 4) + i % 4]) < __builtin_inff())) o[q][i] = __builtin_nanf("");

@@ -72,3 +72,31 @@ def test_gradients_of_small_dout(dtype, sd, sv, sk, sq, hk, plus):
     g = torch.Generator().manual_seed(2)
     q, k, v = _of(g, 70, 2, 64, sq, dtype, plus), _of(g, 70, hk, 64, sk, dtype, plus), _of(g, 70, hk, 64, sv, dtype, plus)
     _against(dtype, q, k, v, torch.tensor([0.003, 0.05]), 0.125, dout=_of(g, 70, 2, 64, sd, dtype, plus), far=70 * 0.05)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n", [32, 72])
+@pytest.mark.parametrize("zero", ["keys", "values"])
+def test_old_rows_of_fast_heads(dtype, n, zero):
+    """Rows 0, 32 and 64 alone add something; what the rows behind them leave of it is exact to its own size, however little."""
+    for decays in ([0.2, 0.35], [0.5, 0.7], [0.84, 2.0]):
+        g = torch.Generator().manual_seed(3)
+        q, k, v = _of(g, n, 2, 64, 4.0, dtype), _of(g, n, 2, 64, 4.0, dtype), _of(g, n, 2, 64, 100.0, dtype)
+        for row in range(n):
+            if row % 32:
+                (k if zero == "keys" else v)[row] = 0
+        _against(dtype, q, k, v, torch.tensor(decays), 0.125, far=n * max(decays))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("d", [0.0, 0.5])
+def test_columns_and_rows_far_apart_in_size(dtype, d):
+    """Columns of v 2^24 apart in one state; elements of q, k and v from 2^-6 to 2^6 each, and whole rows from 2^-4 to 2^4."""
+    g = torch.Generator().manual_seed(4)
+    dec = torch.tensor([d, d])
+    q, k, v = _of(g, 100, 2, 64, 1.0, dtype), _of(g, 100, 2, 64, 1.0, dtype), _of(g, 100, 2, 64, 1.0, dtype)
+    wide = v * torch.exp2(12.0 - 2.0 * (torch.arange(64) % 13)).to(v.dtype)
+    _against(dtype, q, k, wide, dec, 2.0 ** -10, far=100 * d)
+    mixed = [x * torch.exp2(torch.randint(-6, 7, x.shape, generator=g).float() + torch.randint(-4, 5, x.shape[:1], generator=g).float()[:, None, None]).to(x.dtype)
+             for x in (q, k, v)]
+    _against(dtype, *mixed, dec, 2.0 ** -22, far=100 * d)
