@@ -23,7 +23,8 @@
 // are products of dout and v), a row weighted by 2^-40 may be all that there is, columns may be 2^24 apart. There every operand
 // that carries a weight is taken in bf16, whose range is fp32's: the rows of y, weighted as they are put into LDS (once for all waves), in PIECES
 // parts, z in two (all of its 11 bits), a weighted score in two. Products of parts that the result does not resolve are left out: three a
-// product remain, five where a state is a result. S alone is an fp16 operand, brought to a power of two of its own before.
+// product remain, five where a state is a result. S alone is an fp16 operand, each of its columns brought to a power of two of its own
+// before: what is under 2^-27 of the column's largest value loses bits there (2^-38 of that value is the most it is off by).
 //   The decay of S is put off: the accumulators hold S lambda^-lag, `lag` the rows since they were last brought up to
 // date, and what a chunk adds is weighted up by as much, until lambda^lag leaves 2^+-kLaLag. Each rounding of such a factor
 // then touches what is about to be forgotten only, where one for each chunk would add up over all that a slow decay
@@ -131,20 +132,6 @@ __device__ __forceinline__ typename La<T>::F la_cols(const T* tile, int ct, int 
     for (int j = 0; j < 8; j++) f[j] = at[(8 * (j / 4) + j % 4) * LD];
     return f;
   }
-}
-
-// The largest of a wave's values, in a scalar register: within rows of 16 lanes by DPP, across rows by swaps.
-__device__ __forceinline__ float la_wave_max(float x) {
-  auto dpp = [](float v, auto ctrl) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
-  };
-  x = fmaxf(x, dpp(x, std::integral_constant<int, 0xb1>{}));    // quad_perm 1 0 3 2
-  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x4e>{}));    // quad_perm 2 3 0 1
-  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x141>{}));   // row_half_mirror
-  x = fmaxf(x, dpp(x, std::integral_constant<int, 0x140>{}));   // row_mirror
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 
 // The power of two that brings a largest magnitude m into [2^13, 2^14), its inverse in `inv`; 1 for zero, and for what is no number.
@@ -365,6 +352,7 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
   __shared__ __align__(16) T lds[NX + NY + PIECES * NV + (HALF ? 2 : 1) * NZ];
   __shared__ float pw[STATE ? 1 : C + 32];                    // pscale lambda^k at k + 31; zeros for k < 0
   __shared__ __align__(16) float pu[HALF ? 4 : C];            // weights of the rows in the update
+  __shared__ __align__(16) float pn[HALF && !STATE ? DB : 4]; // fp16: what undoes the powers of two of S's columns
   T* const tx = lds;
   T* const ty = lds + NX;
   U* const tw = (U*)(ty + NY);
@@ -596,7 +584,8 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
     };
 
     f32x16 sc[NB][NB], o[NB];                                  // [key block][query block], transposed
-    float norm = 1.0f, inv = 1.0f;
+    float norm = 1.0f;
+    f32x4 undo[4];                                             // for the lane's rows of o
     if constexpr (!STATE) {
 #pragma unroll
       for (int q = 0; q < NB; q++) {
@@ -613,7 +602,12 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
         for (int t = 0; t < KT; t++)
 #pragma unroll
           for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(S[t][i]));
-        norm = la_norm(la_wave_max(m), inv);
+        float inv;
+        norm = la_norm(half_max(m), inv);
+        pn[32 * wave + r] = inv;
+        __builtin_amdgcn_wave_barrier();                       // (a wave's own LDS accesses are in order)
+#pragma unroll
+        for (int i = 0; i < 4; i++) undo[i] = *(const f32x4*)(pn + 32 * wave + 8 * i + 4 * g);
       }
 #pragma unroll
       for (int s = 0; s < DA / 16; s++) {
@@ -650,13 +644,13 @@ __global__ __launch_bounds__(NW * 64, la_waves(DA)) void la_kernel(LaPasses) {
     float lw[NB];
     if constexpr (!STATE)
 #pragma unroll
-      for (int q = 0; q < NB; q++) lw[q] = p.iscale * inv * exp2_fast(-dl2 * (float)(32 * q + r + 1 + lag));
+      for (int q = 0; q < NB; q++) lw[q] = p.iscale * exp2_fast(-dl2 * (float)(32 * q + r + 1 + lag));
     auto weighted = [&](int part, int parts) {
 #pragma unroll
       for (int q = 0; q < NB; q++)
 #pragma unroll
         for (int i = 16 * part / parts; i < 16 * (part + 1) / parts; i++) {
-          o[q][i] *= lw[q];
+          o[q][i] *= HALF ? lw[q] * undo[i / 4][i % 4] : lw[q];
 #pragma unroll
           for (int k = 0; k <= q; k++) {
             const float w = weight[32 * (q - k) - (8 * (i / 4) + i % 4)];

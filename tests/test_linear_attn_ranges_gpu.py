@@ -100,3 +100,31 @@ def test_columns_and_rows_far_apart_in_size(dtype, d):
     mixed = [x * torch.exp2(torch.randint(-6, 7, x.shape, generator=g).float() + torch.randint(-4, 5, x.shape[:1], generator=g).float()[:, None, None]).to(x.dtype)
              for x in (q, k, v)]
     _against(dtype, *mixed, dec, 2.0 ** -22, far=100 * d)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_states_columns_far_apart(dtype):
+    """An initial state whose columns are 2^31 apart, read one element at a time."""
+    g = torch.Generator().manual_seed(5)
+    state = (1 + 0.9 * torch.rand(2, 64, 64, generator=g)) * torch.where(torch.arange(64) % 2 == 0, 2.0 ** 23, 2.0 ** -8)
+    q = torch.eye(64)[:, None].repeat(1, 2, 1).to(DT[dtype])
+    zero = torch.zeros(64, 2, 64, dtype=DT[dtype])
+    _against(dtype, q, zero, zero, torch.zeros(2), 2.0 ** -8, state=state)
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_an_infinite_column_of_a_state(dtype):
+    """It makes its own column of the outputs infinite, or no number; the others, past fp16's range as they are, stay what they were."""
+    fa = _fa()
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (_of(g, 40, 2, 64, 1.0, dtype) for _ in range(3))
+    state = torch.rand(1, 2, 64, 64, generator=g) * 2.0 ** 18
+    dec = torch.tensor([0.0, 0.1], device="cuda")
+    run = lambda s: fa.linear_attn_func(q.cuda()[None], k.cuda()[None], v.cuda()[None], dec, scale=2.0 ** -12, initial_state=s.cuda())
+    want = run(state)
+    state[:, 1, 5, 9] = float("inf")
+    got = run(state)
+    keep = torch.ones(64, dtype=torch.bool)
+    keep[9] = False
+    assert torch.isfinite(want).all() and not torch.isfinite(got[:, :, 1, 9]).any()
+    assert torch.equal(got[:, :, 0], want[:, :, 0]) and torch.equal(got[:, :, 1, keep], want[:, :, 1, keep])
