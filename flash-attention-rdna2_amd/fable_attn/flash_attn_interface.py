@@ -26,6 +26,7 @@ import threading
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _C, _lib
 
@@ -542,6 +543,12 @@ def _paged_prefill(q, k_cache, v_cache, block_table, cu_q, cu_k, max_sq, max_sk,
     return _C.fwd_paged(q, k_cache, v_cache, idx(block_table), idx(cu_q), idx(cu_k), int(max_sq), spec.scale,
                         bool(spec.causal), spec.wl, spec.wr, spec.softcap, spec.alibi, spec.chunk,
                         idx(seqused_q), idx(seqused_k))
+
+
+def _no_tangents(*tensors):
+    """Called at a dual level (fwAD._current_level >= 0): a launch sees primal values only, its result would come back without a tangent."""
+    if any(torch.is_tensor(t) and fwAD.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("fable_attn: no forward-mode derivative; pass tensors without tangents")
 
 
 def _no_grad8(q):

@@ -13,15 +13,17 @@ is zero-padded). decay is (nheads) or (batch, nheads), as the slopes that flash_
 at least 0, 0 for no decay, infinity for a head that sees only the token itself; like those it gets no gradient.
 What is no number (or infinite) in a row of k or v makes the outputs of its heads so (in v: of its column) from that row on, in a row
 of q that row's only; rows before it and other sequences keep their bits.
+Tensors that carry a tangent (forward-mode differentiation) are refused.
 All calls capture into HIP graphs; a captured backward pass wants leaves that no eager graph still holds, because torch's own
 accumulation would run on that graph's stream.
 """
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from . import _C, _lib
-from .flash_attn_interface import (MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _kernel_width, _place, _plans, _remember, _sig,
+from .flash_attn_interface import (MAX_HEAD_DIM, _DTYPES, _aligned, _as_index, _kernel_width, _no_tangents, _place, _plans, _remember, _sig,
                                    _with_width)
 
 # rows per sequence up to which linear_attn_with_state goes token by token
@@ -134,6 +136,8 @@ class _LinearAttention(torch.autograd.Function):
 
 
 def _attend(pack, q, k, v, decay, scale, state, want):
+    if fwAD._current_level >= 0:
+        _no_tangents(q, k, v, decay, state)
     batch = pack[0].numel() - 1 if pack is not None else q.shape[0]
     decay, scale = _check(q, k, v, decay, pack is not None, scale)
     dk, dv = q.shape[-1], v.shape[-1]
@@ -202,6 +206,8 @@ def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu
     no sequence (a padded batch): its rows of out are zeros and no state changes. Two sequences of one call must not name one state; a
     new request starts from a state that the caller has zeroed. Returns out as linear_attn_func. Up to 16 new tokens per sequence
     run token by token, each state read and written once; more run by chunks. Head dims are multiples of 8. No gradient passes through."""
+    if fwAD._current_level >= 0:
+        _no_tangents(q, k, v, state, decay)
     key, plans = None, _plans("linear_step_plans")
     scale = None if scale is None else float(scale)
     max_seqlen = None if max_seqlen is None else int(max_seqlen)

@@ -6,10 +6,11 @@ they write a cache), and the tables, scaled for contexts longer than the trained
     flash_attn_rotary_tables  cosines and sines of all positions
 """
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from . import _C, _lib
-from .flash_attn_interface import _DTYPES, _as_index, _place, _plans, _remember, _sig
+from .flash_attn_interface import _DTYPES, _as_index, _no_tangents, _place, _plans, _remember, _sig
 
 
 def _flat(t):
@@ -77,7 +78,7 @@ def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=T
     columns behind it are copied. Token t of sequence b has row rotary_seqlens[b] + t (an int or int32 (batch); default 0), the last
     row serving those past it, as in flash_attn_append_kvcache. rotary_interleaved: pairs are columns 2 i and 2 i + 1,
     else i and i + rotary_dim / 2. Returns (q, k), or q alone without a k, in new tensors; rows of no sequence come back as zeros.
-    Gradients flow to q and k."""
+    Gradients flow to q and k; tensors that carry a tangent (forward-mode differentiation) are refused."""
     if not q.is_cuda:
         raise ValueError("fable_attn: tensors must be on the GPU (q.is_cuda == False)")
     if q.dtype not in _DTYPES:
@@ -85,6 +86,8 @@ def flash_attn_rotary_func(q, k, rotary_cos, rotary_sin, *, rotary_interleaved=T
     if q.dim() != (4 if cu_seqlens is None else 3):
         raise ValueError(f"fable_attn: q must be (batch, seqlen, nheads, headdim), or (total, nheads, headdim) with cu_seqlens; "
                          f"got {tuple(q.shape)}")
+    if fwAD._current_level >= 0:
+        _no_tangents(q, k, rotary_cos, rotary_sin)
     grad = torch.is_grad_enabled()
     if grad and (rotary_cos.requires_grad or rotary_sin.requires_grad):
         raise NotImplementedError("fable_attn: rotary tables get no gradient; pass them detached")

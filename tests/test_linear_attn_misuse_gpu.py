@@ -1,0 +1,50 @@
+"""Calls of linear attention and the rotation that are refused because a derivative would be lost, and outputs that ask for none."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+pytestmark = pytest.mark.gpu
+
+
+def _fa():
+    import fable_attn
+    return fable_attn
+
+
+def _x(*shape, dtype=torch.float32):
+    return torch.randn(*shape, device="cuda", dtype=dtype)
+
+
+def test_tangents_are_refused():
+    """There is no forward-mode derivative: a dual tensor raises, whichever input it is and whatever else asks for a gradient."""
+    fa = _fa()
+    q, k, v, dec = _x(2, 20, 2, 32), _x(2, 20, 2, 32), _x(2, 20, 2, 32), torch.tensor([0.1, 0.2], device="cuda")
+    state, cu = _x(2, 2, 32, 32), torch.tensor([0, 20, 40], dtype=torch.int32, device="cuda")
+    cos, sin = fa.flash_attn_rotary_tables(20, 32)
+    flat = lambda t: t.flatten(0, 1) if t.dim() == 4 and t.shape[1] == 20 else t
+    for _ in range(2):                                             # (also calls whose signature is known)
+        fa.linear_attn_func(q, k, v, dec, initial_state=state)
+        fa.linear_attn_with_state(q[:, :1], k[:, :1], v[:, :1], state, dec)
+        fa.flash_attn_rotary_func(q, k, cos, sin)
+    with fwAD.dual_level():
+        for grad in (False, True):
+            for i in range(5):
+                x = [t.clone() for t in (q, k, v, dec, state)]
+                x[1].requires_grad_(grad)
+                x[i] = fwAD.make_dual(x[i], torch.ones_like(x[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fa.linear_attn_func(*x[:4], initial_state=x[4])
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fa.linear_attn_varlen_func(*(flat(t) for t in x[:3]), cu, 20, x[3], initial_state=x[4])
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fa.linear_attn_with_state(x[0][:, :1], x[1].detach()[:, :1] if i != 1 else x[1][:, :1], x[2][:, :1], x[4], x[3])
+            for i in range(4):
+                x = [t.clone() for t in (q, k, cos, sin)]
+                x[1].requires_grad_(grad)
+                x[i] = fwAD.make_dual(x[i], torch.ones_like(x[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fa.flash_attn_rotary_func(*x)
+        # other tensors of a dual level are served
+        want = fa.linear_attn_func(q, k, v, dec)
+        turned = fa.flash_attn_rotary_func(q, k, cos, sin)
+    assert torch.equal(fa.linear_attn_func(q, k, v, dec), want) and torch.equal(fa.flash_attn_rotary_func(q, k, cos, sin)[1], turned[1])
