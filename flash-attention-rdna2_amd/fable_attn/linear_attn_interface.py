@@ -202,20 +202,24 @@ def _step_fast(plan, q, k, v, state, decay, idx, cu):
 def linear_attn_with_state(q, k, v, state, decay, state_idx=None, scale=None, cu_seqlens=None, max_seqlen=None):
     """Serving: new tokens q, k, v (batch, seqlen_new, nheads, ...), or packed (total, nheads, ...) with cu_seqlens int32 (batch+1) and
     max_seqlen (default: total), go on from the states of a pool, float32 (num_states, nheads, d, dv), which are
-    updated in place (which autograd sees as it sees any change in place). state_idx int32 (batch): the state of each sequence (default: its own number); an entry outside the pool names
-    no sequence (a padded batch): its rows of out are zeros and no state changes. Two sequences of one call must not name one state; a
-    new request starts from a state that the caller has zeroed. Returns out as linear_attn_func. Up to 16 new tokens per sequence
-    run token by token, each state read and written once; more run by chunks. Head dims are multiples of 8. No gradient passes through."""
+    updated in place (autograd sees that as any change in place). state_idx int32 (batch): the state of each sequence (default: its
+    own number); an entry outside the pool names no sequence (a padded batch): its rows of out are zeros and no state changes. Two
+    sequences of one call must not name one state; a new request starts from a state that the caller has zeroed. Returns out as
+    linear_attn_func. Up to 16 new tokens per sequence (by max_seqlen where packed) run token by token, each state read and written
+    once; more run by chunks. Head dims are multiples of 8. There is no gradient: where one is asked for, run it under torch.no_grad()."""
     if fwAD._current_level >= 0:
         _no_tangents(q, k, v, state, decay)
-    key, plans = None, _plans("linear_step_plans")
+    key, plans, asks = None, _plans("linear_step_plans"), False
     scale = None if scale is None else float(scale)
     max_seqlen = None if max_seqlen is None else int(max_seqlen)
     try:
         key = (_place(q), _place(k), _place(v), _place(state), _sig(decay), _sig(state_idx), _sig(cu_seqlens), scale, max_seqlen)
         plan = plans.get(key)
+        asks = q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or decay.requires_grad
     except (AttributeError, TypeError, ValueError, RuntimeError):   # not tensors, or no key
         key = plan = None
+    if asks and torch.is_grad_enabled():
+        raise NotImplementedError("fable_attn: linear_attn_with_state has no gradient; run it under torch.no_grad()")
     if plan is not None:
         out = _step_fast(plan, q, k, v, state, decay, state_idx, cu_seqlens)
         if out is not None:

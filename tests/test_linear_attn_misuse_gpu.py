@@ -48,3 +48,21 @@ def test_tangents_are_refused():
         want = fa.linear_attn_func(q, k, v, dec)
         turned = fa.flash_attn_rotary_func(q, k, cos, sin)
     assert torch.equal(fa.linear_attn_func(q, k, v, dec), want) and torch.equal(fa.flash_attn_rotary_func(q, k, cos, sin)[1], turned[1])
+
+
+@pytest.mark.parametrize("n", [1, 17])
+def test_steps_refuse_what_asks_for_a_gradient(n):
+    """They give none: a q, k, v, pool or decay that requires one raises, but for torch.no_grad(), where results are the same."""
+    fa = _fa()
+    x = [_x(2, n, 2, 32) for _ in range(3)] + [_x(2, 2, 32, 32), torch.tensor([0.1, 0.2], device="cuda")]
+    pool = x[3].clone()
+    want = fa.linear_attn_with_state(*x[:3], pool, x[4])
+    for _ in range(2):
+        for i in range(5):
+            y = [t.clone() for t in x]
+            y[i].requires_grad_()
+            with pytest.raises(NotImplementedError, match="no_grad"):
+                fa.linear_attn_with_state(*y)
+            assert torch.equal(y[3], x[3])
+            with torch.no_grad():
+                assert torch.equal(fa.linear_attn_with_state(*y), want) and torch.equal(y[3], pool)
