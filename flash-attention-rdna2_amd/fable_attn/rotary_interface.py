@@ -59,7 +59,13 @@ class _Rotary(torch.autograd.Function):
         ctx.interleaved = interleaved
         ctx.set_materialize_grads(False)
         qo, ko = _turn(q, k, cos, sin, interleaved, cu, start, False)
-        return (qo, ko) if k is not None else qo
+        if k is None:
+            return qo
+        # (one launch turns both; what needs no gradient asks for none further on either)
+        needs = ctx.needs_input_grad
+        if not (needs[0] and needs[1]):
+            ctx.mark_non_differentiable(ko if needs[0] else qo)
+        return qo, ko
 
     @staticmethod
     @once_differentiable

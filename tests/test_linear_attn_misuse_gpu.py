@@ -66,3 +66,20 @@ def test_steps_refuse_what_asks_for_a_gradient(n):
             assert torch.equal(y[3], x[3])
             with torch.no_grad():
                 assert torch.equal(fa.linear_attn_with_state(*y), want) and torch.equal(y[3], pool)
+
+
+def test_rotation_asks_for_no_more_gradients_than_its_inputs():
+    fa = _fa()
+    q, k = _x(2, 20, 4, 32), _x(2, 20, 2, 32)
+    cos, sin = fa.flash_attn_rotary_tables(20, 32)
+    turn = lambda t: fa._C.rotary(t, None, cos, sin, True, conj=True)[0]
+    for need in ((True, False), (False, True), (True, True), (False, False)):
+        a, b = q.clone().requires_grad_(need[0]), k.clone().requires_grad_(need[1])
+        out = fa.flash_attn_rotary_func(a, b, cos, sin)
+        assert (out[0].requires_grad, out[1].requires_grad) == need
+        wants = [x for x, n in zip((a, b), need) if n]
+        outs = [x for x, n in zip(out, need) if n]
+        if wants:
+            douts = [torch.randn_like(x) for x in outs]
+            for got, d in zip(torch.autograd.grad(outs, wants, douts), douts):
+                assert torch.equal(got, turn(d))
