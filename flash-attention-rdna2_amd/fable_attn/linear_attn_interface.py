@@ -47,6 +47,8 @@ def _check(q, k, v, decay, packed, scale):
                          f"cu_seqlens; got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     if q.shape[-2] == 0 or k.shape[-2] == 0 or q.shape[-2] % k.shape[-2]:
         raise ValueError(f"fable_attn: nheads_q={q.shape[-2]} is not a multiple of nheads_k={k.shape[-2]} (GQA)")
+    if k.shape[-1] != q.shape[-1]:
+        raise ValueError(f"fable_attn: q and k must share a head_dim, got {q.shape[-1]} and {k.shape[-1]}")
     if max(q.shape[-1], v.shape[-1]) > MAX_HEAD_DIM or min(q.shape[-1], v.shape[-1]) < 1:
         raise ValueError(f"fable_attn: head_dim={q.shape[-1]} and {v.shape[-1]}: 1 to {MAX_HEAD_DIM}")
     if not torch.is_tensor(decay):

@@ -83,3 +83,19 @@ def test_rotation_asks_for_no_more_gradients_than_its_inputs():
             douts = [torch.randn_like(x) for x in outs]
             for got, d in zip(torch.autograd.grad(outs, wants, douts), douts):
                 assert torch.equal(got, turn(d))
+
+
+@pytest.mark.parametrize("dq,dk", [(60, 64), (64, 60), (60, 40), (64, 128), (5, 8), (64, 32)])
+def test_keys_of_another_width_are_refused(dq, dk):
+    """Also where the width that is zero-padded to would fit both."""
+    fa = _fa()
+    dec, cu = torch.tensor([0.1, 0.2], device="cuda"), torch.tensor([0, 20, 40], dtype=torch.int32, device="cuda")
+    q, k, v = _x(2, 20, 2, dq), _x(2, 20, 2, dk), _x(2, 20, 2, 32)
+    with pytest.raises((ValueError, RuntimeError)):
+        fa.linear_attn_func(q, k, v, dec)
+    with pytest.raises((ValueError, RuntimeError)):
+        fa.linear_attn_varlen_func(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cu, 20, dec)
+    pool = torch.zeros(2, 2, dq, 32, device="cuda")
+    with pytest.raises((ValueError, RuntimeError)):
+        fa.linear_attn_with_state(q, k, v, pool, dec)
+    assert not pool.any()
