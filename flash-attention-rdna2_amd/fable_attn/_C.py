@@ -760,9 +760,9 @@ def _linear_params(q, k, v, decay, scale, cu, max_seqlen, state_in=None, slots=N
     p = _lib.FableLinearParams()
     if packed:
         _check_index("cu_seqlens", cu, dev)
-        p.batch, p.n, p.total, p.cu = cu.numel() - 1, int(max_seqlen), q.shape[0], cu.data_ptr()
+        _req(max_seqlen >= 0, f"max_seqlen={max_seqlen}")
+        p.batch, p.n, p.total, p.cu = cu.numel() - 1, min(int(max_seqlen), q.shape[0]), q.shape[0], cu.data_ptr()
         _req(p.batch >= 0, "cu_seqlens must have batch+1 entries")
-        _req(p.n >= 0, f"max_seqlen={p.n}")
     else:
         p.batch, p.n = q.shape[0], q.shape[1]
     _check_f32("decay", decay, dev)

@@ -99,3 +99,22 @@ def test_keys_of_another_width_are_refused(dq, dk):
     with pytest.raises((ValueError, RuntimeError)):
         fa.linear_attn_with_state(q, k, v, pool, dec)
     assert not pool.any()
+
+
+def test_max_seqlen_of_any_size():
+    """It only sizes the launch, also past what 32 bits count; below 0 it is refused."""
+    fa = _fa()
+    dec, cu = torch.tensor([0.1, 0.2], device="cuda"), torch.tensor([0, 20, 400], dtype=torch.int32, device="cuda")
+    q, k, v = (_x(400, 2, 32) for _ in range(3))
+    want = fa.linear_attn_varlen_func(q, k, v, cu, 400, dec)
+    pools = [torch.zeros(2, 2, 32, 32, device="cuda") for _ in range(2)]
+    steps = fa.linear_attn_with_state(q, k, v, pools[0], dec, cu_seqlens=cu, max_seqlen=400)
+    for most in (401, 2 ** 30 + 1, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 40):
+        assert torch.equal(fa.linear_attn_varlen_func(q, k, v, cu, most, dec), want)
+        pools[1].zero_()
+        assert torch.equal(fa.linear_attn_with_state(q, k, v, pools[1], dec, cu_seqlens=cu, max_seqlen=most), steps) and torch.equal(*pools)
+    for most in (-1, -2 ** 32 + 5):
+        with pytest.raises(RuntimeError, match="max_seqlen"):
+            fa.linear_attn_varlen_func(q, k, v, cu, most, dec)
+        with pytest.raises(RuntimeError, match="max_seqlen"):
+            fa.linear_attn_with_state(q, k, v, pools[1], dec, cu_seqlens=cu, max_seqlen=most)
