@@ -14,7 +14,7 @@ namespace fa {
 
 // Segment sg's addition to the state stands where the state before segment sg + 1 is to be; the state before the first is written
 // where the call overwrites it. A thread carries four elements along; its loads of the next four segments do not wait for
-// the sum (B2 S4096 H32 D128, 8 segments: 10 us, 64 MB).
+// the sum (B2 S4096 H32 D128, 8 segments: 11 us, 64 MB).
 __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs p) {
   const int n = p.da * p.db, nb = (n / 4 + 255) / 256;
   const int e = 4 * ((blockIdx.x % nb) * 256 + threadIdx.x);

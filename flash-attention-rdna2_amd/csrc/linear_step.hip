@@ -5,7 +5,7 @@
 // there are few states (the latency of the loads is the time: more workgroups, fewer loads each), 128 else. A thread holds
 // four columns of R consecutive rows. q, k and v pass through LDS in fp32, TB tokens at a time; the products with q are summed
 // over a wave by lane exchanges and over the four waves through LDS, in a fixed order.
-//   Measured, bf16, states of 128 x 128: 48 sequences x 64 heads (403 MB) 79 us, 5.1 TB/s; one sequence 5.6 us, its latency.
+//   Measured, bf16, states of 128 x 128: 48 sequences x 64 heads (403 MB) 80 us, 5.0 TB/s; one sequence x 32 heads 5 us, its latency.
 #include "linear_kernel.hpp"
 
 namespace fa {
@@ -99,6 +99,8 @@ void la_step_rows(const LaArgs& p, hipStream_t st) {
   else hipLaunchKernelGGL((la_step_kernel<T, CT, 256 / RG>), grid, dim3(256), 0, st, p);
 }
 
+// Columns of a workgroup. Heads of 128, 32 columns against 128, us on the device one call after another: 32 states 4.6 / 5.2, 128 6.0 / 6.2,
+// 256 8.5 / 7.6, 512 12.4 / 10.5, 3072 62.7 / 64.8; 128 heads of 64 4.2 / 5.2, 1024 10.3 / 9.0; 256 heads of 256 (512 tiles) 24.1 / 27.1.
 template <typename T>
 void la_step_type(const LaArgs& p, hipStream_t st) {
   if ((long long)p.batch * p.NH * ((p.db + 127) / 128) < 512 || p.db <= 32) la_step_rows<T, 32>(p, st);

@@ -171,7 +171,9 @@ void rot_launch(RotArgs a, bool wide, hipStream_t st) {
   }
   a.units = (p.rotary == 1 ? p.rotary_dim / 2 / N : p.rotary_dim / N) + (p.HD - p.rotary_dim) / N;
   const int per = a.units >= 64 ? 1 : 64 / a.units, turns = (heads + per - 1) / per;
-  // waves of a token: up to one per turn of the loop while the chip has fewer than 2048 waves
+  // Waves of a token: up to one per turn of the loop while the chip has fewer than 2048 waves. bf16, 64 + 8 heads of 128, us on the device with
+  // one wave a token / 1024 / 2048 / 4096 in all / one per turn: 48 tokens 8.1 / 3.5 / 3.5 / 3.5 / 3.5, 512 8.9 / 6.7 / 6.0 / 6.0 / 7.1,
+  // 1024 12.1 / 12.2 / 8.9 / 8.4 / 11.4, 2048 16.6 / 17.0 / 16.6 / 14.8 / 18.8.
   long long split = a.tokens > 0 ? 2048 / a.tokens : 1;
   a.split = (int)(split < 1 ? 1 : split > turns ? turns : split);
   const dim3 grid((unsigned)((a.tokens * a.split + 3) / 4));
@@ -272,7 +274,9 @@ extern "C" int fable_attn_rotary_tables(FableRotaryTableParams p, void* stream) 
   a.step = log2(p.base) / p.pairs;
   const int columns = wide ? p.pairs / 4 : p.pairs;
   a.columns = columns < 256 ? columns : 256;
-  // eight rows a thread at least where there are enough of them to fill the chip
+  // Eight rows a thread at least where there are enough of them to fill the chip, for the frequencies formed once. 64 pairs, us on the
+  // device, this rule / at most 1024 workgroups / a row a thread: 32768 positions 7.7 / 7.6 / 8.6, 131072 16.0 / 15.7 / 22.0, 1048576
+  // 120 / 119 / 157.
   const long long groups = (p.rows + 256 / a.columns - 1) / (256 / a.columns);
   const unsigned grid = (unsigned)(groups < 1024 ? groups : groups / 8 < 1024 ? 1024 : groups / 8 < 4096 ? groups / 8 : 4096);
   if (wide) hipLaunchKernelGGL(rot_table_kernel<4>, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
