@@ -31,7 +31,7 @@
 // remembers; and for all but fast decays that spares most of the DA / 2 multiplications per lane and chunk.
 //
 // Measured, bf16, heads of 128: B2 S4096 H32 (268 MB) 54 to 60 us, 4.5 to 5.0 TB/s, of the 5.2 that a large copy reaches
-// here; the states of its segments beside that 35 us, and 11 to chain them. fp16: forward 131 us with all, 104 in bf16. What bounds it is the bytes and, as much, the issue of vector and
+// here; the states of its segments beside that 35 us, and 11 to chain them. fp16: a whole forward call 131 us, 104 in bf16. What bounds it is the bytes and, as much, the issue of vector and
 // matrix instructions, which are busy 80% of a CU's cycles together. Where a SIMD has one wave, the chain of a chunk's steps
 // does: 1.9 us per chunk, 60 ns per row. Not kept, because slower or no faster: three waves per SIMD (387 against 371 us forward
 // and backward: fewer loads of operands in flight), two chunks' tiles ahead in registers, two LDS buffers, the operands of
