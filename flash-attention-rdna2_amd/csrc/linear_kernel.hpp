@@ -31,8 +31,9 @@
 // remembers; and for all but fast decays that spares most of the DA / 2 multiplications per lane and chunk.
 //
 // Measured, bf16, heads of 128: B2 S4096 H32 (268 MB) 54 to 60 us, 4.5 to 5.0 TB/s, of the 5.2 that a large copy reaches
-// here; the states of its segments beside that 35 us, and 11 to chain them. fp16: a whole forward call 131 us, 104 in bf16. What bounds it is the bytes and, as much, the issue of vector and
-// matrix instructions, which are busy 80% of a CU's cycles together. Where a SIMD has one wave, the chain of a chunk's steps
+// here; the states of its segments beside that 35 us, and 11 to chain them; a whole call 103, in fp16 124 to 131. What bounds it
+// is the bytes and, as much, the issue of vector and matrix instructions, which are busy 80% of a CU's cycles together. Where a
+// SIMD has one wave, the chain of a chunk's steps
 // does: 1.9 us per chunk, 60 ns per row. Not kept, because slower or no faster: three waves per SIMD (387 against 371 us forward
 // and backward: fewer loads of operands in flight), two chunks' tiles ahead in registers, two LDS buffers, the operands of
 // four steps read ahead, C = 64 (registers spill).
@@ -100,7 +101,7 @@ struct La<float> {
 
 // LDS tiles, rows of LD values. Rows of x and y are read by 32 lanes at one column (8 bytes each) and y by columns, 4 rows
 // x 32 columns at a time: a row is 7 units of 8 bytes longer than a multiple of the 64 banks (or of half of them), so the
-// first meets every bank once and the second nearly so; z is read by columns only and is 8 units longer. (fp32: one unit of
+// first meets every bank once and the second nearly so; z, and fp16's weighted y, are read by columns only and 8 units longer. (fp32: one unit of
 // 16 bytes.) Padding, not a turned order within the row, because then all addresses are one register and constants.
 template <typename T, int W>
 constexpr int kLaRow = W + (sizeof(T) == 2 ? 28 : 4);

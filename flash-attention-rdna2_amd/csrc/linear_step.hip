@@ -100,7 +100,7 @@ void la_step_rows(const LaArgs& p, hipStream_t st) {
 }
 
 // Columns of a workgroup. Heads of 128, 32 columns against 128, us on the device one call after another: 32 states 4.6 / 5.2, 128 6.0 / 6.2,
-// 256 8.5 / 7.6, 512 12.4 / 10.5, 3072 62.7 / 64.8; 128 heads of 64 4.2 / 5.2, 1024 10.3 / 9.0; 256 heads of 256 (512 tiles) 24.1 / 27.1.
+// 256 8.5 / 7.6, 512 12.4 / 10.5, 48 x 64 62.7 / 64.8; 128 heads of 64 4.2 / 5.2, 1024 10.3 / 9.0; 256 heads of 256 (512 tiles) 24.1 / 27.1.
 template <typename T>
 void la_step_type(const LaArgs& p, hipStream_t st) {
   if ((long long)p.batch * p.NH * ((p.db + 127) / 128) < 512 || p.db <= 32) la_step_rows<T, 32>(p, st);
